@@ -22,6 +22,7 @@
 #ifndef KQ_H
 #define KQ_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -255,6 +256,93 @@ int kq_subblock_sums(const void* w, int R, int C, int type, const void* xq, int 
  */
 int kq_dequant_rows(const void* w, int R, int C, int type, int row0, int nrows, float* y,
                     int64_t ldy, void* stream);
+
+/*
+ * Decoding with a paged key-value cache.  No counterpart in the reference's Q4 path, whose engine keeps one
+ * contiguous cache (engine.py:255-280); these operators serve several requests from one pool of pages, on
+ * the fp32 activations that the products above read and write.
+ *
+ * A cache holds `pages` pages of `page_size` positions for `heads` key-value heads of `dim` values: element d
+ * of (page, head, position) lies at page * page_stride + head * head_stride + position * pos_stride + d, the
+ * same for k and v, in elements.  KQ_KV_I8 stores codes in -127..127 and one fp32 scale per (page, head,
+ * position), at the scale strides: a value is code * scale.  Requirements: dim a multiple of 16 up to 256,
+ * page_size a power of two, k and v 16-byte aligned, strides multiples of 16 bytes and at least dim.
+ *
+ * A request's positions lie in the pages that its row of the page table names: position p in page
+ * table[seq * ldt + p / page_size].  An entry outside 0..pages-1 is a hole: nothing is stored there, and
+ * attention passes over its positions.  Tables, positions and lengths are int32 on the device and are read
+ * when the kernel runs; a request holds at most width * page_size positions (at most 2^30).
+ */
+#define KQ_KV_F16 1
+#define KQ_KV_I8 24
+#define KQ_KV_BF16 30
+
+typedef struct kq_kv {
+    void* k;
+    void* v;
+    float* k_scale;          /* KQ_KV_I8 only */
+    float* v_scale;
+    int type, heads, dim, pages, page_size;
+    int64_t page_stride, head_stride, pos_stride;
+    int64_t scale_page_stride, scale_head_stride, scale_pos_stride;
+} kq_kv;
+
+/*
+ * Append N tokens: token n belongs to request seq[n] and stands at position pos[n].  Its keys k[n] (heads x dim
+ * floats, row stride ldk) are rotated and stored with its values v[n]; its queries q[n] (q_heads x dim, row stride
+ * ldq) are rotated into q_out[n] (row stride ldqo; q_out may be q).  q and q_out NULL: keys and values only.
+ * The first `rot` values of a head turn (a, b) -> (a cos - b sin, b cos + a sin), each product and sum
+ * rounded to fp32, where a pair is (i, i + rot/2), or (2i, 2i + 1) with `interleaved`; rope holds for each of
+ * rope_rows positions rot/2 cosines, then rot/2 sines (rot a multiple of 8; rope NULL: nothing turns).  f16
+ * and bf16 round to nearest even; KQ_KV_I8: scale = max|x| / 127, code = x / scale to nearest even.  Inputs must be
+ * finite there.  A token whose seq is outside 0..seqs-1, or whose pos is outside the request's positions or the rope
+ * table, is skipped: nothing of it is read or written.  Tokens of one call must have different places.  All float
+ * pointers 4-byte aligned.
+ */
+int kq_kv_append(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, int N, const int32_t* seq,
+                 const int32_t* pos, const float* q, int64_t ldq, int q_heads, float* q_out, int64_t ldqo, const float* k,
+                 int64_t ldk, const float* v, int64_t ldv, const float* rope, int rope_rows, int rot, int interleaved,
+                 void* stream);
+
+/* Bytes of device workspace kq_attn_paged needs (0 for invalid sizes). */
+size_t kq_attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len);
+
+/*
+ * Attention of the last T (1..16) tokens of each request over its cache, T = 1 for decoding, more to verify a draft
+ * (kq_gemv_q8k's rows).  lens[b] counts request b's positions, the new tokens included (values above max_len or
+ * the table's positions count as those); row b * T + t of q and out (q_heads x dim floats, row strides ldq, ldo) is
+ * token t, which sees the positions below lens[b] - T + 1 + t.  Query head h reads key-value head
+ * h / (q_heads / heads).  out = sum_p softmax_p(scale * q.k_p) v_p, summed in fp32; a row that sees no position
+ * is 0.  A row's result depends only on its query, its cache and how many positions it sees, not on T, on max_len or
+ * on the other requests.  out must not overlap q.  ws: 256-byte aligned, kq_attn_paged_workspace bytes; calls
+ * sharing it must be ordered.  Float pointers 4-byte aligned.  Allocates nothing.
+ */
+int kq_attn_paged(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, const int32_t* lens,
+                  int max_len, int T, const float* q, int64_t ldq, int q_heads, float scale, float* out, int64_t ldo,
+                  void* ws, size_t ws_bytes, void* stream);
+
+/* Bytes of workspace kq_logits_penalize needs for B rows with a pick (0 for invalid sizes). */
+size_t kq_logits_workspace(int B);
+
+/*
+ * Penalties, biases and a grammar mask on B rows of V logits, with the greedy pick.  For each row b, with its history
+ * hist[b][0..hist_len[b]-1] of token ids (row stride ldh >= max_hist; lengths count up to max_hist; ids outside
+ * 0..V-1 are passed over), of which the first prompt_len[b] are the prompt:
+ *   y = x;  where the id occurs in the history:  y = y > 0 ? y / rep[b] : y * rep[b];
+ *   y -= freq[b] * c, y -= pres[b] where c > 0, with c the occurrences after the prompt;
+ *   y += bias_val[b][i] where bias_id[b][i] is the id (nb entries, row stride ldb; an id's last entry counts);
+ *   y = -inf where bit id % 32 of allowed[b][id / 32] (row stride ldm words; 0: one row for all) is 0,
+ * each step rounded to fp32.  hist, prompt_len, rep, freq, pres, bias_id and allowed may each be NULL: without that
+ * step (prompt_len: no prompt).  y (row stride ldy; may be x) receives the rows, or is NULL; picked[b] receives the
+ * index of the row's largest value, the smallest index among equal ones, NaN never, and -1 when nothing is above
+ * -1e30, or is NULL; one of the two is needed.  ws (for picked): 256-byte aligned, kq_logits_workspace(B) bytes,
+ * zero-filled before its first use (each call leaves it ready for the next); calls sharing it must be ordered.
+ */
+int kq_logits_penalize(const float* x, int64_t ldx, int B, int V, const int32_t* hist, int64_t ldh, int max_hist,
+                       const int32_t* hist_len, const int32_t* prompt_len, const float* rep, const float* freq,
+                       const float* pres, const int32_t* bias_id, const float* bias_val, int64_t ldb, int nb,
+                       const uint32_t* allowed, int64_t ldm, float* y, int64_t ldy, void* ws, size_t ws_bytes,
+                       int32_t* picked, void* stream);
 
 #ifdef __cplusplus
 }

@@ -449,4 +449,183 @@ int kq_dequant_rows(const void* w, int R, int C, int type, int row0, int nrows, 
     return check_launch(fn);
 }
 
+// A cache's own rules (include/kq.h, kq_kv).
+static int check_kv(const kq_kv* kv, const char* fn) {
+    if (!kv) return fail(KQ_ERR_ARG, "%s: kv is NULL", fn);
+    if (kv->type != KQ_KV_F16 && kv->type != KQ_KV_BF16 && kv->type != KQ_KV_I8)
+        return fail(KQ_ERR_ARG, "%s: cache type %d is not f16 (1), i8 (24) or bf16 (30)", fn, kv->type);
+    if (kv->heads < 1 || kv->heads > 4096) return fail(KQ_ERR_ARG, "%s: heads=%d must be 1..4096", fn, kv->heads);
+    if (kv->dim < 16 || kv->dim > 256 || kv->dim % 16)
+        return fail(KQ_ERR_ARG, "%s: dim=%d must be a multiple of 16 up to 256", fn, kv->dim);
+    if (kv->page_size < 1 || kv->page_size > (1 << 20) || (kv->page_size & (kv->page_size - 1)))
+        return fail(KQ_ERR_ARG, "%s: page_size=%d must be a power of two up to 2^20", fn, kv->page_size);
+    if (kv->pages < 1) return fail(KQ_ERR_ARG, "%s: pages=%d must be positive", fn, kv->pages);
+    KQ_TRY(check_ptr(kv->k, 16, "k of the cache", fn));
+    KQ_TRY(check_ptr(kv->v, 16, "v of the cache", fn));
+    const int64_t unit = kv->type == KQ_KV_I8 ? 16 : 8;
+    for (int64_t st : {kv->page_stride, kv->head_stride, kv->pos_stride})
+        if (st < kv->dim || st % unit || st > (INT64_MAX >> 33))
+            return fail(KQ_ERR_ARG, "%s: stride %lld of the cache must be a multiple of %lld, at least dim=%d", fn,
+                        (long long)st, (long long)unit, kv->dim);
+    if (kv->type == KQ_KV_I8) {
+        KQ_TRY(check_ptr(kv->k_scale, 4, "k_scale of the cache", fn));
+        KQ_TRY(check_ptr(kv->v_scale, 4, "v_scale of the cache", fn));
+        for (int64_t st : {kv->scale_page_stride, kv->scale_head_stride, kv->scale_pos_stride})
+            if (st < 1 || st > (INT64_MAX >> 33))
+                return fail(KQ_ERR_ARG, "%s: scale stride %lld of the cache must be positive", fn, (long long)st);
+    }
+    return KQ_OK;
+}
+
+static int check_table(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, const char* fn,
+                       PageTable* out) {
+    KQ_TRY(check_ptr(table, 4, "table", fn));
+    if (seqs < 1 || seqs > 65535) return fail(KQ_ERR_ARG, "%s: seqs=%d must be 1..65535", fn, seqs);
+    if (width < 1 || (int64_t)width * kv->page_size > (1 << 30))
+        return fail(KQ_ERR_ARG, "%s: width=%d pages of %d positions must be 1..2^30 positions", fn, width, kv->page_size);
+    if (ldt < width) return fail(KQ_ERR_ARG, "%s: ldt=%lld is smaller than width=%d", fn, (long long)ldt, width);
+    *out = PageTable{table, ldt, seqs, width * kv->page_size};
+    return KQ_OK;
+}
+
+static int check_rows(const void* p, int64_t ld, int64_t n, int64_t row, const char* what, const char* fn) {
+    KQ_TRY(check_ptr(p, 4, what, fn));
+    if (n > 1 && ld < row)
+        return fail(KQ_ERR_ARG, "%s: row stride %lld of %s is smaller than %lld", fn, (long long)ld, what, (long long)row);
+    return KQ_OK;
+}
+
+static int check_q_heads(const kq_kv* kv, int q_heads, const char* fn) {
+    if (q_heads < 1 || q_heads > 4096 || q_heads % kv->heads)
+        return fail(KQ_ERR_ARG, "%s: q_heads=%d must be a multiple of the cache's %d heads, up to 4096", fn, q_heads,
+                    kv->heads);
+    return KQ_OK;
+}
+
+int kq_kv_append(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, int N, const int32_t* seq,
+                 const int32_t* pos, const float* q, int64_t ldq, int q_heads, float* q_out, int64_t ldqo, const float* k,
+                 int64_t ldk, const float* v, int64_t ldv, const float* rope, int rope_rows, int rot, int interleaved,
+                 void* stream) {
+    static const char* fn = "kq_kv_append";
+    AppendArgs a = {};
+    KQ_TRY(check_kv(kv, fn));
+    KQ_TRY(check_table(kv, table, ldt, seqs, width, fn, &a.table));
+    if (N < 0) return fail(KQ_ERR_ARG, "%s: N=%d is negative", fn, N);
+    if ((q != nullptr) != (q_out != nullptr)) return fail(KQ_ERR_ARG, "%s: q and q_out go together", fn);
+    if (q) KQ_TRY(check_q_heads(kv, q_heads, fn));
+    if (rope) {
+        KQ_TRY(check_ptr(rope, 4, "rope", fn));
+        if (rot < 8 || rot % 8 || rot > kv->dim)
+            return fail(KQ_ERR_ARG, "%s: rot=%d must be a multiple of 8 up to dim=%d", fn, rot, kv->dim);
+        if (rope_rows < 1) return fail(KQ_ERR_ARG, "%s: rope_rows=%d must be positive", fn, rope_rows);
+    }
+    if (N == 0) return KQ_OK;
+    KQ_TRY(check_ptr(seq, 4, "seq", fn));
+    KQ_TRY(check_ptr(pos, 4, "pos", fn));
+    const int64_t kw = (int64_t)kv->heads * kv->dim, qw = (int64_t)q_heads * kv->dim;
+    KQ_TRY(check_rows(k, ldk, N, kw, "k", fn));
+    KQ_TRY(check_rows(v, ldv, N, kw, "v", fn));
+    if (q) {
+        KQ_TRY(check_rows(q, ldq, N, qw, "q", fn));
+        KQ_TRY(check_rows(q_out, ldqo, N, qw, "q_out", fn));
+    }
+    a.kv = *kv;
+    a.N = N;
+    a.q_heads = q ? q_heads : 0;
+    if ((int64_t)N * (a.q_heads + 2 * kv->heads) > (1 << 30))
+        return fail(KQ_ERR_ARG, "%s: N=%d tokens are too many for one call", fn, N);
+    a.rope_rows = rope_rows;
+    a.rot = rope ? rot : 0;
+    a.interleaved = interleaved;
+    a.seq = seq, a.pos = pos, a.q = q, a.k = k, a.v = v, a.rope = rope, a.q_out = q_out;
+    a.ldq = ldq, a.ldqo = ldqo, a.ldk = ldk, a.ldv = ldv;
+    launch_kv_append(a, as_stream(stream));
+    return check_launch(fn);
+}
+
+size_t kq_attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len) {
+    if (seqs < 1 || seqs > 65535 || q_heads < 1 || q_heads > 4096 || dim < 16 || dim > 256 || dim % 16 || T < 1 ||
+        T > KQ_MAX_BATCH || max_len < 1 || max_len > (1 << 30))
+        return 0;
+    return attn_paged_workspace(seqs, q_heads, dim, T, max_len);
+}
+
+int kq_attn_paged(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, const int32_t* lens,
+                  int max_len, int T, const float* q, int64_t ldq, int q_heads, float scale, float* out, int64_t ldo,
+                  void* ws, size_t ws_bytes, void* stream) {
+    static const char* fn = "kq_attn_paged";
+    AttnArgs a = {};
+    KQ_TRY(check_kv(kv, fn));
+    KQ_TRY(check_table(kv, table, ldt, seqs, width, fn, &a.table));
+    KQ_TRY(check_q_heads(kv, q_heads, fn));
+    KQ_TRY(check_ptr(lens, 4, "lens", fn));
+    if (T < 1 || T > KQ_MAX_BATCH) return fail(KQ_ERR_ARG, "%s: T=%d must be 1..%d", fn, T, KQ_MAX_BATCH);
+    if (max_len < 1 || max_len > (1 << 30)) return fail(KQ_ERR_ARG, "%s: max_len=%d must be 1..2^30", fn, max_len);
+    const int64_t rows = (int64_t)seqs * T, qw = (int64_t)q_heads * kv->dim;
+    KQ_TRY(check_rows(q, ldq, rows, qw, "q", fn));
+    KQ_TRY(check_rows(out, ldo, rows, qw, "out", fn));
+    if (!(scale - scale == 0)) return fail(KQ_ERR_ARG, "%s: scale must be finite", fn);
+    KQ_TRY(check_ptr(ws, 256, "ws", fn));
+    const size_t need = attn_paged_workspace(seqs, q_heads, kv->dim, T, max_len);
+    if (ws_bytes < need)
+        return fail(KQ_ERR_ARG, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, need);
+    a.kv = *kv;
+    a.lens = lens;
+    a.max_len = max_len < a.table.cap ? max_len : a.table.cap;
+    a.T = T;
+    a.q_heads = q_heads;
+    a.q = q, a.ldq = ldq, a.out = out, a.ldo = ldo;
+    a.scale = scale;
+    a.ws = static_cast<uint8_t*>(ws);
+    launch_attn_paged(a, as_stream(stream));
+    return check_launch(fn);
+}
+
+size_t kq_logits_workspace(int B) { return B < 1 || B > 65535 ? 0 : logits_workspace(B); }
+
+int kq_logits_penalize(const float* x, int64_t ldx, int B, int V, const int32_t* hist, int64_t ldh, int max_hist,
+                       const int32_t* hist_len, const int32_t* prompt_len, const float* rep, const float* freq,
+                       const float* pres, const int32_t* bias_id, const float* bias_val, int64_t ldb, int nb,
+                       const uint32_t* allowed, int64_t ldm, float* y, int64_t ldy, void* ws, size_t ws_bytes,
+                       int32_t* picked, void* stream) {
+    static const char* fn = "kq_logits_penalize";
+    if (B < 1 || B > 65535) return fail(KQ_ERR_ARG, "%s: B=%d must be 1..65535", fn, B);
+    if (V < 1 || V > (1 << 30)) return fail(KQ_ERR_ARG, "%s: V=%d must be 1..2^30", fn, V);
+    KQ_TRY(check_rows(x, ldx, B, V, "x", fn));
+    if (hist) {
+        if (max_hist < 0) return fail(KQ_ERR_ARG, "%s: max_hist=%d is negative", fn, max_hist);
+        KQ_TRY(check_rows(hist, ldh, B, max_hist, "hist", fn));
+        KQ_TRY(check_ptr(hist_len, 4, "hist_len", fn));
+    }
+    if (bias_id) {
+        if (nb < 0) return fail(KQ_ERR_ARG, "%s: nb=%d is negative", fn, nb);
+        KQ_TRY(check_rows(bias_id, ldb, B, nb, "bias_id", fn));
+        KQ_TRY(check_ptr(bias_val, 4, "bias_val", fn));
+    }
+    if (allowed) {
+        KQ_TRY(check_ptr(allowed, 4, "allowed", fn));
+        if (ldm < 0 || (ldm > 0 && ldm < (V + 31) / 32))
+            return fail(KQ_ERR_ARG, "%s: ldm=%lld words must be 0 or at least %d", fn, (long long)ldm, (V + 31) / 32);
+    }
+    for (const void* p : {(const void*)prompt_len, (const void*)rep, (const void*)freq, (const void*)pres})
+        if (p) KQ_TRY(check_ptr(p, 4, "a per-row array", fn));
+    if (!y && !picked) return fail(KQ_ERR_ARG, "%s: neither y nor picked is given", fn);
+    if (y) KQ_TRY(check_rows(y, ldy, B, V, "y", fn));
+    if (picked) {
+        KQ_TRY(check_ptr(picked, 4, "picked", fn));
+        KQ_TRY(check_ptr(ws, 256, "ws", fn));
+        if (ws_bytes < logits_workspace(B))
+            return fail(KQ_ERR_ARG, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, logits_workspace(B));
+    }
+    LogitsArgs a = {};
+    a.x = x, a.ldx = ldx, a.B = B, a.V = V;
+    a.hist = hist, a.ldh = ldh, a.max_hist = max_hist, a.hist_len = hist_len, a.prompt_len = prompt_len;
+    a.rep = rep, a.freq = freq, a.pres = pres;
+    a.bias_id = bias_id, a.bias_val = bias_val, a.ldb = ldb, a.nb = nb;
+    a.allowed = allowed, a.ldm = ldm;
+    a.y = y, a.ldy = ldy, a.ws = static_cast<uint8_t*>(ws), a.picked = picked;
+    launch_logits(a, as_stream(stream));
+    return check_launch(fn);
+}
+
 }  // extern "C"

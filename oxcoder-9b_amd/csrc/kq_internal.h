@@ -110,4 +110,50 @@ void launch_gemv_f32_rows(int n, const uint8_t* const* w, const int* R, int C, i
 void launch_dequant_rows(const uint8_t* w, int R, int C, int type, int row0, int nrows, float* y,
                          int64_t ldy, hipStream_t s);
 
+// Decoding with a paged cache.  A request's page table, as the kernels take it: positions are clamped or tested
+// against cap = width * page_size, page numbers against the cache's pages, before any address is formed.
+struct PageTable {
+    const int32_t* pages;
+    int64_t ld;
+    int seqs, cap;
+};
+struct AppendArgs {
+    kq_kv kv;
+    PageTable table;
+    int N, q_heads, rope_rows, rot, interleaved;
+    const int32_t *seq, *pos;
+    const float *q, *k, *v, *rope;
+    float* q_out;
+    int64_t ldq, ldqo, ldk, ldv;
+};
+void launch_kv_append(const AppendArgs& a, hipStream_t s);
+struct AttnArgs {
+    kq_kv kv;
+    PageTable table;
+    const int32_t* lens;
+    int max_len, T, q_heads;
+    const float* q;
+    int64_t ldq, ldo;
+    float scale;
+    float* out;
+    uint8_t* ws;
+};
+size_t attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len);
+void launch_attn_paged(const AttnArgs& a, hipStream_t s);
+struct LogitsArgs {
+    const float* x;
+    int64_t ldx, ldh, ldb, ldm, ldy;
+    int B, V, max_hist, nb;
+    const int32_t *hist, *hist_len, *prompt_len;
+    const float *rep, *freq, *pres;
+    const int32_t* bias_id;
+    const float* bias_val;
+    const uint32_t* allowed;
+    float* y;
+    uint8_t* ws;
+    int32_t* picked;
+};
+size_t logits_workspace(int B);
+void launch_logits(const LogitsArgs& a, hipStream_t s);
+
 }  // namespace kq

@@ -12,6 +12,16 @@ LIBKQHOST = os.path.join(HERE, "libkqhost.so")
 
 # Every symbol include/kq.h declares, with (restype, argtypes).
 _vp, _i, _i64 = C.c_void_p, C.c_int, C.c_int64
+
+
+class KV(C.Structure):
+    """kq_kv: a paged key-value cache (include/kq.h)."""
+    _fields_ = ([("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp)]
+                + [(n, _i) for n in ("type", "heads", "dim", "pages", "page_size")]
+                + [(n, _i64) for n in ("page_stride", "head_stride", "pos_stride", "scale_page_stride",
+                                       "scale_head_stride", "scale_pos_stride")])
+
+
 KQ_SYMBOLS = {
     "kq_last_error": (C.c_char_p, []),
     "kq_version": (_i, []),
@@ -42,6 +52,14 @@ KQ_SYMBOLS = {
     "kq_gemm_q8k_static": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _i64, _vp]),
     "kq_subblock_sums": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp]),
     "kq_dequant_rows": (_i, [_vp, _i, _i, _i, _i, _i, _vp, _i64, _vp]),
+    "kq_kv_append": (_i, [_vp, _vp, _i64, _i, _i, _i, _vp, _vp, _vp, _i64, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i,
+                          _i, _i, _vp]),
+    "kq_attn_paged_workspace": (C.c_size_t, [_i, _i, _i, _i, _i]),
+    "kq_attn_paged": (_i, [_vp, _vp, _i64, _i, _i, _vp, _i, _i, _vp, _i64, _i, C.c_float, _vp, _i64, _vp, C.c_size_t,
+                           _vp]),
+    "kq_logits_workspace": (C.c_size_t, [_i]),
+    "kq_logits_penalize": (_i, [_vp, _i64, _i, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _vp,
+                                _i64, _vp, _i64, _vp, C.c_size_t, _vp, _vp]),
 }
 KQHOST_SYMBOLS = {
     "kq_host_quantize_q4k": (_i, [_vp, _i64, _i, _vp]),
@@ -55,6 +73,7 @@ KQ_ERR_ARG = -1
 KQ_ERR_HIP = -2
 KQ_MAX_BATCH = 16
 KQ_GEMM_STATIC_SCRATCH_BYTES = 32 << 20
+KQ_KV_F16, KQ_KV_I8, KQ_KV_BF16 = 1, 24, 30
 
 _libs = {}
 

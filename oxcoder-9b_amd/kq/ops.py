@@ -431,3 +431,111 @@ def dequant_rows(w, R, C_, ty, row0, nrows, y=None):
     _lib.check(_lib.kq().kq_dequant_rows(pw, R, C_, ty, row0, nrows, _dev(y, "y", torch.float32), ld,
                                          _stream(w.device)))
     return y
+
+
+def _opt(t, name, dtype, n):
+    """Pointer of an optional contiguous 1-D device tensor of at least n values."""
+    if t is None:
+        return None
+    if t.numel() < n or not t.is_contiguous():
+        raise ValueError("%s must hold %d values, contiguous" % (name, n))
+    return _dev(t, name, dtype)
+
+
+def _mat(t, name, dtype, rows, cols):
+    """(pointer, row stride) of a 2-D device tensor of at least rows x cols with contiguous rows."""
+    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols:
+        raise ValueError("%s must be [%d][%d], got %s" % (name, rows, cols, list(t.shape)))
+    return _dev(t, name, dtype), t.stride(0)
+
+
+def _table(t):
+    """(pointer, row stride, rows, columns) of a page table."""
+    if t.dim() != 2:
+        raise ValueError("table must be [requests][pages]")
+    seqs, width = t.shape
+    return _dev(t, "table", torch.int32), t.stride(0) if seqs > 1 else width, seqs, width
+
+
+def kv_append(cache, table, q, k, v, seq, pos, q_out, q_heads, rope=None, interleaved=False):
+    """Rotate q [N][q_heads * dim] into q_out and k [N][heads * dim], and store k and v of token n at position pos[n]
+    of request seq[n] in ``cache`` (a kv.KVCache) under ``table`` int32 [requests][width] (kq_kv_append).
+    q and q_out None: keys and values only; rope: kv.rope_table's, or None."""
+    N, heads, D = k.shape[0], cache.heads, cache.dim
+    pk, ldk = _mat(k, "k", torch.float32, N, heads * D)
+    pv, ldv = _mat(v, "v", torch.float32, N, heads * D)
+    pq = po = None
+    ldq = ldo = 0
+    if (q is None) != (q_out is None):
+        raise ValueError("q and q_out go together")
+    if q is not None:
+        pq, ldq = _mat(q, "q", torch.float32, N, q_heads * D)
+        po, ldo = _mat(q_out, "q_out", torch.float32, N, q_heads * D)
+    pr, rows, rot = None, 0, 0
+    if rope is not None:
+        rows, rot = rope.shape
+        if not rope.is_contiguous():
+            raise ValueError("rope must be contiguous")
+        pr = _dev(rope, "rope", torch.float32)
+    pt, ldt, seqs, width = _table(table)
+    _lib.check(_lib.kq().kq_kv_append(cache.ref, pt, ldt, seqs, width, N, _opt(seq, "seq", torch.int32, N),
+                                      _opt(pos, "pos", torch.int32, N), pq, ldq, q_heads, po, ldo, pk, ldk, pv, ldv, pr, rows, rot, 1 if interleaved else 0,
+                                      _stream(cache.device)))
+    return q_out
+
+
+def attn_paged_workspace_bytes(seqs, q_heads, dim, tokens, max_len):
+    """Device bytes of workspace attn_paged needs (kq_attn_paged_workspace; 0 for sizes it does not take)."""
+    return int(_lib.kq().kq_attn_paged_workspace(seqs, q_heads, dim, tokens, max_len))
+
+
+def attn_paged(cache, table, q, lens, out, q_heads, tokens, scale, max_len, ws):
+    """Attention of the last ``tokens`` tokens of each request over ``cache`` (a kv.KVCache) under ``table``
+    int32 [requests][width]: q, out [requests * tokens][q_heads * dim], lens int32 [requests] counting the new
+    tokens, at most max_len; ws of attn_paged_workspace_bytes, 256-byte aligned (kq_attn_paged)."""
+    pt, ldt, seqs, width = _table(table)
+    pq, ldq = _mat(q, "q", torch.float32, seqs * tokens, q_heads * cache.dim)
+    po, ldo = _mat(out, "out", torch.float32, seqs * tokens, q_heads * cache.dim)
+    _lib.check(_lib.kq().kq_attn_paged(cache.ref, pt, ldt, seqs, width, _opt(lens, "lens", torch.int32, seqs), max_len,
+                                       tokens, pq, ldq, q_heads, scale, po, ldo, _dev(ws, "ws", torch.uint8), ws.numel(), _stream(cache.device)))
+    return out
+
+
+def logits_workspace_bytes(rows):
+    """Device bytes of zero-filled workspace logits_penalize needs (kq_logits_workspace; 0 for sizes it does not take)."""
+    return int(_lib.kq().kq_logits_workspace(rows))
+
+
+def logits_penalize(x, history=None, length=None, prompt=None, repetition=None, frequency=None, presence=None,
+                    bias_ids=None, bias_values=None, allowed=None, y=None, picked=None, ws=None):
+    """Penalties, biases and a grammar mask on logits x [B][V] into y (may be x) and the greedy pick into picked
+    int32 [B] (ws: zero-filled, logits_workspace_bytes, 256-byte aligned); either may be None
+    (kq_logits_penalize; the arguments are sampling.Picker.pick's)."""
+    B, V = x.shape
+    px, ldx = _mat(x, "x", torch.float32, B, V)
+    ph = pb = pv = pm = py = None
+    ldh = hist = ldb = nb = ldm = ldy = 0
+    if history is not None:
+        if length is None:
+            raise ValueError("history needs its length")
+        hist = history.shape[-1]
+        ph, ldh = _mat(history, "history", torch.int32, B, hist)
+    if bias_ids is not None:
+        nb = bias_ids.shape[-1]
+        pb, ldb = _mat(bias_ids, "bias_ids", torch.int32, B, nb)
+        if bias_values is None or bias_values.shape != bias_ids.shape or bias_values.stride() != bias_ids.stride():
+            raise ValueError("bias_values must have the shape and strides of bias_ids")
+        pv = _dev(bias_values, "bias_values", torch.float32)
+    if allowed is not None:
+        shared = allowed.dim() == 2 and allowed.shape[0] == 1 and B > 1
+        pm, ldm = _mat(allowed, "allowed", torch.int32, 1 if shared else B, (V + 31) // 32)
+        ldm = 0 if shared else ldm
+    if y is not None:
+        py, ldy = _mat(y, "y", torch.float32, B, V)
+    _lib.check(_lib.kq().kq_logits_penalize(
+        px, ldx, B, V, ph, ldh, hist, _opt(length, "length", torch.int32, B), _opt(prompt, "prompt", torch.int32, B),
+        _opt(repetition, "repetition", torch.float32, B), _opt(frequency, "frequency", torch.float32, B),
+        _opt(presence, "presence", torch.float32, B), pb, pv, ldb, nb, pm, ldm, py, ldy,
+        _opt(ws, "ws", torch.uint8, 0), 0 if ws is None else ws.numel(), _opt(picked, "picked", torch.int32, B),
+        _stream(x.device)))
+    return y

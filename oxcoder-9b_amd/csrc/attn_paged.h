@@ -1,0 +1,534 @@
+// Attention over a paged key-value cache, the part that reads the cache (attn_paged.hip joins the parts).
+//
+//   out = sum_p e_p v_p / sum_p e_p,   e_p = 2^(x_p - m),   x_p = scale log2(e) q.k_p,   m = max x_p
+//
+// A request's positions fall into chunks of AT_CHUNK; one workgroup takes one chunk of one key-value head for all rows
+// (tokens x query heads of the group) that read it, so the cache is read once however many rows there are.  It
+// leaves each row's m, sum e and sum e v; chunks lie at fixed places, so a row's result does not depend on what else runs.
+// A wave takes 64 neighbouring positions in steps of 32, keys and values straight from memory to registers and the next
+// step's in flight while it computes, with 16x16x32 MFMAs for 16 rows at a time:
+//   S^T [position][row] = K [position][d] Q^T [d][row],   O^T [d][row] += V^T [d][position] E^T [position][row].
+// The result layout of the first (lane: row lane % 16, positions 4 (lane / 16) + 0..3 of a tile) is the operand layout of the
+// second for an order of positions that V's loads follow, so e never leaves its lane.  V^T comes from V by byte
+// permutes: a lane loads 1, 2, 4 or 8 neighbouring d of the 8 positions whose values it feeds.
+//
+// q and e are fp32; the cache's types multiply them exactly when they are cut into three parts of 8 (bf16) or
+// 11 (f16) bits, each part truncated from what the one before left, so products are those of fp32 and the sums fp32.
+// Three products in place of one cost little: the kernel waits for memory.
+#pragma once
+#include "kv_device.h"
+
+namespace kq {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int AT_CHUNK = 256;                 // positions of a workgroup
+constexpr int AT_WAVES = 4;
+
+// v_perm: bytes 0..3 of the second operand are selected by 0..3, of the first by 4..7.
+__device__ __forceinline__ uint32_t lo_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ uint32_t hi_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+__device__ __forceinline__ float fbits(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t ubits(float f) { return __builtin_bit_cast(uint32_t, f); }
+
+// Both elements' three parts, packed in pairs.  A part that is left with nothing becomes a number of x's sign far
+// below the last part's step (0 for x = 0), so that an infinite factor gives an infinity and not 0 * inf.
+template <class KV>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+    if constexpr (KV::id == KQ_KV_F16) {
+        auto cut = [](float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); };
+        auto least = [](float a) { return a == 0.0f ? 0.0f : __builtin_copysignf(0x1p-24f, a); };
+        const float tx = least(x), ty = least(y);
+        p0 = cut(x, y);
+        const float rx = x - f16_lo(p0) + tx, ry = y - f16_hi(p0) + ty;
+        p1 = cut(rx, ry);
+        p2 = cut(rx - f16_lo(p1) + tx, ry - f16_hi(p1) + ty);
+    } else {
+        auto cut = [](float a) { return fbits(ubits(a) & 0xffff0000u); };
+        // a rest that is not 0 is at least 2^-24 |x| and has at most 16 bits: the sum with 2^-50 x rounds back to it
+        const float tx = x * 0x1p-50f, ty = y * 0x1p-50f;
+        const float rx = x - cut(x), ry = y - cut(y), sx = rx - cut(rx), sy = ry - cut(ry);
+        p0 = hi_halves(ubits(x), ubits(y));
+        p1 = hi_halves(ubits(rx + tx), ubits(ry + ty));
+        p2 = hi_halves(ubits(sx + tx), ubits(sy + ty));
+    }
+}
+
+template <class KV>
+__device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (KV::id == KQ_KV_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Four codes (bytes of w) as floats' bits; their high halves are the codes in bf16.
+__device__ __forceinline__ u32x4 code_floats(uint32_t w) {
+    return u32x4{ubits((float)(int8_t)(w & 0xff)), ubits((float)(int8_t)(w >> 8 & 0xff)),
+                 ubits((float)(int8_t)(w >> 16 & 0xff)), ubits((float)(int8_t)(w >> 24))};
+}
+
+// W neighbouring elements of V as dwords (one element: in the low half).
+template <int BYTES>
+struct VRaw {
+    static constexpr int N = (BYTES + 3) / 4;
+    uint32_t u[N];
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        if constexpr (BYTES == 16) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+            u[0] = x.x, u[1] = x.y, u[2] = x.z, u[3] = x.w;
+        } else if constexpr (BYTES == 8) {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+            u[0] = x.x, u[1] = x.y;
+        } else if constexpr (BYTES == 4) u[0] = *reinterpret_cast<const uint32_t*>(p);
+        else if constexpr (BYTES == 2) u[0] = *reinterpret_cast<const uint16_t*>(p);
+        else u[0] = *p;
+    }
+};
+
+// ND = dim / 16, taken in strips of 16 W values, W = 8, 4, 2 or 1 per lane.
+constexpr int at_strips(int nd) { return nd / 8 + (nd >> 2 & 1) + (nd >> 1 & 1) + (nd & 1); }
+constexpr int at_width(int nd, int s) {
+    if (s < nd / 8) return 8;
+    s -= nd / 8;
+    for (int w = 4; w; w >>= 1)
+        if (nd & w) {
+            if (s == 0) return w;
+            s--;
+        }
+    return 0;
+}
+constexpr int at_first(int nd, int s) {           // first value of strip s, in 16ths
+    int n = 0;
+    for (int i = 0; i < s; i++) n += at_width(nd, i);
+    return n;
+}
+
+template <class KV, int ND>
+struct Attn {
+    static constexpr bool I8 = KV::id == KQ_KV_I8;
+    static constexpr int D = 16 * ND, EB = I8 ? 1 : 2;
+    static constexpr int KL = I8 ? (ND + 3) / 4 : (ND + 1) / 2;  // 16-byte loads of a key by its 4 lanes
+    static constexpr int KS = I8 ? 2 * KL : KL;                  // k-steps of 32
+    static constexpr bool K_WHOLE = I8 ? ND % 4 == 0 : ND % 2 == 0;
+    static constexpr int LD = D + 4;                             // row stride of the waves' sums in LDS
+    static constexpr float BIAS = KV::id == KQ_KV_F16 ? 14.0f : 0.0f;   // f16: e is held times 2^14, clear of subnormals
+    static constexpr int VW = [] { int n = 0; for (int s = 0; s < at_strips(ND); s++) n += (at_width(ND, s) * EB + 3) / 4; return n; }();
+
+    // First of the 8 values that lane group g feeds to k-step ks.
+    static __device__ __forceinline__ int k_dim(int ks, int g) { return I8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g; }
+
+    // Lane i of the wave: where position first + i lies in the pool, in bytes (a place that is there where the position
+    // is not), and its scales; there: the positions to be read.
+    int first;
+    uint32_t at_lo, at_hi;
+    float mine_ks, mine_vs;
+    uint64_t there;
+    const uint8_t *kb, *vb;
+    u32x4 k[2][KL];                      // of position 16 t + lane % 16 of the step
+    uint32_t v[2][4][VW];                // of positions 16 t + 4 (lane / 16) + i
+
+    __device__ __forceinline__ void open(const AttnArgs& a, int b, int kh, int from, int len, int lane) {
+        first = from;
+        const int p = from + lane;
+        int page = -1;
+        if (p < len) page = a.table.pages[(int64_t)b * a.table.ld + (p >> a.page_shift)];
+        const bool ok = (unsigned)page < (unsigned)a.kv.pages;
+        page = ok ? page : 0;
+        const int off = ok ? p & (a.kv.page_size - 1) : 0;
+        there = __ballot(ok);
+        const int64_t at = (page * a.kv.page_stride + off * a.kv.pos_stride) * EB;
+        at_lo = (uint32_t)at;
+        at_hi = (uint32_t)(at >> 32);
+        if constexpr (I8) {
+            const int64_t e = page * a.kv.scale_page_stride + kh * a.kv.scale_head_stride + off * a.kv.scale_pos_stride;
+            mine_ks = a.kv.k_scale[e];
+            mine_vs = a.kv.v_scale[e];
+        }
+        kb = static_cast<const uint8_t*>(a.kv.k) + (int64_t)kh * a.kv.head_stride * EB;
+        vb = static_cast<const uint8_t*>(a.kv.v) + (int64_t)kh * a.kv.head_stride * EB;
+    }
+    // Byte offset of the wave's position i.
+    __device__ __forceinline__ int64_t place(int i) const {
+        return (int64_t)((uint64_t)(uint32_t)__shfl((int)at_hi, i, 64) << 32 | (uint32_t)__shfl((int)at_lo, i, 64));
+    }
+    // Keeps what follows from the lanes' places from being computed once for every step and held in registers.
+    __device__ __forceinline__ void here() { asm volatile("" : "+v"(at_lo), "+v"(at_hi)); }
+    __device__ __forceinline__ void load_k(int u, int r, int g) {
+        here();
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint8_t* row = kb + place(32 * u + 16 * t + r);
+#pragma unroll
+            for (int s = 0; s < KL; s++) {
+                const int piece = 4 * s + g;
+                if (s == KL - 1 && !K_WHOLE) {
+                    constexpr int PIECES = D * EB / 16;
+                    const u32x4 x = *reinterpret_cast<const u32x4*>(row + 16 * (piece < PIECES ? piece : 0));
+                    k[t][s] = piece < PIECES ? x : u32x4{0, 0, 0, 0};
+                } else {
+                    k[t][s] = *reinterpret_cast<const u32x4*>(row + 16 * piece);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(int u, int r, int g) {
+        here();
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) load_strip<0, 0>(v[t][i], vb + place(32 * u + 16 * t + 4 * g + i), r);
+    }
+    template <int S, int AT>
+    static __device__ __forceinline__ void load_strip(uint32_t* to, const uint8_t* row, int r) {
+        if constexpr (S < at_strips(ND)) {
+            constexpr int W = at_width(ND, S);
+            VRaw<W * EB> x;
+            x.load(row + (16 * at_first(ND, S) + W * r) * EB);
+#pragma unroll
+            for (int j = 0; j < VRaw<W * EB>::N; j++) to[AT + j] = x.u[j];
+            load_strip<S + 1, AT + VRaw<W * EB>::N>(to, row, r);
+        }
+    }
+
+    // Key fragment of k-step s for tile t.
+    __device__ __forceinline__ u32x4 k_frag(int t, int s) const {
+        if constexpr (I8) {
+            const u32x4 raw = k[t][s >> 1];
+            const u32x4 x = code_floats(raw[2 * (s & 1)]), y = code_floats(raw[2 * (s & 1) + 1]);
+            return u32x4{hi_halves(x.x, x.y), hi_halves(x.z, x.w), hi_halves(y.x, y.y), hi_halves(y.z, y.w)};
+        } else {
+            return k[t][s];
+        }
+    }
+
+    // Bit 4 t + i: position 16 t + 4 g + i of step u is a hole, or not below `to`.
+    __device__ __forceinline__ uint32_t hidden(int u, int to, int g) const {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const int at = 32 * u + 16 * t + 4 * g, n = to - first - at;      // n of the four are below `to`
+            const uint32_t out = ~(uint32_t)(there >> at) | ~0u << min(max(n, 0), 4);
+            bits |= (out & 15u) << (4 * t);
+        }
+        return bits;
+    }
+    __device__ __forceinline__ void clear_v(uint32_t bits) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool out = bits >> (4 * t + i) & 1u;
+#pragma unroll
+                for (int j = 0; j < VW; j++) v[t][i][j] = out ? 0u : v[t][i][j];
+            }
+    }
+    // Whether a value at one of the positions is an infinity or NaN.
+    __device__ __forceinline__ bool v_not_finite(uint32_t bits) const {
+        if constexpr (I8) return false;                // codes; a position's scale counts only where e does
+        constexpr uint32_t E = KV::id == KQ_KV_F16 ? 0x7c00u : 0x7f80u;
+        bool any = false;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (bits >> (4 * t + i) & 1u)
+#pragma unroll
+                    for (int j = 0; j < VW; j++) any |= (v[t][i][j] & E) == E || (v[t][i][j] >> 16 & E) == E;
+        return __any(any);
+    }
+
+    template <int S, int AT>
+    __device__ __forceinline__ void pv_strip(const u32x4 (&p)[3], f32x4 (&o)[ND]) const {
+        if constexpr (S < at_strips(ND)) {
+            constexpr int W = at_width(ND, S), F = at_first(ND, S), NW = VRaw<W * EB>::N;
+            auto raw = [&](int kk, int d) { return v[kk >> 2][kk & 3][AT + d]; };
+            if constexpr (I8) {
+#pragma unroll
+                for (int d = 0; d < NW; d++) {
+                    u32x4 x[8];
+#pragma unroll
+                    for (int kk = 0; kk < 8; kk++) x[kk] = code_floats(raw(kk, d));
+#pragma unroll
+                    for (int w = 4 * d; w < W && w < 4 * d + 4; w++) {
+                        const u32x4 f = {hi_halves(x[0][w & 3], x[1][w & 3]), hi_halves(x[2][w & 3], x[3][w & 3]),
+                                         hi_halves(x[4][w & 3], x[5][w & 3]), hi_halves(x[6][w & 3], x[7][w & 3])};
+#pragma unroll
+                        for (int n = 0; n < 3; n++) o[F + w] = mma<KV>(f, p[n], o[F + w]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    u32x4 f;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        f[j] = w & 1 ? hi_halves(raw(2 * j, w >> 1), raw(2 * j + 1, w >> 1))
+                                     : lo_halves(raw(2 * j, w >> 1), raw(2 * j + 1, w >> 1));
+#pragma unroll
+                    for (int n = 0; n < 3; n++) o[F + w] = mma<KV>(f, p[n], o[F + w]);
+                }
+            }
+            pv_strip<S + 1, AT + NW>(p, o);
+        }
+    }
+    // o += V^T E^T of the step; e[t][i] of position 16 t + 4 g + i, 0 where the row does not see it.
+    __device__ __forceinline__ void pv(const float (&e)[2][4], f32x4 (&o)[ND], int u, int g) const {
+        u32x4 p[3];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int t = j >> 1, i = 2 * (j & 1);
+            float x = e[t][i], y = e[t][i + 1];
+            if constexpr (I8) {                                  // a NaN stays one, a 0 takes no part
+                const int at = 32 * u + 16 * t + 4 * g + i;
+                const float sx = __shfl(mine_vs, at, 64), sy = __shfl(mine_vs, at + 1, 64);
+                x = x == 0.0f ? x : x * sx;
+                y = y == 0.0f ? y : y * sy;
+            }
+            uint32_t p0, p1, p2;
+            split2<KV>(x, y, p0, p1, p2);
+            p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
+        }
+        pv_strip<0, 0>(p, o);
+    }
+};
+
+// o's values of strip S into a row of LDS.
+template <int ND, int S>
+__device__ __forceinline__ void put_o(float* row, const f32x4 (&o)[ND], int g) {
+    if constexpr (S < at_strips(ND)) {
+        constexpr int W = at_width(ND, S), F = at_first(ND, S);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float* to = row + 16 * F + (4 * g + i) * W;
+            if constexpr (W >= 4) {
+#pragma unroll
+                for (int w = 0; w < W; w += 4)
+                    *reinterpret_cast<f32x4*>(to + w) = f32x4{o[F + w][i], o[F + w + 1][i], o[F + w + 2][i], o[F + w + 3][i]};
+            } else {
+#pragma unroll
+                for (int w = 0; w < W; w++) to[w] = o[F + w][i];
+            }
+        }
+        put_o<ND, S + 1>(row, o, g);
+    }
+}
+
+template <class KV, int ND>
+__global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_attn_part(AttnArgs a) {
+    typedef Attn<KV, ND> A;
+    // the rows' parts [k-step][part][lane], later the waves' sums [wave][row][LD]
+    constexpr int Q_BYTES = A::KS * 3 * 1024, O_BYTES = AT_WAVES * 16 * A::LD * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
+    __shared__ float sm[AT_WAVES][16], sl[AT_WAVES][16];
+    auto sq = reinterpret_cast<u32x4 (*)[3][64]>(lds);
+    auto so = reinterpret_cast<float (*)[16][A::LD]>(lds);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int c = blockIdx.x, kh = blockIdx.y, b = blockIdx.z;
+    const int len = min(a.lens[b], a.max_len);
+    if (c * AT_CHUNK >= len && (c || a.joined)) return;         // the join knows the chunks that are there
+    const int G = a.q_heads / a.kv.heads, R = a.T * G;
+    const int all = len - a.T + 1;                              // positions that every token sees
+    const int first = c * AT_CHUNK + 64 * wave;
+    A s;
+    s.open(a, b, kh, first, len, lane);
+    bool apart = false;                                         // token by token (below)
+    int tok = 0;
+    for (int r0 = 0; r0 < R;) {
+        const int row = r0 + r, t = row / G, h = kh * G + row % G;
+        const int see = row < R ? all + t : 0;                  // positions that the lane's row sees
+        if (first < len) {
+            s.load_k(0, r, g);
+            s.load_v(0, r, g);
+        }
+        // q's parts; each wave cuts a share
+        const float* q = a.q + ((int64_t)b * a.T + (row < R ? t : 0)) * a.ldq + (int64_t)(row < R ? h : 0) * A::D;
+        float f = a.scale * 1.44269504088896341f, up = 1.0f;
+        auto q8 = [&](int n, f32x4 (&x)[2]) {
+            const int d = A::k_dim(n, g);
+            const bool ok = A::K_WHOLE || d < A::D;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                x[j] = *reinterpret_cast<const f32x4_a4*>(q + (ok ? d : 0) + 4 * j);
+                if (!ok) x[j] = f32x4{0, 0, 0, 0};
+            }
+        };
+        if constexpr (KV::id == KQ_KV_F16) {
+            // times a power of two that puts the row's largest near 2^14
+            float top = 0.0f;
+#pragma unroll
+            for (int n = 0; n < A::KS; n++) {
+                f32x4 x[2];
+                q8(n, x);
+#pragma unroll
+                for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[j >> 2][j & 3]));
+            }
+            top = xor32_max(xor16_max(top));
+            const uint32_t ex = max(ubits(top) >> 23, 15u);
+            up = fbits(min(268u - ex, 254u) << 23);
+            f *= fbits((ex - 14u) << 23);
+        }
+#pragma unroll
+        for (int n0 = 0; n0 < A::KS; n0 += AT_WAVES) {
+            const int n = n0 + wave;
+            if (n < A::KS) {
+                f32x4 x[2];
+                q8(n, x);
+                u32x4 p[3];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint32_t p0, p1, p2;
+                    split2<KV>(x[j >> 1][2 * (j & 1)] * up, x[j >> 1][2 * (j & 1) + 1] * up, p0, p1, p2);
+                    p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
+                }
+#pragma unroll
+                for (int j = 0; j < 3; j++) sq[n][j][lane] = p[j];
+            }
+        }
+        __syncthreads();
+        float m = -INFINITY, l = 0.0f;
+        f32x4 o[ND];
+#pragma unroll
+        for (int n = 0; n < ND; n++) o[n] = f32x4{0, 0, 0, 0};
+        int found = 0;
+#pragma unroll 1
+        for (int u = 0; u < 2; u++) {
+            const int base = first + 32 * u;
+            if (base >= len) break;
+            f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            if constexpr (A::I8) asm volatile("" : "+v"(s.mine_ks), "+v"(s.mine_vs));   // as here()
+#pragma unroll
+            for (int n = 0; n < A::KS; n++) {
+                u32x4 qp[3];
+#pragma unroll
+                for (int j = 0; j < 3; j++) qp[j] = sq[n][j][lane];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const u32x4 kf = s.k_frag(i, n);
+#pragma unroll
+                    for (int j = 2; j >= 0; j--) acc[i] = mma<KV>(kf, qp[j], acc[i]);
+                }
+            }
+            const bool next = u == 0 && base + 32 < len;
+            if (next) s.load_k(1, r, g);
+            float e[2][4], top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float x = acc[i][j];
+                    if constexpr (A::I8) x *= __shfl(s.mine_ks, 32 * u + 16 * i + 4 * g + j, 64);
+                    e[i][j] = x * f;
+                }
+            // some row does not see some position
+            const bool partly = (uint32_t)(s.there >> (32 * u)) != ~0u || base + 32 > all;
+            if (partly) {
+                const uint32_t hid = s.hidden(u, see, g);
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (hid >> (4 * i + j) & 1u) e[i][j] = -INFINITY;
+                // An infinity or NaN that only some tokens see would reach the others as 0 * inf: then the rows are done
+                // again, token by token, with the values that it does not see cleared.
+                const uint32_t gone = s.hidden(u, apart ? all + tok : len, g);
+                if (a.T > 1 && !apart) found |= s.v_not_finite(s.hidden(u, all, g) & ~gone);
+                s.clear_v(gone);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) top = fmaxf(top, e[i][j]);
+            top = fmaxf(m, xor32_max(xor16_max(top)));
+            const float keep = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+            if (!__all(keep == 1.0f)) {
+                l *= keep;
+#pragma unroll
+                for (int n = 0; n < ND; n++) o[n] *= keep;
+            }
+            m = top;
+            const float from = (m == -INFINITY ? 0.0f : m) - A::BIAS;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    e[i][j] = __builtin_amdgcn_exp2f(e[i][j] - from);
+                    l += e[i][j];
+                }
+            s.pv(e, o, u, g);
+            if (next) s.load_v(1, r, g);
+        }
+        if (a.T > 1 && !apart) {
+            if (__syncthreads_or(found)) {
+                apart = true;
+                tok = a.T - 1;
+                r0 = 0;
+                continue;
+            }
+        } else {
+            __syncthreads();                                    // the parts of q have left LDS
+        }
+        // the waves' sums, joined
+        l = xor32_sum(xor16_sum(l));
+        if (row < R) {
+            if (g == 0) sm[wave][r] = m, sl[wave][r] = l;
+            put_o<ND, 0>(so[wave][r], o, g);
+        }
+        __syncthreads();
+        constexpr int Q = A::D / 4;
+        for (int i = tid; i < min(16, R - r0) * Q; i += 64 * AT_WAVES) {
+            const int rr = i / Q, d = 4 * (i % Q), tt = (r0 + rr) / G, hh = kh * G + (r0 + rr) % G;
+            if (apart && tt != tok) continue;
+            float top = sm[0][rr];
+#pragma unroll
+            for (int w = 1; w < AT_WAVES; w++) top = fmaxf(top, sm[w][rr]);
+            f32x4 sum = {0, 0, 0, 0};
+            float total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < AT_WAVES; w++) {
+                const float lw = sl[w][rr];
+                if (lw != 0.0f) {                               // 0: the wave saw nothing (a NaN counts)
+                    const float k = __builtin_amdgcn_exp2f(sm[w][rr] - top);
+                    sum += *reinterpret_cast<const f32x4*>(&so[w][rr][d]) * k;
+                    total += lw * k;
+                }
+            }
+            const int64_t at = (int64_t)b * a.T + tt;
+            if (a.joined) {
+                const int64_t part = (at * a.q_heads + hh) * a.chunks + c;
+                *reinterpret_cast<f32x4*>(a.po + part * A::D + d) = sum;
+                if (d == 0) a.pml[part] = AttnMl{top, total};
+            } else {
+                *reinterpret_cast<f32x4_a4*>(a.out + at * a.ldo + (int64_t)hh * A::D + d) =
+                    total == 0.0f ? f32x4{0, 0, 0, 0} : sum / total;
+            }
+        }
+        if (!apart || tok == 0) {
+            r0 += 16;
+            tok = a.T - 1;
+        } else {
+            tok--;
+        }
+        if (r0 < R) __syncthreads();                            // the sums have left LDS
+    }
+}
+
+template <class KV, int ND>
+void launch_attn_part_nd(const AttnArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((k_attn_part<KV, ND>), dim3(a.chunks, a.kv.heads, a.table.seqs), dim3(64 * AT_WAVES), 0, s, a);
+}
+
+template <class KV>
+void launch_attn_part(const AttnArgs& a, hipStream_t s) {
+    static constexpr void (*go[16])(const AttnArgs&, hipStream_t) = {
+        launch_attn_part_nd<KV, 1>, launch_attn_part_nd<KV, 2>, launch_attn_part_nd<KV, 3>, launch_attn_part_nd<KV, 4>,
+        launch_attn_part_nd<KV, 5>, launch_attn_part_nd<KV, 6>, launch_attn_part_nd<KV, 7>, launch_attn_part_nd<KV, 8>,
+        launch_attn_part_nd<KV, 9>, launch_attn_part_nd<KV, 10>, launch_attn_part_nd<KV, 11>, launch_attn_part_nd<KV, 12>,
+        launch_attn_part_nd<KV, 13>, launch_attn_part_nd<KV, 14>, launch_attn_part_nd<KV, 15>, launch_attn_part_nd<KV, 16>};
+    go[a.kv.dim / 16 - 1](a, s);
+}
+
+}  // namespace kq

@@ -1,66 +1,73 @@
-// Attention of each request's last tokens over a paged key-value cache (include/kq.h: kq_attn_paged).
-#include "kv_device.h"
+// Attention of each request's last tokens over a paged key-value cache (include/kq.h: kq_attn_paged): the join of the chunks'
+// parts that attn_paged.h's kernels leave.
+#include <math.h>
+
+#include "attn_paged.h"
 
 namespace kq {
 
-// One workgroup per row; its waves take every fourth position, a lane up to 4 values of the head.
-template <class KV>
-__global__ void __launch_bounds__(256) k_attn_rows(AttnArgs a) {
-    __shared__ float sm[4], sl[4], so[4][256];
-    const int D = a.kv.dim, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int h = blockIdx.x, b = blockIdx.y / a.T, t = blockIdx.y % a.T;
-    const int len = min(min(a.lens[b], a.max_len), a.table.cap), upto = len - a.T + 1 + t;
-    const int kh = h / (a.q_heads / a.kv.heads);
-    float q[4], o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
-    for (int i = 0; i < 4; i++)
-        q[i] = lane + 64 * i < D ? a.q[(int64_t)blockIdx.y * a.ldq + (int64_t)h * D + lane + 64 * i] * a.scale : 0.0f;
-    for (int p = wave; p < upto; p += 4) {
-        const int page = a.table.pages[(int64_t)b * a.table.ld + p / a.kv.page_size];
-        if (page < 0 || page >= a.kv.pages) continue;
-        const int off = p & (a.kv.page_size - 1);
-        const int64_t at = page * a.kv.page_stride + kh * a.kv.head_stride + off * a.kv.pos_stride;
-        float ks = 1, vs = 1;
-        if constexpr (KV::id == KQ_KV_I8) {
-            const int64_t sat = page * a.kv.scale_page_stride + kh * a.kv.scale_head_stride + off * a.kv.scale_pos_stride;
-            ks = a.kv.k_scale[sat];
-            vs = a.kv.v_scale[sat];
-        }
-        auto val = [&](const void* base, int i) {
-            const typename KV::T x = static_cast<const typename KV::T*>(base)[at + lane + 64 * i];
-            if constexpr (KV::id == KQ_KV_BF16) return __builtin_bit_cast(float, (uint32_t)x << 16);
-            else return (float)x;
-        };
-        float s = 0;
-        for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < D) s += q[i] * val(a.kv.k, i);
-        for (int w = 32; w; w >>= 1) s += __shfl_xor(s, w, 64);
-        s *= ks;
-        const float mn = fmaxf(m, s), keep = mn == m ? 1.0f : expf(m - mn), e = expf(s - mn);
-        for (int i = 0; i < 4; i++) o[i] = o[i] * keep + (lane + 64 * i < D ? e * vs * val(a.kv.v, i) : 0.0f);
-        l = l * keep + e;
-        m = mn;
-    }
-    if (lane == 0) { sm[wave] = m; sl[wave] = l; }
-    for (int i = 0; i < 4; i++) so[wave][lane + 64 * i] = o[i];
+// One workgroup per row.  Lane groups of dim / 4 take every n-th chunk, then the groups are added in order: a row's
+// result depends on its number of chunks alone.
+__global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) f32x4 so[256];
+    __shared__ float sl[64], sm[4];
+    const int tid = threadIdx.x, b = blockIdx.x / a.T, h = blockIdx.y, D = a.kv.dim, Q = D / 4, groups = 256 / Q;
+    const int j = tid / Q, d = 4 * (tid % Q);
+    const int len = min(a.lens[b], a.max_len), n = len <= 0 ? 0 : (len + AT_CHUNK - 1) / AT_CHUNK;
+    const int64_t row = ((int64_t)blockIdx.x * a.q_heads + h) * a.chunks;
+    float top = -INFINITY;
+    for (int c = tid; c < n; c += 256) top = fmaxf(top, a.pml[row + c].m);
+    for (int w = 32; w; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
+    if ((tid & 63) == 0) sm[tid >> 6] = top;
     __syncthreads();
-    if ((int)threadIdx.x >= D) return;
-    const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    float sum = 0, val = 0;
-    for (int w = 0; w < 4; w++) {
-        const float f = sm[w] == -INFINITY ? 0.0f : expf(sm[w] - top);
-        sum += sl[w] * f;
-        val += so[w][threadIdx.x] * f;
+    top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    f32x4 sum = {0, 0, 0, 0};
+    float total = 0.0f;
+    if (j < groups) {
+#pragma unroll 4
+        for (int c = j; c < n; c += groups) {
+            const AttnMl ml = a.pml[row + c];
+            const f32x4 x = *reinterpret_cast<const f32x4*>(a.po + (row + c) * D + d);
+            if (ml.l != 0.0f) {
+                const float k = __builtin_amdgcn_exp2f(ml.m - top);
+                sum += x * k;
+                total += ml.l * k;
+            }
+        }
+        so[tid] = sum;
+        if (d == 0) sl[j] = total;
     }
-    a.out[(int64_t)blockIdx.y * a.ldo + (int64_t)h * D + threadIdx.x] = sum == 0 ? 0.0f : val / sum;
+    __syncthreads();
+    if (j) return;
+    for (int i = 1; i < groups; i++) {
+        sum += so[i * Q + tid];
+        total += sl[i];
+    }
+    *reinterpret_cast<f32x4_a4*>(a.out + (int64_t)blockIdx.x * a.ldo + (int64_t)h * D + d) =
+        total == 0.0f ? f32x4{0, 0, 0, 0} : sum / total;
 }
 
-size_t attn_paged_workspace(int, int, int, int, int) { return 256; }
+static int chunks_of(int max_len) { return max_len / AT_CHUNK + (max_len % AT_CHUNK != 0); }
+static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-void launch_attn_paged(const AttnArgs& a, hipStream_t s) {
-    const dim3 grid(a.q_heads, a.table.seqs * a.T);
-    if (a.kv.type == KQ_KV_F16) hipLaunchKernelGGL(k_attn_rows<KvF16>, grid, dim3(256), 0, s, a);
-    else if (a.kv.type == KQ_KV_BF16) hipLaunchKernelGGL(k_attn_rows<KvBf16>, grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(k_attn_rows<KvI8>, grid, dim3(256), 0, s, a);
+size_t attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len) {
+    const size_t parts = (size_t)seqs * T * q_heads * chunks_of(max_len);
+    return max_len <= AT_CHUNK ? 256 : up256(parts * dim * 4) + up256(parts * sizeof(AttnMl));
+}
+
+void launch_attn_paged(const AttnArgs& args, hipStream_t s) {
+    AttnArgs a = args;
+    a.page_shift = __builtin_ctz((unsigned)a.kv.page_size);
+    a.chunks = chunks_of(a.max_len);
+    a.joined = a.chunks > 1;
+    const size_t parts = (size_t)a.table.seqs * a.T * a.q_heads * a.chunks;
+    a.po = reinterpret_cast<float*>(a.ws);
+    a.pml = reinterpret_cast<AttnMl*>(a.ws + up256(parts * a.kv.dim * 4));
+    if (a.kv.type == KQ_KV_F16) launch_attn_part<KvF16>(a, s);
+    else if (a.kv.type == KQ_KV_BF16) launch_attn_part<KvBf16>(a, s);
+    else launch_attn_part<KvI8>(a, s);
+    if (a.joined)
+        hipLaunchKernelGGL(k_attn_join, dim3(a.table.seqs * a.T, a.q_heads), dim3(256), 0, s, a);
 }
 
 }  // namespace kq

@@ -127,6 +127,9 @@ struct AppendArgs {
     int64_t ldq, ldqo, ldk, ldv;
 };
 void launch_kv_append(const AppendArgs& a, hipStream_t s);
+struct AttnMl {
+    float m, l;                // a row's largest score in a chunk (times log2 e), its sum of 2^(score - m)
+};
 struct AttnArgs {
     kq_kv kv;
     PageTable table;
@@ -137,7 +140,13 @@ struct AttnArgs {
     float scale;
     float* out;
     uint8_t* ws;
+    // set by launch_attn_paged
+    int page_shift, chunks, joined;     // joined: parts go to po and pml [row][head][chunk]
+    float* po;
+    AttnMl* pml;
 };
+template <class KV>
+void launch_attn_part(const AttnArgs& a, hipStream_t s);
 size_t attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len);
 void launch_attn_paged(const AttnArgs& a, hipStream_t s);
 struct LogitsArgs {

@@ -6,43 +6,44 @@
 
 namespace kq {
 
-// One workgroup per row.  Lane groups of dim / 4 take every n-th chunk, then the groups are added in order: a row's
-// result depends on its number of chunks alone.
+// One workgroup per row and 32 of its values: 32 groups of 8 lanes take every 32nd chunk, then the groups are added as a
+// tree: a row's result depends on its number of chunks alone.
 __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
-    __shared__ __attribute__((aligned(16))) f32x4 so[256];
-    __shared__ float sl[64], sm[4];
-    const int tid = threadIdx.x, b = blockIdx.x / a.T, h = blockIdx.y, D = a.kv.dim, Q = D / 4, groups = 256 / Q;
-    const int j = tid / Q, d = 4 * (tid % Q);
+    __shared__ __attribute__((aligned(16))) f32x4 so[4][8];
+    __shared__ float sl[4], sm[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, D = a.kv.dim;
+    const int b = blockIdx.x / a.T, h = blockIdx.y, d = 32 * blockIdx.z + 4 * (tid & 7);
     const int len = min(a.lens[b], a.max_len), n = len <= 0 ? 0 : (len + AT_CHUNK - 1) / AT_CHUNK;
     const int64_t row = ((int64_t)blockIdx.x * a.q_heads + h) * a.chunks;
     float top = -INFINITY;
     for (int c = tid; c < n; c += 256) top = fmaxf(top, a.pml[row + c].m);
     for (int w = 32; w; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
-    if ((tid & 63) == 0) sm[tid >> 6] = top;
+    if (lane == 0) sm[wave] = top;
     __syncthreads();
     top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
     f32x4 sum = {0, 0, 0, 0};
     float total = 0.0f;
-    if (j < groups) {
-#pragma unroll 4
-        for (int c = j; c < n; c += groups) {
-            const AttnMl ml = a.pml[row + c];
-            const f32x4 x = *reinterpret_cast<const f32x4*>(a.po + (row + c) * D + d);
-            if (ml.l != 0.0f) {
-                const float k = __builtin_amdgcn_exp2f(ml.m - top);
-                sum += x * k;
-                total += ml.l * k;
-            }
+#pragma unroll 8
+    for (int c = tid >> 3; c < n; c += 32) {
+        const AttnMl ml = a.pml[row + c];
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.po + (row + c) * D + (d < D ? d : 0));
+        if (ml.l != 0.0f) {
+            const float k = __builtin_amdgcn_exp2f(ml.m - top);
+            sum += x * k;
+            total += ml.l * k;
         }
-        so[tid] = sum;
-        if (d == 0) sl[j] = total;
     }
+    for (int w = 8; w < 64; w <<= 1) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) sum[i] += __shfl_xor(sum[i], w, 64);
+        total += __shfl_xor(total, w, 64);
+    }
+    if (lane < 8) so[wave][lane] = sum;
+    if (lane == 0) sl[wave] = total;
     __syncthreads();
-    if (j) return;
-    for (int i = 1; i < groups; i++) {
-        sum += so[i * Q + tid];
-        total += sl[i];
-    }
+    if (tid >= 8 || d >= D) return;
+    sum = (so[0][tid] + so[1][tid]) + (so[2][tid] + so[3][tid]);
+    total = (sl[0] + sl[1]) + (sl[2] + sl[3]);
     *reinterpret_cast<f32x4_a4*>(a.out + (int64_t)blockIdx.x * a.ldo + (int64_t)h * D + d) =
         total == 0.0f ? f32x4{0, 0, 0, 0} : sum / total;
 }
@@ -67,7 +68,7 @@ void launch_attn_paged(const AttnArgs& args, hipStream_t s) {
     else if (a.kv.type == KQ_KV_BF16) launch_attn_part<KvBf16>(a, s);
     else launch_attn_part<KvI8>(a, s);
     if (a.joined)
-        hipLaunchKernelGGL(k_attn_join, dim3(a.table.seqs * a.T, a.q_heads), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(k_attn_join, dim3(a.table.seqs * a.T, a.q_heads, (a.kv.dim + 31) / 32), dim3(256), 0, s, a);
 }
 
 }  // namespace kq

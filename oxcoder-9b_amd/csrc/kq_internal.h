@@ -141,7 +141,7 @@ struct AttnArgs {
     float* out;
     uint8_t* ws;
     // set by launch_attn_paged
-    int page_shift, chunks, joined;     // joined: parts go to po and pml [row][head][chunk]
+    int page_shift, chunks, chunk0, joined;     // joined: parts go to po and pml [row][head][chunk]
     float* po;
     AttnMl* pml;
 };

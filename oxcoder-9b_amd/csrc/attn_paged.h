@@ -14,7 +14,8 @@
 //
 // q and e are fp32; the cache's types multiply them exactly when they are cut into three parts of 8 (bf16) or
 // 11 (f16) bits, each part truncated from what the one before left, so products are those of fp32 and the sums fp32.
-// Three products in place of one cost little: the kernel waits for memory.
+// Three products in place of one cost little: the kernel waits for memory.  An 8-bit cache's codes are bf16 values to e,
+// and meet q as integers: q in units of its row's largest / 8.35e6 is three bytes, the sums of their products are exact.
 #pragma once
 #include "kv_device.h"
 
@@ -22,6 +23,7 @@ namespace kq {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int AT_CHUNK = 256;                 // positions of a workgroup
 constexpr int AT_WAVES = 4;
@@ -111,14 +113,11 @@ struct Attn {
     static constexpr bool I8 = KV::id == KQ_KV_I8;
     static constexpr int D = 16 * ND, EB = I8 ? 1 : 2;
     static constexpr int KL = I8 ? (ND + 3) / 4 : (ND + 1) / 2;  // 16-byte loads of a key by its 4 lanes
-    static constexpr int KS = I8 ? 2 * KL : KL;                  // k-steps of 32
+    static constexpr int QW = I8 ? 4 : 2;                        // a lane's share of q for a load, in fours
     static constexpr bool K_WHOLE = I8 ? ND % 4 == 0 : ND % 2 == 0;
     static constexpr int LD = D + 4;                             // row stride of the waves' sums in LDS
     static constexpr float BIAS = KV::id == KQ_KV_F16 ? 14.0f : 0.0f;   // f16: e is held times 2^14, clear of subnormals
     static constexpr int VW = [] { int n = 0; for (int s = 0; s < at_strips(ND); s++) n += (at_width(ND, s) * EB + 3) / 4; return n; }();
-
-    // First of the 8 values that lane group g feeds to k-step ks.
-    static __device__ __forceinline__ int k_dim(int ks, int g) { return I8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g; }
 
     // Lane i of the wave: where position first + i lies in the pool, in bytes (a place that is there where the position
     // is not), and its scales; there: the positions to be read.
@@ -130,12 +129,11 @@ struct Attn {
     u32x4 k[2][KL];                      // of position 16 t + lane % 16 of the step
     uint32_t v[2][4][VW];                // of positions 16 t + 4 (lane / 16) + i
 
-    __device__ __forceinline__ void open(const AttnArgs& a, int b, int kh, int from, int len, int lane) {
+    // page: the table's entry for the lane's position, or any other's where that is not below len.
+    __device__ __forceinline__ void open(const AttnArgs& a, int page, int kh, int from, int len, int lane) {
         first = from;
         const int p = from + lane;
-        int page = -1;
-        if (p < len) page = a.table.pages[(int64_t)b * a.table.ld + (p >> a.page_shift)];
-        const bool ok = (unsigned)page < (unsigned)a.kv.pages;
+        const bool ok = p < len && (unsigned)page < (unsigned)a.kv.pages;
         page = ok ? page : 0;
         const int off = ok ? p & (a.kv.page_size - 1) : 0;
         there = __ballot(ok);
@@ -190,17 +188,6 @@ struct Attn {
 #pragma unroll
             for (int j = 0; j < VRaw<W * EB>::N; j++) to[AT + j] = x.u[j];
             load_strip<S + 1, AT + VRaw<W * EB>::N>(to, row, r);
-        }
-    }
-
-    // Key fragment of k-step s for tile t.
-    __device__ __forceinline__ u32x4 k_frag(int t, int s) const {
-        if constexpr (I8) {
-            const u32x4 raw = k[t][s >> 1];
-            const u32x4 x = code_floats(raw[2 * (s & 1)]), y = code_floats(raw[2 * (s & 1) + 1]);
-            return u32x4{hi_halves(x.x, x.y), hi_halves(x.z, x.w), hi_halves(y.x, y.y), hi_halves(y.z, y.w)};
-        } else {
-            return k[t][s];
         }
     }
 
@@ -319,8 +306,8 @@ __device__ __forceinline__ void put_o(float* row, const f32x4 (&o)[ND], int g) {
 template <class KV, int ND>
 __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_attn_part(AttnArgs a) {
     typedef Attn<KV, ND> A;
-    // the rows' parts [k-step][part][lane], later the waves' sums [wave][row][LD]
-    constexpr int Q_BYTES = A::KS * 3 * 1024, O_BYTES = AT_WAVES * 16 * A::LD * 4;
+    // q's parts [load][part][lane], later the waves' sums [wave][row][LD]
+    constexpr int Q_BYTES = A::KL * 3 * 1024, O_BYTES = AT_WAVES * 16 * A::LD * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
     __shared__ float sm[AT_WAVES][16], sl[AT_WAVES][16];
     auto sq = reinterpret_cast<u32x4 (*)[3][64]>(lds);
@@ -331,61 +318,93 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
     // different lengths load the XCDs alike (chunks side by side: the 48 requests below 8192 positions took 209 us, XCD 0
     // with 1.5 times the chunks of XCD 7)
     const int c = a.chunk0 + blockIdx.z, kh = blockIdx.x, b = (blockIdx.y + (uint32_t)c) % gridDim.y;
+    // every argument in one go, then the length and the table's entry side by side
+    KQ_ARGS_READY("s"(a.kv.k), "s"(a.kv.v), "s"(a.kv.k_scale), "s"(a.kv.v_scale), "s"(a.kv.page_stride), "s"(a.kv.head_stride),
+                  "s"(a.kv.pos_stride), "s"(a.table.pages), "s"(a.table.ld), "s"(a.lens), "s"(a.q), "s"(a.ldq));
+    const int first = c * AT_CHUNK + 64 * wave;
     const int len = min(a.lens[b], a.max_len);
+    int page = a.table.pages[(int64_t)b * a.table.ld + (min(first + lane, a.table.cap - 1) >> a.page_shift)];
+    asm volatile("" : "+v"(page));
     if (c * AT_CHUNK >= len && (c || a.joined)) return;         // the join knows the chunks that are there
     const int G = a.q_heads / a.kv.heads, R = a.T * G;
     const int all = len - a.T + 1;                              // positions that every token sees
-    const int first = c * AT_CHUNK + 64 * wave;
     A s;
-    s.open(a, b, kh, first, len, lane);
+    s.open(a, page, kh, first, len, lane);
     bool apart = false;                                         // token by token (below)
     int tok = 0;
     for (int r0 = 0; r0 < R;) {
         const int row = r0 + r, t = row / G, h = kh * G + row % G;
         const int see = row < R ? all + t : 0;                  // positions that the lane's row sees
-        if (first < len) {
-            s.load_k(0, r, g);
-            s.load_v(0, r, g);
-        }
         // q's parts; each wave cuts a share
         const float* q = a.q + ((int64_t)b * a.T + (row < R ? t : 0)) * a.ldq + (int64_t)(row < R ? h : 0) * A::D;
-        float f = a.scale * 1.44269504088896341f, up = 1.0f;
-        auto q8 = [&](int n, f32x4 (&x)[2]) {
-            const int d = A::k_dim(n, g);
+        float f = a.scale * 1.44269504088896341f, top = 0.0f, bad = 0.0f;
+        typedef f32x4 Share[A::QW];
+        auto share = [&](int n, Share& x) {
+            const int d = 16 * A::QW * n + 4 * A::QW * g;
             const bool ok = A::K_WHOLE || d < A::D;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < A::QW; j++) {
                 x[j] = *reinterpret_cast<const f32x4_a4*>(q + (ok ? d : 0) + 4 * j);
                 if (!ok) x[j] = f32x4{0, 0, 0, 0};
             }
         };
+        constexpr int SHARES = (A::KL + AT_WAVES - 1) / AT_WAVES;
+        Share mine[SHARES], whole[KV::id == KQ_KV_BF16 ? 1 : A::KL];
+#pragma unroll
+        for (int i = 0; i < SHARES; i++) share(min(AT_WAVES * i + wave, A::KL - 1), mine[i]);
+        if constexpr (KV::id != KQ_KV_BF16)
+#pragma unroll
+            for (int n = 0; n < A::KL; n++) share(n, whole[n]);
+        s.load_k(0, r, g);
+        s.load_v(0, r, g);
+        if constexpr (KV::id != KQ_KV_BF16) {
+#pragma unroll
+            for (int n = 0; n < A::KL; n++)
+#pragma unroll
+                for (int j = 0; j < 4 * A::QW; j++) {
+                    const float x = whole[n][j >> 2][j & 3];
+                    top = fmaxf(top, fabsf(x));
+                    if constexpr (A::I8) bad = __builtin_fmaf(x, 0.0f, bad);
+                }
+            top = xor32_max(xor16_max(top));
+            if constexpr (A::I8) bad = xor32_sum(xor16_sum(bad));
+        }
+        float up = 1.0f;
         if constexpr (KV::id == KQ_KV_F16) {
             // times a power of two that puts the row's largest near 2^14
-            float top = 0.0f;
-#pragma unroll
-            for (int n = 0; n < A::KS; n++) {
-                f32x4 x[2];
-                q8(n, x);
-#pragma unroll
-                for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[j >> 2][j & 3]));
-            }
-            top = xor32_max(xor16_max(top));
             const uint32_t ex = max(ubits(top) >> 23, 15u);
             up = fbits(min(268u - ex, 254u) << 23);
             f *= fbits((ex - 14u) << 23);
         }
+        if constexpr (A::I8) {
+            up = 8.35e6f / fmaxf(top, 1e-30f);
+            f = f * (fmaxf(top, 1e-30f) / 8.35e6f) + bad;            // bad: NaN for a row with an infinity or NaN
+        }
 #pragma unroll
-        for (int n0 = 0; n0 < A::KS; n0 += AT_WAVES) {
-            const int n = n0 + wave;
-            if (n < A::KS) {
-                f32x4 x[2];
-                q8(n, x);
+        for (int i = 0; i < SHARES; i++) {
+            const int n = AT_WAVES * i + wave;
+            if (n < A::KL) {
                 u32x4 p[3];
+                if constexpr (A::I8) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    uint32_t p0, p1, p2;
-                    split2<KV>(x[j >> 1][2 * (j & 1)] * up, x[j >> 1][2 * (j & 1) + 1] * up, p0, p1, p2);
-                    p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t p0 = 0, p1 = 0, p2 = 0;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const int x = (int)rintf(mine[i][j][k] * up), y = (x + 0x80) >> 8, z = (y + 0x80) >> 8;
+                            p0 |= ((uint32_t)z & 0xffu) << (8 * k);      // x = 65536 z + 256 (int8)y + (int8)x
+                            p1 |= ((uint32_t)y & 0xffu) << (8 * k);
+                            p2 |= ((uint32_t)x & 0xffu) << (8 * k);
+                        }
+                        p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t p0, p1, p2;
+                        split2<KV>(mine[i][j >> 1][2 * (j & 1)] * up, mine[i][j >> 1][2 * (j & 1) + 1] * up, p0, p1, p2);
+                        p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
+                    }
                 }
 #pragma unroll
                 for (int j = 0; j < 3; j++) sq[n][j][lane] = p[j];
@@ -401,31 +420,51 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
         for (int u = 0; u < 2; u++) {
             const int base = first + 32 * u;
             if (base >= len) break;
-            f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-            if constexpr (A::I8) asm volatile("" : "+v"(s.mine_ks), "+v"(s.mine_vs));   // as here()
+            float e[2][4];
+            if constexpr (A::I8) {
+                i32x4 acc[2][3] = {};
 #pragma unroll
-            for (int n = 0; n < A::KS; n++) {
-                u32x4 qp[3];
+                for (int n = 0; n < A::KL; n++)
 #pragma unroll
-                for (int j = 0; j < 3; j++) qp[j] = sq[n][j][lane];
+                    for (int j = 0; j < 3; j++) {
+                        const i32x4 qp = __builtin_bit_cast(i32x4, sq[n][j][lane]);
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const u32x4 kf = s.k_frag(i, n);
+                        for (int i = 0; i < 2; i++)
+                            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, s.k[i][n]), qp, acc[i][j], 0, 0, 0);
+                    }
 #pragma unroll
-                    for (int j = 2; j >= 0; j--) acc[i] = mma<KV>(kf, qp[j], acc[i]);
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        e[i][j] = __builtin_fmaf(__builtin_fmaf((float)acc[i][0][j], 256.0f, (float)acc[i][1][j]), 256.0f, (float)acc[i][2][j]);
+            } else {
+                f32x4 acc[2] = {};
+#pragma unroll
+                for (int n = 0; n < A::KL; n++) {
+                    u32x4 qp[3];
+#pragma unroll
+                    for (int j = 0; j < 3; j++) qp[j] = sq[n][j][lane];
+#pragma unroll
+                    for (int j = 2; j >= 0; j--)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) acc[i] = mma<KV>(s.k[i][n], qp[j], acc[i]);
                 }
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) e[i][j] = acc[i][j];
             }
             const bool next = u == 0 && base + 32 < len;
             if (next) s.load_k(1, r, g);
-            float e[2][4], top = -INFINITY;
+            if constexpr (A::I8) asm volatile("" : "+v"(s.mine_ks), "+v"(s.mine_vs));   // as here()
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    float x = acc[i][j];
-                    if constexpr (A::I8) x *= __shfl(s.mine_ks, 32 * u + 16 * i + 4 * g + j, 64);
-                    e[i][j] = x * f;
+                    if constexpr (A::I8) e[i][j] *= __shfl(s.mine_ks, 32 * u + 16 * i + 4 * g + j, 64);
+                    e[i][j] *= f;
                 }
+            top = -INFINITY;
             // some row does not see some position
             const bool partly = (uint32_t)(s.there >> (32 * u)) != ~0u || base + 32 > all;
             if (partly) {

@@ -161,6 +161,7 @@ struct LogitsArgs {
     float* y;
     uint8_t* ws;
     int32_t* picked;
+    int slice;                 // set by launch_logits
 };
 size_t logits_workspace(int B);
 void launch_logits(const LogitsArgs& a, hipStream_t s);

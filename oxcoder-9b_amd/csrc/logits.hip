@@ -2,94 +2,47 @@
 // kq_logits_penalize).
 //
 // A workgroup takes a slice of one row's vocabulary.  The history and the bias list name few ids anywhere in the row, so
-// each workgroup scans them once and notes in LDS, per id of its slice, how often it occurs after the prompt, whether
-// it occurs at all (integer atomics: any order gives the same) and its last bias entry.  Then one pass over the
-// slice's logits applies the steps and keeps the best; the pick folds into one key per row, as argmax_block.h does
-// for a single row.
+// each workgroup scans them once, notes in LDS per id of its slice how often it occurs after the prompt, whether it
+// occurs at all and its last bias entry (integer atomics: any order gives the same), and lists the ids that have a note.
+// The listed ids are stepped first, packed into full waves, and their notes replaced by the results; then one pass over the
+// slice takes each logit from the row or from its note, applies the mask and keeps the best.  The pick folds into one
+// key per row, as argmax_block.h does for a single row.  The row's first values are fetched ahead of the scan.
 #include "argmax_block.h"
 #include "kq_internal.h"
 
 namespace kq {
 
-constexpr int LG_SLICE = 4096;               // ids of a workgroup: 32 KB of LDS for the two notes
-constexpr uint32_t LG_SEEN = 0x80000000u;    // the id occurs; the low bits count occurrences after the prompt
+constexpr int LG_T = 512;                    // threads
+constexpr int LG_STEP = 4 * LG_T;            // ids of a workgroup's pass of 16-byte loads
+constexpr int LG_MOST = 4 * LG_STEP;         // ids of the largest slice: 48 KB of LDS, three workgroups a CU
+// A note, held inverted (an id without one: all ones, as no result is)
+constexpr uint32_t LG_SEEN = 0x80000000u;    // the id occurs
+constexpr int LG_ENTRY = 20;                 // from this bit on: its last bias entry + 1; below: occurrences after the prompt
+constexpr int LG_MOST_HIST = 1 << LG_ENTRY, LG_MOST_BIAS = 1 << (31 - LG_ENTRY);
 constexpr int LG_ROW_BYTES = 2 * ARG_LINE;   // workspace of a row: the key's line, the ticket's line
 
-template <bool V4>
-__global__ void __launch_bounds__(256) k_logits(LogitsArgs a) {
-    __shared__ __attribute__((aligned(16))) uint32_t note[LG_SLICE], bias[LG_SLICE];
-    __shared__ ArgBest wave_best[4];
-    const int b = blockIdx.y, v0 = blockIdx.x * LG_SLICE, nv = min(LG_SLICE, a.V - v0), tid = threadIdx.x;
-    const int nh = a.hist ? min(max(a.hist_len[b], 0), a.max_hist) : 0, nb = a.bias_id ? a.nb : 0;
-    if (nh | nb) {
-        for (int i = 4 * tid; i < LG_SLICE; i += 1024) {
-            *reinterpret_cast<u32x4*>(note + i) = u32x4{0, 0, 0, 0};
-            *reinterpret_cast<u32x4*>(bias + i) = u32x4{0, 0, 0, 0};
-        }
-        __syncthreads();
-        const int prompt = a.prompt_len ? a.prompt_len[b] : 0;
-        const int32_t* hist = a.hist + (int64_t)b * a.ldh;
-        for (int i = tid; i < nh; i += 256) {
-            const uint32_t id = (uint32_t)hist[i] - (uint32_t)v0;
-            if (id < (uint32_t)nv) {
-                atomicOr(&note[id], LG_SEEN);
-                if (i >= prompt) atomicAdd(&note[id], 1u);
-            }
-        }
-        for (int i = tid; i < nb; i += 256) {
-            const uint32_t id = (uint32_t)a.bias_id[(int64_t)b * a.ldb + i] - (uint32_t)v0;
-            if (id < (uint32_t)nv) atomicMax(&bias[id], (uint32_t)i + 1u);
-        }
-        __syncthreads();
+// y after the penalties and the bias, each step rounded.
+__device__ __forceinline__ float lg_step(const LogitsArgs& a, int b, float t, bool seen, uint32_t count, uint32_t entry) {
+    if (seen && a.rep) {
+        const float rep = a.rep[b];
+        t = t > 0.0f ? t / rep : t * rep;
     }
-    const float rep = a.rep ? a.rep[b] : 1.0f, freq = a.freq ? a.freq[b] : 0.0f, pres = a.pres ? a.pres[b] : 0.0f;
-    const float* x = a.x + (int64_t)b * a.ldx + v0;
-    float* y = a.y ? a.y + (int64_t)b * a.ldy + v0 : nullptr;
-    const uint32_t* allowed = a.allowed ? a.allowed + (int64_t)b * a.ldm + (v0 >> 5) : nullptr;
-    ArgBest best{-1e30f, -1};
-    auto step = [&](float t, uint32_t seen, uint32_t entry, bool ok) {
-        if (seen) {
-            if (a.rep) t = t > 0.0f ? t / rep : t * rep;
-            const uint32_t c = seen & ~LG_SEEN;
-            if (c) {
-                t = t - freq * (float)c;
-                t = t - pres;
-            }
-        }
-        if (entry) t = t + a.bias_val[(int64_t)b * a.ldb + entry - 1];
-        return ok ? t : -INFINITY;
-    };
-    auto allowed_at = [&](int i) { return allowed ? allowed[i >> 5] >> (i & 31) : ~0u; };
-    auto one = [&](int i) {
-        const float t = step(x[i], nh ? note[i] : 0u, nb ? bias[i] : 0u, allowed_at(i) & 1u);
-        if (y) y[i] = t;
-        arg_take(best, t, v0 + i);
-    };
-    if constexpr (V4) {
-        const u32x4 none = {0, 0, 0, 0};
-        for (int i = 4 * tid; i + 3 < nv; i += 1024) {
-            f32x4 t = *reinterpret_cast<const f32x4*>(x + i);
-            const u32x4 n4 = nh ? *reinterpret_cast<const u32x4*>(note + i) : none;
-            const u32x4 b4 = nb ? *reinterpret_cast<const u32x4*>(bias + i) : none;
-            const uint32_t ok = allowed_at(i);
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                t[k] = step(t[k], n4[k], b4[k], (ok >> k) & 1u);
-                arg_take(best, t[k], v0 + i + k);
-            }
-            if (y) *reinterpret_cast<f32x4*>(y + i) = t;
-        }
-        for (int i = (nv & ~3) + tid; i < nv; i += 256) one(i);
-    } else {
-        for (int i = tid; i < nv; i += 256) one(i);
+    if (count) {
+        if (a.freq) t = t - a.freq[b] * (float)count;
+        if (a.pres) t = t - a.pres[b];
     }
-    if (!a.picked) return;
+    if (entry) t = t + a.bias_val[(int64_t)b * a.ldb + entry - 1];
+    return t;
+}
+
+// Folds the workgroup's best into the row's key; whoever takes the row's last ticket reads the key and clears both.
+__device__ __forceinline__ void lg_finish(const LogitsArgs& a, int b, ArgBest best) {
+    __shared__ ArgBest wave_best[LG_T / 64];
     best = arg_wave_reduce(best);
-    if ((tid & 63) == 0) wave_best[tid >> 6] = best;
+    if ((threadIdx.x & 63) == 0) wave_best[threadIdx.x >> 6] = best;
     __syncthreads();
-    if (tid) return;
-    for (int w = 0; w < 4; w++) best = arg_combine(best, wave_best[w]);
-    // fold into the row's key; whoever takes the row's last ticket reads the key and clears both
+    if (threadIdx.x) return;
+    for (int w = 0; w < LG_T / 64; w++) best = arg_combine(best, wave_best[w]);
     auto* key = reinterpret_cast<unsigned long long*>(a.ws + (size_t)b * LG_ROW_BYTES);
     auto* ticket = reinterpret_cast<unsigned int*>(a.ws + (size_t)b * LG_ROW_BYTES + ARG_LINE);
     atomicMax(key, arg_key(best));
@@ -99,13 +52,139 @@ __global__ void __launch_bounds__(256) k_logits(LogitsArgs a) {
     atomicExch(ticket, 0u);
 }
 
+template <bool V4>
+__global__ void __launch_bounds__(LG_T) k_logits(LogitsArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t note[];       // [slice], then the list of ids [slice] in 16 bits
+    __shared__ int listed;
+    uint16_t* const list = reinterpret_cast<uint16_t*>(note + a.slice);
+    const int b = blockIdx.y, v0 = blockIdx.x * a.slice, nv = min(a.slice, a.V - v0), tid = threadIdx.x;
+    const float* x = a.x + (int64_t)b * a.ldx + v0;
+    f32x4 t[LG_MOST / LG_STEP];
+#pragma unroll
+    for (int n = 0; n < LG_MOST / LG_STEP; n++) {
+        const int i = n * LG_STEP + 4 * tid;
+        if constexpr (V4) {
+            if (i + 3 < nv) t[n] = *reinterpret_cast<const f32x4*>(x + i);
+        } else if (i + 3 < nv) {
+            t[n] = *reinterpret_cast<const f32x4_a4*>(x + i);
+        }
+    }
+    const int nh = a.hist ? min(max(a.hist_len[b], 0), a.max_hist) : 0, nb = a.bias_id ? a.nb : 0;
+    const bool notes = nh | nb;
+    if (notes) {
+        if (tid == 0) listed = 0;
+        for (int i = 4 * tid; i < a.slice; i += LG_STEP) *reinterpret_cast<u32x4*>(note + i) = u32x4{~0u, ~0u, ~0u, ~0u};
+        __syncthreads();
+        auto enlist = [&](uint32_t before, uint32_t id) {
+            if (before == ~0u) list[atomicAdd(&listed, 1)] = (uint16_t)id;
+        };
+        for (int i = tid; i < nb; i += LG_T) {
+            const uint32_t id = (uint32_t)a.bias_id[(int64_t)b * a.ldb + i] - (uint32_t)v0;
+            if (id < (uint32_t)nv) enlist(atomicMin(&note[id], ~((uint32_t)(i + 1) << LG_ENTRY)), id);
+        }
+        if (nb) __syncthreads();
+        const int prompt = a.prompt_len ? a.prompt_len[b] : 0;
+        const int32_t* hist = a.hist + (int64_t)b * a.ldh;
+        for (int i0 = tid; i0 < nh; i0 += 4 * LG_T) {
+            uint32_t id[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) id[k] = i0 + k * LG_T < nh ? (uint32_t)hist[i0 + k * LG_T] - (uint32_t)v0 : ~0u;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (id[k] < (uint32_t)nv) {
+                    enlist(atomicAnd(&note[id[k]], ~LG_SEEN), id[k]);
+                    if (i0 + k * LG_T >= prompt) atomicSub(&note[id[k]], 1u);
+                }
+        }
+        __syncthreads();
+        for (int i = tid; i < listed; i += LG_T) {
+            const int id = list[i];
+            const uint32_t n = ~note[id];
+            const float u = lg_step(a, b, x[id], n >= LG_SEEN, n & (LG_MOST_HIST - 1), (n & ~LG_SEEN) >> LG_ENTRY);
+            note[id] = u == u ? __builtin_bit_cast(uint32_t, u) : 0x7fc00000u;
+        }
+        __syncthreads();
+    }
+    float* y = a.y ? a.y + (int64_t)b * a.ldy + v0 : nullptr;
+    const uint32_t* allowed = a.allowed ? a.allowed + (int64_t)b * a.ldm + (v0 >> 5) : nullptr;
+    ArgBest best{-1e30f, -1};
+    auto allowed_at = [&](int i) { return allowed ? allowed[i >> 5] >> (i & 31) : ~0u; };
+#pragma unroll
+    for (int n = 0; n < LG_MOST / LG_STEP; n++) {
+        const int i = n * LG_STEP + 4 * tid;
+        if (i + 3 >= nv) continue;
+        const uint32_t ok = allowed_at(i);
+        const u32x4 noted = notes ? *reinterpret_cast<const u32x4*>(note + i) : u32x4{~0u, ~0u, ~0u, ~0u};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t m = noted[k];
+            const float u = (ok >> k) & 1u ? (m != ~0u ? __builtin_bit_cast(float, m) : t[n][k]) : -INFINITY;
+            t[n][k] = u;
+            arg_take_ascending(best, u, v0 + i + k);
+        }
+        if (y) {
+            if constexpr (V4) *reinterpret_cast<f32x4*>(y + i) = t[n];
+            else *reinterpret_cast<f32x4_a4*>(y + i) = t[n];
+        }
+    }
+    if (tid < (nv & 3)) {                                                  // the last one to three ids
+        const int i = (nv & ~3) + tid;
+        const uint32_t noted = notes ? note[i] : ~0u;
+        float u = noted != ~0u ? __builtin_bit_cast(float, noted) : x[i];
+        u = allowed_at(i) & 1u ? u : -INFINITY;
+        arg_take(best, u, v0 + i);
+        if (y) y[i] = u;
+    }
+    if (a.picked) lg_finish(a, b, best);
+}
+
+// Histories or bias lists too long for a note's fields: two notes per id, and every id stepped in place.
+constexpr int LG_WIDE = 4096;
+__global__ void __launch_bounds__(LG_T) k_logits_wide(LogitsArgs a) {
+    __shared__ uint32_t note[LG_WIDE], bias[LG_WIDE];
+    const int b = blockIdx.y, v0 = blockIdx.x * LG_WIDE, nv = min(LG_WIDE, a.V - v0), tid = threadIdx.x;
+    const int nh = a.hist ? min(max(a.hist_len[b], 0), a.max_hist) : 0, nb = a.bias_id ? a.nb : 0;
+    for (int i = tid; i < LG_WIDE; i += LG_T) note[i] = bias[i] = 0;
+    __syncthreads();
+    const int prompt = a.prompt_len ? a.prompt_len[b] : 0;
+    for (int i = tid; i < nh; i += LG_T) {
+        const uint32_t id = (uint32_t)a.hist[(int64_t)b * a.ldh + i] - (uint32_t)v0;
+        if (id < (uint32_t)nv) {
+            atomicOr(&note[id], LG_SEEN);
+            if (i >= prompt) atomicAdd(&note[id], 1u);
+        }
+    }
+    for (int i = tid; i < nb; i += LG_T) {
+        const uint32_t id = (uint32_t)a.bias_id[(int64_t)b * a.ldb + i] - (uint32_t)v0;
+        if (id < (uint32_t)nv) atomicMax(&bias[id], (uint32_t)i + 1u);
+    }
+    __syncthreads();
+    ArgBest best{-1e30f, -1};
+    for (int i = tid; i < nv; i += LG_T) {
+        float t = lg_step(a, b, a.x[(int64_t)b * a.ldx + v0 + i], note[i] != 0, note[i] & ~LG_SEEN, bias[i]);
+        if (a.allowed && !(a.allowed[(int64_t)b * a.ldm + ((v0 + i) >> 5)] >> ((v0 + i) & 31) & 1u)) t = -INFINITY;
+        if (a.y) a.y[(int64_t)b * a.ldy + v0 + i] = t;
+        arg_take(best, t, v0 + i);
+    }
+    if (a.picked) lg_finish(a, b, best);
+}
+
 size_t logits_workspace(int B) { return (size_t)B * LG_ROW_BYTES; }
 
-void launch_logits(const LogitsArgs& a, hipStream_t s) {
-    const dim3 grid((a.V + LG_SLICE - 1) / LG_SLICE, a.B);
+void launch_logits(const LogitsArgs& args, hipStream_t s) {
+    LogitsArgs a = args;
+    if ((a.hist && a.max_hist >= LG_MOST_HIST) || (a.bias_id && a.nb >= LG_MOST_BIAS)) {
+        hipLaunchKernelGGL(k_logits_wide, dim3((a.V + LG_WIDE - 1) / LG_WIDE, a.B), dim3(LG_T), 0, s, a);
+        return;
+    }
+    // the largest slice that leaves two workgroups a CU: every slice scans the whole history
+    a.slice = LG_MOST;
+    while (a.slice > LG_STEP && (int64_t)a.B * ((a.V + a.slice - 1) / a.slice) < 2 * device_cus()) a.slice /= 2;
+    const dim3 grid((a.V + a.slice - 1) / a.slice, a.B);
+    const size_t lds = a.hist || a.bias_id ? (size_t)a.slice * 6 : 0;
     auto al = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0; };
-    if (al(a.x, a.ldx) && (!a.y || al(a.y, a.ldy))) hipLaunchKernelGGL(k_logits<true>, grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(k_logits<false>, grid, dim3(256), 0, s, a);
+    if (al(a.x, a.ldx) && (!a.y || al(a.y, a.ldy))) hipLaunchKernelGGL(k_logits<true>, grid, dim3(LG_T), lds, s, a);
+    else hipLaunchKernelGGL(k_logits<false>, grid, dim3(LG_T), lds, s, a);
 }
 
 }  // namespace kq

@@ -192,3 +192,15 @@ def test_other_stream_and_graph(dev):
         torch.cuda.synchronize()
         a, y = p.picked.clone(), out.clone()
         assert torch.equal(p.pick(x, out=out, **args), a) and torch.equal(out, y)
+
+
+@pytest.mark.parametrize("B,V", [(200, 9001), (600, 5000), (300, 20003)])
+def test_slices(dev, B, V):
+    """Batches whose rows are cut into fewer, larger slices."""
+    check(dev, *inputs(B, V, 70, 6, True, seed=B))
+
+
+@pytest.mark.parametrize("L,nb", [(3000, 2047), (3000, 2048), (3000, 5000), (1 << 20, 10), ((1 << 20) - 1, 10)])
+def test_long_lists(dev, L, nb):
+    """Bias lists and histories on both sides of what one note per id holds."""
+    check(dev, *inputs(2, 6000, L, nb, True, seed=nb))

@@ -1,12 +1,11 @@
 // Penalties, biases and a grammar mask on the requests' logits, with the greedy pick (include/kq.h:
 // kq_logits_penalize).
 //
-// A workgroup takes a slice of one row's vocabulary.  The history and the bias list name few ids anywhere in the row, so
-// each workgroup scans them once, notes in LDS per id of its slice how often it occurs after the prompt, whether it
-// occurs at all and its last bias entry (integer atomics: any order gives the same), and lists the ids that have a note.
-// The listed ids are stepped first, packed into full waves, and their notes replaced by the results; then one pass over the
-// slice takes each logit from the row or from its note, applies the mask and keeps the best.  The pick folds into one
-// key per row, as argmax_block.h does for a single row.  The row's first values are fetched ahead of the scan.
+// A workgroup takes a slice of one row's vocabulary, its logits and mask on their way to registers from the start.  The
+// history and the bias list name few ids anywhere in the row, so each workgroup scans them once and notes in LDS, per id of its
+// slice, how often it occurs after the prompt, whether it occurs at all and its last bias entry (integer atomics: any
+// order gives the same).  Then every thread steps its logits and keeps the best.  The pick folds into one key per row, as
+// argmax_block.h does for a single row.
 #include "argmax_block.h"
 #include "kq_internal.h"
 
@@ -14,24 +13,26 @@ namespace kq {
 
 constexpr int LG_T = 512;                    // threads
 constexpr int LG_STEP = 4 * LG_T;            // ids of a workgroup's pass of 16-byte loads
-constexpr int LG_MOST = 4 * LG_STEP;         // ids of the largest slice: 48 KB of LDS, three workgroups a CU
-// A note, held inverted (an id without one: all ones, as no result is)
-constexpr uint32_t LG_SEEN = 0x80000000u;    // the id occurs
+constexpr int LG_MOST = 4 * LG_STEP;         // ids of the largest slice: 32 KB of notes, four workgroups a CU
+constexpr uint32_t LG_SEEN = 0x80000000u;    // a note: the id occurs;
 constexpr int LG_ENTRY = 20;                 // from this bit on: its last bias entry + 1; below: occurrences after the prompt
 constexpr int LG_MOST_HIST = 1 << LG_ENTRY, LG_MOST_BIAS = 1 << (31 - LG_ENTRY);
 constexpr int LG_ROW_BYTES = 2 * ARG_LINE;   // workspace of a row: the key's line, the ticket's line
 
-// y after the penalties and the bias, each step rounded.
-__device__ __forceinline__ float lg_step(const LogitsArgs& a, int b, float t, bool seen, uint32_t count, uint32_t entry) {
-    if (seen && a.rep) {
-        const float rep = a.rep[b];
-        t = t > 0.0f ? t / rep : t * rep;
-    }
-    if (count) {
-        if (a.freq) t = t - a.freq[b] * (float)count;
-        if (a.pres) t = t - a.pres[b];
-    }
-    if (entry) t = t + a.bias_val[(int64_t)b * a.ldb + entry - 1];
+// A row's penalties.
+struct LgRow {
+    float rep, freq, pres;
+    bool has_rep, has_freq, has_pres;
+};
+__device__ __forceinline__ LgRow lg_row(const LogitsArgs& a, int b) {
+    return LgRow{a.rep ? a.rep[b] : 1.0f, a.freq ? a.freq[b] : 0.0f, a.pres ? a.pres[b] : 0.0f, a.rep != nullptr, a.freq != nullptr,
+                 a.pres != nullptr};
+}
+// t after the penalties, each step rounded.
+__device__ __forceinline__ float lg_step(const LgRow& r, float t, bool seen, uint32_t count) {
+    if (seen && r.has_rep) t = t > 0.0f ? t / r.rep : t * r.rep;
+    if (count && r.has_freq) t = t - r.freq * (float)count;
+    if (count && r.has_pres) t = t - r.pres;
     return t;
 }
 
@@ -54,35 +55,38 @@ __device__ __forceinline__ void lg_finish(const LogitsArgs& a, int b, ArgBest be
 
 template <bool V4>
 __global__ void __launch_bounds__(LG_T) k_logits(LogitsArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint32_t note[];       // [slice], then the list of ids [slice] in 16 bits
-    __shared__ int listed;
-    uint16_t* const list = reinterpret_cast<uint16_t*>(note + a.slice);
+    extern __shared__ __attribute__((aligned(16))) uint32_t note[];       // [slice], then the biases [nb]
+    float* const bias = reinterpret_cast<float*>(note + a.slice);
     const int b = blockIdx.y, v0 = blockIdx.x * a.slice, nv = min(a.slice, a.V - v0), tid = threadIdx.x;
     const float* x = a.x + (int64_t)b * a.ldx + v0;
+    const uint32_t* allowed = a.allowed ? a.allowed + (int64_t)b * a.ldm + (v0 >> 5) : nullptr;
     f32x4 t[LG_MOST / LG_STEP];
+    uint32_t ok[LG_MOST / LG_STEP];
 #pragma unroll
     for (int n = 0; n < LG_MOST / LG_STEP; n++) {
         const int i = n * LG_STEP + 4 * tid;
-        if constexpr (V4) {
-            if (i + 3 < nv) t[n] = *reinterpret_cast<const f32x4*>(x + i);
-        } else if (i + 3 < nv) {
-            t[n] = *reinterpret_cast<const f32x4_a4*>(x + i);
+        ok[n] = ~0u;
+        if (i + 3 < nv) {
+            if constexpr (V4) t[n] = *reinterpret_cast<const f32x4*>(x + i);
+            else t[n] = *reinterpret_cast<const f32x4_a4*>(x + i);
+            if (allowed) ok[n] = allowed[i >> 5];
         }
     }
+    const LgRow row = lg_row(a, b);
     const int nh = a.hist ? min(max(a.hist_len[b], 0), a.max_hist) : 0, nb = a.bias_id ? a.nb : 0;
     const bool notes = nh | nb;
     if (notes) {
-        if (tid == 0) listed = 0;
-        for (int i = 4 * tid; i < a.slice; i += LG_STEP) *reinterpret_cast<u32x4*>(note + i) = u32x4{~0u, ~0u, ~0u, ~0u};
+        for (int i = 4 * tid; i < a.slice; i += LG_STEP) *reinterpret_cast<u32x4*>(note + i) = u32x4{0, 0, 0, 0};
         __syncthreads();
-        auto enlist = [&](uint32_t before, uint32_t id) {
-            if (before == ~0u) list[atomicAdd(&listed, 1)] = (uint16_t)id;
-        };
-        for (int i = tid; i < nb; i += LG_T) {
-            const uint32_t id = (uint32_t)a.bias_id[(int64_t)b * a.ldb + i] - (uint32_t)v0;
-            if (id < (uint32_t)nv) enlist(atomicMin(&note[id], ~((uint32_t)(i + 1) << LG_ENTRY)), id);
+        if (nb) {
+            for (int i = tid; i < nb; i += LG_T) {
+                const int64_t at = (int64_t)b * a.ldb + i;
+                const uint32_t id = (uint32_t)a.bias_id[at] - (uint32_t)v0;
+                bias[i] = a.bias_val[at];
+                if (id < (uint32_t)nv) atomicMax(&note[id], (uint32_t)(i + 1) << LG_ENTRY);
+            }
+            __syncthreads();
         }
-        if (nb) __syncthreads();
         const int prompt = a.prompt_len ? a.prompt_len[b] : 0;
         const int32_t* hist = a.hist + (int64_t)b * a.ldh;
         for (int i0 = tid; i0 < nh; i0 += 4 * LG_T) {
@@ -92,33 +96,33 @@ __global__ void __launch_bounds__(LG_T) k_logits(LogitsArgs a) {
 #pragma unroll
             for (int k = 0; k < 4; k++)
                 if (id[k] < (uint32_t)nv) {
-                    enlist(atomicAnd(&note[id[k]], ~LG_SEEN), id[k]);
-                    if (i0 + k * LG_T >= prompt) atomicSub(&note[id[k]], 1u);
+                    atomicOr(&note[id[k]], LG_SEEN);
+                    if (i0 + k * LG_T >= prompt) atomicAdd(&note[id[k]], 1u);
                 }
-        }
-        __syncthreads();
-        for (int i = tid; i < listed; i += LG_T) {
-            const int id = list[i];
-            const uint32_t n = ~note[id];
-            const float u = lg_step(a, b, x[id], n >= LG_SEEN, n & (LG_MOST_HIST - 1), (n & ~LG_SEEN) >> LG_ENTRY);
-            note[id] = u == u ? __builtin_bit_cast(uint32_t, u) : 0x7fc00000u;
         }
         __syncthreads();
     }
     float* y = a.y ? a.y + (int64_t)b * a.ldy + v0 : nullptr;
-    const uint32_t* allowed = a.allowed ? a.allowed + (int64_t)b * a.ldm + (v0 >> 5) : nullptr;
     ArgBest best{-1e30f, -1};
-    auto allowed_at = [&](int i) { return allowed ? allowed[i >> 5] >> (i & 31) : ~0u; };
+    auto noted = [&](float u, uint32_t n) {
+        if (n) {
+            u = lg_step(row, u, n >= LG_SEEN, n & (LG_MOST_HIST - 1));
+            const uint32_t entry = (n & ~LG_SEEN) >> LG_ENTRY;
+            if (entry) u = u + bias[entry - 1];
+        }
+        return u;
+    };
 #pragma unroll
     for (int n = 0; n < LG_MOST / LG_STEP; n++) {
         const int i = n * LG_STEP + 4 * tid;
         if (i + 3 >= nv) continue;
-        const uint32_t ok = allowed_at(i);
-        const u32x4 noted = notes ? *reinterpret_cast<const u32x4*>(note + i) : u32x4{~0u, ~0u, ~0u, ~0u};
+        const u32x4 m = notes ? *reinterpret_cast<const u32x4*>(note + i) : u32x4{0, 0, 0, 0};
+        const uint32_t bits = ok[n] >> (i & 31);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const uint32_t m = noted[k];
-            const float u = (ok >> k) & 1u ? (m != ~0u ? __builtin_bit_cast(float, m) : t[n][k]) : -INFINITY;
+            float u = t[n][k];
+            u = noted(u, m[k]);
+            u = (bits >> k) & 1u ? u : -INFINITY;
             t[n][k] = u;
             arg_take_ascending(best, u, v0 + i + k);
         }
@@ -129,9 +133,8 @@ __global__ void __launch_bounds__(LG_T) k_logits(LogitsArgs a) {
     }
     if (tid < (nv & 3)) {                                                  // the last one to three ids
         const int i = (nv & ~3) + tid;
-        const uint32_t noted = notes ? note[i] : ~0u;
-        float u = noted != ~0u ? __builtin_bit_cast(float, noted) : x[i];
-        u = allowed_at(i) & 1u ? u : -INFINITY;
+        float u = noted(x[i], notes ? note[i] : 0u);
+        if (allowed && !(allowed[i >> 5] >> (i & 31) & 1u)) u = -INFINITY;
         arg_take(best, u, v0 + i);
         if (y) y[i] = u;
     }
@@ -159,9 +162,11 @@ __global__ void __launch_bounds__(LG_T) k_logits_wide(LogitsArgs a) {
         if (id < (uint32_t)nv) atomicMax(&bias[id], (uint32_t)i + 1u);
     }
     __syncthreads();
+    const LgRow row = lg_row(a, b);
     ArgBest best{-1e30f, -1};
     for (int i = tid; i < nv; i += LG_T) {
-        float t = lg_step(a, b, a.x[(int64_t)b * a.ldx + v0 + i], note[i] != 0, note[i] & ~LG_SEEN, bias[i]);
+        float t = lg_step(row, a.x[(int64_t)b * a.ldx + v0 + i], note[i] != 0, note[i] & ~LG_SEEN);
+        if (bias[i]) t = t + a.bias_val[(int64_t)b * a.ldb + bias[i] - 1];
         if (a.allowed && !(a.allowed[(int64_t)b * a.ldm + ((v0 + i) >> 5)] >> ((v0 + i) & 31) & 1u)) t = -INFINITY;
         if (a.y) a.y[(int64_t)b * a.ldy + v0 + i] = t;
         arg_take(best, t, v0 + i);
@@ -181,7 +186,7 @@ void launch_logits(const LogitsArgs& args, hipStream_t s) {
     a.slice = LG_MOST;
     while (a.slice > LG_STEP && (int64_t)a.B * ((a.V + a.slice - 1) / a.slice) < 2 * device_cus()) a.slice /= 2;
     const dim3 grid((a.V + a.slice - 1) / a.slice, a.B);
-    const size_t lds = a.hist || a.bias_id ? (size_t)a.slice * 6 : 0;
+    const size_t lds = a.hist || a.bias_id ? ((size_t)a.slice + (a.bias_id ? a.nb : 0)) * 4 : 0;
     auto al = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0; };
     if (al(a.x, a.ldx) && (!a.y || al(a.y, a.ldy))) hipLaunchKernelGGL(k_logits<true>, grid, dim3(LG_T), lds, s, a);
     else hipLaunchKernelGGL(k_logits<false>, grid, dim3(LG_T), lds, s, a);

@@ -92,7 +92,7 @@ def _load(path, symbols):
 
 
 def kq():
-    return _load(LIBKQ, KQ_SYMBOLS)
+    return _libs.get(LIBKQ) or _load(LIBKQ, KQ_SYMBOLS)
 
 
 def kqhost():

@@ -92,6 +92,7 @@ class PagedAttention:
     tokens per request that attend will see (1..16); max_len: the most positions a request will hold
     (default: what its row of the table covers); rope: rope_table's, or None (nothing is rotated), whose width is
     the number of values that turn; interleaved: pairs (2i, 2i + 1) instead of (i, i + rot/2); scale: default dim ** -0.5.
+    These are for the object's life: another table or rotation takes another object, what is in them may change.
     Calls on one PagedAttention share its workspace and so must be ordered: one stream, or synchronised."""
 
     def __init__(self, caches, table, q_heads, tokens=1, max_len=None, rope=None, interleaved=False, scale=None):
@@ -106,8 +107,8 @@ class PagedAttention:
             raise ValueError("tokens must be 1..%d" % _lib.KQ_MAX_BATCH)
         if q_heads < 1 or q_heads % c.heads:
             raise ValueError("q_heads must be a multiple of the cache's %d heads" % c.heads)
-        self.caches, self.table, self.q_heads, self.tokens = list(caches), table, q_heads, tokens
-        self.rope, self.interleaved = rope, bool(interleaved)
+        self.caches, self.table, self.q_heads, self.tokens = tuple(caches), table, q_heads, tokens
+        self.rope, self._interleaved = rope, 1 if interleaved else 0
         self.scale = c.dim ** -0.5 if scale is None else float(scale)
         self.max_len = table.shape[1] * c.page_size if max_len is None else int(max_len)
         n = ops.attn_paged_workspace_bytes(table.shape[0], q_heads, c.dim, tokens, self.max_len)
@@ -116,16 +117,22 @@ class PagedAttention:
                              % (table.shape[0], self.max_len, q_heads, c.dim))
         buf = torch.empty(n + 256, dtype=torch.uint8, device=c.device)
         self.ws = buf[-buf.data_ptr() % 256:][:n]
+        # what every call passes on
+        self._ws = self.ws.data_ptr(), n
+        self._table = self._rope = None
+        if c.device.type == "cuda":
+            self._table, self._rope = ops._table(table), ops._rope(rope)
 
     def append(self, layer, q, k, v, seq, pos, q_out=None):
         """Rotate q [N][q_heads * dim] into q_out (q itself: in place; None: a new tensor) and k
         [N][heads * dim], store k and v for token n of request seq[n] at position pos[n] (both int32 [N]).
         q None: keys and values only.  Returns q_out."""
+        if self._table is None:
+            raise ValueError("the caches must be device tensors")
         if q is not None and q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ops.kv_append(self.caches[layer], self.table, q, k, v, seq, pos, q_out, self.q_heads, self.rope,
-                      self.interleaved)
-        return q_out
+        return ops._kv_append(self.caches[layer], self._table, q, k, v, seq, pos, q_out, self.q_heads, self._rope,
+                              self._interleaved)
 
     def attend(self, layer, q, lens, out=None, tokens=None):
         """Attention of the last ``tokens`` (default: the constructor's) tokens of each request; q and out
@@ -133,7 +140,9 @@ class PagedAttention:
         T = self.tokens if tokens is None else tokens
         if not 1 <= T <= self.tokens:
             raise ValueError("tokens must be 1..%d" % self.tokens)
+        if self._table is None:
+            raise ValueError("the caches must be device tensors")
         if out is None:
             out = torch.empty((q.shape[0], self.q_heads * self.caches[layer].dim), device=q.device)
-        return ops.attn_paged(self.caches[layer], self.table, q, lens, out, self.q_heads, T, self.scale, self.max_len,
-                              self.ws)
+        return ops._attn_paged(self.caches[layer], self._table, q, lens, out, self.q_heads, T, self.scale, self.max_len,
+                               *self._ws)

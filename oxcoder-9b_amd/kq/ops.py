@@ -433,20 +433,29 @@ def dequant_rows(w, R, C_, ty, row0, nrows, y=None):
     return y
 
 
+# Arguments of the operators of a token loop, whose calls take a few microseconds: one look at each attribute where the
+# tensor is as it should be, and the words of what is wrong where it is not.
+
 def _opt(t, name, dtype, n):
     """Pointer of an optional contiguous 1-D device tensor of at least n values."""
     if t is None:
         return None
-    if t.numel() < n or not t.is_contiguous():
-        raise ValueError("%s must hold %d values, contiguous" % (name, n))
-    return _dev(t, name, dtype)
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.is_contiguous() and t.numel() >= n:
+        return t.data_ptr()
+    _dev(t, name, dtype)
+    raise ValueError("%s must hold %d values, contiguous" % (name, n))
 
 
 def _mat(t, name, dtype, rows, cols):
     """(pointer, row stride) of a 2-D device tensor of at least rows x cols with contiguous rows."""
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols:
-        raise ValueError("%s must be [%d][%d], got %s" % (name, rows, cols, list(t.shape)))
-    return _dev(t, name, dtype), t.stride(0)
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype:
+        shape = t.shape
+        if len(shape) == 2 and shape[0] >= rows and shape[1] >= cols:
+            ld, step = t.stride()
+            if step == 1 or shape[1] <= 1:
+                return t.data_ptr(), ld
+    _dev(t, name, dtype)
+    raise ValueError("%s must be [%d][%d], got %s" % (name, rows, cols, list(t.shape)))
 
 
 def _table(t):
@@ -457,30 +466,43 @@ def _table(t):
     return _dev(t, "table", torch.int32), t.stride(0) if seqs > 1 else width, seqs, width
 
 
+def _rope(rope):
+    """(pointer, positions, values that turn) of a rotation table or None."""
+    if rope is None:
+        return None, 0, 0
+    if rope.dim() != 2 or not rope.is_contiguous():
+        raise ValueError("rope must be [positions][values], contiguous")
+    return (_dev(rope, "rope", torch.float32), *rope.shape)
+
+
 def kv_append(cache, table, q, k, v, seq, pos, q_out, q_heads, rope=None, interleaved=False):
     """Rotate q [N][q_heads * dim] into q_out and k [N][heads * dim], and store k and v of token n at position pos[n]
     of request seq[n] in ``cache`` (a kv.KVCache) under ``table`` int32 [requests][width] (kq_kv_append).
     q and q_out None: keys and values only; rope: kv.rope_table's, or None."""
-    N, heads, D = k.shape[0], cache.heads, cache.dim
-    pk, ldk = _mat(k, "k", torch.float32, N, heads * D)
-    pv, ldv = _mat(v, "v", torch.float32, N, heads * D)
-    pq = po = None
-    ldq = ldo = 0
-    if (q is None) != (q_out is None):
+    return _kv_append(cache, _table(table), q, k, v, seq, pos, q_out, q_heads, _rope(rope), 1 if interleaved else 0)
+
+
+def _kv_append(cache, table, q, k, v, seq, pos, q_out, q_heads, rope, interleaved):
+    f32, i32, D = torch.float32, torch.int32, cache.dim
+    cols = cache.heads * D
+    if q is None:
+        if q_out is not None:
+            raise ValueError("q and q_out go together")
+        N = k.shape[0]
+        pq = po = None
+        ldq = ldo = 0
+    elif q_out is None:
         raise ValueError("q and q_out go together")
-    if q is not None:
-        pq, ldq = _mat(q, "q", torch.float32, N, q_heads * D)
-        po, ldo = _mat(q_out, "q_out", torch.float32, N, q_heads * D)
-    pr, rows, rot = None, 0, 0
-    if rope is not None:
-        rows, rot = rope.shape
-        if not rope.is_contiguous():
-            raise ValueError("rope must be contiguous")
-        pr = _dev(rope, "rope", torch.float32)
-    pt, ldt, seqs, width = _table(table)
-    _lib.check(_lib.kq().kq_kv_append(cache.ref, pt, ldt, seqs, width, N, _opt(seq, "seq", torch.int32, N),
-                                      _opt(pos, "pos", torch.int32, N), pq, ldq, q_heads, po, ldo, pk, ldk, pv, ldv, pr, rows, rot, 1 if interleaved else 0,
-                                      _stream(cache.device)))
+    else:
+        N = k.shape[0]
+        pq, ldq = _mat(q, "q", f32, N, q_heads * D)
+        po, ldo = (pq, ldq) if q_out is q else _mat(q_out, "q_out", f32, N, q_heads * D)
+    pk, ldk = _mat(k, "k", f32, N, cols)
+    pv, ldv = _mat(v, "v", f32, N, cols)
+    rc = _lib.kq().kq_kv_append(cache.ref, *table, N, _opt(seq, "seq", i32, N), _opt(pos, "pos", i32, N), pq, ldq, q_heads,
+                                po, ldo, pk, ldk, pv, ldv, *rope, interleaved, _stream(cache.device))
+    if rc:
+        _lib.check(rc)
     return q_out
 
 
@@ -493,11 +515,18 @@ def attn_paged(cache, table, q, lens, out, q_heads, tokens, scale, max_len, ws):
     """Attention of the last ``tokens`` tokens of each request over ``cache`` (a kv.KVCache) under ``table``
     int32 [requests][width]: q, out [requests * tokens][q_heads * dim], lens int32 [requests] counting the new
     tokens, at most max_len; ws of attn_paged_workspace_bytes, 256-byte aligned (kq_attn_paged)."""
-    pt, ldt, seqs, width = _table(table)
-    pq, ldq = _mat(q, "q", torch.float32, seqs * tokens, q_heads * cache.dim)
-    po, ldo = _mat(out, "out", torch.float32, seqs * tokens, q_heads * cache.dim)
-    _lib.check(_lib.kq().kq_attn_paged(cache.ref, pt, ldt, seqs, width, _opt(lens, "lens", torch.int32, seqs), max_len,
-                                       tokens, pq, ldq, q_heads, scale, po, ldo, _dev(ws, "ws", torch.uint8), ws.numel(), _stream(cache.device)))
+    return _attn_paged(cache, _table(table), q, lens, out, q_heads, tokens, scale, max_len, _dev(ws, "ws", torch.uint8),
+                       ws.numel())
+
+
+def _attn_paged(cache, table, q, lens, out, q_heads, tokens, scale, max_len, ws, ws_bytes):
+    seqs, cols = table[2], q_heads * cache.dim
+    pq, ldq = _mat(q, "q", torch.float32, seqs * tokens, cols)
+    po, ldo = _mat(out, "out", torch.float32, seqs * tokens, cols)
+    rc = _lib.kq().kq_attn_paged(cache.ref, *table, _opt(lens, "lens", torch.int32, seqs), max_len, tokens, pq, ldq, q_heads,
+                                 scale, po, ldo, ws, ws_bytes, _stream(cache.device))
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -511,31 +540,41 @@ def logits_penalize(x, history=None, length=None, prompt=None, repetition=None, 
     """Penalties, biases and a grammar mask on logits x [B][V] into y (may be x) and the greedy pick into picked
     int32 [B] (ws: zero-filled, logits_workspace_bytes, 256-byte aligned); either may be None
     (kq_logits_penalize; the arguments are sampling.Picker.pick's)."""
+    return _logits_penalize(x, history, length, prompt, repetition, frequency, presence, bias_ids, bias_values, allowed, y,
+                            _opt(picked, "picked", torch.int32, x.shape[0]), _opt(ws, "ws", torch.uint8, 0),
+                            0 if ws is None else ws.numel())
+
+
+def _logits_penalize(x, history, length, prompt, repetition, frequency, presence, bias_ids, bias_values, allowed, y, picked,
+                     ws, ws_bytes):
+    f32, i32 = torch.float32, torch.int32
     B, V = x.shape
-    px, ldx = _mat(x, "x", torch.float32, B, V)
+    px, ldx = _mat(x, "x", f32, B, V)
     ph = pb = pv = pm = py = None
     ldh = hist = ldb = nb = ldm = ldy = 0
     if history is not None:
         if length is None:
             raise ValueError("history needs its length")
         hist = history.shape[-1]
-        ph, ldh = _mat(history, "history", torch.int32, B, hist)
+        ph, ldh = _mat(history, "history", i32, B, hist)
     if bias_ids is not None:
         nb = bias_ids.shape[-1]
-        pb, ldb = _mat(bias_ids, "bias_ids", torch.int32, B, nb)
+        pb, ldb = _mat(bias_ids, "bias_ids", i32, B, nb)
         if bias_values is None or bias_values.shape != bias_ids.shape or bias_values.stride() != bias_ids.stride():
             raise ValueError("bias_values must have the shape and strides of bias_ids")
-        pv = _dev(bias_values, "bias_values", torch.float32)
+        pv = _mat(bias_values, "bias_values", f32, B, nb)[0]
     if allowed is not None:
-        shared = allowed.dim() == 2 and allowed.shape[0] == 1 and B > 1
-        pm, ldm = _mat(allowed, "allowed", torch.int32, 1 if shared else B, (V + 31) // 32)
-        ldm = 0 if shared else ldm
+        words = (V + 31) // 32
+        if B > 1 and allowed.dim() == 2 and allowed.shape[0] == 1:
+            pm, ldm = _mat(allowed, "allowed", i32, 1, words)[0], 0
+        else:
+            pm, ldm = _mat(allowed, "allowed", i32, B, words)
     if y is not None:
-        py, ldy = _mat(y, "y", torch.float32, B, V)
-    _lib.check(_lib.kq().kq_logits_penalize(
-        px, ldx, B, V, ph, ldh, hist, _opt(length, "length", torch.int32, B), _opt(prompt, "prompt", torch.int32, B),
-        _opt(repetition, "repetition", torch.float32, B), _opt(frequency, "frequency", torch.float32, B),
-        _opt(presence, "presence", torch.float32, B), pb, pv, ldb, nb, pm, ldm, py, ldy,
-        _opt(ws, "ws", torch.uint8, 0), 0 if ws is None else ws.numel(), _opt(picked, "picked", torch.int32, B),
-        _stream(x.device)))
+        py, ldy = _mat(y, "y", f32, B, V)
+    rc = _lib.kq().kq_logits_penalize(
+        px, ldx, B, V, ph, ldh, hist, _opt(length, "length", i32, B), _opt(prompt, "prompt", i32, B),
+        _opt(repetition, "repetition", f32, B), _opt(frequency, "frequency", f32, B), _opt(presence, "presence", f32, B),
+        pb, pv, ldb, nb, pm, ldm, py, ldy, ws, ws_bytes, picked, _stream(x.device))
+    if rc:
+        _lib.check(rc)
     return y

@@ -20,6 +20,8 @@ class Picker:
         self.ws = buf[-buf.data_ptr() % 256:][:n]
         self.rows = rows
         self.picked = torch.empty(rows, dtype=torch.int32, device=device)
+        self._held = self.picked.data_ptr(), self.ws.data_ptr(), n       # what every call passes on
+        self._device = self.ws.device
 
     def pick(self, logits, history=None, length=None, prompt=None, repetition=None, frequency=None, presence=None,
              bias_ids=None, bias_values=None, allowed=None, out=None):
@@ -35,9 +37,11 @@ class Picker:
         if logits.dim() == 1:
             logits = logits.unsqueeze(0)
             out = out.unsqueeze(0) if out is not None and out.dim() == 1 else out
-        if logits.shape[0] > self.rows:
-            raise ValueError("%d rows, the picker holds %d" % (logits.shape[0], self.rows))
-        picked = self.picked if logits.shape[0] == self.rows else self.picked[:logits.shape[0]]
-        ops.logits_penalize(logits, history, length, prompt, repetition, frequency, presence, bias_ids, bias_values,
-                            allowed, out, picked, self.ws)
-        return picked
+        rows = logits.shape[0]
+        if rows > self.rows:
+            raise ValueError("%d rows, the picker holds %d" % (rows, self.rows))
+        if logits.device != self._device:
+            raise ValueError("logits must be a device tensor, on the picker's device")
+        ops._logits_penalize(logits, history, length, prompt, repetition, frequency, presence, bias_ids, bias_values,
+                             allowed, out, *self._held)
+        return self.picked if rows == self.rows else self.picked[:rows]

@@ -27,11 +27,9 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
     for (int c = tid >> 3; c < n; c += 32) {
         const AttnMl ml = a.pml[row + c];
         const f32x4 x = *reinterpret_cast<const f32x4*>(a.po + (row + c) * D + (d < D ? d : 0));
-        if (ml.l != 0.0f) {
-            const float k = __builtin_amdgcn_exp2f(ml.m - top);
-            sum += x * k;
-            total += ml.l * k;
-        }
+        const float k = ml.l != 0.0f ? __builtin_amdgcn_exp2f(ml.m - top) : 0.0f;   // 0: the row saw nothing (a NaN counts)
+        sum += x * k;
+        total += ml.l * k;
     }
     for (int w = 8; w < 64; w <<= 1) {
 #pragma unroll

@@ -261,3 +261,35 @@ def test_workspace_grows_with_its_sizes():
     base = ops.attn_paged_workspace_bytes(4, 8, 64, 1, 5000)
     for more in ((8, 8, 64, 1, 5000), (4, 16, 64, 1, 5000), (4, 8, 128, 1, 5000), (4, 8, 64, 2, 5000), (4, 8, 64, 1, 50000)):
         assert ops.attn_paged_workspace_bytes(*more) >= base
+
+
+@pytest.mark.parametrize("dtype,D,T", [("bf16", 128, 1), ("f16", 256, 4), ("i8", 80, 3)])
+def test_a_longer_bound_changes_no_bit(dev, dtype, D, T):
+    """Tables for contexts of one chunk, of some and of very many: the joins that each leads to agree."""
+    H, lens = 8, [130, 256, 0, 3]
+    cache, table, q = setup(dev, dtype, D, H, 2, 16, lens, T)
+    narrow = attend(dev, cache, table, q, lens, T, H)
+    for width in (17, 100, 1200, 40000):
+        wide = torch.full((len(lens), width), -1, dtype=torch.int32)
+        wide[:, :table.shape[1]] = table
+        assert torch.equal(attend(dev, cache, wide, q, lens, T, H), narrow), width
+    lens = [700, 5000, 255, 1025]
+    cache, table, q = setup(dev, dtype, D, H, 2, 16, lens, T)
+    here = attend(dev, cache, table, q, lens, T, H)
+    wide = torch.full((len(lens), 3000), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    assert torch.equal(attend(dev, cache, wide, q, lens, T, H), here)
+
+
+def test_repeated_calls_leave_the_workspace_ready(dev):
+    """Calls of changing tokens, lengths and bounds on one workspace: each as on a new one."""
+    H, D = 8, 64
+    cache, table, _ = setup(dev, "bf16", D, H, 2, 16, [2000, 900, 40], 1)
+    att = kv.PagedAttention([cache], table.to(dev), H, tokens=16)
+    g = torch.Generator().manual_seed(3)
+    for i in range(30):
+        T = [1, 4, 16][i % 3]
+        lens = [int(torch.randint(0, n + 1, (1,), generator=g)) for n in (2000, 900, 40)]
+        q = torch.randn((3 * T, H * D), generator=g)
+        got = att.attend(0, q.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), tokens=T)
+        assert torch.equal(got, attend(dev, cache, table, q, lens, T, H)), (i, lens)

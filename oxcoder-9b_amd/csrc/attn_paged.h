@@ -17,6 +17,8 @@
 // Three products in place of one cost little: the kernel waits for memory.  An 8-bit cache's codes are bf16 values to e,
 // and meet q as integers: q in units of its row's largest / 8.35e6 is three bytes, the sums of their products are exact.
 #pragma once
+#include <type_traits>
+
 #include "kv_device.h"
 
 namespace kq {
@@ -31,6 +33,9 @@ constexpr int AT_WAVES = 4;
 // v_perm: bytes 0..3 of the second operand are selected by 0..3, of the first by 4..7.
 __device__ __forceinline__ uint32_t lo_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t hi_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// Lane i's v.
+__device__ __forceinline__ uint32_t of_lane(int i, uint32_t v) { return (uint32_t)__builtin_amdgcn_ds_bpermute(i << 2, (int)v); }
 
 __device__ __forceinline__ float fbits(uint32_t u) { return __builtin_bit_cast(float, u); }
 __device__ __forceinline__ uint32_t ubits(float f) { return __builtin_bit_cast(uint32_t, f); }
@@ -78,11 +83,13 @@ struct VRaw {
     static constexpr int N = (BYTES + 3) / 4;
     uint32_t u[N];
     __device__ __forceinline__ void load(const uint8_t* p) {
+        // read once, so first to leave the caches: the parts that the join reads stay (the 48 requests below 8192 positions
+        // 178 -> 169 us; K's rows come in quarters and need the cache)
         if constexpr (BYTES == 16) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+            const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
             u[0] = x.x, u[1] = x.y, u[2] = x.z, u[3] = x.w;
         } else if constexpr (BYTES == 8) {
-            const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+            const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
             u[0] = x.x, u[1] = x.y;
         } else if constexpr (BYTES == 4) u[0] = *reinterpret_cast<const uint32_t*>(p);
         else if constexpr (BYTES == 2) u[0] = *reinterpret_cast<const uint16_t*>(p);
@@ -115,42 +122,45 @@ struct Attn {
     static constexpr int KL = I8 ? (ND + 3) / 4 : (ND + 1) / 2;  // 16-byte loads of a key by its 4 lanes
     static constexpr int QW = I8 ? 4 : 2;                        // a lane's share of q for a load, in fours
     static constexpr bool K_WHOLE = I8 ? ND % 4 == 0 : ND % 2 == 0;
-    static constexpr int LD = D + 4;                             // row stride of the waves' sums in LDS
+    static constexpr int WIDE = D > 128 ? 128 : D, LD = WIDE + 4; // values of a round of the waves' join, row stride in LDS
     static constexpr float BIAS = KV::id == KQ_KV_F16 ? 14.0f : 0.0f;   // f16: e is held times 2^14, clear of subnormals
     static constexpr int VW = [] { int n = 0; for (int s = 0; s < at_strips(ND); s++) n += (at_width(ND, s) * EB + 3) / 4; return n; }();
 
-    // Lane i of the wave: where position first + i lies in the pool, in bytes (a place that is there where the position
-    // is not), and its scales; there: the positions to be read.
-    int first;
+    // Lane i of the wave: where position i of the chunk that is fetched lies in the pool, in bytes (a place that is there
+    // where the position is not).
     uint32_t at_lo, at_hi;
-    float mine_ks, mine_vs;
-    uint64_t there;
+    // The wave's 64 positions of a chunk: their first, which of them are to be read, lane i's scales.
+    struct Span {
+        int first;
+        uint64_t there;
+        float ks, vs;
+    };
     const uint8_t *kb, *vb;
     u32x4 k[2][KL];                      // of position 16 t + lane % 16 of the step
     uint32_t v[2][4][VW];                // of positions 16 t + 4 (lane / 16) + i
 
     // page: the table's entry for the lane's position, or any other's where that is not below len.
-    __device__ __forceinline__ void open(const AttnArgs& a, int page, int kh, int from, int len, int lane) {
-        first = from;
-        const int p = from + lane;
+    __device__ __forceinline__ Span open(const AttnArgs& a, int page, int kh, int first, int len, int lane) {
+        Span n;
+        n.first = first;
+        const int p = first + lane;
         const bool ok = p < len && (unsigned)page < (unsigned)a.kv.pages;
         page = ok ? page : 0;
         const int off = ok ? p & (a.kv.page_size - 1) : 0;
-        there = __ballot(ok);
+        n.there = __ballot(ok);
         const int64_t at = (page * a.kv.page_stride + off * a.kv.pos_stride) * EB;
         at_lo = (uint32_t)at;
         at_hi = (uint32_t)(at >> 32);
         if constexpr (I8) {
             const int64_t e = page * a.kv.scale_page_stride + kh * a.kv.scale_head_stride + off * a.kv.scale_pos_stride;
-            mine_ks = a.kv.k_scale[e];
-            mine_vs = a.kv.v_scale[e];
+            n.ks = a.kv.k_scale[e];
+            n.vs = a.kv.v_scale[e];
         }
-        kb = static_cast<const uint8_t*>(a.kv.k) + (int64_t)kh * a.kv.head_stride * EB;
-        vb = static_cast<const uint8_t*>(a.kv.v) + (int64_t)kh * a.kv.head_stride * EB;
+        return n;
     }
     // Byte offset of the wave's position i.
     __device__ __forceinline__ int64_t place(int i) const {
-        return (int64_t)((uint64_t)(uint32_t)__shfl((int)at_hi, i, 64) << 32 | (uint32_t)__shfl((int)at_lo, i, 64));
+        return (int64_t)((uint64_t)of_lane(i, at_hi) << 32 | of_lane(i, at_lo));
     }
     // Keeps what follows from the lanes' places from being computed once for every step and held in registers.
     __device__ __forceinline__ void here() { asm volatile("" : "+v"(at_lo), "+v"(at_hi)); }
@@ -192,12 +202,12 @@ struct Attn {
     }
 
     // Bit 4 t + i: position 16 t + 4 g + i of step u is a hole, or not below `to`.
-    __device__ __forceinline__ uint32_t hidden(int u, int to, int g) const {
+    static __device__ __forceinline__ uint32_t hidden(const Span& w, int u, int to, int g) {
         uint32_t bits = 0;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const int at = 32 * u + 16 * t + 4 * g, n = to - first - at;      // n of the four are below `to`
-            const uint32_t out = ~(uint32_t)(there >> at) | ~0u << min(max(n, 0), 4);
+            const int at = 32 * u + 16 * t + 4 * g, n = to - w.first - at;    // n of the four are below `to`
+            const uint32_t out = ~(uint32_t)(w.there >> at) | ~0u << min(max(n, 0), 4);
             bits |= (out & 15u) << (4 * t);
         }
         return bits;
@@ -262,7 +272,7 @@ struct Attn {
         }
     }
     // o += V^T E^T of the step; e[t][i] of position 16 t + 4 g + i, 0 where the row does not see it.
-    __device__ __forceinline__ void pv(const float (&e)[2][4], f32x4 (&o)[ND], int u, int g) const {
+    __device__ __forceinline__ void pv(const Span& w, const float (&e)[2][4], f32x4 (&o)[ND], int u, int g) const {
         u32x4 p[3];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -270,7 +280,7 @@ struct Attn {
             float x = e[t][i], y = e[t][i + 1];
             if constexpr (I8) {                                  // a NaN stays one, a 0 takes no part
                 const int at = 32 * u + 16 * t + 4 * g + i;
-                const float sx = __shfl(mine_vs, at, 64), sy = __shfl(mine_vs, at + 1, 64);
+                const float sx = fbits(of_lane(at, ubits(w.vs))), sy = fbits(of_lane(at + 1, ubits(w.vs)));
                 x = x == 0.0f ? x : x * sx;
                 y = y == 0.0f ? y : y * sy;
             }
@@ -282,135 +292,151 @@ struct Attn {
     }
 };
 
-// o's values of strip S into a row of LDS.
-template <int ND, int S>
-__device__ __forceinline__ void put_o(float* row, const f32x4 (&o)[ND], int g) {
+// o's values in [16 FROM, 16 TO), times k, into a row of LDS; S: the strip.
+template <int ND, int FROM, int TO, int S = 0>
+__device__ __forceinline__ void put_o(float* row, const f32x4 (&o)[ND], float k, int g) {
     if constexpr (S < at_strips(ND)) {
         constexpr int W = at_width(ND, S), F = at_first(ND, S);
+        if constexpr (F >= FROM && F < TO) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float* to = row + 16 * F + (4 * g + i) * W;
-            if constexpr (W >= 4) {
+            for (int i = 0; i < 4; i++) {
+                float* to = row + 16 * (F - FROM) + (4 * g + i) * W;
+                if constexpr (W >= 4) {
 #pragma unroll
-                for (int w = 0; w < W; w += 4)
-                    *reinterpret_cast<f32x4*>(to + w) = f32x4{o[F + w][i], o[F + w + 1][i], o[F + w + 2][i], o[F + w + 3][i]};
-            } else {
+                    for (int w = 0; w < W; w += 4)
+                        *reinterpret_cast<f32x4*>(to + w) =
+                            f32x4{o[F + w][i], o[F + w + 1][i], o[F + w + 2][i], o[F + w + 3][i]} * k;
+                } else {
 #pragma unroll
-                for (int w = 0; w < W; w++) to[w] = o[F + w][i];
+                    for (int w = 0; w < W; w++) to[w] = o[F + w][i] * k;
+                }
             }
         }
-        put_o<ND, S + 1>(row, o, g);
+        put_o<ND, FROM, TO, S + 1>(row, o, k, g);
     }
 }
 
 template <class KV, int ND>
 __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_attn_part(AttnArgs a) {
     typedef Attn<KV, ND> A;
-    // q's parts [load][part][lane], later the waves' sums [wave][row][LD]
-    constexpr int Q_BYTES = A::KL * 3 * 1024, O_BYTES = AT_WAVES * 16 * A::LD * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
-    __shared__ float sm[AT_WAVES][16], sl[AT_WAVES][16];
-    auto sq = reinterpret_cast<u32x4 (*)[3][64]>(lds);
-    auto so = reinterpret_cast<float (*)[16][A::LD]>(lds);
+    __shared__ u32x4 sq[A::KL][3][64];                          // q's parts [load][part][lane]
+    __shared__ __attribute__((aligned(16))) float so[AT_WAVES][16][A::LD];
+    __shared__ float sm[AT_WAVES][16], sl[AT_WAVES][16], st[16];
+    __shared__ int sf[AT_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
     // Workgroups go to the XCDs in turn: neighbours are heads, then requests, turned by the chunk, so that requests of
     // different lengths load the XCDs alike (chunks side by side: the 48 requests below 8192 positions took 209 us, XCD 0
     // with 1.5 times the chunks of XCD 7)
-    const int c = a.chunk0 + blockIdx.z, kh = blockIdx.x, b = (blockIdx.y + (uint32_t)c) % gridDim.y;
+    int c = blockIdx.z;
+    const int kh = blockIdx.x, b = __builtin_amdgcn_readfirstlane((blockIdx.y + (uint32_t)c) % gridDim.y), stride = gridDim.z;
     // every argument in one go, then the length and the table's entry side by side
     KQ_ARGS_READY("s"(a.kv.k), "s"(a.kv.v), "s"(a.kv.k_scale), "s"(a.kv.v_scale), "s"(a.kv.page_stride), "s"(a.kv.head_stride),
                   "s"(a.kv.pos_stride), "s"(a.table.pages), "s"(a.table.ld), "s"(a.lens), "s"(a.q), "s"(a.ldq));
-    const int first = c * AT_CHUNK + 64 * wave;
-    const int len = min(a.lens[b], a.max_len);
-    int page = a.table.pages[(int64_t)b * a.table.ld + (min(first + lane, a.table.cap - 1) >> a.page_shift)];
+    const int32_t* table = a.table.pages + (int64_t)b * a.table.ld;
+    auto entry = [&](int first) { return table[min(first + lane, a.table.cap - 1) >> a.page_shift]; };
+    const int length = a.lens[b];
+    int page = entry(c * AT_CHUNK + 64 * wave);
     asm volatile("" : "+v"(page));
+    const int len = min(__builtin_amdgcn_readfirstlane(length), a.max_len);
     if (c * AT_CHUNK >= len && (c || a.joined)) return;         // the join knows the chunks that are there
-    const int G = a.q_heads / a.kv.heads, R = a.T * G;
+    const int G = a.group, R = a.T * G;
     const int all = len - a.T + 1;                              // positions that every token sees
     A s;
-    s.open(a, page, kh, first, len, lane);
+    s.kb = static_cast<const uint8_t*>(a.kv.k) + (int64_t)kh * a.kv.head_stride * A::EB;
+    s.vb = static_cast<const uint8_t*>(a.kv.v) + (int64_t)kh * a.kv.head_stride * A::EB;
+    typename A::Span w;
+    bool ready = false;                                         // the chunk's first step is in flight and q's parts are there
     bool apart = false;                                         // token by token (below)
-    int tok = 0;
-    for (int r0 = 0; r0 < R;) {
-        const int row = r0 + r, t = row / G, h = kh * G + row % G;
+    int tok = 0, r0 = 0;
+    float f = 0.0f;
+    for (;;) {
+        const int row = r0 + r, t = row / G;
         const int see = row < R ? all + t : 0;                  // positions that the lane's row sees
-        // q's parts; each wave cuts a share
-        const float* q = a.q + ((int64_t)b * a.T + (row < R ? t : 0)) * a.ldq + (int64_t)(row < R ? h : 0) * A::D;
-        float f = a.scale * 1.44269504088896341f, top = 0.0f, bad = 0.0f;
-        typedef f32x4 Share[A::QW];
-        auto share = [&](int n, Share& x) {
-            const int d = 16 * A::QW * n + 4 * A::QW * g;
-            const bool ok = A::K_WHOLE || d < A::D;
+        if (!ready) {
+            w = s.open(a, page, kh, c * AT_CHUNK + 64 * wave, len, lane);
+            // q's parts; each wave cuts a share
+            const float* q = a.q + ((int64_t)b * a.T + (row < R ? t : 0)) * a.ldq + (int64_t)(row < R ? kh * G + row % G : 0) * A::D;
+            typedef f32x4 Share[A::QW];
+            auto share = [&](int n, Share& x) {
+                const int d = 16 * A::QW * n + 4 * A::QW * g;
+                const bool ok = A::K_WHOLE || d < A::D;
 #pragma unroll
-            for (int j = 0; j < A::QW; j++) {
-                x[j] = *reinterpret_cast<const f32x4_a4*>(q + (ok ? d : 0) + 4 * j);
-                if (!ok) x[j] = f32x4{0, 0, 0, 0};
-            }
-        };
-        constexpr int SHARES = (A::KL + AT_WAVES - 1) / AT_WAVES;
-        Share mine[SHARES], whole[KV::id == KQ_KV_BF16 ? 1 : A::KL];
-#pragma unroll
-        for (int i = 0; i < SHARES; i++) share(min(AT_WAVES * i + wave, A::KL - 1), mine[i]);
-        if constexpr (KV::id != KQ_KV_BF16)
-#pragma unroll
-            for (int n = 0; n < A::KL; n++) share(n, whole[n]);
-        s.load_k(0, r, g);
-        s.load_v(0, r, g);
-        if constexpr (KV::id != KQ_KV_BF16) {
-#pragma unroll
-            for (int n = 0; n < A::KL; n++)
-#pragma unroll
-                for (int j = 0; j < 4 * A::QW; j++) {
-                    const float x = whole[n][j >> 2][j & 3];
-                    top = fmaxf(top, fabsf(x));
-                    if constexpr (A::I8) bad = __builtin_fmaf(x, 0.0f, bad);
+                for (int j = 0; j < A::QW; j++) {
+                    x[j] = *reinterpret_cast<const f32x4_a4*>(q + (ok ? d : 0) + 4 * j);
+                    if (!ok) x[j] = f32x4{0, 0, 0, 0};
                 }
-            top = xor32_max(xor16_max(top));
-            if constexpr (A::I8) bad = xor32_sum(xor16_sum(bad));
-        }
-        float up = 1.0f;
-        if constexpr (KV::id == KQ_KV_F16) {
-            // times a power of two that puts the row's largest near 2^14
-            const uint32_t ex = max(ubits(top) >> 23, 15u);
-            up = fbits(min(268u - ex, 254u) << 23);
-            f *= fbits((ex - 14u) << 23);
-        }
-        if constexpr (A::I8) {
-            up = 8.35e6f / fmaxf(top, 1e-30f);
-            f = f * (fmaxf(top, 1e-30f) / 8.35e6f) + bad;            // bad: NaN for a row with an infinity or NaN
-        }
+            };
+            constexpr int SHARES = (A::KL + AT_WAVES - 1) / AT_WAVES;
+            Share mine[SHARES], whole[KV::id == KQ_KV_BF16 ? 1 : A::KL];
 #pragma unroll
-        for (int i = 0; i < SHARES; i++) {
-            const int n = AT_WAVES * i + wave;
-            if (n < A::KL) {
-                u32x4 p[3];
-                if constexpr (A::I8) {
+            for (int i = 0; i < SHARES; i++) share(min(AT_WAVES * i + wave, A::KL - 1), mine[i]);
+            if constexpr (KV::id != KQ_KV_BF16)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        uint32_t p0 = 0, p1 = 0, p2 = 0;
+                for (int n = 0; n < A::KL; n++) share(n, whole[n]);
+            s.load_k(0, r, g);
+            s.load_v(0, r, g);
+            float top = 0.0f, bad = 0.0f, up = 1.0f;
+            f = a.scale * 1.44269504088896341f;
+            if constexpr (KV::id != KQ_KV_BF16) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const int x = (int)rintf(mine[i][j][k] * up), y = (x + 0x80) >> 8, z = (y + 0x80) >> 8;
-                            p0 |= ((uint32_t)z & 0xffu) << (8 * k);      // x = 65536 z + 256 (int8)y + (int8)x
-                            p1 |= ((uint32_t)y & 0xffu) << (8 * k);
-                            p2 |= ((uint32_t)x & 0xffu) << (8 * k);
+                for (int n = 0; n < A::KL; n++)
+#pragma unroll
+                    for (int j = 0; j < 4 * A::QW; j++) {
+                        const float x = whole[n][j >> 2][j & 3];
+                        top = fmaxf(top, fabsf(x));
+                        if constexpr (A::I8) bad = __builtin_fmaf(x, 0.0f, bad);
+                    }
+                top = xor32_max(xor16_max(top));
+                if constexpr (A::I8) bad = xor32_sum(xor16_sum(bad));
+            }
+            if constexpr (KV::id == KQ_KV_F16) {
+                // times a power of two that puts the row's largest near 2^14
+                const uint32_t ex = max(ubits(top) >> 23, 15u);
+                up = fbits(min(268u - ex, 254u) << 23);
+                f *= fbits((ex - 14u) << 23);
+            }
+            if constexpr (A::I8) {
+                up = 8.35e6f / fmaxf(top, 1e-30f);
+                f = f * (fmaxf(top, 1e-30f) / 8.35e6f) + bad;            // bad: NaN for a row with an infinity or NaN
+            }
+#pragma unroll
+            for (int i = 0; i < SHARES; i++) {
+                const int n = AT_WAVES * i + wave;
+                if (n < A::KL) {
+                    u32x4 p[3];
+                    if constexpr (A::I8) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            uint32_t p0 = 0, p1 = 0, p2 = 0;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const int x = (int)rintf(mine[i][j][k] * up), y = (x + 0x80) >> 8, z = (y + 0x80) >> 8;
+                                p0 |= ((uint32_t)z & 0xffu) << (8 * k);      // x = 65536 z + 256 (int8)y + (int8)x
+                                p1 |= ((uint32_t)y & 0xffu) << (8 * k);
+                                p2 |= ((uint32_t)x & 0xffu) << (8 * k);
+                            }
+                            p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
                         }
-                        p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
-                    }
-                } else {
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        uint32_t p0, p1, p2;
-                        split2<KV>(mine[i][j >> 1][2 * (j & 1)] * up, mine[i][j >> 1][2 * (j & 1) + 1] * up, p0, p1, p2);
-                        p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
+                        for (int j = 0; j < 4; j++) {
+                            uint32_t p0, p1, p2;
+                            split2<KV>(mine[i][j >> 1][2 * (j & 1)] * up, mine[i][j >> 1][2 * (j & 1) + 1] * up, p0, p1, p2);
+                            p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
+                        }
                     }
+#pragma unroll
+                    for (int j = 0; j < 3; j++) sq[n][j][lane] = p[j];
                 }
-#pragma unroll
-                for (int j = 0; j < 3; j++) sq[n][j][lane] = p[j];
             }
+            __syncthreads();
         }
-        __syncthreads();
+        // The next chunk, if its rows are these: it is whole up to its own, so every wave has both its steps here.
+        const int after = c + stride;
+        const bool on = R <= 16 && !apart && (int64_t)after * AT_CHUNK < len;
+        int page_on = -1;
+        typename A::Span wn = w;
         float m = -INFINITY, l = 0.0f;
         f32x4 o[ND];
 #pragma unroll
@@ -418,7 +444,7 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
         int found = 0;
 #pragma unroll 1
         for (int u = 0; u < 2; u++) {
-            const int base = first + 32 * u;
+            const int base = w.first + 32 * u;
             if (base >= len) break;
             float e[2][4];
             if constexpr (A::I8) {
@@ -454,21 +480,24 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
 #pragma unroll
                     for (int j = 0; j < 4; j++) e[i][j] = acc[i][j];
             }
-            const bool next = u == 0 && base + 32 < len;
-            if (next) s.load_k(1, r, g);
-            if constexpr (A::I8) asm volatile("" : "+v"(s.mine_ks), "+v"(s.mine_vs));   // as here()
+            // What the next step reads is fetched whether there is one or not (no place that is not there is read, all lanes
+            // take the pool's first): the waits below then know how many loads are younger than theirs.
+            if (u) wn = s.open(a, on ? page_on : -1, kh, after * AT_CHUNK + 64 * wave, len, lane);
+            s.load_k(1 - u, r, g);
+            page_on = entry(after * AT_CHUNK + 64 * wave);
+            if constexpr (A::I8) asm volatile("" : "+v"(w.ks), "+v"(w.vs));   // as here()
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    if constexpr (A::I8) e[i][j] *= __shfl(s.mine_ks, 32 * u + 16 * i + 4 * g + j, 64);
+                    if constexpr (A::I8) e[i][j] *= fbits(of_lane(32 * u + 16 * i + 4 * g + j, ubits(w.ks)));
                     e[i][j] *= f;
                 }
-            top = -INFINITY;
+            float top = -INFINITY;
             // some row does not see some position
-            const bool partly = (uint32_t)(s.there >> (32 * u)) != ~0u || base + 32 > all;
+            const bool partly = (uint32_t)(w.there >> (32 * u)) != ~0u || base + 32 > all;
             if (partly) {
-                const uint32_t hid = s.hidden(u, see, g);
+                const uint32_t hid = A::hidden(w, u, see, g);
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -476,8 +505,8 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
                         if (hid >> (4 * i + j) & 1u) e[i][j] = -INFINITY;
                 // An infinity or NaN that only some tokens see would reach the others as 0 * inf: then the rows are done
                 // again, token by token, with the values that it does not see cleared.
-                const uint32_t gone = s.hidden(u, apart ? all + tok : len, g);
-                if (a.T > 1 && !apart) found |= s.v_not_finite(s.hidden(u, all, g) & ~gone);
+                const uint32_t gone = A::hidden(w, u, apart ? all + tok : len, g);
+                if (a.T > 1 && !apart) found |= s.v_not_finite(A::hidden(w, u, all, g) & ~gone);
                 s.clear_v(gone);
             }
 #pragma unroll
@@ -500,71 +529,96 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
                     e[i][j] = __builtin_amdgcn_exp2f(e[i][j] - from);
                     l += e[i][j];
                 }
-            s.pv(e, o, u, g);
-            if (next) s.load_v(1, r, g);
+            s.pv(w, e, o, u, g);
+            s.load_v(1 - u, r, g);
         }
-        if (a.T > 1 && !apart) {
-            if (__syncthreads_or(found)) {
-                apart = true;
-                tok = a.T - 1;
-                r0 = 0;
-                continue;
-            }
-        } else {
-            __syncthreads();                                    // the parts of q have left LDS
-        }
-        // the waves' sums, joined
+        // The waves' sums, joined: each scaled to the workgroup's maximum, then added.  (From here on the thread's place is
+        // taken anew, so that no address is held through the steps.)
         l = xor32_sum(xor16_sum(l));
-        if (row < R) {
-            if (g == 0) sm[wave][r] = m, sl[wave][r] = l;
-            put_o<ND, 0>(so[wave][r], o, g);
-        }
+        int me = tid;
+        asm volatile("" : "+v"(me));
+        const int r = me & 15, g = me >> 4 & 3;
+        if (g == 0) sm[wave][r] = m, sl[wave][r] = l;
+        if (g == 0 && r == 0) sf[wave] = found;
         __syncthreads();
-        constexpr int Q = A::D / 4;
-        for (int i = tid; i < min(16, R - r0) * Q; i += 64 * AT_WAVES) {
-            const int rr = i / Q, d = 4 * (i % Q), tt = (r0 + rr) / G, hh = kh * G + (r0 + rr) % G;
-            if (apart && tt != tok) continue;
-            float top = sm[0][rr];
-#pragma unroll
-            for (int w = 1; w < AT_WAVES; w++) top = fmaxf(top, sm[w][rr]);
-            f32x4 sum = {0, 0, 0, 0};
+        if (a.T > 1 && !apart && (sf[0] | sf[1] | sf[2] | sf[3])) {
+            apart = true;
+            tok = a.T - 1;
+            ready = false;
+            page = entry(c * AT_CHUNK + 64 * wave);
+            __syncthreads();
+            continue;
+        }
+        const float top = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+        if (wave == 0 && g == 0) {
             float total = 0.0f;
 #pragma unroll
-            for (int w = 0; w < AT_WAVES; w++) {
-                const float lw = sl[w][rr];
-                if (lw != 0.0f) {                               // 0: the wave saw nothing (a NaN counts)
-                    const float k = __builtin_amdgcn_exp2f(sm[w][rr] - top);
-                    sum += *reinterpret_cast<const f32x4*>(&so[w][rr][d]) * k;
-                    total += lw * k;
+            for (int i = 0; i < AT_WAVES; i++) {
+                const float li = sl[i][r];                      // 0: the wave saw nothing (a NaN counts)
+                total += li != 0.0f ? li * __builtin_amdgcn_exp2f(sm[i][r] - top) : 0.0f;
+            }
+            st[r] = total;
+            if (a.joined && row < R && (!apart || t == tok))
+                a.pml[(((int64_t)b * a.kv.heads + kh) * R + row) * a.chunks + c] = AttnMl{top, total};
+        }
+        const float k = l != 0.0f ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
+        auto round = [&](auto from, auto to) {
+            constexpr int FROM = decltype(from)::value, TO = decltype(to)::value, Q = 4 * (TO - FROM);
+            if (FROM) __syncthreads();                          // the round before has left LDS
+            if (row < R) {
+                if (l != 0.0f) {
+                    put_o<ND, FROM, TO>(so[wave][r], o, k, g);
+                } else {
+#pragma unroll
+                    for (int i = g; i < Q; i += 4) *reinterpret_cast<f32x4*>(&so[wave][r][4 * i]) = f32x4{0, 0, 0, 0};
                 }
             }
-            const int64_t at = (int64_t)b * a.T + tt;
-            if (a.joined) {
-                const int64_t part = (at * a.q_heads + hh) * a.chunks + c;
-                *reinterpret_cast<f32x4*>(a.po + part * A::D + d) = sum;
-                if (d == 0) a.pml[part] = AttnMl{top, total};
-            } else {
-                *reinterpret_cast<f32x4_a4*>(a.out + at * a.ldo + (int64_t)hh * A::D + d) =
-                    total == 0.0f ? f32x4{0, 0, 0, 0} : sum / total;
+            __syncthreads();
+            for (int i = me; i < min(16, R - r0) * Q; i += 64 * AT_WAVES) {
+                const int rr = i / Q, d = 4 * (i % Q);
+                auto part = [&](int n) { return *reinterpret_cast<const f32x4*>(&so[n][rr][d]); };
+                const f32x4 sum = (part(0) + part(1)) + (part(2) + part(3));
+                if (a.joined && !apart) {
+                    *reinterpret_cast<f32x4*>(a.po + ((((int64_t)b * a.kv.heads + kh) * R + r0 + rr) * a.chunks + c) * A::D +
+                                              16 * FROM + d) = sum;
+                    continue;
+                }
+                const int tt = (r0 + rr) / G, hh = kh * G + (r0 + rr) % G;
+                if (apart && tt != tok) continue;
+                if (a.joined)
+                    *reinterpret_cast<f32x4*>(a.po + ((((int64_t)b * a.kv.heads + kh) * R + r0 + rr) * a.chunks + c) * A::D +
+                                              16 * FROM + d) = sum;
+                else
+                    *reinterpret_cast<f32x4_a4*>(a.out + ((int64_t)b * a.T + tt) * a.ldo + (int64_t)hh * A::D + 16 * FROM + d) =
+                        st[rr] == 0.0f ? f32x4{0, 0, 0, 0} : sum / st[rr];
             }
-        }
-        if (!apart || tok == 0) {
+        };
+        round(std::integral_constant<int, 0>(), std::integral_constant<int, (ND < 8 ? ND : 8)>());
+        if constexpr (ND > 8) round(std::integral_constant<int, 8>(), std::integral_constant<int, ND>());
+        // what comes next: this chunk's next token or rows, or the next chunk
+        ready = on;
+        w = wn;
+        if (apart && tok > 0) {
+            tok--;
+        } else if (r0 + 16 < R) {
             r0 += 16;
             tok = a.T - 1;
         } else {
-            tok--;
+            c = after;
+            r0 = 0;
+            apart = false;
+            if ((int64_t)c * AT_CHUNK >= len) return;
         }
-        if (r0 < R) __syncthreads();                            // the sums have left LDS
+        if (!ready) {
+            page = entry(c * AT_CHUNK + 64 * wave);
+            __syncthreads();                                    // q's parts and the sums have left LDS
+        }
     }
 }
 
 template <class KV, int ND>
 void launch_attn_part_nd(const AttnArgs& a, hipStream_t s) {
-    AttnArgs p = a;
-    for (p.chunk0 = 0; p.chunk0 < a.chunks; p.chunk0 += 32768) {
-        const int n = a.chunks - p.chunk0 < 32768 ? a.chunks - p.chunk0 : 32768;
-        hipLaunchKernelGGL((k_attn_part<KV, ND>), dim3(a.kv.heads, a.table.seqs, n), dim3(64 * AT_WAVES), 0, s, p);
-    }
+    hipLaunchKernelGGL((k_attn_part<KV, ND>), dim3(a.kv.heads, a.table.seqs, a.groups), dim3(64 * AT_WAVES), 0, s, a);
 }
 
 template <class KV>

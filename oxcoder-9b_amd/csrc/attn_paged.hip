@@ -6,44 +6,52 @@
 
 namespace kq {
 
-// One workgroup per row and 32 of its values: 32 groups of 8 lanes take every 32nd chunk, then the groups are added as a
-// tree: a row's result depends on its number of chunks alone.
+// One workgroup per row and 32 N of its values: 32 groups of 8 lanes take every 32nd chunk, then the groups are added as
+// a tree: a row's result depends on its number of chunks alone.
+template <int N>
 __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
-    __shared__ __attribute__((aligned(16))) f32x4 so[4][8];
+    __shared__ __attribute__((aligned(16))) f32x4 so[4][N][8];
     __shared__ float sl[4], sm[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, D = a.kv.dim;
-    const int b = blockIdx.x / a.T, h = blockIdx.y, d = 32 * blockIdx.z + 4 * (tid & 7);
+    const int b = blockIdx.x / a.T, h = blockIdx.y, G = a.group, d = 32 * N * blockIdx.z + 4 * (tid & 7);
     const int len = min(a.lens[b], a.max_len), n = len <= 0 ? 0 : (len + AT_CHUNK - 1) / AT_CHUNK;
-    const int64_t row = ((int64_t)blockIdx.x * a.q_heads + h) * a.chunks;
+    const int64_t row = (((int64_t)b * a.kv.heads + h / G) * a.T * G + blockIdx.x % a.T * G + h % G) * a.chunks;
     float top = -INFINITY;
     for (int c = tid; c < n; c += 256) top = fmaxf(top, a.pml[row + c].m);
     for (int w = 32; w; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
     if (lane == 0) sm[wave] = top;
     __syncthreads();
     top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    f32x4 sum = {0, 0, 0, 0};
+    f32x4 sum[N] = {};
     float total = 0.0f;
-#pragma unroll 8
+#pragma unroll 8 / N
     for (int c = tid >> 3; c < n; c += 32) {
         const AttnMl ml = a.pml[row + c];
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.po + (row + c) * D + (d < D ? d : 0));
+        f32x4 x[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = *reinterpret_cast<const f32x4*>(a.po + (row + c) * D + (d + 32 * i < D ? d + 32 * i : 0));
         const float k = ml.l != 0.0f ? __builtin_amdgcn_exp2f(ml.m - top) : 0.0f;   // 0: the row saw nothing (a NaN counts)
-        sum += x * k;
+#pragma unroll
+        for (int i = 0; i < N; i++) sum[i] += x[i] * k;
         total += ml.l * k;
     }
+#pragma unroll
     for (int w = 8; w < 64; w <<= 1) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) sum[i] += __shfl_xor(sum[i], w, 64);
+        for (int i = 0; i < 4 * N; i++) sum[i >> 2][i & 3] += __shfl_xor(sum[i >> 2][i & 3], w, 64);
         total += __shfl_xor(total, w, 64);
     }
-    if (lane < 8) so[wave][lane] = sum;
+    if (lane < 8)
+#pragma unroll
+        for (int i = 0; i < N; i++) so[wave][i][lane] = sum[i];
     if (lane == 0) sl[wave] = total;
     __syncthreads();
-    if (tid >= 8 || d >= D) return;
-    sum = (so[0][tid] + so[1][tid]) + (so[2][tid] + so[3][tid]);
+    const int i = tid >> 3, at = 32 * N * blockIdx.z + 4 * tid;
+    if (i >= N || at >= D) return;
+    const f32x4 all = (so[0][i][tid & 7] + so[1][i][tid & 7]) + (so[2][i][tid & 7] + so[3][i][tid & 7]);
     total = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-    *reinterpret_cast<f32x4_a4*>(a.out + (int64_t)blockIdx.x * a.ldo + (int64_t)h * D + d) =
-        total == 0.0f ? f32x4{0, 0, 0, 0} : sum / total;
+    *reinterpret_cast<f32x4_a4*>(a.out + (int64_t)blockIdx.x * a.ldo + (int64_t)h * D + at) =
+        total == 0.0f ? f32x4{0, 0, 0, 0} : all / total;
 }
 
 static int chunks_of(int max_len) { return max_len / AT_CHUNK + (max_len % AT_CHUNK != 0); }
@@ -56,17 +64,31 @@ size_t attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len) 
 
 void launch_attn_paged(const AttnArgs& args, hipStream_t s) {
     AttnArgs a = args;
+    a.group = a.q_heads / a.kv.heads;
     a.page_shift = __builtin_ctz((unsigned)a.kv.page_size);
     a.chunks = chunks_of(a.max_len);
     a.joined = a.chunks > 1;
+    // A workgroup takes up to three chunks, the next one's first step in flight while it ends one, if that leaves eight
+    // workgroups a CU (32 requests of 16384 8-bit positions: 159, 151, 146, 147 us with one to four; one request of 100001:
+    // 87, 87, 89, 93 us; 8 requests of 5003: 34, 46, 41 us).
+    int64_t per = (int64_t)a.chunks * a.kv.heads * a.table.seqs / (8 * device_cus());
+    per = per < 1 ? 1 : per > 3 ? 3 : per;
+    a.groups = (int)((a.chunks + per - 1) / per);
+    if (a.groups > 65535) a.groups = 65535;                    // a workgroup goes on until no chunk is left
     const size_t parts = (size_t)a.table.seqs * a.T * a.q_heads * a.chunks;
     a.po = reinterpret_cast<float*>(a.ws);
     a.pml = reinterpret_cast<AttnMl*>(a.ws + up256(parts * a.kv.dim * 4));
     if (a.kv.type == KQ_KV_F16) launch_attn_part<KvF16>(a, s);
     else if (a.kv.type == KQ_KV_BF16) launch_attn_part<KvBf16>(a, s);
     else launch_attn_part<KvI8>(a, s);
-    if (a.joined)
-        hipLaunchKernelGGL(k_attn_join, dim3(a.table.seqs * a.T, a.q_heads, (a.kv.dim + 31) / 32), dim3(256), 0, s, a);
+    if (!a.joined) return;
+    // rows enough for the chip: four times fewer workgroups, that scan a row's maxima once for 128 values (512 rows of 20 chunks and
+    // 256 values 7.4 -> 5 us; the 32 rows of 391 chunks 8 us with 32 values each, 13 us with 128)
+    const int64_t rows = (int64_t)a.table.seqs * a.T * a.q_heads;
+    if (rows >= device_cus())
+        hipLaunchKernelGGL(k_attn_join<4>, dim3(a.table.seqs * a.T, a.q_heads, (a.kv.dim + 127) / 128), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL(k_attn_join<1>, dim3(a.table.seqs * a.T, a.q_heads, (a.kv.dim + 31) / 32), dim3(256), 0, s, a);
 }
 
 }  // namespace kq

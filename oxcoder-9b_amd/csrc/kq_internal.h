@@ -141,7 +141,8 @@ struct AttnArgs {
     float* out;
     uint8_t* ws;
     // set by launch_attn_paged
-    int page_shift, chunks, chunk0, joined;     // joined: parts go to po and pml [row][head][chunk]
+    int group, page_shift, chunks, joined;     // group: query heads of a key-value head; joined: parts go to po and pml [request][key-value head][token, query head][chunk]
+    int groups;                         // workgroups that share a request and head's chunks
     float* po;
     AttnMl* pml;
 };

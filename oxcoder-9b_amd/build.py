@@ -2,6 +2,7 @@
 
 * ``kq/libkq.so``     -- HIP kernels + C ABI (include/kq.h), gfx950 only, built with hipcc.
 * ``kq/libkqhost.so`` -- host-side synthetic weight quantizer (include/kq_host.h), g++ + OpenMP.
+* ``kq/_calls.so``   -- the token loop's calls from Python (a CPython module on torch's headers), g++.
 
 Every HIP translation unit is compiled with -ffp-contract=off (the numerical contract of the
 kernels spells out each fused multiply-add explicitly) and with packed fp32 instructions disabled.
@@ -12,6 +13,7 @@ import hashlib
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -48,6 +50,8 @@ HIP_EXTRA = {"gemm_q8k.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 HOST_SOURCES = ["host/quantize_weights.cpp"]
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-shared", "-fopenmp", "-ffp-contract=off",
               "-fno-math-errno", "-Wall", "-I" + os.path.join(ROOT, "include")]
+CALLS_SOURCE = "host/calls.cpp"
+CALLS_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-I" + os.path.join(ROOT, "include")]
 
 
 def _run(cmd):
@@ -83,9 +87,21 @@ def _compile_hip(src):
     return obj
 
 
+def _compile_calls():
+    import torch
+    from torch.utils import cpp_extension
+
+    dirs = cpp_extension.include_paths() + [sysconfig.get_paths()["include"]]
+    obj = os.path.join(OBJ, "calls.o")
+    _run(["g++", *CALLS_FLAGS, "-D__HIP_PLATFORM_AMD__", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+          *[f for d in dirs for f in ("-isystem", d)], "-c", os.path.join(CSRC, CALLS_SOURCE), "-o", obj])
+    return obj, os.path.join(os.path.dirname(torch.__file__), "lib")
+
+
 def build(jobs=8):
     os.makedirs(OBJ, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        calls = ex.submit(_compile_calls)
         objs = list(ex.map(_compile_hip, HIP_SOURCES))
     so = os.path.join(OUT, "libkq.so")
     _run([HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC", *objs, "-o", so + ".tmp"])
@@ -93,6 +109,12 @@ def build(jobs=8):
     host = os.path.join(OUT, "libkqhost.so")
     _run(["g++", *HOST_FLAGS, *[os.path.join(CSRC, s) for s in HOST_SOURCES], "-o", host + ".tmp"])
     os.replace(host + ".tmp", host)
+    obj, torch_lib = calls.result()
+    py = os.path.join(OUT, "_calls.so")
+    # torch's libraries are in the process before the module is loaded; libkq.so lies beside it
+    _run(["g++", "-shared", obj, "-L" + OUT, "-l:libkq.so", "-L" + torch_lib, "-ltorch_python", "-ltorch_cpu", "-lc10",
+          "-Wl,-rpath,$ORIGIN", "-o", py + ".tmp"])
+    os.replace(py + ".tmp", py)
     return so, host
 
 

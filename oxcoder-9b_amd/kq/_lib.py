@@ -9,6 +9,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIBKQ = os.path.join(HERE, "libkq.so")
 LIBKQHOST = os.path.join(HERE, "libkqhost.so")
+CALLS = os.path.join(HERE, "_calls.so")
 
 # Every symbol include/kq.h declares, with (restype, argtypes).
 _vp, _i, _i64 = C.c_void_p, C.c_int, C.c_int64
@@ -93,6 +94,19 @@ def _load(path, symbols):
 
 def kq():
     return _libs.get(LIBKQ) or _load(LIBKQ, KQ_SYMBOLS)
+
+
+def calls():
+    """The compiled form of the token loop's calls (csrc/host/calls.cpp)."""
+    if CALLS not in _libs:
+        if not os.path.exists(CALLS):
+            raise RuntimeError("%s is not built; run `python oxcoder-9b_amd/build.py`" % os.path.basename(CALLS))
+        import torch  # noqa: F401 (its libraries, which the module needs in the process)
+
+        kq()
+        from . import _calls
+        _libs[CALLS] = _calls
+    return _libs[CALLS]
 
 
 def kqhost():

@@ -117,22 +117,26 @@ class PagedAttention:
                              % (table.shape[0], self.max_len, q_heads, c.dim))
         buf = torch.empty(n + 256, dtype=torch.uint8, device=c.device)
         self.ws = buf[-buf.data_ptr() % 256:][:n]
-        # what every call passes on
-        self._ws = self.ws.data_ptr(), n
-        self._table = self._rope = None
+        # what every call passes on, as addresses: the tensors stay as long as the plan
+        self._plan, self._keep = None, (table, rope, buf)
         if c.device.type == "cuda":
-            self._table, self._rope = ops._table(table), ops._rope(rope)
+            self._calls = _lib.calls()
+            self._plan = self._calls.plan(ops._table(table), ops._rope(rope), q_heads, c.heads, c.dim, self.max_len,
+                                          self._interleaved, self.scale, (self.ws.data_ptr(), n))
 
     def append(self, layer, q, k, v, seq, pos, q_out=None):
         """Rotate q [N][q_heads * dim] into q_out (q itself: in place; None: a new tensor) and k
         [N][heads * dim], store k and v for token n of request seq[n] at position pos[n] (both int32 [N]).
         q None: keys and values only.  Returns q_out."""
-        if self._table is None:
-            raise ValueError("the caches must be device tensors")
         if q is not None and q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        return ops._kv_append(self.caches[layer], self._table, q, k, v, seq, pos, q_out, self.q_heads, self._rope,
-                              self._interleaved)
+        c = self.caches[layer]
+        rc = self._plan and self._calls.append(self._plan, c.ref, ops._stream(c.device), q, k, v, seq, pos, q_out)
+        if rc is None:                       # a tensor is not as it should be
+            ops.kv_append(c, self.table, q, k, v, seq, pos, q_out, self.q_heads, self.rope, self._interleaved)
+        elif rc:
+            _lib.check(rc)
+        return q_out
 
     def attend(self, layer, q, lens, out=None, tokens=None):
         """Attention of the last ``tokens`` (default: the constructor's) tokens of each request; q and out
@@ -140,9 +144,12 @@ class PagedAttention:
         T = self.tokens if tokens is None else tokens
         if not 1 <= T <= self.tokens:
             raise ValueError("tokens must be 1..%d" % self.tokens)
-        if self._table is None:
-            raise ValueError("the caches must be device tensors")
+        c = self.caches[layer]
         if out is None:
-            out = torch.empty((q.shape[0], self.q_heads * self.caches[layer].dim), device=q.device)
-        return ops._attn_paged(self.caches[layer], self._table, q, lens, out, self.q_heads, T, self.scale, self.max_len,
-                               *self._ws)
+            out = torch.empty((q.shape[0], self.q_heads * c.dim), device=q.device)
+        rc = self._plan and self._calls.attend(self._plan, c.ref, ops._stream(c.device), q, lens, out, T)
+        if rc is None:                       # a tensor is not as it should be
+            ops.attn_paged(c, self.table, q, lens, out, self.q_heads, T, self.scale, self.max_len, self.ws)
+        elif rc:
+            _lib.check(rc)
+        return out

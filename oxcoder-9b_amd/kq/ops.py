@@ -433,9 +433,6 @@ def dequant_rows(w, R, C_, ty, row0, nrows, y=None):
     return y
 
 
-# Arguments of the operators of a token loop, whose calls take a few microseconds: one look at each attribute where the
-# tensor is as it should be, and the words of what is wrong where it is not.
-
 def _opt(t, name, dtype, n):
     """Pointer of an optional contiguous 1-D device tensor of at least n values."""
     if t is None:
@@ -444,6 +441,11 @@ def _opt(t, name, dtype, n):
         return t.data_ptr()
     _dev(t, name, dtype)
     raise ValueError("%s must hold %d values, contiguous" % (name, n))
+
+
+def _need(t, name, dtype, n):
+    """_opt's pointer of a tensor that may not be left out."""
+    return _dev(t, name, dtype) if t is None else _opt(t, name, dtype, n)
 
 
 def _mat(t, name, dtype, rows, cols):
@@ -479,30 +481,20 @@ def kv_append(cache, table, q, k, v, seq, pos, q_out, q_heads, rope=None, interl
     """Rotate q [N][q_heads * dim] into q_out and k [N][heads * dim], and store k and v of token n at position pos[n]
     of request seq[n] in ``cache`` (a kv.KVCache) under ``table`` int32 [requests][width] (kq_kv_append).
     q and q_out None: keys and values only; rope: kv.rope_table's, or None."""
-    return _kv_append(cache, _table(table), q, k, v, seq, pos, q_out, q_heads, _rope(rope), 1 if interleaved else 0)
-
-
-def _kv_append(cache, table, q, k, v, seq, pos, q_out, q_heads, rope, interleaved):
     f32, i32, D = torch.float32, torch.int32, cache.dim
-    cols = cache.heads * D
-    if q is None:
-        if q_out is not None:
-            raise ValueError("q and q_out go together")
-        N = k.shape[0]
-        pq = po = None
-        ldq = ldo = 0
-    elif q_out is None:
+    N, cols = k.shape[0], cache.heads * D
+    if (q is None) != (q_out is None):
         raise ValueError("q and q_out go together")
-    else:
-        N = k.shape[0]
+    pq = po = None
+    ldq = ldo = 0
+    if q is not None:
         pq, ldq = _mat(q, "q", f32, N, q_heads * D)
-        po, ldo = (pq, ldq) if q_out is q else _mat(q_out, "q_out", f32, N, q_heads * D)
+        po, ldo = _mat(q_out, "q_out", f32, N, q_heads * D)
     pk, ldk = _mat(k, "k", f32, N, cols)
     pv, ldv = _mat(v, "v", f32, N, cols)
-    rc = _lib.kq().kq_kv_append(cache.ref, *table, N, _opt(seq, "seq", i32, N), _opt(pos, "pos", i32, N), pq, ldq, q_heads,
-                                po, ldo, pk, ldk, pv, ldv, *rope, interleaved, _stream(cache.device))
-    if rc:
-        _lib.check(rc)
+    _lib.check(_lib.kq().kq_kv_append(cache.ref, *_table(table), N, _need(seq, "seq", i32, N), _need(pos, "pos", i32, N), pq, ldq,
+                                      q_heads, po, ldo, pk, ldk, pv, ldv, *_rope(rope), 1 if interleaved else 0,
+                                      _stream(cache.device)))
     return q_out
 
 
@@ -515,18 +507,12 @@ def attn_paged(cache, table, q, lens, out, q_heads, tokens, scale, max_len, ws):
     """Attention of the last ``tokens`` tokens of each request over ``cache`` (a kv.KVCache) under ``table``
     int32 [requests][width]: q, out [requests * tokens][q_heads * dim], lens int32 [requests] counting the new
     tokens, at most max_len; ws of attn_paged_workspace_bytes, 256-byte aligned (kq_attn_paged)."""
-    return _attn_paged(cache, _table(table), q, lens, out, q_heads, tokens, scale, max_len, _dev(ws, "ws", torch.uint8),
-                       ws.numel())
-
-
-def _attn_paged(cache, table, q, lens, out, q_heads, tokens, scale, max_len, ws, ws_bytes):
-    seqs, cols = table[2], q_heads * cache.dim
-    pq, ldq = _mat(q, "q", torch.float32, seqs * tokens, cols)
-    po, ldo = _mat(out, "out", torch.float32, seqs * tokens, cols)
-    rc = _lib.kq().kq_attn_paged(cache.ref, *table, _opt(lens, "lens", torch.int32, seqs), max_len, tokens, pq, ldq, q_heads,
-                                 scale, po, ldo, ws, ws_bytes, _stream(cache.device))
-    if rc:
-        _lib.check(rc)
+    table = _table(table)
+    rows, cols = table[2] * tokens, q_heads * cache.dim
+    pq, ldq = _mat(q, "q", torch.float32, rows, cols)
+    po, ldo = _mat(out, "out", torch.float32, rows, cols)
+    _lib.check(_lib.kq().kq_attn_paged(cache.ref, *table, _need(lens, "lens", torch.int32, table[2]), max_len, tokens, pq, ldq,
+                                       q_heads, scale, po, ldo, _dev(ws, "ws", torch.uint8), ws.numel(), _stream(cache.device)))
     return out
 
 
@@ -540,13 +526,6 @@ def logits_penalize(x, history=None, length=None, prompt=None, repetition=None, 
     """Penalties, biases and a grammar mask on logits x [B][V] into y (may be x) and the greedy pick into picked
     int32 [B] (ws: zero-filled, logits_workspace_bytes, 256-byte aligned); either may be None
     (kq_logits_penalize; the arguments are sampling.Picker.pick's)."""
-    return _logits_penalize(x, history, length, prompt, repetition, frequency, presence, bias_ids, bias_values, allowed, y,
-                            _opt(picked, "picked", torch.int32, x.shape[0]), _opt(ws, "ws", torch.uint8, 0),
-                            0 if ws is None else ws.numel())
-
-
-def _logits_penalize(x, history, length, prompt, repetition, frequency, presence, bias_ids, bias_values, allowed, y, picked,
-                     ws, ws_bytes):
     f32, i32 = torch.float32, torch.int32
     B, V = x.shape
     px, ldx = _mat(x, "x", f32, B, V)
@@ -571,10 +550,9 @@ def _logits_penalize(x, history, length, prompt, repetition, frequency, presence
             pm, ldm = _mat(allowed, "allowed", i32, B, words)
     if y is not None:
         py, ldy = _mat(y, "y", f32, B, V)
-    rc = _lib.kq().kq_logits_penalize(
+    _lib.check(_lib.kq().kq_logits_penalize(
         px, ldx, B, V, ph, ldh, hist, _opt(length, "length", i32, B), _opt(prompt, "prompt", i32, B),
         _opt(repetition, "repetition", f32, B), _opt(frequency, "frequency", f32, B), _opt(presence, "presence", f32, B),
-        pb, pv, ldb, nb, pm, ldm, py, ldy, ws, ws_bytes, picked, _stream(x.device))
-    if rc:
-        _lib.check(rc)
+        pb, pv, ldb, nb, pm, ldm, py, ldy, _opt(ws, "ws", torch.uint8, 0), 0 if ws is None else ws.numel(),
+        _opt(picked, "picked", i32, B), _stream(x.device)))
     return y

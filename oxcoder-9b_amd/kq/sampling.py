@@ -5,7 +5,7 @@ logits of a batch and applies what a serving program is asked for on the way, in
 """
 import torch
 
-from . import ops
+from . import _lib, ops
 
 
 class Picker:
@@ -20,8 +20,9 @@ class Picker:
         self.ws = buf[-buf.data_ptr() % 256:][:n]
         self.rows = rows
         self.picked = torch.empty(rows, dtype=torch.int32, device=device)
-        self._held = self.picked.data_ptr(), self.ws.data_ptr(), n       # what every call passes on
-        self._device = self.ws.device
+        # what every call passes on, as addresses: the tensors stay as long as the picker
+        self._held, self._keep = (self.picked.data_ptr(), self.ws.data_ptr(), n), (self.picked, buf)
+        self._device, self._calls = self.ws.device, _lib.calls()
 
     def pick(self, logits, history=None, length=None, prompt=None, repetition=None, frequency=None, presence=None,
              bias_ids=None, bias_values=None, allowed=None, out=None):
@@ -42,6 +43,12 @@ class Picker:
             raise ValueError("%d rows, the picker holds %d" % (rows, self.rows))
         if logits.device != self._device:
             raise ValueError("logits must be a device tensor, on the picker's device")
-        ops._logits_penalize(logits, history, length, prompt, repetition, frequency, presence, bias_ids, bias_values,
-                             allowed, out, *self._held)
-        return self.picked if rows == self.rows else self.picked[:rows]
+        rc = self._calls.pick(*self._held, ops._stream(self._device) if logits.is_cuda else None, logits, history, length, prompt,
+                              repetition, frequency, presence, bias_ids, bias_values, allowed, out)
+        picked = self.picked if rows == self.rows else self.picked[:rows]
+        if rc is None:                       # a tensor is not as it should be
+            ops.logits_penalize(logits, history, length, prompt, repetition, frequency, presence, bias_ids, bias_values,
+                                allowed, out, picked, self.ws)
+        elif rc:
+            _lib.check(rc)
+        return picked

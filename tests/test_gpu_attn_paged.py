@@ -293,3 +293,27 @@ def test_repeated_calls_leave_the_workspace_ready(dev):
         q = torch.randn((3 * T, H * D), generator=g)
         got = att.attend(0, q.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), tokens=T)
         assert torch.equal(got, attend(dev, cache, table, q, lens, T, H)), (i, lens)
+
+
+def test_refusals_on_the_device(dev):
+    """Device tensors of another type, too small, of another layout or left out: refused before any launch."""
+    H, D = 4, 64
+    cache, table, q = setup(dev, "bf16", D, H, 2, 16, [40, 40], 1)
+    att = kv.PagedAttention([cache], table.to(dev), H, rope=kv.rope_table(64, D, device=dev))
+    q, lens = q.to(dev), torch.tensor([40, 40], dtype=torch.int32, device=dev)
+    new = torch.randn(2, 2 * D, device=dev)
+    seq, pos = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([0, 1], [39, 39]))
+    before = cache.k.clone()
+    for a in ((q.half(), lens), (q[:1], lens), (q[:, :-1], lens), (q.t().contiguous().t(), lens), (q.view(-1), lens),
+              (q, lens.long()), (q, lens[:1]), (q, None), (q.cpu(), lens), (None, lens, torch.empty_like(q))):
+        with pytest.raises(ValueError):
+            att.attend(0, *a)
+    for a in ((q, new.half(), new, seq, pos), (q, new, new[:1], seq, pos), (q, new, new[:, :-1], seq, pos),
+              (q, new, new, seq.long(), pos), (q, new, new, seq, pos[:1]), (q, new, new, None, pos), (q[:1], new, new, seq, pos),
+              (q, new, new, torch.stack([seq, seq], 1)[:, 0], pos), (None, new, new, seq, pos, q)):
+        with pytest.raises(ValueError):
+            att.append(0, *a)
+    torch.cuda.synchronize()
+    assert torch.equal(cache.k, before)
+    att.append(0, q, new, new, seq, pos)
+    assert not torch.equal(cache.k, before)

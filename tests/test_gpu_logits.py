@@ -204,3 +204,22 @@ def test_slices(dev, B, V):
 def test_long_lists(dev, L, nb):
     """Bias lists and histories on both sides of what one note per id holds."""
     check(dev, *inputs(2, 6000, L, nb, True, seed=nb))
+
+
+def test_refusals_on_the_device(dev):
+    """Device tensors of another type, too small, of another layout or left out: refused before any launch."""
+    B, V = 2, 300
+    x, *args = (torch.from_numpy(a).to(dev) for a in inputs(B, V, 20, 5, True))
+    good = dict(zip(NAMES, args))
+    p = sampling.Picker(B, dev)
+    for name, bad in (("history", good["history"].long()), ("history", good["history"][:1]), ("length", None),
+                      ("length", good["length"][:1]), ("prompt", good["prompt"].long()), ("repetition", good["repetition"].double()),
+                      ("frequency", good["frequency"][:1]), ("bias_values", None), ("bias_values", good["bias_values"][:, :4]),
+                      ("bias_ids", good["bias_ids"].t().contiguous().t()), ("allowed", good["allowed"][:, :9]),
+                      ("out", torch.empty(B, V - 1, device=dev)), ("out", torch.empty(B, V)), ("out", torch.empty(V, B, device=dev).t())):
+        with pytest.raises(ValueError):
+            p.pick(x, **{**good, name: bad})
+    for logits in (x.double(), x.t().contiguous().t(), x.cpu()):
+        with pytest.raises(ValueError):
+            p.pick(logits, **good)
+    assert p.pick(x, **good).cpu().tolist() == picks(steps(x.cpu().numpy(), *[a.cpu().numpy() for a in args]))

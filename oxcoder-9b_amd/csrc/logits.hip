@@ -13,10 +13,12 @@ namespace kq {
 
 constexpr int LG_T = 512;                    // threads
 constexpr int LG_STEP = 4 * LG_T;            // ids of a workgroup's pass of 16-byte loads
+constexpr int LG_AHEAD = 4;                  // history ids a thread fetches ahead
 constexpr int LG_MOST = 4 * LG_STEP;         // ids of the largest slice: 32 KB of notes, four workgroups a CU
-constexpr uint32_t LG_SEEN = 0x80000000u;    // a note: the id occurs;
-constexpr int LG_ENTRY = 20;                 // from this bit on: its last bias entry + 1; below: occurrences after the prompt
-constexpr int LG_MOST_HIST = 1 << LG_ENTRY, LG_MOST_BIAS = 1 << (31 - LG_ENTRY);
+// A note: the last bias entry + 1, whether the id occurs, occurrences after the prompt.
+constexpr int LG_ENTRY = 21, LG_COUNT = 20;
+constexpr uint32_t LG_SEEN = 1u << LG_COUNT;
+constexpr int LG_MOST_HIST = 1 << LG_COUNT, LG_MOST_BIAS = 1 << (32 - LG_ENTRY);
 constexpr int LG_ROW_BYTES = 2 * ARG_LINE;   // workspace of a row: the key's line, the ticket's line
 
 // A row's penalties.
@@ -72,33 +74,53 @@ __global__ void __launch_bounds__(LG_T) k_logits(LogitsArgs a) {
             if (allowed) ok[n] = allowed[i >> 5];
         }
     }
+    // the lists' first entries as well, read before the history's length is known: its row holds max_hist ids
+    const int32_t* hist = a.hist + (int64_t)b * a.ldh;
+    const int64_t bias0 = (int64_t)b * a.ldb;
+    const int held = a.hist ? a.max_hist : 0, nb = a.bias_id ? a.nb : 0;
+    uint32_t id[LG_AHEAD], bias_id = ~0u;
+    float bias_val = 0.0f;
+#pragma unroll
+    for (int k = 0; k < LG_AHEAD; k++) id[k] = tid + k * LG_T < held ? (uint32_t)hist[tid + k * LG_T] : ~0u;
+    if (tid < nb) {
+        bias_id = (uint32_t)a.bias_id[bias0 + tid];
+        bias_val = a.bias_val[bias0 + tid];
+    }
     const LgRow row = lg_row(a, b);
-    const int nh = a.hist ? min(max(a.hist_len[b], 0), a.max_hist) : 0, nb = a.bias_id ? a.nb : 0;
+    const int nh = a.hist ? min(max(a.hist_len[b], 0), a.max_hist) : 0;
     const bool notes = nh | nb;
     if (notes) {
         for (int i = 4 * tid; i < a.slice; i += LG_STEP) *reinterpret_cast<u32x4*>(note + i) = u32x4{0, 0, 0, 0};
-        __syncthreads();
-        if (nb) {
-            for (int i = tid; i < nb; i += LG_T) {
-                const int64_t at = (int64_t)b * a.ldb + i;
-                const uint32_t id = (uint32_t)a.bias_id[at] - (uint32_t)v0;
-                bias[i] = a.bias_val[at];
-                if (id < (uint32_t)nv) atomicMax(&note[id], (uint32_t)(i + 1) << LG_ENTRY);
-            }
-            __syncthreads();
-        }
         const int prompt = a.prompt_len ? a.prompt_len[b] : 0;
-        const int32_t* hist = a.hist + (int64_t)b * a.ldh;
-        for (int i0 = tid; i0 < nh; i0 += 4 * LG_T) {
-            uint32_t id[4];
+        __syncthreads();
+        auto occurs = [&](uint32_t v, int i) {
+            const uint32_t at = v - (uint32_t)v0;
+            if (at < (uint32_t)nv && i < nh) {
+                atomicOr(&note[at], LG_SEEN);
+                if (i >= prompt) atomicAdd(&note[at], 1u);
+            }
+        };
+        auto biased = [&](uint32_t v, float value, int i) {
+            bias[i] = value;
+            const uint32_t at = v - (uint32_t)v0, entry = (uint32_t)(i + 1) << LG_ENTRY;
+            if (at >= (uint32_t)nv) return;
+            uint32_t old = note[at];
+            while (old < entry) {                                          // the fields below may change meanwhile
+                const uint32_t was = atomicCAS(&note[at], old, (old & ((1u << LG_ENTRY) - 1)) | entry);
+                if (was == old) break;
+                old = was;
+            }
+        };
+        if (tid < nb) biased(bias_id, bias_val, tid);
+        for (int i = tid + LG_T; i < nb; i += LG_T) biased((uint32_t)a.bias_id[bias0 + i], a.bias_val[bias0 + i], i);
 #pragma unroll
-            for (int k = 0; k < 4; k++) id[k] = i0 + k * LG_T < nh ? (uint32_t)hist[i0 + k * LG_T] - (uint32_t)v0 : ~0u;
+        for (int k = 0; k < LG_AHEAD; k++) occurs(id[k], tid + k * LG_T);
+        for (int i0 = tid + LG_AHEAD * LG_T; i0 < nh; i0 += 4 * LG_T) {
+            uint32_t v[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (id[k] < (uint32_t)nv) {
-                    atomicOr(&note[id[k]], LG_SEEN);
-                    if (i0 + k * LG_T >= prompt) atomicAdd(&note[id[k]], 1u);
-                }
+            for (int k = 0; k < 4; k++) v[k] = i0 + k * LG_T < nh ? (uint32_t)hist[i0 + k * LG_T] : ~0u;
+#pragma unroll
+            for (int k = 0; k < 4; k++) occurs(v[k], i0 + k * LG_T);
         }
         __syncthreads();
     }
@@ -106,8 +128,8 @@ __global__ void __launch_bounds__(LG_T) k_logits(LogitsArgs a) {
     ArgBest best{-1e30f, -1};
     auto noted = [&](float u, uint32_t n) {
         if (n) {
-            u = lg_step(row, u, n >= LG_SEEN, n & (LG_MOST_HIST - 1));
-            const uint32_t entry = (n & ~LG_SEEN) >> LG_ENTRY;
+            u = lg_step(row, u, n & LG_SEEN, n & (LG_SEEN - 1));
+            const uint32_t entry = n >> LG_ENTRY;
             if (entry) u = u + bias[entry - 1];
         }
         return u;
@@ -153,7 +175,7 @@ __global__ void __launch_bounds__(LG_T) k_logits_wide(LogitsArgs a) {
     for (int i = tid; i < nh; i += LG_T) {
         const uint32_t id = (uint32_t)a.hist[(int64_t)b * a.ldh + i] - (uint32_t)v0;
         if (id < (uint32_t)nv) {
-            atomicOr(&note[id], LG_SEEN);
+            atomicOr(&note[id], 1u << 31);
             if (i >= prompt) atomicAdd(&note[id], 1u);
         }
     }
@@ -165,7 +187,7 @@ __global__ void __launch_bounds__(LG_T) k_logits_wide(LogitsArgs a) {
     const LgRow row = lg_row(a, b);
     ArgBest best{-1e30f, -1};
     for (int i = tid; i < nv; i += LG_T) {
-        float t = lg_step(row, a.x[(int64_t)b * a.ldx + v0 + i], note[i] != 0, note[i] & ~LG_SEEN);
+        float t = lg_step(row, a.x[(int64_t)b * a.ldx + v0 + i], note[i] != 0, note[i] & ~(1u << 31));
         if (bias[i]) t = t + a.bias_val[(int64_t)b * a.ldb + bias[i] - 1];
         if (a.allowed && !(a.allowed[(int64_t)b * a.ldm + ((v0 + i) >> 5)] >> ((v0 + i) & 31) & 1u)) t = -INFINITY;
         if (a.y) a.y[(int64_t)b * a.ldy + v0 + i] = t;

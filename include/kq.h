@@ -294,7 +294,7 @@ typedef struct kq_kv {
  * The first `rot` values of a head turn (a, b) -> (a cos - b sin, b cos + a sin), each product and sum
  * rounded to fp32, where a pair is (i, i + rot/2), or (2i, 2i + 1) with `interleaved`; rope holds for each of
  * rope_rows positions rot/2 cosines, then rot/2 sines (rot a multiple of 8; rope NULL: nothing turns).  f16
- * and bf16 round to nearest even; KQ_KV_I8: scale = max|x| / 127, code = x / scale to nearest even.  Inputs must be
+ * and bf16 round to nearest even; KQ_KV_I8: scale = max|x| * fl(1/127), code = x / scale to nearest even.  Inputs must be
  * finite there.  A token whose seq is outside 0..seqs-1, or whose pos is outside the request's positions or the rope
  * table, is skipped: nothing of it is read or written.  Tokens of one call must have different places.  All float
  * pointers 4-byte aligned.

@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(256) k_kv_append(AppendArgs a, int lanes) {
         float m = fmaxf(fmaxf(fabsf(lo.x), fabsf(lo.y)), fmaxf(fabsf(lo.z), fabsf(lo.w)));
         m = fmaxf(m, fmaxf(fmaxf(fabsf(hi.x), fabsf(hi.y)), fmaxf(fabsf(hi.z), fabsf(hi.w))));
         for (int w = lanes >> 1; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
-        scale = m / 127.0f;
+        scale = m * (1.0f / 127.0f);
         if (i == 0)
             (is_v ? a.kv.v_scale : a.kv.k_scale)[page * a.kv.scale_page_stride + kh * a.kv.scale_head_stride +
                                                  off * a.kv.scale_pos_stride] = scale;

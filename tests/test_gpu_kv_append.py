@@ -26,7 +26,7 @@ def turned(x, pos, rope, rot, interleaved, dt):
 def stored(x, dtype):
     """(elements, scales or None) of x [N][heads][D] fp32."""
     if dtype == "i8":
-        scale = np.abs(x).max(-1) / F32(127)
+        scale = np.abs(x).max(-1) * (F32(1) / F32(127))
         return np.where(scale[..., None] > 0, np.rint(x / np.where(scale > 0, scale, 1)[..., None]), 0).astype(np.int8), scale
     t = torch.from_numpy(x).to(kv.DTYPES[dtype])
     return t.view(torch.int16).numpy(), None

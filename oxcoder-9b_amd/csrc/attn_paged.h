@@ -115,7 +115,7 @@ constexpr int at_first(int nd, int s) {           // first value of strip s, in 
     return n;
 }
 
-template <class KV, int ND>
+template <class KV, int ND, int NR>
 struct Attn {
     static constexpr bool I8 = KV::id == KQ_KV_I8;
     static constexpr int D = 16 * ND, EB = I8 ? 1 : 2;
@@ -238,7 +238,7 @@ struct Attn {
     }
 
     template <int S, int AT>
-    __device__ __forceinline__ void pv_strip(const u32x4 (&p)[3], f32x4 (&o)[ND]) const {
+    __device__ __forceinline__ void pv_strip(const u32x4 (&p)[NR][3], f32x4 (&o)[NR][ND]) const {
         if constexpr (S < at_strips(ND)) {
             constexpr int W = at_width(ND, S), F = at_first(ND, S), NW = VRaw<W * EB>::N;
             auto raw = [&](int kk, int d) { return v[kk >> 2][kk & 3][AT + d]; };
@@ -253,7 +253,7 @@ struct Attn {
                         const u32x4 f = {hi_halves(x[0][w & 3], x[1][w & 3]), hi_halves(x[2][w & 3], x[3][w & 3]),
                                          hi_halves(x[4][w & 3], x[5][w & 3]), hi_halves(x[6][w & 3], x[7][w & 3])};
 #pragma unroll
-                        for (int n = 0; n < 3; n++) o[F + w] = mma<KV>(f, p[n], o[F + w]);
+                        for (int n = 0; n < 3 * NR; n++) o[n % NR][F + w] = mma<KV>(f, p[n % NR][n / NR], o[n % NR][F + w]);
                     }
                 }
             } else {
@@ -265,28 +265,34 @@ struct Attn {
                         f[j] = w & 1 ? hi_halves(raw(2 * j, w >> 1), raw(2 * j + 1, w >> 1))
                                      : lo_halves(raw(2 * j, w >> 1), raw(2 * j + 1, w >> 1));
 #pragma unroll
-                    for (int n = 0; n < 3; n++) o[F + w] = mma<KV>(f, p[n], o[F + w]);
+                    for (int n = 0; n < 3 * NR; n++) o[n % NR][F + w] = mma<KV>(f, p[n % NR][n / NR], o[n % NR][F + w]);
                 }
             }
             pv_strip<S + 1, AT + NW>(p, o);
         }
     }
-    // o += V^T E^T of the step; e[t][i] of position 16 t + 4 g + i, 0 where the row does not see it.
-    __device__ __forceinline__ void pv(const Span& w, const float (&e)[2][4], f32x4 (&o)[ND], int u, int g) const {
-        u32x4 p[3];
+    // o += V^T E^T of the step, for NR tiles of rows; e[n][t][i] of position 16 t + 4 g + i, 0 where the row does not see it.
+    __device__ __forceinline__ void pv(const Span& w, const float (&e)[NR][2][4], f32x4 (&o)[NR][ND], int u, int g) const {
+        u32x4 p[NR][3];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int t = j >> 1, i = 2 * (j & 1);
-            float x = e[t][i], y = e[t][i + 1];
-            if constexpr (I8) {                                  // a NaN stays one, a 0 takes no part
+            float sx = 1.0f, sy = 1.0f;
+            if constexpr (I8) {
                 const int at = 32 * u + 16 * t + 4 * g + i;
-                const float sx = fbits(of_lane(at, ubits(w.vs))), sy = fbits(of_lane(at + 1, ubits(w.vs)));
-                x = x == 0.0f ? x : x * sx;
-                y = y == 0.0f ? y : y * sy;
+                sx = fbits(of_lane(at, ubits(w.vs))), sy = fbits(of_lane(at + 1, ubits(w.vs)));
             }
-            uint32_t p0, p1, p2;
-            split2<KV>(x, y, p0, p1, p2);
-            p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
+#pragma unroll
+            for (int n = 0; n < NR; n++) {
+                float x = e[n][t][i], y = e[n][t][i + 1];
+                if constexpr (I8) {                              // a NaN stays one, a 0 takes no part
+                    x = x == 0.0f ? x : x * sx;
+                    y = y == 0.0f ? y : y * sy;
+                }
+                uint32_t p0, p1, p2;
+                split2<KV>(x, y, p0, p1, p2);
+                p[n][0][j] = p0, p[n][1][j] = p1, p[n][2][j] = p2;
+            }
         }
         pv_strip<0, 0>(p, o);
     }
@@ -316,12 +322,13 @@ __device__ __forceinline__ void put_o(float* row, const f32x4 (&o)[ND], float k,
     }
 }
 
-template <class KV, int ND>
-__global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_attn_part(AttnArgs a) {
-    typedef Attn<KV, ND> A;
-    __shared__ u32x4 sq[A::KL][3][64];                          // q's parts [load][part][lane]
+// NR: tiles of 16 rows that a workgroup takes at once.
+template <class KV, int ND, int NR>
+__global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ? 3 : 4) k_attn_part(AttnArgs a) {
+    typedef Attn<KV, ND, NR> A;
+    __shared__ u32x4 sq[NR][A::KL][3][64];                      // q's parts [tile][load][part][lane]
     __shared__ __attribute__((aligned(16))) float so[AT_WAVES][16][A::LD];
-    __shared__ float sm[AT_WAVES][16], sl[AT_WAVES][16], st[16];
+    __shared__ float sm[AT_WAVES][16 * NR], sl[AT_WAVES][16 * NR], st[16 * NR];
     __shared__ int sf[AT_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
@@ -329,7 +336,8 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
     // different lengths load the XCDs alike (chunks side by side: the 48 requests below 8192 positions took 209 us, XCD 0
     // with 1.5 times the chunks of XCD 7)
     int c = blockIdx.z;
-    const int kh = blockIdx.x, b = __builtin_amdgcn_readfirstlane((blockIdx.y + (uint32_t)c) % gridDim.y), stride = gridDim.z;
+    const int group = a.row_groups > 1 ? blockIdx.x / a.kv.heads : 0, kh = blockIdx.x - group * a.kv.heads, r0 = 16 * NR * group;
+    const int b = __builtin_amdgcn_readfirstlane((blockIdx.y + (uint32_t)c) % gridDim.y), stride = gridDim.z;
     // every argument in one go, then the length and the table's entry side by side
     KQ_ARGS_READY("s"(a.kv.k), "s"(a.kv.v), "s"(a.kv.k_scale), "s"(a.kv.v_scale), "s"(a.kv.page_stride), "s"(a.kv.head_stride),
                   "s"(a.kv.pos_stride), "s"(a.table.pages), "s"(a.table.ld), "s"(a.lens), "s"(a.q), "s"(a.ldq));
@@ -348,17 +356,19 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
     typename A::Span w;
     bool ready = false;                                         // the chunk's first step is in flight and q's parts are there
     bool apart = false;                                         // token by token (below)
-    int tok = 0, r0 = 0;
-    float f = 0.0f;
+    int tok = 0;
+    float f[NR];
     for (;;) {
-        const int row = r0 + r, t = row / G;
-        const int see = row < R ? all + t : 0;                  // positions that the lane's row sees
+        int row[NR], t[NR];
+#pragma unroll
+        for (int n = 0; n < NR; n++) row[n] = r0 + 16 * n + r, t[n] = row[n] / G;
         if (!ready) {
             w = s.open(a, page, kh, c * AT_CHUNK + 64 * wave, len, lane);
             // q's parts; each wave cuts a share
-            const float* q = a.q + ((int64_t)b * a.T + (row < R ? t : 0)) * a.ldq + (int64_t)(row < R ? kh * G + row % G : 0) * A::D;
             typedef f32x4 Share[A::QW];
-            auto share = [&](int n, Share& x) {
+            auto share = [&](int tile, int n, Share& x) {
+                const float* q = a.q + ((int64_t)b * a.T + (row[tile] < R ? t[tile] : 0)) * a.ldq +
+                                 (int64_t)(row[tile] < R ? kh * G + row[tile] % G : 0) * A::D;
                 const int d = 16 * A::QW * n + 4 * A::QW * g;
                 const bool ok = A::K_WHOLE || d < A::D;
 #pragma unroll
@@ -367,118 +377,125 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
                     if (!ok) x[j] = f32x4{0, 0, 0, 0};
                 }
             };
-            constexpr int SHARES = (A::KL + AT_WAVES - 1) / AT_WAVES;
-            Share mine[SHARES], whole[KV::id == KQ_KV_BF16 ? 1 : A::KL];
+            constexpr int SHARES = (A::KL + AT_WAVES - 1) / AT_WAVES, WHOLE = KV::id == KQ_KV_BF16 ? 0 : A::KL;
+            Share mine[NR][SHARES], whole[NR][WHOLE ? WHOLE : 1];
 #pragma unroll
-            for (int i = 0; i < SHARES; i++) share(min(AT_WAVES * i + wave, A::KL - 1), mine[i]);
-            if constexpr (KV::id != KQ_KV_BF16)
+            for (int tile = 0; tile < NR; tile++) {
 #pragma unroll
-                for (int n = 0; n < A::KL; n++) share(n, whole[n]);
+                for (int i = 0; i < SHARES; i++) share(tile, min(AT_WAVES * i + wave, A::KL - 1), mine[tile][i]);
+#pragma unroll
+                for (int n = 0; n < WHOLE; n++) share(tile, n, whole[tile][n]);
+            }
             s.load_k(0, r, g);
             s.load_v(0, r, g);
-            float top = 0.0f, bad = 0.0f, up = 1.0f;
-            f = a.scale * 1.44269504088896341f;
-            if constexpr (KV::id != KQ_KV_BF16) {
 #pragma unroll
-                for (int n = 0; n < A::KL; n++)
+            for (int tile = 0; tile < NR; tile++) {
+                float top = 0.0f, bad = 0.0f, up = 1.0f;
+                f[tile] = a.scale * 1.44269504088896341f;
+#pragma unroll
+                for (int n = 0; n < WHOLE; n++)
 #pragma unroll
                     for (int j = 0; j < 4 * A::QW; j++) {
-                        const float x = whole[n][j >> 2][j & 3];
+                        const float x = whole[tile][n][j >> 2][j & 3];
                         top = fmaxf(top, fabsf(x));
                         if constexpr (A::I8) bad = __builtin_fmaf(x, 0.0f, bad);
                     }
-                top = xor32_max(xor16_max(top));
+                if constexpr (WHOLE) top = xor32_max(xor16_max(top));
                 if constexpr (A::I8) bad = xor32_sum(xor16_sum(bad));
-            }
-            if constexpr (KV::id == KQ_KV_F16) {
-                // times a power of two that puts the row's largest near 2^14
-                const uint32_t ex = max(ubits(top) >> 23, 15u);
-                up = fbits(min(268u - ex, 254u) << 23);
-                f *= fbits((ex - 14u) << 23);
-            }
-            if constexpr (A::I8) {
-                up = 8.35e6f / fmaxf(top, 1e-30f);
-                f = f * (fmaxf(top, 1e-30f) / 8.35e6f) + bad;            // bad: NaN for a row with an infinity or NaN
-            }
+                if constexpr (KV::id == KQ_KV_F16) {
+                    // times a power of two that puts the row's largest near 2^14
+                    const uint32_t ex = max(ubits(top) >> 23, 15u);
+                    up = fbits(min(268u - ex, 254u) << 23);
+                    f[tile] *= fbits((ex - 14u) << 23);
+                }
+                if constexpr (A::I8) {
+                    up = 8.35e6f / fmaxf(top, 1e-30f);
+                    f[tile] = f[tile] * (fmaxf(top, 1e-30f) / 8.35e6f) + bad;    // bad: NaN for a row with an infinity or NaN
+                }
 #pragma unroll
-            for (int i = 0; i < SHARES; i++) {
-                const int n = AT_WAVES * i + wave;
-                if (n < A::KL) {
-                    u32x4 p[3];
-                    if constexpr (A::I8) {
+                for (int i = 0; i < SHARES; i++) {
+                    const int n = AT_WAVES * i + wave;
+                    if (n < A::KL) {
+                        u32x4 p[3];
+                        if constexpr (A::I8) {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            uint32_t p0 = 0, p1 = 0, p2 = 0;
+                            for (int j = 0; j < 4; j++) {
+                                uint32_t p0 = 0, p1 = 0, p2 = 0;
 #pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                const int x = (int)rintf(mine[i][j][k] * up), y = (x + 0x80) >> 8, z = (y + 0x80) >> 8;
-                                p0 |= ((uint32_t)z & 0xffu) << (8 * k);      // x = 65536 z + 256 (int8)y + (int8)x
-                                p1 |= ((uint32_t)y & 0xffu) << (8 * k);
-                                p2 |= ((uint32_t)x & 0xffu) << (8 * k);
+                                for (int k = 0; k < 4; k++) {
+                                    const int x = (int)rintf(mine[tile][i][j][k] * up), y = (x + 0x80) >> 8, z = (y + 0x80) >> 8;
+                                    p0 |= ((uint32_t)z & 0xffu) << (8 * k);      // x = 65536 z + 256 (int8)y + (int8)x
+                                    p1 |= ((uint32_t)y & 0xffu) << (8 * k);
+                                    p2 |= ((uint32_t)x & 0xffu) << (8 * k);
+                                }
+                                p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
                             }
-                            p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
-                        }
-                    } else {
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            uint32_t p0, p1, p2;
-                            split2<KV>(mine[i][j >> 1][2 * (j & 1)] * up, mine[i][j >> 1][2 * (j & 1) + 1] * up, p0, p1, p2);
-                            p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
+                            for (int j = 0; j < 4; j++) {
+                                uint32_t p0, p1, p2;
+                                split2<KV>(mine[tile][i][j >> 1][2 * (j & 1)] * up, mine[tile][i][j >> 1][2 * (j & 1) + 1] * up, p0, p1, p2);
+                                p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
+                            }
                         }
+#pragma unroll
+                        for (int j = 0; j < 3; j++) sq[tile][n][j][lane] = p[j];
                     }
-#pragma unroll
-                    for (int j = 0; j < 3; j++) sq[n][j][lane] = p[j];
                 }
             }
             __syncthreads();
         }
-        // The next chunk, if its rows are these: it is whole up to its own, so every wave has both its steps here.
+        // The next chunk: where there is one, every wave has both its steps in this one.
         const int after = c + stride;
-        const bool on = R <= 16 && !apart && (int64_t)after * AT_CHUNK < len;
+        const bool on = !apart && (int64_t)after * AT_CHUNK < len;
         int page_on = -1;
         typename A::Span wn = w;
-        float m = -INFINITY, l = 0.0f;
-        f32x4 o[ND];
+        float m[NR], l[NR];
+        f32x4 o[NR][ND] = {};
 #pragma unroll
-        for (int n = 0; n < ND; n++) o[n] = f32x4{0, 0, 0, 0};
+        for (int n = 0; n < NR; n++) m[n] = -INFINITY, l[n] = 0.0f;
         int found = 0;
 #pragma unroll 1
         for (int u = 0; u < 2; u++) {
             const int base = w.first + 32 * u;
             if (base >= len) break;
-            float e[2][4];
+            float e[NR][2][4];
             if constexpr (A::I8) {
-                i32x4 acc[2][3] = {};
+                i32x4 acc[NR][2][3] = {};
 #pragma unroll
                 for (int n = 0; n < A::KL; n++)
 #pragma unroll
-                    for (int j = 0; j < 3; j++) {
-                        const i32x4 qp = __builtin_bit_cast(i32x4, sq[n][j][lane]);
+                    for (int j = 0; j < 3; j++)
 #pragma unroll
-                        for (int i = 0; i < 2; i++)
-                            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, s.k[i][n]), qp, acc[i][j], 0, 0, 0);
+                        for (int tile = 0; tile < NR; tile++) {
+                            const i32x4 qp = __builtin_bit_cast(i32x4, sq[tile][n][j][lane]);
+#pragma unroll
+                            for (int i = 0; i < 2; i++)
+                                acc[tile][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, s.k[i][n]), qp,
+                                                                                        acc[tile][i][j], 0, 0, 0);
+                        }
+#pragma unroll
+                for (int j = 0; j < 8 * NR; j++) {
+                    const i32x4* x = acc[j >> 3][j >> 2 & 1];
+                    e[j >> 3][j >> 2 & 1][j & 3] =
+                        __builtin_fmaf(__builtin_fmaf((float)x[0][j & 3], 256.0f, (float)x[1][j & 3]), 256.0f, (float)x[2][j & 3]);
+                }
+            } else {
+                f32x4 acc[NR][2] = {};
+#pragma unroll
+                for (int n = 0; n < A::KL; n++)
+#pragma unroll
+                    for (int tile = 0; tile < NR; tile++) {
+                        u32x4 qp[3];
+#pragma unroll
+                        for (int j = 0; j < 3; j++) qp[j] = sq[tile][n][j][lane];
+#pragma unroll
+                        for (int j = 2; j >= 0; j--)
+#pragma unroll
+                            for (int i = 0; i < 2; i++) acc[tile][i] = mma<KV>(s.k[i][n], qp[j], acc[tile][i]);
                     }
 #pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        e[i][j] = __builtin_fmaf(__builtin_fmaf((float)acc[i][0][j], 256.0f, (float)acc[i][1][j]), 256.0f, (float)acc[i][2][j]);
-            } else {
-                f32x4 acc[2] = {};
-#pragma unroll
-                for (int n = 0; n < A::KL; n++) {
-                    u32x4 qp[3];
-#pragma unroll
-                    for (int j = 0; j < 3; j++) qp[j] = sq[n][j][lane];
-#pragma unroll
-                    for (int j = 2; j >= 0; j--)
-#pragma unroll
-                        for (int i = 0; i < 2; i++) acc[i] = mma<KV>(s.k[i][n], qp[j], acc[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) e[i][j] = acc[i][j];
+                for (int j = 0; j < 8 * NR; j++) e[j >> 3][j >> 2 & 1][j & 3] = acc[j >> 3][j >> 2 & 1][j & 3];
             }
             // What the next step reads is fetched whether there is one or not (no place that is not there is read, all lanes
             // take the pool's first): the waits below then know how many loads are younger than theirs.
@@ -487,22 +504,25 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
             page_on = entry(after * AT_CHUNK + 64 * wave);
             if constexpr (A::I8) asm volatile("" : "+v"(w.ks), "+v"(w.vs));   // as here()
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int j = 0; j < 8; j++) {
+                float ks = 1.0f;
+                if constexpr (A::I8) ks = fbits(of_lane(32 * u + 16 * (j >> 2) + 4 * g + (j & 3), ubits(w.ks)));
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if constexpr (A::I8) e[i][j] *= fbits(of_lane(32 * u + 16 * i + 4 * g + j, ubits(w.ks)));
-                    e[i][j] *= f;
+                for (int n = 0; n < NR; n++) {
+                    if constexpr (A::I8) e[n][j >> 2][j & 3] *= ks;
+                    e[n][j >> 2][j & 3] *= f[n];
                 }
-            float top = -INFINITY;
+            }
             // some row does not see some position
             const bool partly = (uint32_t)(w.there >> (32 * u)) != ~0u || base + 32 > all;
             if (partly) {
-                const uint32_t hid = A::hidden(w, u, see, g);
 #pragma unroll
-                for (int i = 0; i < 2; i++)
+                for (int n = 0; n < NR; n++) {
+                    const uint32_t hid = A::hidden(w, u, row[n] < R ? all + t[n] : 0, g);
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (hid >> (4 * i + j) & 1u) e[i][j] = -INFINITY;
+                    for (int j = 0; j < 8; j++)
+                        if (hid >> j & 1u) e[n][j >> 2][j & 3] = -INFINITY;
+                }
                 // An infinity or NaN that only some tokens see would reach the others as 0 * inf: then the rows are done
                 // again, token by token, with the values that it does not see cleared.
                 const uint32_t gone = A::hidden(w, u, apart ? all + tok : len, g);
@@ -510,35 +530,39 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
                 s.clear_v(gone);
             }
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int n = 0; n < NR; n++) {
+                float top = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 4; j++) top = fmaxf(top, e[i][j]);
-            top = fmaxf(m, xor32_max(xor16_max(top)));
-            const float keep = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
-            if (!__all(keep == 1.0f)) {
-                l *= keep;
+                for (int j = 0; j < 8; j++) top = fmaxf(top, e[n][j >> 2][j & 3]);
+                top = fmaxf(m[n], xor32_max(xor16_max(top)));
+                const float keep = m[n] == top ? 1.0f : __builtin_amdgcn_exp2f(m[n] - top);
+                if (!__all(keep == 1.0f)) {
+                    l[n] *= keep;
 #pragma unroll
-                for (int n = 0; n < ND; n++) o[n] *= keep;
-            }
-            m = top;
-            const float from = (m == -INFINITY ? 0.0f : m) - A::BIAS;
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    e[i][j] = __builtin_amdgcn_exp2f(e[i][j] - from);
-                    l += e[i][j];
+                    for (int d = 0; d < ND; d++) o[n][d] *= keep;
                 }
+                m[n] = top;
+                const float from = (top == -INFINITY ? 0.0f : top) - A::BIAS;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float x = __builtin_amdgcn_exp2f(e[n][j >> 2][j & 3] - from);
+                    e[n][j >> 2][j & 3] = x;
+                    l[n] += x;
+                }
+            }
             s.pv(w, e, o, u, g);
             s.load_v(1 - u, r, g);
         }
         // The waves' sums, joined: each scaled to the workgroup's maximum, then added.  (From here on the thread's place is
         // taken anew, so that no address is held through the steps.)
-        l = xor32_sum(xor16_sum(l));
         int me = tid;
         asm volatile("" : "+v"(me));
         const int r = me & 15, g = me >> 4 & 3;
-        if (g == 0) sm[wave][r] = m, sl[wave][r] = l;
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            l[n] = xor32_sum(xor16_sum(l[n]));
+            if (g == 0) sm[wave][16 * n + r] = m[n], sl[wave][16 * n + r] = l[n];
+        }
         if (g == 0 && r == 0) sf[wave] = found;
         __syncthreads();
         if (a.T > 1 && !apart && (sf[0] | sf[1] | sf[2] | sf[3])) {
@@ -549,63 +573,63 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
             __syncthreads();
             continue;
         }
-        const float top = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
-        if (wave == 0 && g == 0) {
-            float total = 0.0f;
+        const int64_t part0 = (((int64_t)b * a.kv.heads + kh) * R + r0) * a.chunks + c;      // part of the group's first row
 #pragma unroll
-            for (int i = 0; i < AT_WAVES; i++) {
-                const float li = sl[i][r];                      // 0: the wave saw nothing (a NaN counts)
-                total += li != 0.0f ? li * __builtin_amdgcn_exp2f(sm[i][r] - top) : 0.0f;
+        for (int n = 0; n < NR; n++) {
+            const int at = 16 * n + r;
+            const float top = fmaxf(fmaxf(sm[0][at], sm[1][at]), fmaxf(sm[2][at], sm[3][at]));
+            if (wave == 0 && g == 0) {
+                float total = 0.0f;
+#pragma unroll
+                for (int i = 0; i < AT_WAVES; i++) {
+                    const float li = sl[i][at];                 // 0: the wave saw nothing (a NaN counts)
+                    total += li != 0.0f ? li * __builtin_amdgcn_exp2f(sm[i][at] - top) : 0.0f;
+                }
+                st[at] = total;
+                if (a.joined && row[n] < R && (!apart || t[n] == tok)) a.pml[part0 + (int64_t)at * a.chunks] = AttnMl{top, total};
             }
-            st[r] = total;
-            if (a.joined && row < R && (!apart || t == tok))
-                a.pml[(((int64_t)b * a.kv.heads + kh) * R + row) * a.chunks + c] = AttnMl{top, total};
+            const float k = l[n] != 0.0f ? __builtin_amdgcn_exp2f(m[n] - top) : 0.0f;
+            auto round = [&](auto from, auto to) {
+                constexpr int FROM = decltype(from)::value, TO = decltype(to)::value, Q = 4 * (TO - FROM);
+                if (FROM || n) __syncthreads();                 // the round before has left LDS
+                if (row[n] < R) {
+                    if (l[n] != 0.0f) {
+                        put_o<ND, FROM, TO>(so[wave][r], o[n], k, g);
+                    } else {
+#pragma unroll
+                        for (int i = g; i < Q; i += 4) *reinterpret_cast<f32x4*>(&so[wave][r][4 * i]) = f32x4{0, 0, 0, 0};
+                    }
+                }
+                __syncthreads();
+                for (int i = me; i < min(16, R - r0 - 16 * n) * Q; i += 64 * AT_WAVES) {
+                    const int rr = i / Q, d = 4 * (i % Q);
+                    auto of = [&](int w) { return *reinterpret_cast<const f32x4*>(&so[w][rr][d]); };
+                    const f32x4 sum = (of(0) + of(1)) + (of(2) + of(3));
+                    float* const part = a.po + (part0 + (int64_t)(16 * n + rr) * a.chunks) * A::D + 16 * FROM + d;
+                    if (a.joined && !apart) {
+                        *reinterpret_cast<f32x4*>(part) = sum;
+                        continue;
+                    }
+                    const int tt = (r0 + 16 * n + rr) / G, hh = kh * G + (r0 + 16 * n + rr) % G;
+                    if (apart && tt != tok) continue;
+                    const float total = st[16 * n + rr];
+                    if (a.joined)
+                        *reinterpret_cast<f32x4*>(part) = sum;
+                    else
+                        *reinterpret_cast<f32x4_a4*>(a.out + ((int64_t)b * a.T + tt) * a.ldo + (int64_t)hh * A::D + 16 * FROM + d) =
+                            total == 0.0f ? f32x4{0, 0, 0, 0} : sum / total;
+                }
+            };
+            round(std::integral_constant<int, 0>(), std::integral_constant<int, (ND < 8 ? ND : 8)>());
+            if constexpr (ND > 8) round(std::integral_constant<int, 8>(), std::integral_constant<int, ND>());
         }
-        const float k = l != 0.0f ? __builtin_amdgcn_exp2f(m - top) : 0.0f;
-        auto round = [&](auto from, auto to) {
-            constexpr int FROM = decltype(from)::value, TO = decltype(to)::value, Q = 4 * (TO - FROM);
-            if (FROM) __syncthreads();                          // the round before has left LDS
-            if (row < R) {
-                if (l != 0.0f) {
-                    put_o<ND, FROM, TO>(so[wave][r], o, k, g);
-                } else {
-#pragma unroll
-                    for (int i = g; i < Q; i += 4) *reinterpret_cast<f32x4*>(&so[wave][r][4 * i]) = f32x4{0, 0, 0, 0};
-                }
-            }
-            __syncthreads();
-            for (int i = me; i < min(16, R - r0) * Q; i += 64 * AT_WAVES) {
-                const int rr = i / Q, d = 4 * (i % Q);
-                auto part = [&](int n) { return *reinterpret_cast<const f32x4*>(&so[n][rr][d]); };
-                const f32x4 sum = (part(0) + part(1)) + (part(2) + part(3));
-                if (a.joined && !apart) {
-                    *reinterpret_cast<f32x4*>(a.po + ((((int64_t)b * a.kv.heads + kh) * R + r0 + rr) * a.chunks + c) * A::D +
-                                              16 * FROM + d) = sum;
-                    continue;
-                }
-                const int tt = (r0 + rr) / G, hh = kh * G + (r0 + rr) % G;
-                if (apart && tt != tok) continue;
-                if (a.joined)
-                    *reinterpret_cast<f32x4*>(a.po + ((((int64_t)b * a.kv.heads + kh) * R + r0 + rr) * a.chunks + c) * A::D +
-                                              16 * FROM + d) = sum;
-                else
-                    *reinterpret_cast<f32x4_a4*>(a.out + ((int64_t)b * a.T + tt) * a.ldo + (int64_t)hh * A::D + 16 * FROM + d) =
-                        st[rr] == 0.0f ? f32x4{0, 0, 0, 0} : sum / st[rr];
-            }
-        };
-        round(std::integral_constant<int, 0>(), std::integral_constant<int, (ND < 8 ? ND : 8)>());
-        if constexpr (ND > 8) round(std::integral_constant<int, 8>(), std::integral_constant<int, ND>());
-        // what comes next: this chunk's next token or rows, or the next chunk
+        // what comes next: this chunk's next token, or the next chunk
         ready = on;
         w = wn;
         if (apart && tok > 0) {
             tok--;
-        } else if (r0 + 16 < R) {
-            r0 += 16;
-            tok = a.T - 1;
         } else {
             c = after;
-            r0 = 0;
             apart = false;
             if ((int64_t)c * AT_CHUNK >= len) return;
         }
@@ -616,9 +640,19 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 ? 2 : ND > 4 ? 3 : 4) k_
     }
 }
 
+template <class KV, int ND, int NR>
+void launch_attn_part_nr(const AttnArgs& args, hipStream_t s) {
+    AttnArgs a = args;
+    const int R = a.T * a.group;
+    a.row_groups = (R + 16 * NR - 1) / (16 * NR);
+    hipLaunchKernelGGL((k_attn_part<KV, ND, NR>), dim3(a.kv.heads * a.row_groups, a.table.seqs, a.groups), dim3(64 * AT_WAVES), 0, s, a);
+}
+
 template <class KV, int ND>
 void launch_attn_part_nd(const AttnArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((k_attn_part<KV, ND>), dim3(a.kv.heads, a.table.seqs, a.groups), dim3(64 * AT_WAVES), 0, s, a);
+    if constexpr (ND <= 8)
+        if (a.T * a.group > 16) return launch_attn_part_nr<KV, ND, 2>(a, s);
+    launch_attn_part_nr<KV, ND, 1>(a, s);
 }
 
 template <class KV>

@@ -143,6 +143,7 @@ struct AttnArgs {
     // set by launch_attn_paged
     int group, page_shift, chunks, joined;     // group: query heads of a key-value head; joined: parts go to po and pml [request][key-value head][token, query head][chunk]
     int groups;                         // workgroups that share a request and head's chunks
+    int row_groups;                     // workgroups that share a chunk, each for its rows
     float* po;
     AttnMl* pml;
 };

@@ -359,9 +359,11 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
     int tok = 0;
     float f[NR];
     for (;;) {
-        int row[NR], t[NR];
+        // (Taken anew for each chunk, as the thread's place below: what queries' addresses come from is not held.)
+        int row[NR], t[NR], lane_row = r0 + r;
+        asm volatile("" : "+v"(lane_row));
 #pragma unroll
-        for (int n = 0; n < NR; n++) row[n] = r0 + 16 * n + r, t[n] = row[n] / G;
+        for (int n = 0; n < NR; n++) row[n] = lane_row + 16 * n, t[n] = row[n] / G;
         if (!ready) {
             w = s.open(a, page, kh, c * AT_CHUNK + 64 * wave, len, lane);
             // q's parts; each wave cuts a share

@@ -6,6 +6,11 @@
 // slice, how often it occurs after the prompt, whether it occurs at all and its last bias entry (integer atomics: any
 // order gives the same).  Then every thread steps its logits and keeps the best.  The pick folds into one key per row, as
 // argmax_block.h does for a single row.
+//
+// 128 rows of 248320 with histories of 4000, 20 biases and a mask: 260 MB in 55 us, 4.7 TB/s, a large copy's rate.  Listing the noted ids
+// and stepping them packed, ahead of the pass, took 79 us: it read their logits a second time, one round trip later.
+// 32 rows of 151936: 12 us (39 MB), 608 workgroups on 256 CUs and one scan's latency; halving the slices scans more (15 us).
+// One row: 5.5 us, the launch and the chain of list, barrier, logits and the pick's two atomics.
 #include "argmax_block.h"
 #include "kq_internal.h"
 

@@ -317,3 +317,21 @@ def test_refusals_on_the_device(dev):
     assert torch.equal(cache.k, before)
     att.append(0, q, new, new, seq, pos)
     assert not torch.equal(cache.k, before)
+
+
+@pytest.mark.parametrize("dtype,D,q_heads", [("bf16", 64, 4), ("f16", 128, 8), ("f16", 256, 4), ("bf16", 240, 6)])
+@pytest.mark.parametrize("n", [3, 40, 258, 515])
+def test_infinities_that_some_tokens_see(dev, dtype, D, q_heads, n):
+    """Drafted tokens that bring infinities and NaN: each row is what it is alone, at its own length."""
+    T, heads, lens = 5, 2, [n, 700]
+    cache, table, q = setup(dev, dtype, D, q_heads, heads, 16, lens, T, seed=n)
+    page, off = (table[0, (n - 1) // 16], (n - 1) % 16), (table[0, max(n - 3, 0) // 16], max(n - 3, 0) % 16)
+    cache.v[page[0], 1, page[1], 7] = float("inf")
+    cache.v[off[0], 0, off[1], D - 1] = float("nan")
+    cache.k[off[0], 1, off[1], 0] = float("-inf")
+    rows = attend(dev, cache, table, q, lens, T, q_heads).view(2, T, -1)
+    qs = q.view(2, T, -1)
+    for t in range(T):
+        alone = attend(dev, cache, table, qs[:, t].contiguous(), [m - T + 1 + t for m in lens], 1, q_heads)
+        torch.testing.assert_close(rows[:, t], alone, rtol=0, atol=0, equal_nan=True)
+    assert torch.isfinite(rows[1]).all() and not torch.isfinite(rows[0, -1]).all()

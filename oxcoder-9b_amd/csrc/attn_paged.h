@@ -130,7 +130,7 @@ struct Attn {
     static constexpr int KL = I8 ? (ND + 3) / 4 : (ND + 1) / 2;  // 16-byte loads of a key by its 4 lanes
     static constexpr int QW = I8 ? 4 : 2;                        // a lane's share of q for a load, in fours
     static constexpr bool K_WHOLE = I8 ? ND % 4 == 0 : ND % 2 == 0;
-    static constexpr int WIDE = D > 128 ? 128 : D, LD = WIDE + 4; // values of a round of the waves' join, row stride in LDS
+    static constexpr int WIDE = D > 128 ? 128 : D, LD = WIDE == 128 ? 128 : WIDE + 4; // values of a round of the waves' join, row stride in LDS
     static constexpr float BIAS = KV::id == KQ_KV_F16 ? 14.0f : 0.0f;   // f16: e is held times 2^14, clear of subnormals
     static constexpr int VW = [] { int n = 0; for (int s = 0; s < at_strips(ND); s++) n += (at_width(ND, s) * EB + 3) / 4; return n; }();
 
@@ -306,27 +306,44 @@ struct Attn {
     }
 };
 
-// o's values in [16 FROM, 16 TO), times k, into a row of LDS; S: the strip.
+// Where value d of row r lies in its row of LDS: rows of 128 have no gap between them, and fours change places instead.
+template <int ND>
+__device__ __forceinline__ int in_row(int r, int d) { return ND < 8 ? d : d ^ (r & 7) << 2; }
+
+// The scales that bring two parts to their common maximum.
+struct AtPair {
+    float top, k0, k1, l;
+};
+__device__ __forceinline__ AtPair at_pair(AttnMl a, AttnMl b) {
+    AtPair p;
+    p.top = fmaxf(a.m, b.m);
+    p.k0 = a.l != 0.0f ? __builtin_amdgcn_exp2f(a.m - p.top) : 0.0f;         // 0: the row saw nothing (a NaN counts)
+    p.k1 = b.l != 0.0f ? __builtin_amdgcn_exp2f(b.m - p.top) : 0.0f;
+    p.l = a.l * p.k0 + b.l * p.k1;
+    return p;
+}
+
+// o's values in [16 FROM, 16 TO), times k, into row r of LDS; S: the strip.
 template <int ND, int FROM, int TO, int S = 0>
-__device__ __forceinline__ void put_o(float* row, const f32x4 (&o)[ND], float k, int g) {
+__device__ __forceinline__ void put_o(float* row, const f32x4 (&o)[ND], float k, int r, int g) {
     if constexpr (S < at_strips(ND)) {
         constexpr int W = at_width(ND, S), F = at_first(ND, S);
         if constexpr (F >= FROM && F < TO) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                float* to = row + 16 * (F - FROM) + (4 * g + i) * W;
+                const int d = 16 * (F - FROM) + (4 * g + i) * W;
                 if constexpr (W >= 4) {
 #pragma unroll
                     for (int w = 0; w < W; w += 4)
-                        *reinterpret_cast<f32x4*>(to + w) =
+                        *reinterpret_cast<f32x4*>(row + in_row<ND>(r, d + w)) =
                             f32x4{o[F + w][i], o[F + w + 1][i], o[F + w + 2][i], o[F + w + 3][i]} * k;
                 } else {
 #pragma unroll
-                    for (int w = 0; w < W; w++) to[w] = o[F + w][i] * k;
+                    for (int w = 0; w < W; w++) row[in_row<ND>(r, d + w)] = o[F + w][i] * k;
                 }
             }
         }
-        put_o<ND, FROM, TO, S + 1>(row, o, k, g);
+        put_o<ND, FROM, TO, S + 1>(row, o, k, r, g);
     }
 }
 
@@ -335,17 +352,26 @@ template <class KV, int ND, int NR>
 __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ? 3 : 4) k_attn_part(AttnArgs a) {
     typedef Attn<KV, ND, NR> A;
     __shared__ u32x4 sq[NR][A::KL][3][64];                      // q's parts [tile][load][part][lane]
-    __shared__ __attribute__((aligned(16))) float so[AT_WAVES][16][A::LD];
     __shared__ float sm[AT_WAVES][16 * NR], sl[AT_WAVES][16 * NR], st[16 * NR];
+    // the first chunk of a pair: its m and l; the pair's scales
+    __shared__ AttnMl held_ml[16 * NR];
+    __shared__ float k0[16 * NR], k1[16 * NR];
     __shared__ int sf[AT_WAVES];
+    // the waves' sums of up to 16 rows [wave][row][LD], then the first chunk's of a pair [tile][round][row, value], which only
+    // the thread that put them there reads (as many rows as there are, so that three workgroups fit a CU)
+    extern __shared__ __attribute__((aligned(16))) float sums[];
+    constexpr int ROUNDS = ND > 8 ? 2 : 1;
+    const int live = min(16, a.T * a.group);
+    auto so = [&](int w, int row) { return sums + (w * live + row) * A::LD; };
+    f32x4* const held = reinterpret_cast<f32x4*>(sums + AT_WAVES * live * A::LD);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
     // Workgroups go to the XCDs in turn: neighbours are heads, then requests, turned by the chunk, so that requests of
     // different lengths load the XCDs alike (chunks side by side: the 48 requests below 8192 positions took 209 us, XCD 0
     // with 1.5 times the chunks of XCD 7)
-    int c = blockIdx.z;
+    int c = a.paired ? 2 * blockIdx.z : blockIdx.z;
     const int group = a.row_groups > 1 ? blockIdx.x / a.kv.heads : 0, kh = blockIdx.x - group * a.kv.heads, r0 = 16 * NR * group;
-    const int b = __builtin_amdgcn_readfirstlane((blockIdx.y + (uint32_t)c) % gridDim.y), stride = gridDim.z;
+    const int b = __builtin_amdgcn_readfirstlane((blockIdx.y + blockIdx.z) % gridDim.y), stride = gridDim.z;
     // every argument in one go, then the length and the table's entry side by side
     KQ_ARGS_READY("s"(a.kv.k), "s"(a.kv.v), "s"(a.kv.k_scale), "s"(a.kv.v_scale), "s"(a.kv.page_stride), "s"(a.kv.head_stride),
                   "s"(a.kv.pos_stride), "s"(a.table.pages), "s"(a.table.ld), "s"(a.lens), "s"(a.q), "s"(a.ldq));
@@ -456,7 +482,8 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
             __syncthreads();
         }
         // The next chunk: where there is one, every wave has both its steps in this one.
-        const int after = c + stride;
+        const bool first_of_two = a.paired && !(c & 1) && (int64_t)(c + 1) * AT_CHUNK < len;
+        const int after = first_of_two ? c + 1 : a.paired ? (c & ~1) + 2 * stride : c + stride;
         const bool on = !apart && (int64_t)after * AT_CHUNK < len;
         int page_on = -1;
         typename A::Span wn = w;
@@ -583,7 +610,9 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
             __syncthreads();
             continue;
         }
-        const int64_t part0 = (((int64_t)b * a.kv.heads + kh) * R + r0) * a.chunks + c;      // part of the group's first row
+        // part of the group's first row
+        const int64_t part0 = (((int64_t)b * a.kv.heads + kh) * R + r0) * a.parts + (a.paired ? c >> 1 : c);
+        const bool second_of_two = a.paired && (c & 1);
 #pragma unroll
         for (int n = 0; n < NR; n++) {
             const int at = 16 * n + r;
@@ -596,7 +625,16 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
                     total += li != 0.0f ? li * __builtin_amdgcn_exp2f(sm[i][at] - top) : 0.0f;
                 }
                 st[at] = total;
-                if (a.joined && row[n] < R && (!apart || t[n] == tok)) a.pml[part0 + (int64_t)at * a.chunks] = AttnMl{top, total};
+                if (a.joined && row[n] < R && (!apart || t[n] == tok)) {
+                    AttnMl ml{top, total};
+                    if (second_of_two) {
+                        const AtPair p = at_pair(held_ml[at], ml);
+                        k0[at] = p.k0, k1[at] = p.k1;
+                        ml = AttnMl{p.top, p.l};
+                    }
+                    if (first_of_two) held_ml[at] = ml;
+                    else a.pml[part0 + (int64_t)at * a.parts] = ml;
+                }
             }
             const float k = l[n] != 0.0f ? __builtin_amdgcn_exp2f(m[n] - top) : 0.0f;
             auto round = [&](auto from, auto to) {
@@ -604,30 +642,32 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
                 if (FROM || n) __syncthreads();                 // the round before has left LDS
                 if (row[n] < R) {
                     if (l[n] != 0.0f) {
-                        put_o<ND, FROM, TO>(so[wave][r], o[n], k, g);
+                        put_o<ND, FROM, TO>(so(wave, r), o[n], k, r, g);
                     } else {
 #pragma unroll
-                        for (int i = g; i < Q; i += 4) *reinterpret_cast<f32x4*>(&so[wave][r][4 * i]) = f32x4{0, 0, 0, 0};
+                        for (int i = g; i < Q; i += 4) *reinterpret_cast<f32x4*>(so(wave, r) + in_row<ND>(r, 4 * i)) = f32x4{0, 0, 0, 0};
                     }
                 }
                 __syncthreads();
                 for (int i = me; i < min(16, R - r0 - 16 * n) * Q; i += 64 * AT_WAVES) {
                     const int rr = i / Q, d = 4 * (i % Q);
-                    auto of = [&](int w) { return *reinterpret_cast<const f32x4*>(&so[w][rr][d]); };
-                    const f32x4 sum = (of(0) + of(1)) + (of(2) + of(3));
-                    float* const part = a.po + (part0 + (int64_t)(16 * n + rr) * a.chunks) * A::D + 16 * FROM + d;
-                    if (a.joined && !apart) {
-                        *reinterpret_cast<f32x4*>(part) = sum;
+                    auto of = [&](int w) { return *reinterpret_cast<const f32x4*>(so(w, rr) + in_row<ND>(rr, d)); };
+                    f32x4 sum = (of(0) + of(1)) + (of(2) + of(3));
+                    if (apart && (r0 + 16 * n + rr) / G != tok) continue;
+                    if (a.joined) {
+                        f32x4& first = held[(n * ROUNDS + FROM / 8) * 32 * live + i];
+                        if (first_of_two) {
+                            first = sum;
+                            continue;
+                        }
+                        if (second_of_two) sum = first * k0[16 * n + rr] + sum * k1[16 * n + rr];
+                        *reinterpret_cast<f32x4*>(a.po + (part0 + (int64_t)(16 * n + rr) * a.parts) * A::D + 16 * FROM + d) = sum;
                         continue;
                     }
                     const int tt = (r0 + 16 * n + rr) / G, hh = kh * G + (r0 + 16 * n + rr) % G;
-                    if (apart && tt != tok) continue;
                     const float total = st[16 * n + rr];
-                    if (a.joined)
-                        *reinterpret_cast<f32x4*>(part) = sum;
-                    else
-                        *reinterpret_cast<f32x4_a4*>(a.out + ((int64_t)b * a.T + tt) * a.ldo + (int64_t)hh * A::D + 16 * FROM + d) =
-                            total == 0.0f ? f32x4{0, 0, 0, 0} : sum / total;
+                    *reinterpret_cast<f32x4_a4*>(a.out + ((int64_t)b * a.T + tt) * a.ldo + (int64_t)hh * A::D + 16 * FROM + d) =
+                        total == 0.0f ? f32x4{0, 0, 0, 0} : sum / total;
                 }
             };
             round(std::integral_constant<int, 0>(), std::integral_constant<int, (ND < 8 ? ND : 8)>());
@@ -655,7 +695,9 @@ void launch_attn_part_nr(const AttnArgs& args, hipStream_t s) {
     AttnArgs a = args;
     const int R = a.T * a.group;
     a.row_groups = (R + 16 * NR - 1) / (16 * NR);
-    hipLaunchKernelGGL((k_attn_part<KV, ND, NR>), dim3(a.kv.heads * a.row_groups, a.table.seqs, a.groups), dim3(64 * AT_WAVES), 0, s, a);
+    const int live = R < 16 ? R : 16, held = a.paired ? NR * (ND > 8 ? 2 : 1) * 512 : 0;
+    const size_t lds = (size_t)live * (AT_WAVES * Attn<KV, ND, NR>::LD * 4 + held);
+    hipLaunchKernelGGL((k_attn_part<KV, ND, NR>), dim3(a.kv.heads * a.row_groups, a.table.seqs, a.groups), dim3(64 * AT_WAVES), lds, s, a);
 }
 
 template <class KV, int ND>

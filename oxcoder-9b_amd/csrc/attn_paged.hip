@@ -6,34 +6,59 @@
 
 namespace kq {
 
-// One workgroup per row and 32 N of its values: 32 groups of 8 lanes take every 32nd chunk, then the groups are added as
-// a tree: a row's result depends on its number of chunks alone.
+// One workgroup per row and 32 N of its values: 32 groups of 8 lanes take every 32nd pair of chunks, in the steps of
+// the workgroup that had both where there was one; then the groups are added as a tree: a row's result depends on its
+// number of chunks alone.
 template <int N>
 __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 so[4][N][8];
     __shared__ float sl[4], sm[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, D = a.kv.dim;
     const int b = blockIdx.x / a.T, h = blockIdx.y, G = a.group, d = 32 * N * blockIdx.z + 4 * (tid & 7);
-    const int len = min(a.lens[b], a.max_len), n = len <= 0 ? 0 : (len + AT_CHUNK - 1) / AT_CHUNK;
-    const int64_t row = (((int64_t)b * a.kv.heads + h / G) * a.T * G + blockIdx.x % a.T * G + h % G) * a.chunks;
+    const int len = min(a.lens[b], a.max_len), n = len <= 0 ? 0 : (len + AT_CHUNK - 1) / AT_CHUNK, pairs = (n + 1) / 2;
+    const int64_t row = (((int64_t)b * a.kv.heads + h / G) * a.T * G + blockIdx.x % a.T * G + h % G) * a.parts;
     float top = -INFINITY;
-    for (int c = tid; c < n; c += 256) top = fmaxf(top, a.pml[row + c].m);
+    for (int c = tid; c < (a.paired ? pairs : n); c += 256) top = fmaxf(top, a.pml[row + c].m);
     for (int w = 32; w; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
     if (lane == 0) sm[wave] = top;
     __syncthreads();
     top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
     f32x4 sum[N] = {};
     float total = 0.0f;
-#pragma unroll 8 / N
-    for (int c = tid >> 3; c < n; c += 32) {
-        const AttnMl ml = a.pml[row + c];
-        f32x4 x[N];
+    auto load = [&](int64_t part, f32x4 (&x)[N]) {
 #pragma unroll
-        for (int i = 0; i < N; i++) x[i] = *reinterpret_cast<const f32x4*>(a.po + (row + c) * D + (d + 32 * i < D ? d + 32 * i : 0));
+        for (int i = 0; i < N; i++) x[i] = *reinterpret_cast<const f32x4*>(a.po + part * D + (d + 32 * i < D ? d + 32 * i : 0));
+    };
+    auto add = [&](AttnMl ml, const f32x4 (&x)[N]) {
         const float k = ml.l != 0.0f ? __builtin_amdgcn_exp2f(ml.m - top) : 0.0f;   // 0: the row saw nothing (a NaN counts)
 #pragma unroll
         for (int i = 0; i < N; i++) sum[i] += x[i] * k;
         total += ml.l * k;
+    };
+    if (a.paired) {
+#pragma unroll 8 / N
+        for (int c = tid >> 3; c < pairs; c += 32) {
+            f32x4 x[N];
+            load(row + c, x);
+            add(a.pml[row + c], x);
+        }
+    } else {
+#pragma unroll 4 / N
+        for (int c = tid >> 3; c < pairs; c += 32) {
+            const int64_t p0 = row + 2 * c, p1 = 2 * c + 1 < n ? p0 + 1 : p0;
+            const AttnMl m0 = a.pml[p0];
+            AttnMl m1 = a.pml[p1];
+            f32x4 x[N], y[N];
+            load(p0, x);
+            load(p1, y);
+            if (p1 != p0) {
+                const AtPair p = at_pair(m0, m1);
+#pragma unroll
+                for (int i = 0; i < N; i++) x[i] = x[i] * p.k0 + y[i] * p.k1;
+                m1 = AttnMl{p.top, p.l};
+            }
+            add(m1, x);
+        }
     }
 #pragma unroll
     for (int w = 8; w < 64; w <<= 1) {
@@ -68,14 +93,16 @@ void launch_attn_paged(const AttnArgs& args, hipStream_t s) {
     a.page_shift = __builtin_ctz((unsigned)a.kv.page_size);
     a.chunks = chunks_of(a.max_len);
     a.joined = a.chunks > 1;
-    // A workgroup takes up to three chunks, the next one's first step in flight while it ends one, if that leaves eight
-    // workgroups a CU (32 requests of 16384 8-bit positions: 159, 151, 146, 147 us with one to four; one request of 100001:
-    // 87, 87, 89, 93 us; 8 requests of 5003: 34, 46, 41 us).
-    int64_t per = (int64_t)a.chunks * a.kv.heads * a.table.seqs / (8 * device_cus());
-    per = per < 1 ? 1 : per > 3 ? 3 : per;
-    a.groups = (int)((a.chunks + per - 1) / per);
+    // Where that leaves six workgroups a CU, a workgroup takes two chunks, the second's first step in flight while it ends the first, and
+    // leaves one part for both; four chunks where that leaves sixteen.  One, two, four chunks: 48 requests below 8192
+    // positions 169, 154, 160 us, one request of 100001 86, 82, 88, 32 requests of 16384 8-bit positions 161, 145, 143, 51 requests
+    // of 16 tokens 277, 254, 248; but 8 requests of 5003, 640 chunks in all, 32, 45, 48.
+    const int64_t all = (int64_t)a.chunks * a.kv.heads * a.table.seqs * ((a.T * a.group + 15) / 16), cus = device_cus();
+    a.paired = a.joined && all >= 12 * cus;
+    a.parts = a.paired ? (a.chunks + 1) / 2 : a.chunks;
+    a.groups = all >= 64 * cus ? (a.parts + 1) / 2 : a.parts;
     if (a.groups > 65535) a.groups = 65535;                    // a workgroup goes on until no chunk is left
-    const size_t parts = (size_t)a.table.seqs * a.T * a.q_heads * a.chunks;
+    const size_t parts = (size_t)a.table.seqs * a.T * a.q_heads * a.parts;
     a.po = reinterpret_cast<float*>(a.ws);
     a.pml = reinterpret_cast<AttnMl*>(a.ws + up256(parts * a.kv.dim * 4));
     if (a.kv.type == KQ_KV_F16) launch_attn_part<KvF16>(a, s);

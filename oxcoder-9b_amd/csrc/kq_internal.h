@@ -141,8 +141,9 @@ struct AttnArgs {
     float* out;
     uint8_t* ws;
     // set by launch_attn_paged
-    int group, page_shift, chunks, joined;     // group: query heads of a key-value head; joined: parts go to po and pml [request][key-value head][token, query head][chunk]
+    int group, page_shift, chunks, joined;     // group: query heads of a key-value head; joined: parts go to po and pml [request][key-value head][token, query head][part]
     int groups;                         // workgroups that share a request and head's chunks
+    int paired, parts;                  // paired: a part is two chunks, joined where both are; parts: chunks or pairs of a row
     int row_groups;                     // workgroups that share a chunk, each for its rows
     float* po;
     AttnMl* pml;

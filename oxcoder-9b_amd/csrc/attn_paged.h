@@ -2,11 +2,12 @@
 //
 //   out = sum_p e_p v_p / sum_p e_p,   e_p = 2^(x_p - m),   x_p = scale log2(e) q.k_p,   m = max x_p
 //
-// A request's positions fall into chunks of AT_CHUNK; a workgroup takes one to three chunks of one key-value head for up to 16
-// or 32 of the rows (tokens x query heads of the group) that read them.  It leaves each row's m, sum e and sum e v of
-// each chunk; chunks lie at fixed places, so a row's result does not depend on what else runs.  A wave takes 64
-// neighbouring positions in steps of 32, keys and values straight from memory to registers and the next step's (or the next
-// chunk's) in flight while it computes, with 16x16x32 MFMAs for 16 rows at a time:
+// A request's positions fall into chunks of AT_CHUNK; a workgroup takes one, two or four chunks of one key-value head for up to
+// 16 or 32 of the rows (tokens x query heads of the group) that read them.  It leaves each row's m, sum e and sum e v of each
+// chunk, or of each pair of chunks; chunks and pairs lie at fixed places and are joined in the same steps wherever that
+// happens, so a row's result does not depend on what else runs.  A wave takes 64 neighbouring positions in steps
+// of 32, keys and values straight from memory to registers and the next step's (or the next chunk's) in flight while it
+// computes, with 16x16x32 MFMAs for 16 rows at a time:
 //   S^T [position][row] = K [position][d] Q^T [d][row],   O^T [d][row] += V^T [d][position] E^T [position][row].
 // The result layout of the first (lane: row lane % 16, positions 4 (lane / 16) + 0..3 of a tile) is the operand layout of the
 // second for an order of positions that V's loads follow, so e never leaves its lane.  V^T comes from V by byte
@@ -17,13 +18,13 @@
 // Three products in place of one cost little: the kernel waits for memory.  An 8-bit cache's codes are bf16 values to e,
 // and meet q as integers: q in units of its row's largest / 8.35e6 is three bytes, the sums of their products are exact.
 //
-// Measured: 48 requests of up to 8191 positions, 32 query heads on 8 of 128 bf16 values, pages of 16 (823 MB) 153 us, 5.4 TB/s
+// Measured: 48 requests of up to 8191 positions, 32 query heads on 8 of 128 bf16 values, pages of 16 (823 MB) 146 us, 5.6 TB/s
 // where a bare read of the same places reaches 6.1; matrix units busy 11 % of the time, vector units 24 %, waves wait to
-// issue loads 54 % and for data 31 % of theirs.  With two of three products left out, with all matrix instructions
-// replaced and with no exponentials the time stays; without the parts' stores (2 KB a chunk, 13 MB) it falls by 16 us, more than their bytes
-// explain.  32 requests of 16384 8-bit positions (572 MB): 131 us, 4.4 TB/s, vector units 52 % (64 conversions and 32 byte
-// permutes of the 300 instructions of a step).  Joining in the last workgroup to end, with tickets, in place of a launch of its own
-// measured slower everywhere (8 requests of 5003, 4 tokens: 34 -> 82 us; 48 requests: 173 -> 181 us).
+// issue loads half of theirs and for data a third.  With two of three products left out, with all matrix instructions
+// replaced and with no exponentials the time stays; a part for every chunk (2 KB) instead of every second one costs 9 us, more
+// than its bytes explain.  32 requests of 16384 8-bit positions (572 MB): 131 us, 4.4 TB/s, vector units 52 % (64 conversions and 32
+// byte permutes of the 300 instructions of a step).  Joining in the last workgroup to end, with tickets, in place of a launch of its
+// own measured slower everywhere (8 requests of 5003, 4 tokens: 34 -> 82 us; 48 requests: 173 -> 181 us).
 #pragma once
 #include <type_traits>
 
@@ -35,7 +36,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int AT_CHUNK = 256;                 // positions of a part
+constexpr int AT_CHUNK = 256;                 // positions of a chunk
 constexpr int AT_WAVES = 4;
 
 // v_perm: bytes 0..3 of the second operand are selected by 0..3, of the first by 4..7.
@@ -347,8 +348,9 @@ __device__ __forceinline__ void put_o(float* row, const f32x4 (&o)[ND], float k,
     }
 }
 
-// NR: tiles of 16 rows that a workgroup takes at once.
-template <class KV, int ND, int NR>
+// NR: tiles of 16 rows that a workgroup takes at once; PAIRED: it takes chunks by twos (apart from the other, whose way is
+// shorter: one request of 611 positions 7.8 -> 7.0 us).
+template <class KV, int ND, int NR, bool PAIRED>
 __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ? 3 : 4) k_attn_part(AttnArgs a) {
     typedef Attn<KV, ND, NR> A;
     __shared__ u32x4 sq[NR][A::KL][3][64];                      // q's parts [tile][load][part][lane]
@@ -358,10 +360,10 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
     __shared__ float k0[16 * NR], k1[16 * NR];
     __shared__ int sf[AT_WAVES];
     // the waves' sums of up to 16 rows [wave][row][LD], then the first chunk's of a pair [tile][round][row, value], which only
-    // the thread that put them there reads (as many rows as there are, so that three workgroups fit a CU)
+    // the thread that put them there reads (with these as many rows as there are, so that three workgroups fit a CU)
     extern __shared__ __attribute__((aligned(16))) float sums[];
     constexpr int ROUNDS = ND > 8 ? 2 : 1;
-    const int live = min(16, a.T * a.group);
+    const int live = PAIRED ? min(16, a.T * a.group) : 16;
     auto so = [&](int w, int row) { return sums + (w * live + row) * A::LD; };
     f32x4* const held = reinterpret_cast<f32x4*>(sums + AT_WAVES * live * A::LD);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
     // Workgroups go to the XCDs in turn: neighbours are heads, then requests, turned by the chunk, so that requests of
     // different lengths load the XCDs alike (chunks side by side: the 48 requests below 8192 positions took 209 us, XCD 0
     // with 1.5 times the chunks of XCD 7)
-    int c = a.paired ? 2 * blockIdx.z : blockIdx.z;
+    int c = PAIRED ? 2 * blockIdx.z : blockIdx.z;
     const int group = a.row_groups > 1 ? blockIdx.x / a.kv.heads : 0, kh = blockIdx.x - group * a.kv.heads, r0 = 16 * NR * group;
     const int b = __builtin_amdgcn_readfirstlane((blockIdx.y + blockIdx.z) % gridDim.y), stride = gridDim.z;
     // every argument in one go, then the length and the table's entry side by side
@@ -482,8 +484,8 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
             __syncthreads();
         }
         // The next chunk: where there is one, every wave has both its steps in this one.
-        const bool first_of_two = a.paired && !(c & 1) && (int64_t)(c + 1) * AT_CHUNK < len;
-        const int after = first_of_two ? c + 1 : a.paired ? (c & ~1) + 2 * stride : c + stride;
+        const bool first_of_two = PAIRED && !(c & 1) && (int64_t)(c + 1) * AT_CHUNK < len;
+        const int after = first_of_two ? c + 1 : PAIRED ? (c & ~1) + 2 * stride : c + stride;
         const bool on = !apart && (int64_t)after * AT_CHUNK < len;
         int page_on = -1;
         typename A::Span wn = w;
@@ -611,8 +613,8 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
             continue;
         }
         // part of the group's first row
-        const int64_t part0 = (((int64_t)b * a.kv.heads + kh) * R + r0) * a.parts + (a.paired ? c >> 1 : c);
-        const bool second_of_two = a.paired && (c & 1);
+        const int64_t part0 = (((int64_t)b * a.kv.heads + kh) * R + r0) * a.parts + (PAIRED ? c >> 1 : c);
+        const bool second_of_two = PAIRED && (c & 1);
 #pragma unroll
         for (int n = 0; n < NR; n++) {
             const int at = 16 * n + r;
@@ -695,9 +697,11 @@ void launch_attn_part_nr(const AttnArgs& args, hipStream_t s) {
     AttnArgs a = args;
     const int R = a.T * a.group;
     a.row_groups = (R + 16 * NR - 1) / (16 * NR);
-    const int live = R < 16 ? R : 16, held = a.paired ? NR * (ND > 8 ? 2 : 1) * 512 : 0;
+    const int live = a.paired && R < 16 ? R : 16, held = a.paired ? NR * (ND > 8 ? 2 : 1) * 512 : 0;
     const size_t lds = (size_t)live * (AT_WAVES * Attn<KV, ND, NR>::LD * 4 + held);
-    hipLaunchKernelGGL((k_attn_part<KV, ND, NR>), dim3(a.kv.heads * a.row_groups, a.table.seqs, a.groups), dim3(64 * AT_WAVES), lds, s, a);
+    const dim3 grid(a.kv.heads * a.row_groups, a.table.seqs, a.groups);
+    if (a.paired) hipLaunchKernelGGL((k_attn_part<KV, ND, NR, true>), grid, dim3(64 * AT_WAVES), lds, s, a);
+    else hipLaunchKernelGGL((k_attn_part<KV, ND, NR, false>), grid, dim3(64 * AT_WAVES), lds, s, a);
 }
 
 template <class KV, int ND>

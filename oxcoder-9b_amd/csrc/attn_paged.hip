@@ -9,7 +9,7 @@ namespace kq {
 // One workgroup per row and 32 N of its values: 32 groups of 8 lanes take every 32nd pair of chunks, in the steps of
 // the workgroup that had both where there was one; then the groups are added as a tree: a row's result depends on its
 // number of chunks alone.
-template <int N>
+template <int N, bool PAIRED>
 __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 so[4][N][8];
     __shared__ float sl[4], sm[4];
@@ -18,7 +18,7 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
     const int len = min(a.lens[b], a.max_len), n = len <= 0 ? 0 : (len + AT_CHUNK - 1) / AT_CHUNK, pairs = (n + 1) / 2;
     const int64_t row = (((int64_t)b * a.kv.heads + h / G) * a.T * G + blockIdx.x % a.T * G + h % G) * a.parts;
     float top = -INFINITY;
-    for (int c = tid; c < (a.paired ? pairs : n); c += 256) top = fmaxf(top, a.pml[row + c].m);
+    for (int c = tid; c < (PAIRED ? pairs : n); c += 256) top = fmaxf(top, a.pml[row + c].m);
     for (int w = 32; w; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
     if (lane == 0) sm[wave] = top;
     __syncthreads();
@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
         for (int i = 0; i < N; i++) sum[i] += x[i] * k;
         total += ml.l * k;
     };
-    if (a.paired) {
+    if constexpr (PAIRED) {
 #pragma unroll 8 / N
         for (int c = tid >> 3; c < pairs; c += 32) {
             f32x4 x[N];
@@ -112,10 +112,11 @@ void launch_attn_paged(const AttnArgs& args, hipStream_t s) {
     // rows enough for the chip: four times fewer workgroups, that scan a row's maxima once for 128 values (512 rows of 20 chunks and
     // 256 values 7.4 -> 5 us; the 32 rows of 391 chunks 8 us with 32 values each, 13 us with 128)
     const int64_t rows = (int64_t)a.table.seqs * a.T * a.q_heads;
-    if (rows >= device_cus())
-        hipLaunchKernelGGL(k_attn_join<4>, dim3(a.table.seqs * a.T, a.q_heads, (a.kv.dim + 127) / 128), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL(k_attn_join<1>, dim3(a.table.seqs * a.T, a.q_heads, (a.kv.dim + 31) / 32), dim3(256), 0, s, a);
+    const bool wide = rows >= device_cus();
+    const dim3 grid(a.table.seqs * a.T, a.q_heads, wide ? (a.kv.dim + 127) / 128 : (a.kv.dim + 31) / 32);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
+    if (a.paired) wide ? go(k_attn_join<4, true>) : go(k_attn_join<1, true>);
+    else wide ? go(k_attn_join<4, false>) : go(k_attn_join<1, false>);
 }
 
 }  // namespace kq

@@ -276,9 +276,10 @@ def test_a_longer_bound_changes_no_bit(dev, dtype, D, T):
     lens = [700, 5000, 255, 1025]
     cache, table, q = setup(dev, dtype, D, H, 2, 16, lens, T)
     here = attend(dev, cache, table, q, lens, T, H)
-    wide = torch.full((len(lens), 3000), -1, dtype=torch.int32)
-    wide[:, :table.shape[1]] = table
-    assert torch.equal(attend(dev, cache, wide, q, lens, T, H), here)
+    for width in (3000, 10000, 40000):              # one, two and four chunks a workgroup
+        wide = torch.full((len(lens), width), -1, dtype=torch.int32)
+        wide[:, :table.shape[1]] = table
+        assert torch.equal(attend(dev, cache, wide, q, lens, T, H), here), width
 
 
 def test_repeated_calls_leave_the_workspace_ready(dev):
@@ -335,3 +336,6 @@ def test_infinities_that_some_tokens_see(dev, dtype, D, q_heads, n):
         alone = attend(dev, cache, table, qs[:, t].contiguous(), [m - T + 1 + t for m in lens], 1, q_heads)
         torch.testing.assert_close(rows[:, t], alone, rtol=0, atol=0, equal_nan=True)
     assert torch.isfinite(rows[1]).all() and not torch.isfinite(rows[0, -1]).all()
+    wide = torch.full((2, 60000), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    torch.testing.assert_close(attend(dev, cache, wide, q, lens, T, q_heads).view(2, T, -1), rows, rtol=0, atol=0, equal_nan=True)

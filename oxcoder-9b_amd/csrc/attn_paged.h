@@ -14,7 +14,8 @@
 // permutes: a lane loads 1, 2, 4 or 8 neighbouring d of the 8 positions whose values it feeds.
 //
 // q and e are fp32; the cache's types multiply them exactly when they are cut into three parts of 8 (bf16) or
-// 11 (f16) bits, each part truncated from what the one before left, so products are those of fp32 and the sums fp32.
+// 11 (f16) bits, each part truncated from what the one before left, so products are those of fp32 and the sums fp32
+// (what f16's range needs for e: pv_f16).
 // Three products in place of one cost little: the kernel waits for memory.  An 8-bit cache's codes are bf16 values to e,
 // and meet q as integers: q in units of its row's largest / 8.35e6 is three bytes, the sums of their products are exact.
 //
@@ -80,6 +81,9 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// One product of four positions, a group of 16 lanes each.
+__device__ __forceinline__ f32x4 mma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
 // Four codes (bytes of w) as floats' bits; their high halves are the codes in bf16.
 __device__ __forceinline__ u32x4 code_floats(uint32_t w) {
     return u32x4{ubits((float)(int8_t)(w & 0xff)), ubits((float)(int8_t)(w >> 8 & 0xff)),
@@ -126,13 +130,13 @@ constexpr int at_first(int nd, int s) {           // first value of strip s, in 
 
 template <class KV, int ND, int NR>
 struct Attn {
-    static constexpr bool I8 = KV::id == KQ_KV_I8;
+    static constexpr bool I8 = KV::id == KQ_KV_I8, F16 = KV::id == KQ_KV_F16;
     static constexpr int D = 16 * ND, EB = I8 ? 1 : 2;
     static constexpr int KL = I8 ? (ND + 3) / 4 : (ND + 1) / 2;  // 16-byte loads of a key by its 4 lanes
     static constexpr int QW = I8 ? 4 : 2;                        // a lane's share of q for a load, in fours
     static constexpr bool K_WHOLE = I8 ? ND % 4 == 0 : ND % 2 == 0;
     static constexpr int WIDE = D > 128 ? 128 : D, LD = WIDE == 128 ? 128 : WIDE + 4; // values of a round of the waves' join, row stride in LDS
-    static constexpr float BIAS = KV::id == KQ_KV_F16 ? 14.0f : 0.0f;   // f16: e is held times 2^14, clear of subnormals
+    static constexpr float BIAS = F16 ? 14.0f : 0.0f;            // f16: e is held times 2^14
     static constexpr int VW = [] { int n = 0; for (int s = 0; s < at_strips(ND); s++) n += (at_width(ND, s) * EB + 3) / 4; return n; }();
 
     // Lane i of the wave: where position i of the chunk that is fetched lies in the pool, in bytes (a place that is there
@@ -280,8 +284,98 @@ struct Attn {
             pv_strip<S + 1, AT + NW>(p, o);
         }
     }
+    // f16: o += V^T (p0 + 2^-11 p1 + 2^-22 p2).
+    template <int S, int AT>
+    __device__ __forceinline__ void pv_strip_f16(const u32x4 (&p)[NR][3], f32x4 (&o)[NR][ND]) const {
+        if constexpr (S < at_strips(ND)) {
+            constexpr int W = at_width(ND, S), F = at_first(ND, S), NW = VRaw<W * EB>::N;
+            auto raw = [&](int kk, int d) { return v[kk >> 2][kk & 3][AT + d]; };
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                u32x4 f;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    f[j] = w & 1 ? hi_halves(raw(2 * j, w >> 1), raw(2 * j + 1, w >> 1))
+                                 : lo_halves(raw(2 * j, w >> 1), raw(2 * j + 1, w >> 1));
+#pragma unroll
+                for (int n = 0; n < NR; n++) {
+                    f32x4 x = mma<KV>(f, p[n][1], mma<KV>(f, p[n][2], f32x4{}) * 0x1p-11f);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(x[i], 0x1p-11f, o[n][F + w][i]);
+                    o[n][F + w] = mma<KV>(f, p[n][0], x);
+                }
+            }
+            pv_strip_f16<S + 1, AT + NW>(p, o);
+        }
+    }
+    // The same in fp32: position kk's values and weights.
+    template <int S, int AT>
+    __device__ __forceinline__ void pv_strip_f32(const float (&e)[NR][2][4], f32x4 (&o)[NR][ND]) const {
+        if constexpr (S < at_strips(ND)) {
+            constexpr int W = at_width(ND, S), F = at_first(ND, S), NW = VRaw<W * EB>::N;
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++)
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    const uint32_t raw = v[kk >> 2][kk & 3][AT + (w >> 1)];
+                    const float x = w & 1 ? f16_hi(raw) : f16_lo(raw);
+#pragma unroll
+                    for (int n = 0; n < NR; n++) o[n][F + w] = mma_f32(x, e[n][kk >> 2][kk & 3], o[n][F + w]);
+                }
+            pv_strip_f32<S + 1, AT + NW>(e, o);
+        }
+    }
+    // f16 weights e 2^14: three f16 parts, each held 2^11 times larger than the one before so that no rest meets f16's last step
+    // before its 24 bits are used up, hold every e >= 2^-37 exactly.  What they leave of a smaller one is added in fp32, and a
+    // step with an infinite value goes that way alone, as a part may be 0 where its weight is not.  (All steps in fp32, 16 times
+    // the matrix time: the 48 requests below 8192 positions 157 -> 164 us, 8 drafts of 4 tokens at 256 values 32.6 -> 36.6.)
+    __device__ __forceinline__ void pv_f16(const float (&e)[NR][2][4], f32x4 (&o)[NR][ND]) const {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        f16x2 zero[4] = {};                                     // NaN once a value is not finite
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int j = 0; j < VW; j++)
+                zero[i & 3] = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, v[i >> 2][i & 3][j]), f16x2{}, zero[i & 3]);
+        const bool bad = __any(__builtin_bit_cast(uint32_t, zero[0] + zero[1] + (zero[2] + zero[3])) != 0);
+        bool small = false;
+#pragma unroll
+        for (int j = 0; j < 8 * NR; j++) small |= ubits(e[j >> 3][j >> 2 & 1][j & 3]) - 1u < ubits(0x1p-23f) - 1u;
+        const bool rest = __any(small);
+        auto cut = [](float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); };
+        if (bad || rest) {
+            float x[NR][2][4];
+#pragma unroll
+            for (int j = 0; j < 8 * NR; j++) {
+                float r = e[j >> 3][j >> 2 & 1][j & 3];
+                if (!bad) {
+#pragma unroll
+                    for (int i = 0; i < 3; i++) r = (r - f16_lo(cut(r, 0.0f))) * 0x1p11f;
+                    r *= 0x1p-33f;
+                }
+                x[j >> 3][j >> 2 & 1][j & 3] = r;
+            }
+            pv_strip_f32<0, 0>(x, o);
+        }
+        if (!bad) {
+            u32x4 p[NR][3];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int n = 0; n < NR; n++) {
+                    float x = e[n][j >> 1][2 * (j & 1)], y = e[n][j >> 1][2 * (j & 1) + 1];
+#pragma unroll
+                    for (int i = 0; i < 3; i++) {
+                        p[n][i][j] = cut(x, y);
+                        x = (x - f16_lo(p[n][i][j])) * 0x1p11f, y = (y - f16_hi(p[n][i][j])) * 0x1p11f;
+                    }
+                }
+            pv_strip_f16<0, 0>(p, o);
+        }
+    }
     // o += V^T E^T of the step, for NR tiles of rows; e[n][t][i] of position 16 t + 4 g + i, 0 where the row does not see it.
     __device__ __forceinline__ void pv(const Span& w, const float (&e)[NR][2][4], f32x4 (&o)[NR][ND], int u, int g) const {
+        if constexpr (F16) return pv_f16(e, o);
         u32x4 p[NR][3];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -396,8 +490,8 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
     float f[NR];
     for (;;) {
         // (Taken anew for each chunk, as the thread's place below: what queries' addresses come from is not held.)
-        int row[NR], t[NR], lane_row = r0 + r;
-        asm volatile("" : "+v"(lane_row));
+        int row[NR], t[NR], lane_row = r0 + r, lane_g = g;
+        asm volatile("" : "+v"(lane_row), "+v"(lane_g));
 #pragma unroll
         for (int n = 0; n < NR; n++) row[n] = lane_row + 16 * n, t[n] = row[n] / G;
         if (!ready) {
@@ -407,7 +501,7 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
             auto share = [&](int tile, int n, Share& x) {
                 const float* q = a.q + ((int64_t)b * a.T + (row[tile] < R ? t[tile] : 0)) * a.ldq +
                                  (int64_t)(row[tile] < R ? kh * G + row[tile] % G : 0) * A::D;
-                const int d = 16 * A::QW * n + 4 * A::QW * g;
+                const int d = 16 * A::QW * n + 4 * A::QW * lane_g;
                 const bool ok = A::K_WHOLE || d < A::D;
 #pragma unroll
                 for (int j = 0; j < A::QW; j++) {

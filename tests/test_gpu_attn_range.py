@@ -1,0 +1,93 @@
+"""Attention where fp32's range and each number's own 24 bits count, against the formula in 64 bits within
+decode_helpers.attention's bound."""
+import math
+
+import pytest
+import torch
+
+from decode_helpers import attention, check_attention, make_cache, page_table
+from test_gpu_attn_paged import attend, setup
+
+pytestmark = pytest.mark.gpu
+
+
+def sinks(dev, dtype, D, gap, lens, T, every=64):
+    """Every 64th position takes all the weight and has a value of 0; the others' scores lie `gap` below.  Two query heads on
+    one key-value head; the score is the first value of the key."""
+    table, pages = page_table(lens, 16)
+    cache = make_cache(dtype, pages, 1, 16, D, dev)
+    flat = torch.zeros(pages * 16, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        p = torch.arange(5, n, every)
+        flat[table[b].long()[p // 16] * 16 + p % 16] = True
+    sink = flat.view(pages, 1, 16).to(dev)
+    cache.k.zero_()
+    if dtype == "i8":
+        cache.k[..., 0] = 127 * sink
+        cache.k_scale.fill_(gap / 127)
+        cache.v.abs_()                                  # of one sign, so that errors of one sign do not cancel
+    else:
+        cache.k[..., 0] = gap * sink
+        cache.v.add_(1)
+    cache.v.masked_fill_(sink[..., None], 0)
+    q = torch.zeros(len(lens) * T, 2 * D)
+    q[:, [0, D]] = 1
+    return cache, table, q
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "i8"])
+@pytest.mark.parametrize("gap", [12, 18, 25, 30, 40, 60, 80])
+@pytest.mark.parametrize("D,T", [(64, 1), (128, 3), (256, 1)])
+def test_weights_far_below_the_largest(dev, dtype, gap, D, T):
+    lens = [40, 65, 700, 4096]
+    print("sinks", dtype, gap, D, T, flush=True)
+    cache, table, q = sinks(dev, dtype, D, gap, lens, T)
+    got = attend(dev, cache, table, q, lens, T, 2, scale=1.0)
+    check_attention(got, *attention(cache, table, q, lens, T, 2, 1.0))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("gap", [0, 20, 40, 80])
+@pytest.mark.parametrize("D,T", [(64, 1), (128, 4), (256, 1)])
+def test_infinite_values_of_small_weight(dev, dtype, gap, D, T):
+    """An infinity or NaN that a row sees counts however small its weight; the other columns keep their sums."""
+    lens = [700, 40]
+    print("infinite values", dtype, gap, D, T, flush=True)
+    cache, table, q = sinks(dev, dtype, D, gap, lens, T)
+    page, off = table[0, 300 // 16], 300 % 16
+    cache.v[page, 0, off:off + 2, 10:14] = 0
+    ref, bound = attention(cache, table, q, lens, T, 2, 1.0)
+    cache.v[page, 0, off, 10:14] = torch.tensor([math.inf, -math.inf, math.nan, math.inf], device=dev).to(cache.v.dtype)
+    cache.v[page, 0, off + 1, 13] = -math.inf
+    got = attend(dev, cache, table, q, lens, T, 2, scale=1.0).view(2, T, 2, D)
+    hit = got[0, :, :, 10:14].cpu()
+    assert (hit[..., 0] == math.inf).all() and (hit[..., 1] == -math.inf).all() and hit[..., 2:].isnan().all()
+    got[0, :, :, 10:14] = 0
+    ref.view(2, T, 2, D)[0, :, :, 10:14] = 0
+    bound.view(2, T, 2, D)[0, :, :, 10:14] = 0
+    check_attention(got.view(2 * T, -1), ref, bound)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D,T", [(64, 1), (128, 4), (240, 1)])
+def test_infinite_keys_that_are_seen(dev, dtype, D, T):
+    """A key of -inf in one channel: no weight where the query is positive there, a NaN row where it is negative."""
+    lens, H = [300, 41], 4
+    print("infinite keys", dtype, D, T, flush=True)
+    cache, table, q = setup(dev, dtype, D, H, 2, 16, lens, T)
+    q.view(-1, H, D)[:, :, 3] = torch.tensor([8.0, -8.0, 1e-6, 8.0])
+    at = (table[0, 100 // 16], slice(None), 100 % 16, 3)
+    cache.k[at] = -60000.0
+    ref, bound = (x.view(2, T, H, D) for x in attention(cache, table, q, lens, T, H, 1.0))
+    far = attend(dev, cache, table, q, lens, T, H, scale=1.0).view(2, T, H, D)
+    cache.k[at] = -math.inf
+    got = attend(dev, cache, table, q, lens, T, H, scale=1.0).view(2, T, H, D)
+    assert got[0, :, 1].isnan().all()
+    for h in (0, 3):                                # there a key of -60000 has no weight either
+        assert torch.equal(got[0, :, h], far[0, :, h])
+    assert torch.equal(got[1], far[1])
+    assert torch.isfinite(got[0, :, 2]).all()       # a small positive query there: no weight, the rest as it is
+    got[0, :, 1:3] = 0
+    ref[0, :, 1:3] = 0
+    bound[0, :, 1:3] = 0
+    check_attention(got.view(2 * T, -1), ref.view(2 * T, -1), bound.view(2 * T, -1))

@@ -16,8 +16,7 @@
 // q and e are fp32; the cache's types multiply them exactly when they are cut into three parts of 8 (bf16) or
 // 11 (f16) bits, each part truncated from what the one before left, so products are those of fp32 and the sums fp32
 // (what f16's range needs for e: pv_f16).
-// Three products in place of one cost little: the kernel waits for memory.  An 8-bit cache's codes are bf16 values to e,
-// and meet q as integers: q in units of its row's largest / 8.35e6 is three bytes, the sums of their products are exact.
+// Three products in place of one cost little: the kernel waits for memory.  An 8-bit cache's codes are bf16 values to q and e.
 //
 // Measured: 48 requests of up to 8191 positions, 32 query heads on 8 of 128 bf16 values, pages of 16 (823 MB) 146 us, 5.6 TB/s
 // where a bare read of the same places reaches 6.1; matrix units busy 11 % of the time, vector units 24 %, waves wait to
@@ -35,7 +34,6 @@ namespace kq {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int AT_CHUNK = 256;                 // positions of a chunk
 constexpr int AT_WAVES = 4;
@@ -89,6 +87,12 @@ __device__ __forceinline__ u32x4 code_floats(uint32_t w) {
     return u32x4{ubits((float)(int8_t)(w & 0xff)), ubits((float)(int8_t)(w >> 8 & 0xff)),
                  ubits((float)(int8_t)(w >> 16 & 0xff)), ubits((float)(int8_t)(w >> 24))};
 }
+// Eight codes as bf16; unpacked here, as the compiler would do it where they are loaded and hold them in four times the registers.
+__device__ __forceinline__ u32x4 code_bf16(uint32_t a, uint32_t b) {
+    asm volatile("" : "+v"(a), "+v"(b));
+    const u32x4 x = code_floats(a), y = code_floats(b);
+    return u32x4{hi_halves(x.x, x.y), hi_halves(x.z, x.w), hi_halves(y.x, y.y), hi_halves(y.z, y.w)};
+}
 
 // W neighbouring elements of V as dwords (one element: in the low half).
 template <int BYTES>
@@ -133,7 +137,7 @@ struct Attn {
     static constexpr bool I8 = KV::id == KQ_KV_I8, F16 = KV::id == KQ_KV_F16;
     static constexpr int D = 16 * ND, EB = I8 ? 1 : 2;
     static constexpr int KL = I8 ? (ND + 3) / 4 : (ND + 1) / 2;  // 16-byte loads of a key by its 4 lanes
-    static constexpr int QW = I8 ? 4 : 2;                        // a lane's share of q for a load, in fours
+    static constexpr int PER = I8 ? 2 : 1, QS = PER * KL;        // products of a load by 8 values of each lane; their sum: q's shares
     static constexpr bool K_WHOLE = I8 ? ND % 4 == 0 : ND % 2 == 0;
     static constexpr int WIDE = D > 128 ? 128 : D, LD = WIDE == 128 ? 128 : WIDE + 4; // values of a round of the waves' join, row stride in LDS
     static constexpr float BIAS = F16 ? 14.0f : 0.0f;            // f16: e is held times 2^14
@@ -447,7 +451,7 @@ __device__ __forceinline__ void put_o(float* row, const f32x4 (&o)[ND], float k,
 template <class KV, int ND, int NR, bool PAIRED>
 __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ? 3 : 4) k_attn_part(AttnArgs a) {
     typedef Attn<KV, ND, NR> A;
-    __shared__ u32x4 sq[NR][A::KL][3][64];                      // q's parts [tile][load][part][lane]
+    __shared__ u32x4 sq[NR][A::QS][3][64];                      // q's parts [tile][share][part][lane]
     __shared__ float sm[AT_WAVES][16 * NR], sl[AT_WAVES][16 * NR], st[16 * NR];
     // the first chunk of a pair: its m and l; the pair's scales
     __shared__ AttnMl held_ml[16 * NR];
@@ -497,24 +501,24 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
         if (!ready) {
             w = s.open(a, page, kh, c * AT_CHUNK + 64 * wave, len, lane);
             // q's parts; each wave cuts a share
-            typedef f32x4 Share[A::QW];
+            typedef f32x4 Share[2];
             auto share = [&](int tile, int n, Share& x) {
                 const float* q = a.q + ((int64_t)b * a.T + (row[tile] < R ? t[tile] : 0)) * a.ldq +
                                  (int64_t)(row[tile] < R ? kh * G + row[tile] % G : 0) * A::D;
-                const int d = 16 * A::QW * n + 4 * A::QW * lane_g;
+                const int d = 32 * A::PER * (n / A::PER) + 8 * (A::PER * lane_g + n % A::PER);
                 const bool ok = A::K_WHOLE || d < A::D;
 #pragma unroll
-                for (int j = 0; j < A::QW; j++) {
+                for (int j = 0; j < 2; j++) {
                     x[j] = *reinterpret_cast<const f32x4_a4*>(q + (ok ? d : 0) + 4 * j);
                     if (!ok) x[j] = f32x4{0, 0, 0, 0};
                 }
             };
-            constexpr int SHARES = (A::KL + AT_WAVES - 1) / AT_WAVES, WHOLE = KV::id == KQ_KV_BF16 ? 0 : A::KL;
+            constexpr int SHARES = (A::QS + AT_WAVES - 1) / AT_WAVES, WHOLE = A::F16 ? A::QS : 0;
             Share mine[NR][SHARES], whole[NR][WHOLE ? WHOLE : 1];
 #pragma unroll
             for (int tile = 0; tile < NR; tile++) {
 #pragma unroll
-                for (int i = 0; i < SHARES; i++) share(tile, min(AT_WAVES * i + wave, A::KL - 1), mine[tile][i]);
+                for (int i = 0; i < SHARES; i++) share(tile, min(AT_WAVES * i + wave, A::QS - 1), mine[tile][i]);
 #pragma unroll
                 for (int n = 0; n < WHOLE; n++) share(tile, n, whole[tile][n]);
             }
@@ -522,53 +526,29 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
             s.load_v(0, r, g);
 #pragma unroll
             for (int tile = 0; tile < NR; tile++) {
-                float top = 0.0f, bad = 0.0f, up = 1.0f;
+                float top = 0.0f, up = 1.0f;
                 f[tile] = a.scale * 1.44269504088896341f;
 #pragma unroll
                 for (int n = 0; n < WHOLE; n++)
 #pragma unroll
-                    for (int j = 0; j < 4 * A::QW; j++) {
-                        const float x = whole[tile][n][j >> 2][j & 3];
-                        top = fmaxf(top, fabsf(x));
-                        if constexpr (A::I8) bad = __builtin_fmaf(x, 0.0f, bad);
-                    }
-                if constexpr (WHOLE) top = xor32_max(xor16_max(top));
-                if constexpr (A::I8) bad = xor32_sum(xor16_sum(bad));
-                if constexpr (KV::id == KQ_KV_F16) {
+                    for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(whole[tile][n][j >> 2][j & 3]));
+                if constexpr (A::F16) {
+                    top = xor32_max(xor16_max(top));
                     // times a power of two that puts the row's largest near 2^14
                     const uint32_t ex = max(ubits(top) >> 23, 15u);
                     up = fbits(min(268u - ex, 254u) << 23);
                     f[tile] *= fbits((ex - 14u) << 23);
                 }
-                if constexpr (A::I8) {
-                    up = 8.35e6f / fmaxf(top, 1e-30f);
-                    f[tile] = f[tile] * (fmaxf(top, 1e-30f) / 8.35e6f) + bad;    // bad: NaN for a row with an infinity or NaN
-                }
 #pragma unroll
                 for (int i = 0; i < SHARES; i++) {
                     const int n = AT_WAVES * i + wave;
-                    if (n < A::KL) {
+                    if (n < A::QS) {
                         u32x4 p[3];
-                        if constexpr (A::I8) {
 #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                uint32_t p0 = 0, p1 = 0, p2 = 0;
-#pragma unroll
-                                for (int k = 0; k < 4; k++) {
-                                    const int x = (int)rintf(mine[tile][i][j][k] * up), y = (x + 0x80) >> 8, z = (y + 0x80) >> 8;
-                                    p0 |= ((uint32_t)z & 0xffu) << (8 * k);      // x = 65536 z + 256 (int8)y + (int8)x
-                                    p1 |= ((uint32_t)y & 0xffu) << (8 * k);
-                                    p2 |= ((uint32_t)x & 0xffu) << (8 * k);
-                                }
-                                p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                uint32_t p0, p1, p2;
-                                split2<KV>(mine[tile][i][j >> 1][2 * (j & 1)] * up, mine[tile][i][j >> 1][2 * (j & 1) + 1] * up, p0, p1, p2);
-                                p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
-                            }
+                        for (int j = 0; j < 4; j++) {
+                            uint32_t p0, p1, p2;
+                            split2<KV>(mine[tile][i][j >> 1][2 * (j & 1)] * up, mine[tile][i][j >> 1][2 * (j & 1) + 1] * up, p0, p1, p2);
+                            p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
                         }
 #pragma unroll
                         for (int j = 0; j < 3; j++) sq[tile][n][j][lane] = p[j];
@@ -593,43 +573,28 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
             const int base = w.first + 32 * u;
             if (base >= len) break;
             float e[NR][2][4];
-            if constexpr (A::I8) {
-                i32x4 acc[NR][2][3] = {};
+            f32x4 acc[NR][2] = {};
 #pragma unroll
-                for (int n = 0; n < A::KL; n++)
+            for (int n = 0; n < A::QS; n++) {
+                u32x4 key[2];
 #pragma unroll
-                    for (int j = 0; j < 3; j++)
-#pragma unroll
-                        for (int tile = 0; tile < NR; tile++) {
-                            const i32x4 qp = __builtin_bit_cast(i32x4, sq[tile][n][j][lane]);
-#pragma unroll
-                            for (int i = 0; i < 2; i++)
-                                acc[tile][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, s.k[i][n]), qp,
-                                                                                        acc[tile][i][j], 0, 0, 0);
-                        }
-#pragma unroll
-                for (int j = 0; j < 8 * NR; j++) {
-                    const i32x4* x = acc[j >> 3][j >> 2 & 1];
-                    e[j >> 3][j >> 2 & 1][j & 3] =
-                        __builtin_fmaf(__builtin_fmaf((float)x[0][j & 3], 256.0f, (float)x[1][j & 3]), 256.0f, (float)x[2][j & 3]);
+                for (int i = 0; i < 2; i++) {
+                    if constexpr (A::I8) key[i] = code_bf16(s.k[i][n / 2][2 * (n & 1)], s.k[i][n / 2][2 * (n & 1) + 1]);
+                    else key[i] = s.k[i][n];
                 }
-            } else {
-                f32x4 acc[NR][2] = {};
 #pragma unroll
-                for (int n = 0; n < A::KL; n++)
+                for (int tile = 0; tile < NR; tile++) {
+                    u32x4 qp[3];
 #pragma unroll
-                    for (int tile = 0; tile < NR; tile++) {
-                        u32x4 qp[3];
+                    for (int j = 0; j < 3; j++) qp[j] = sq[tile][n][j][lane];
 #pragma unroll
-                        for (int j = 0; j < 3; j++) qp[j] = sq[tile][n][j][lane];
+                    for (int j = 2; j >= 0; j--)
 #pragma unroll
-                        for (int j = 2; j >= 0; j--)
-#pragma unroll
-                            for (int i = 0; i < 2; i++) acc[tile][i] = mma<KV>(s.k[i][n], qp[j], acc[tile][i]);
-                    }
-#pragma unroll
-                for (int j = 0; j < 8 * NR; j++) e[j >> 3][j >> 2 & 1][j & 3] = acc[j >> 3][j >> 2 & 1][j & 3];
+                        for (int i = 0; i < 2; i++) acc[tile][i] = mma<KV>(key[i], qp[j], acc[tile][i]);
+                }
             }
+#pragma unroll
+            for (int j = 0; j < 8 * NR; j++) e[j >> 3][j >> 2 & 1][j & 3] = acc[j >> 3][j >> 2 & 1][j & 3];
             // What the next step reads is fetched whether there is one or not (no place that is not there is read, all lanes
             // take the pool's first): the waits below then know how many loads are younger than theirs.
             if (u) wn = s.open(a, on ? page_on : -1, kh, after * AT_CHUNK + 64 * wave, len, lane);

@@ -91,3 +91,27 @@ def test_infinite_keys_that_are_seen(dev, dtype, D, T):
     ref[0, :, 1:3] = 0
     bound[0, :, 1:3] = 0
     check_attention(got.view(2 * T, -1), ref.view(2 * T, -1), bound.view(2 * T, -1))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "i8"])
+@pytest.mark.parametrize("ratio", [1e2, 1e3, 1e4, 1e6, 1e9, 1e12, 1e20])
+@pytest.mark.parametrize("D", [48, 128])
+def test_a_query_channel_far_above_the_others(dev, dtype, ratio, D):
+    """Where the keys are 0 in that channel, the others' products are the whole score."""
+    lens, T, H = [41, 700], 2, 4
+    print("channel", dtype, ratio, D, flush=True)
+    cache, table, q = setup(dev, dtype, D, H, 2, 16, lens, T)
+    q.view(-1, H, D)[..., 17] = ratio
+    cache.k[..., 17] = 0
+    check_attention(attend(dev, cache, table, q, lens, T, H), *attention(cache, table, q, lens, T, H, D ** -0.5))
+
+
+@pytest.mark.parametrize("keys,queries", [(-100, 100), (60, -60), (95, -95), (104, -95)])
+def test_key_scales_far_from_1(dev, keys, queries):
+    """An 8-bit cache's key scales at 2^keys under queries at 2^queries: ordinary scores."""
+    D, H, lens = 64, 4, [41, 300]
+    print("key scales", keys, queries, flush=True)
+    cache, table, q = setup(dev, "i8", D, H, 2, 16, lens, 1)
+    cache.k_scale.mul_(2.0 ** keys)
+    q, scale = q * 2.0 ** queries, 2.0 ** -(keys + queries) * D ** -0.5
+    check_attention(attend(dev, cache, table, q, lens, 1, H, scale), *attention(cache, table, q, lens, 1, H, scale))

@@ -14,8 +14,8 @@
 // permutes: a lane loads 1, 2, 4 or 8 neighbouring d of the 8 positions whose values it feeds.
 //
 // q and e are fp32; the cache's types multiply them exactly when they are cut into three parts of 8 (bf16) or
-// 11 (f16) bits, each part truncated from what the one before left, so products are those of fp32 and the sums fp32
-// (what f16's range needs for e: pv_f16).
+// 11 (f16) bits, each part truncated from what the one before left, so products are those of fp32 and the sums fp32.  What
+// f16's range does not hold of an element or a weight far below the largest is made up for by fp32 products.
 // Three products in place of one cost little: the kernel waits for memory.  An 8-bit cache's codes are bf16 values to q and e.
 //
 // Measured: 48 requests of up to 8191 positions, 32 query heads on 8 of 128 bf16 values, pages of 16 (823 MB) 146 us, 5.6 TB/s
@@ -48,27 +48,38 @@ __device__ __forceinline__ uint32_t of_lane(int i, uint32_t v) { return (uint32_
 __device__ __forceinline__ float fbits(uint32_t u) { return __builtin_bit_cast(float, u); }
 __device__ __forceinline__ uint32_t ubits(float f) { return __builtin_bit_cast(uint32_t, f); }
 
-// Both elements' three parts, packed in pairs.  A part that is left with nothing becomes a number of x's sign far
+// Both elements' three parts of 8 bits, packed in pairs.  A part that is left with nothing becomes a number of x's sign far
 // below the last part's step (0 for x = 0), so that an infinite factor gives an infinity and not 0 * inf.
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+    auto cut = [](float a) { return fbits(ubits(a) & 0xffff0000u); };
+    // a rest that is not 0 is at least 2^-24 |x| and has at most 16 bits: the sum with 2^-50 x rounds back to it
+    const float tx = x * 0x1p-50f, ty = y * 0x1p-50f;
+    const float rx = x - cut(x), ry = y - cut(y), sx = rx - cut(rx), sy = ry - cut(ry);
+    p0 = hi_halves(ubits(x), ubits(y));
+    p1 = hi_halves(ubits(rx + tx), ubits(ry + ty));
+    p2 = hi_halves(ubits(sx + tx), ubits(sy + ty));
+}
+
+// Three f16 parts of 11 bits of |x|, |y| < 2^15, x = p0 + 2^-11 p1 + 2^-22 p2: held 2^11 times larger than the one before,
+// so that no rest meets f16's last step before its 24 bits are used up.  Exact from 2^-23 on, and for 0.
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+    auto cut = [](float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); };
+    p0 = cut(x, y);
+    const float rx = (x - f16_lo(p0)) * 0x1p11f, ry = (y - f16_hi(p0)) * 0x1p11f;
+    p1 = cut(rx, ry);
+    p2 = cut((rx - f16_lo(p1)) * 0x1p11f, (ry - f16_hi(p1)) * 0x1p11f);
+}
+// What the parts leave of x.
+__device__ __forceinline__ float split_rest(float x) {
+#pragma unroll
+    for (int i = 0; i < 3; i++) x = (x - f16_lo(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, 0.0f)))) * 0x1p11f;
+    return x * 0x1p-33f;
+}
+
 template <class KV>
 __device__ __forceinline__ void split2(float x, float y, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
-    if constexpr (KV::id == KQ_KV_F16) {
-        auto cut = [](float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); };
-        auto least = [](float a) { return a == 0.0f ? 0.0f : __builtin_copysignf(0x1p-24f, a); };
-        const float tx = least(x), ty = least(y);
-        p0 = cut(x, y);
-        const float rx = x - f16_lo(p0) + tx, ry = y - f16_hi(p0) + ty;
-        p1 = cut(rx, ry);
-        p2 = cut(rx - f16_lo(p1) + tx, ry - f16_hi(p1) + ty);
-    } else {
-        auto cut = [](float a) { return fbits(ubits(a) & 0xffff0000u); };
-        // a rest that is not 0 is at least 2^-24 |x| and has at most 16 bits: the sum with 2^-50 x rounds back to it
-        const float tx = x * 0x1p-50f, ty = y * 0x1p-50f;
-        const float rx = x - cut(x), ry = y - cut(y), sx = rx - cut(rx), sy = ry - cut(ry);
-        p0 = hi_halves(ubits(x), ubits(y));
-        p1 = hi_halves(ubits(rx + tx), ubits(ry + ty));
-        p2 = hi_halves(ubits(sx + tx), ubits(sy + ty));
-    }
+    if constexpr (KV::id == KQ_KV_F16) split_f16(x, y, p0, p1, p2);
+    else split_bf16(x, y, p0, p1, p2);
 }
 
 template <class KV>
@@ -329,8 +340,7 @@ struct Attn {
             pv_strip_f32<S + 1, AT + NW>(e, o);
         }
     }
-    // f16 weights e 2^14: three f16 parts, each held 2^11 times larger than the one before so that no rest meets f16's last step
-    // before its 24 bits are used up, hold every e >= 2^-37 exactly.  What they leave of a smaller one is added in fp32, and a
+    // f16 weights e 2^14: the parts hold every e >= 2^-37 exactly.  What they leave of a smaller one is added in fp32, and a
     // step with an infinite value goes that way alone, as a part may be 0 where its weight is not.  (All steps in fp32, 16 times
     // the matrix time: the 48 requests below 8192 positions 157 -> 164 us, 8 drafts of 4 tokens at 256 values 32.6 -> 36.6.)
     __device__ __forceinline__ void pv_f16(const float (&e)[NR][2][4], f32x4 (&o)[NR][ND]) const {
@@ -346,18 +356,12 @@ struct Attn {
 #pragma unroll
         for (int j = 0; j < 8 * NR; j++) small |= ubits(e[j >> 3][j >> 2 & 1][j & 3]) - 1u < ubits(0x1p-23f) - 1u;
         const bool rest = __any(small);
-        auto cut = [](float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b)); };
         if (bad || rest) {
             float x[NR][2][4];
 #pragma unroll
             for (int j = 0; j < 8 * NR; j++) {
-                float r = e[j >> 3][j >> 2 & 1][j & 3];
-                if (!bad) {
-#pragma unroll
-                    for (int i = 0; i < 3; i++) r = (r - f16_lo(cut(r, 0.0f))) * 0x1p11f;
-                    r *= 0x1p-33f;
-                }
-                x[j >> 3][j >> 2 & 1][j & 3] = r;
+                const float r = e[j >> 3][j >> 2 & 1][j & 3];
+                x[j >> 3][j >> 2 & 1][j & 3] = bad ? r : split_rest(r);
             }
             pv_strip_f32<0, 0>(x, o);
         }
@@ -367,12 +371,9 @@ struct Attn {
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int n = 0; n < NR; n++) {
-                    float x = e[n][j >> 1][2 * (j & 1)], y = e[n][j >> 1][2 * (j & 1) + 1];
-#pragma unroll
-                    for (int i = 0; i < 3; i++) {
-                        p[n][i][j] = cut(x, y);
-                        x = (x - f16_lo(p[n][i][j])) * 0x1p11f, y = (y - f16_hi(p[n][i][j])) * 0x1p11f;
-                    }
+                    uint32_t p0, p1, p2;
+                    split_f16(e[n][j >> 1][2 * (j & 1)], e[n][j >> 1][2 * (j & 1) + 1], p0, p1, p2);
+                    p[n][0][j] = p0, p[n][1][j] = p1, p[n][2][j] = p2;
                 }
             pv_strip_f16<0, 0>(p, o);
         }
@@ -397,7 +398,7 @@ struct Attn {
                     y = y == 0.0f ? y : y * sy;
                 }
                 uint32_t p0, p1, p2;
-                split2<KV>(x, y, p0, p1, p2);
+                split_bf16(x, y, p0, p1, p2);
                 p[n][0][j] = p0, p[n][1][j] = p1, p[n][2][j] = p2;
             }
         }
@@ -491,28 +492,33 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
     bool ready = false;                                         // the chunk's first step is in flight and q's parts are there
     bool apart = false;                                         // token by token (below)
     int tok = 0;
-    float f[NR];
+    float f[NR], up[NR];                                        // f: what a score is multiplied by; up: what q's parts were
+    bool rest = false;                                          // f16: they leave something of some element
+#pragma unroll
+    for (int n = 0; n < NR; n++) up[n] = 1.0f;
     for (;;) {
         // (Taken anew for each chunk, as the thread's place below: what queries' addresses come from is not held.)
-        int row[NR], t[NR], lane_row = r0 + r, lane_g = g;
+        int row[NR], t[NR], lane_row = r, lane_g = g;
         asm volatile("" : "+v"(lane_row), "+v"(lane_g));
 #pragma unroll
-        for (int n = 0; n < NR; n++) row[n] = lane_row + 16 * n, t[n] = row[n] / G;
+        for (int n = 0; n < NR; n++) row[n] = r0 + lane_row + 16 * n, t[n] = row[n] / G;
+        typedef f32x4 Share[2];
+        auto share = [&](int tile, int n, Share& x, bool again = false) {
+            int at = row[tile], place = lane_g;
+            if (again) asm volatile("" : "+v"(at), "+v"(place));   // read again, not held
+            const float* q = a.q + ((int64_t)b * a.T + (at < R ? again ? at / G : t[tile] : 0)) * a.ldq +
+                             (int64_t)(at < R ? kh * G + at % G : 0) * A::D;
+            const int d = 32 * A::PER * (n / A::PER) + 8 * (A::PER * place + n % A::PER);
+            const bool ok = A::K_WHOLE || n < A::QS - A::PER || d < A::D;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                x[j] = *reinterpret_cast<const f32x4_a4*>(q + (ok ? d : 0) + 4 * j);
+                if (!ok) x[j] = f32x4{0, 0, 0, 0};
+            }
+        };
         if (!ready) {
             w = s.open(a, page, kh, c * AT_CHUNK + 64 * wave, len, lane);
             // q's parts; each wave cuts a share
-            typedef f32x4 Share[2];
-            auto share = [&](int tile, int n, Share& x) {
-                const float* q = a.q + ((int64_t)b * a.T + (row[tile] < R ? t[tile] : 0)) * a.ldq +
-                                 (int64_t)(row[tile] < R ? kh * G + row[tile] % G : 0) * A::D;
-                const int d = 32 * A::PER * (n / A::PER) + 8 * (A::PER * lane_g + n % A::PER);
-                const bool ok = A::K_WHOLE || d < A::D;
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    x[j] = *reinterpret_cast<const f32x4_a4*>(q + (ok ? d : 0) + 4 * j);
-                    if (!ok) x[j] = f32x4{0, 0, 0, 0};
-                }
-            };
             constexpr int SHARES = (A::QS + AT_WAVES - 1) / AT_WAVES, WHOLE = A::F16 ? A::QS : 0;
             Share mine[NR][SHARES], whole[NR][WHOLE ? WHOLE : 1];
 #pragma unroll
@@ -524,20 +530,27 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
             }
             s.load_k(0, r, g);
             s.load_v(0, r, g);
+            bool small = false;
 #pragma unroll
             for (int tile = 0; tile < NR; tile++) {
-                float top = 0.0f, up = 1.0f;
-                f[tile] = a.scale * 1.44269504088896341f;
+                float top = 0.0f;
+                uint32_t least = ~0u;                           // of the elements that are not 0, less one
+                f[tile] = a.scale;
 #pragma unroll
                 for (int n = 0; n < WHOLE; n++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(whole[tile][n][j >> 2][j & 3]));
+                    for (int j = 0; j < 8; j++) {
+                        const float x = fabsf(whole[tile][n][j >> 2][j & 3]);
+                        top = fmaxf(top, x);
+                        least = min(least, ubits(x) - 1u);
+                    }
                 if constexpr (A::F16) {
-                    top = xor32_max(xor16_max(top));
                     // times a power of two that puts the row's largest near 2^14
+                    top = xor32_max(xor16_max(top));
                     const uint32_t ex = max(ubits(top) >> 23, 15u);
-                    up = fbits(min(268u - ex, 254u) << 23);
+                    up[tile] = fbits(min(268u - ex, 254u) << 23);
                     f[tile] *= fbits((ex - 14u) << 23);
+                    small |= least < ((max(ex, 38u) - 37u) << 23) - 1u;   // an element below 2^-37 of the largest's power
                 }
 #pragma unroll
                 for (int i = 0; i < SHARES; i++) {
@@ -547,14 +560,15 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             uint32_t p0, p1, p2;
-                            split2<KV>(mine[tile][i][j >> 1][2 * (j & 1)] * up, mine[tile][i][j >> 1][2 * (j & 1) + 1] * up, p0, p1, p2);
+                            split2<KV>(mine[tile][i][j >> 1][2 * (j & 1)] * up[tile], mine[tile][i][j >> 1][2 * (j & 1) + 1] * up[tile], p0, p1, p2);
                             p[0][j] = p0, p[1][j] = p1, p[2][j] = p2;
                         }
 #pragma unroll
-                        for (int j = 0; j < 3; j++) sq[tile][n][j][lane] = p[j];
+                        for (int j = 0; j < 3; j++) sq[tile][n][j][16 * lane_g + lane_row] = p[j];
                     }
                 }
             }
+            rest = __any(small);
             __syncthreads();
         }
         // The next chunk: where there is one, every wave has both its steps in this one.
@@ -574,23 +588,74 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
             if (base >= len) break;
             float e[NR][2][4];
             f32x4 acc[NR][2] = {};
+            if constexpr (A::F16) {
 #pragma unroll
-            for (int n = 0; n < A::QS; n++) {
-                u32x4 key[2];
+                for (int j = 2; j >= 0; j--)
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    if constexpr (A::I8) key[i] = code_bf16(s.k[i][n / 2][2 * (n & 1)], s.k[i][n / 2][2 * (n & 1) + 1]);
-                    else key[i] = s.k[i][n];
+                    for (int n = 0; n < A::QS; n++)
+#pragma unroll
+                        for (int tile = 0; tile < NR; tile++) {
+                            const u32x4 qp = sq[tile][n][j][lane];
+#pragma unroll
+                            for (int i = 0; i < 2; i++)
+                                acc[tile][i] = mma<KV>(s.k[i][n], qp, n || j == 2 ? acc[tile][i] : acc[tile][i] * 0x1p-11f);
+                        }
+                // S^T of q's elements, or of what the parts leave of them, in fp32.
+                auto in_fp32 = [&](f32x4 (&to)[NR][2], bool left) {
+#pragma unroll
+                    for (int n = 0; n < A::QS; n++)
+#pragma unroll
+                        for (int tile = 0; tile < NR; tile++) {
+                            __builtin_amdgcn_sched_barrier(0);  // (one share's registers at a time)
+                            Share x;
+                            share(tile, n, x, true);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                float y = x[j >> 2][j & 3] * up[tile];
+                                if (left) y = split_rest(y);
+#pragma unroll
+                                for (int i = 0; i < 2; i++) {
+                                    uint32_t raw = s.k[i][n][j >> 1];
+                                    asm volatile("" : "+v"(raw));
+                                    to[tile][i] = mma_f32(j & 1 ? f16_hi(raw) : f16_lo(raw), y, to[tile][i]);
+                                }
+                            }
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                if (rest) in_fp32(acc, true);
+                bool nan = false;                               // an infinite key, it may be, times a part that is 0
+#pragma unroll
+                for (int j = 0; j < 8 * NR; j += 2)
+                    nan |= __builtin_isunordered(acc[j >> 3][j >> 2 & 1][j & 3], acc[j >> 3][j >> 2 & 1][(j & 3) + 1]);
+                if (__any(nan)) {
+                    f32x4 whole[NR][2] = {};
+                    in_fp32(whole, false);
+#pragma unroll
+                    for (int j = 0; j < 8 * NR; j++) {
+                        const float x = acc[j >> 3][j >> 2 & 1][j & 3];
+                        acc[j >> 3][j >> 2 & 1][j & 3] = x == x ? x : whole[j >> 3][j >> 2 & 1][j & 3];
+                    }
                 }
+            } else {
 #pragma unroll
-                for (int tile = 0; tile < NR; tile++) {
-                    u32x4 qp[3];
+                for (int n = 0; n < A::QS; n++) {
+                    u32x4 key[2];
 #pragma unroll
-                    for (int j = 0; j < 3; j++) qp[j] = sq[tile][n][j][lane];
+                    for (int i = 0; i < 2; i++) {
+                        if constexpr (A::I8) key[i] = code_bf16(s.k[i][n / 2][2 * (n & 1)], s.k[i][n / 2][2 * (n & 1) + 1]);
+                        else key[i] = s.k[i][n];
+                    }
 #pragma unroll
-                    for (int j = 2; j >= 0; j--)
+                    for (int tile = 0; tile < NR; tile++) {
+                        u32x4 qp[3];
 #pragma unroll
-                        for (int i = 0; i < 2; i++) acc[tile][i] = mma<KV>(key[i], qp[j], acc[tile][i]);
+                        for (int j = 0; j < 3; j++) qp[j] = sq[tile][n][j][lane];
+#pragma unroll
+                        for (int j = 2; j >= 0; j--)
+#pragma unroll
+                            for (int i = 0; i < 2; i++) acc[tile][i] = mma<KV>(key[i], qp[j], acc[tile][i]);
+                    }
                 }
             }
 #pragma unroll

@@ -89,6 +89,7 @@ size_t attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len) 
 
 void launch_attn_paged(const AttnArgs& args, hipStream_t s) {
     AttnArgs a = args;
+    a.scale *= 1.44269504088896341f;                           // scores in powers of 2
     a.group = a.q_heads / a.kv.heads;
     a.page_shift = __builtin_ctz((unsigned)a.kv.page_size);
     a.chunks = chunks_of(a.max_len);

@@ -71,29 +71,22 @@ def test_infinite_values_of_small_weight(dev, dtype, gap, D, T):
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("D,T", [(64, 1), (128, 4), (240, 1)])
 def test_infinite_keys_that_are_seen(dev, dtype, D, T):
-    """A key of -inf in one channel: no weight where the query is positive there, a NaN row where it is negative."""
+    """A key of -inf in one channel: no weight where the query is positive there, however small, and a NaN row where it is
+    negative.  Pages of one position, so that a hole is what has no weight."""
     lens, H = [300, 41], 4
     print("infinite keys", dtype, D, T, flush=True)
-    cache, table, q = setup(dev, dtype, D, H, 2, 16, lens, T)
-    q.view(-1, H, D)[:, :, 3] = torch.tensor([8.0, -8.0, 1e-6, 8.0])
-    at = (table[0, 100 // 16], slice(None), 100 % 16, 3)
-    cache.k[at] = -60000.0
-    ref, bound = (x.view(2, T, H, D) for x in attention(cache, table, q, lens, T, H, 1.0))
-    far = attend(dev, cache, table, q, lens, T, H, scale=1.0).view(2, T, H, D)
-    cache.k[at] = -math.inf
-    got = attend(dev, cache, table, q, lens, T, H, scale=1.0).view(2, T, H, D)
-    assert got[0, :, 1].isnan().all()
-    for h in (0, 3):                                # there a key of -60000 has no weight either
-        assert torch.equal(got[0, :, h], far[0, :, h])
-    assert torch.equal(got[1], far[1])
-    assert torch.isfinite(got[0, :, 2]).all()       # a small positive query there: no weight, the rest as it is
-    got[0, :, 1:3] = 0
-    ref[0, :, 1:3] = 0
-    bound[0, :, 1:3] = 0
-    check_attention(got.view(2 * T, -1), ref.view(2 * T, -1), bound.view(2 * T, -1))
+    cache, table, q = setup(dev, dtype, D, H, 2, 1, lens, T)
+    q.view(-1, H, D)[:, :, 3] = torch.tensor([8.0, -8.0, 1e-6, 1e-14])
+    cache.k[table[0, 100], :, 0, 3] = -math.inf
+    got = attend(dev, cache, table, q, lens, T, H).view(2, T, H, D)
+    table[0, 100] = -1
+    want = attend(dev, cache, table, q, lens, T, H).view(2, T, H, D)
+    assert torch.isfinite(want).all()
+    want[0, :, 1] = math.nan
+    torch.testing.assert_close(got, want, rtol=0, atol=0, equal_nan=True)
 
 
-@pytest.mark.parametrize("dtype", ["bf16", "i8"])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "i8"])
 @pytest.mark.parametrize("ratio", [1e2, 1e3, 1e4, 1e6, 1e9, 1e12, 1e20])
 @pytest.mark.parametrize("D", [48, 128])
 def test_a_query_channel_far_above_the_others(dev, dtype, ratio, D):
@@ -104,6 +97,21 @@ def test_a_query_channel_far_above_the_others(dev, dtype, ratio, D):
     q.view(-1, H, D)[..., 17] = ratio
     cache.k[..., 17] = 0
     check_attention(attend(dev, cache, table, q, lens, T, H), *attention(cache, table, q, lens, T, H, D ** -0.5))
+
+
+def test_an_f16_row_beside_rows_of_other_ranges(dev):
+    """Drafted tokens with and without elements that f16 parts do not hold: each row's bits are those it has alone."""
+    D, H, T, lens = 128, 4, 4, [700, 41]
+    cache, table, q = setup(dev, "f16", D, H, 2, 16, lens, T)
+    qs = q.view(2, T, H, D)
+    qs[:, 1, :, 17] = 1e15
+    qs[:, 2, 1, 5:9] = 1e-20
+    cache.k[..., 17] = 0
+    rows = attend(dev, cache, table, q, lens, T, H).view(2, T, -1)
+    for t in range(T):
+        alone = attend(dev, cache, table, qs[:, t].reshape(2, -1).contiguous(), [n - T + 1 + t for n in lens], 1, H)
+        assert torch.equal(alone, rows[:, t]), t
+    check_attention(rows.view(2 * T, -1), *attention(cache, table, q, lens, T, H, D ** -0.5))
 
 
 @pytest.mark.parametrize("keys,queries", [(-100, 100), (60, -60), (95, -95), (104, -95)])

@@ -88,10 +88,11 @@ class KVCache:
 class PagedAttention:
     """The attention of a decoding program over its layers' caches, with the one workspace it needs.
 
-    caches: a KVCache per layer, all of one shape and type; table: int32 [requests][width]; tokens: the most new
-    tokens per request that attend will see (1..16); max_len: the most positions a request will hold
+    caches: a KVCache per layer, all of one shape (types may differ); table: int32 [requests][width]; tokens: the most
+    new tokens per request that attend will see (1..16); max_len: the most positions a request will hold
     (default: what its row of the table covers); rope: rope_table's, or None (nothing is rotated), whose width is
-    the number of values that turn; interleaved: pairs (2i, 2i + 1) instead of (i, i + rot/2); scale: default dim ** -0.5.
+    the number of values that turn (append skips tokens at positions past its rows); interleaved: pairs (2i, 2i + 1)
+    instead of (i, i + rot/2); scale: default dim ** -0.5.
     These are for the object's life: another table or rotation takes another object, what is in them may change.
     Calls on one PagedAttention share its workspace and so must be ordered: one stream, or synchronised."""
 
@@ -99,8 +100,8 @@ class PagedAttention:
         if not caches:
             raise ValueError("one cache per layer")
         c = caches[0]
-        if any((x.heads, x.dim, x.device) != (c.heads, c.dim, c.device) for x in caches):
-            raise ValueError("the layers' caches must have the same heads, dim and device")
+        if any((x.k.shape, x.device) != (c.k.shape, c.device) for x in caches):
+            raise ValueError("the layers' caches must have the same pages, heads, page size, dim and device")
         if table.dim() != 2 or table.dtype != torch.int32 or table.device != c.device:
             raise ValueError("table must be int32 [requests][pages] on the caches' device")
         if not 1 <= tokens <= _lib.KQ_MAX_BATCH:

@@ -1,0 +1,21 @@
+"""What the paged cache's objects take and refuse (host only)."""
+import pytest
+import torch
+
+from kq import kv
+
+TABLE = torch.zeros(1, 4, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("other", [(4, 32, 2, 64), (4, 8, 2, 64), (5, 16, 2, 64), (4, 16, 4, 64), (4, 16, 2, 128)])
+def test_layers_of_another_shape(other):
+    """One table and one bound serve all layers: pages of another size would hold other positions than they say."""
+    caches = [kv.KVCache(4, 16, 2, 64, "bf16", "cpu"), kv.KVCache(*other, "bf16", "cpu")]
+    for pair in (caches, caches[::-1]):
+        with pytest.raises(ValueError, match="same"):
+            kv.PagedAttention(pair, TABLE, 8)
+
+
+def test_layers_of_one_shape_in_any_order_of_memory_and_type():
+    k, v = (torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16).transpose(1, 2) for _ in range(2))
+    kv.PagedAttention([kv.KVCache.over(k, v), *(kv.KVCache(4, 16, 2, 64, t, "cpu") for t in ("bf16", "f16", "i8"))], TABLE, 4)

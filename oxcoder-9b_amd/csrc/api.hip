@@ -511,7 +511,7 @@ int kq_kv_append(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, i
     KQ_TRY(check_kv(kv, fn));
     KQ_TRY(check_table(kv, table, ldt, seqs, width, fn, &a.table));
     if (N < 0) return fail(KQ_ERR_ARG, "%s: N=%d is negative", fn, N);
-    if ((q != nullptr) != (q_out != nullptr)) return fail(KQ_ERR_ARG, "%s: q and q_out go together", fn);
+    if (N && (q != nullptr) != (q_out != nullptr)) return fail(KQ_ERR_ARG, "%s: q and q_out go together", fn);
     if (q) KQ_TRY(check_q_heads(kv, q_heads, fn));
     if (rope) {
         KQ_TRY(check_ptr(rope, 4, "rope", fn));

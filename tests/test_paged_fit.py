@@ -19,3 +19,10 @@ def test_layers_of_another_shape(other):
 def test_layers_of_one_shape_in_any_order_of_memory_and_type():
     k, v = (torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16).transpose(1, 2) for _ in range(2))
     kv.PagedAttention([kv.KVCache.over(k, v), *(kv.KVCache(4, 16, 2, 64, t, "cpu") for t in ("bf16", "f16", "i8"))], TABLE, 4)
+
+
+def test_append_of_no_token_into_rows_that_are_there():
+    """An empty tensor's address is NULL: no token with an output of more rows than that is still nothing to do."""
+    from test_paged_host import P, append, cache_struct
+    for q, out in ((None, P), (P, None)):
+        assert append(cache_struct(), N=0, k=None, v=None, q=q, q_out=out, seq=None, pos=None) == 0

@@ -41,7 +41,8 @@ class KVCache:
             raise ValueError("dtype must be one of %s" % sorted(DTYPES))
         shape, dt = (pages, heads, page_size, dim), DTYPES[dtype]
         k, v = (torch.zeros(shape, dtype=dt, device=device) for _ in range(2))
-        ks, vs = (torch.zeros(shape[:3], device=device) for _ in range(2)) if dt == torch.int8 else (None, None)
+        ks, vs = ((torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)) if dt == torch.int8
+                  else (None, None))
         self._bind(k, v, ks, vs)
 
     @classmethod
@@ -147,7 +148,7 @@ class PagedAttention:
             raise ValueError("tokens must be 1..%d" % self.tokens)
         c = self.caches[layer]
         if out is None:
-            out = torch.empty((q.shape[0], self.q_heads * c.dim), device=q.device)
+            out = torch.empty((q.shape[0], self.q_heads * c.dim), dtype=torch.float32, device=q.device)
         rc = self._plan and self._calls.attend(self._plan, c.ref, ops._stream(c.device), q, lens, out, T)
         if rc is None:                       # a tensor is not as it should be
             ops.attn_paged(c, self.table, q, lens, out, self.q_heads, T, self.scale, self.max_len, self.ws)

@@ -26,3 +26,23 @@ def test_append_of_no_token_into_rows_that_are_there():
     from test_paged_host import P, append, cache_struct
     for q, out in ((None, P), (P, None)):
         assert append(cache_struct(), N=0, k=None, v=None, q=q, q_out=out, seq=None, pos=None) == 0
+
+
+@pytest.fixture
+def bf16_by_default():
+    torch.set_default_dtype(torch.bfloat16)
+    yield
+    torch.set_default_dtype(torch.float32)
+
+
+def test_scales_are_fp32_whatever_the_default_type(bf16_by_default):
+    cache = kv.KVCache(4, 16, 2, 64, "i8", "cpu")
+    assert cache.k_scale.dtype == cache.v_scale.dtype == torch.float32
+
+
+@pytest.mark.gpu
+def test_outputs_are_fp32_whatever_the_default_type(dev, bf16_by_default):
+    cache = kv.KVCache(4, 16, 2, 64, "bf16", dev)
+    att = kv.PagedAttention([cache], TABLE.to(dev), 4)
+    q, lens = torch.zeros(1, 256, dtype=torch.float32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    assert att.attend(0, q, lens).dtype == torch.float32

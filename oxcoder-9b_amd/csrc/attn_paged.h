@@ -18,12 +18,14 @@
 // f16's range does not hold of an element or a weight far below the largest is made up for by fp32 products.
 // Three products in place of one cost little: the kernel waits for memory.  An 8-bit cache's codes are bf16 values to q and e.
 //
-// Measured: 48 requests of up to 8191 positions, 32 query heads on 8 of 128 bf16 values, pages of 16 (823 MB) 146 us, 5.6 TB/s
+// Measured: 48 requests of up to 8191 positions, 32 query heads on 8 of 128 bf16 values, pages of 16 (823 MB) 145 us, 5.7 TB/s
 // where a bare read of the same places reaches 6.1; matrix units busy 11 % of the time, vector units 24 %, waves wait to
 // issue loads half of theirs and for data a third.  With two of three products left out, with all matrix instructions
 // replaced and with no exponentials the time stays; a part for every chunk (2 KB) instead of every second one costs 9 us, more
-// than its bytes explain.  32 requests of 16384 8-bit positions (572 MB): 131 us, 4.4 TB/s, vector units 52 % (64 conversions and 32
-// byte permutes of the 300 instructions of a step).  Joining in the last workgroup to end, with tickets, in place of a launch of its
+// than its bytes explain.  32 requests of 16384 8-bit positions (572 MB): 135 us, 4.2 TB/s, vector units 56 % (a step converts 64
+// codes of keys and 64 of values a lane, with 64 byte permutes; queries as 24-bit integers of their row's largest would spare the
+// keys' half and measured 131, but leave a small element fewer bits).  f16, 8 drafts of 4 tokens, 16 query heads on 4 of 256
+// values (92 MB): 28 us.  Joining in the last workgroup to end, with tickets, in place of a launch of its
 // own measured slower everywhere (8 requests of 5003, 4 tokens: 34 -> 82 us; 48 requests: 173 -> 181 us).
 #pragma once
 #include <type_traits>

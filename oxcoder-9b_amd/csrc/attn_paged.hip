@@ -95,9 +95,10 @@ void launch_attn_paged(const AttnArgs& args, hipStream_t s) {
     a.chunks = chunks_of(a.max_len);
     a.joined = a.chunks > 1;
     // Where that leaves six workgroups a CU, a workgroup takes two chunks, the second's first step in flight while it ends the first, and
-    // leaves one part for both; four chunks where that leaves sixteen.  One, two, four chunks: 48 requests below 8192
-    // positions 169, 154, 160 us, one request of 100001 86, 82, 88, 32 requests of 16384 8-bit positions 161, 145, 143, 51 requests
-    // of 16 tokens 277, 254, 248; but 8 requests of 5003, 640 chunks in all, 32, 45, 48.
+    // leaves one part for both; four chunks where that leaves sixteen.  One, two, four chunks a workgroup, us, requests
+    // of 4096 positions with 8 heads of 128 values, by the chunks of all: bf16 640 21, 25, 26; 1536 37, 38, 42; 2304 60, 59, 63; 3072
+    // 80, 74, 74; 4608 118, 109, 113; 12288 310, 279, 279; 25600 641, 575, 576; 8-bit 640 19, 22, 29; 1536 31, 30, 36; 2304 41,
+    // 42, 45; 3072 51, 49, 47; 4608 81, 76, 78; 12288 213, 197, 192; 25600 432, 398, 380.
     const int64_t all = (int64_t)a.chunks * a.kv.heads * a.table.seqs * ((a.T * a.group + 15) / 16), cus = device_cus();
     a.paired = a.joined && all >= 12 * cus;
     a.parts = a.paired ? (a.chunks + 1) / 2 : a.chunks;

@@ -344,6 +344,81 @@ int kq_logits_penalize(const float* x, int64_t ldx, int B, int V, const int32_t*
                        const uint32_t* allowed, int64_t ldm, float* y, int64_t ldy, void* ws, size_t ws_bytes,
                        int32_t* picked, void* stream);
 
+/*
+ * Trees of drafted tokens.  A step may feed, in place of one token per request, a tree of up to KQ_MAX_TREE of them:
+ * parents[b][t] (row stride ldp; 0: one tree for all requests) is the node that node t follows, below t itself, or -1 for one
+ * that follows the request's context.  Another value, or one that leads to such a node, makes t no node: nothing is
+ * read, written or seen of it.  base[b] counts the request's positions ahead of the tree; node t lies in slot base[b] + t of the
+ * cache and stands at position base[b] plus the number of its ancestors.  A base below 0: the request sits out.
+ */
+#define KQ_MAX_TREE 64
+
+/*
+ * What the calls of every layer of a step take, from the parents, in one launch: seen[b][t], whose bit j says that node t
+ * sees node j (its ancestors and itself; 0: no node), and for kq_kv_append_norm seq (-1 where there is nothing to
+ * append), pos and slot, all [seqs][T].
+ */
+int kq_tree_plan(const int32_t* parents, int64_t ldp, const int32_t* base, int seqs, int T, uint64_t* seen, int32_t* seq,
+                 int32_t* pos, int32_t* slot, void* stream);
+
+/*
+ * kq_kv_append with norms of queries and keys and a place apart from the position.  Each head's values x of q (of k)
+ * become x * r * q_norm[d] (k_norm[d]), r = 1 / sqrt(sum x^2 / dim + eps), in fp32 before they are rotated by pos[n]; NULL: no norm.
+ * Token n is stored at position slot[n] of its request (NULL: at pos[n]); it is skipped as kq_kv_append says, with slot in
+ * the place of pos for the request's positions.  Without norms and slot the results are kq_kv_append's.
+ */
+int kq_kv_append_norm(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, int N, const int32_t* seq,
+                      const int32_t* pos, const int32_t* slot, const float* q, int64_t ldq, int q_heads, float* q_out,
+                      int64_t ldqo, const float* k, int64_t ldk, const float* v, int64_t ldv, const float* rope, int rope_rows,
+                      int rot, int interleaved, const float* q_norm, const float* k_norm, float eps, void* stream);
+
+/* Bytes of device workspace kq_attn_tree needs (0 for invalid sizes). */
+size_t kq_attn_tree_workspace(int seqs, int q_heads, int dim, int T, int max_len);
+
+/*
+ * kq_attn_paged for trees of T (1..KQ_MAX_TREE) nodes: row b * T + t of q and out is node t of request b, which sees the
+ * positions below base[b] and slot base[b] + j for each bit j of seen[b * T + t] (kq_tree_plan's); its own word 0, or a base
+ * below 0: it sees nothing, and its row is 0.  Positions from max_len on, or past the table's, are not there.
+ * What lies in positions that a row does not see, infinities and NaN too, has no effect on it.
+ */
+int kq_attn_tree(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, const int32_t* base,
+                 const uint64_t* seen, int max_len, int T, const float* q, int64_t ldq, int q_heads, float scale, float* out,
+                 int64_t ldo, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Keep the accepted nodes of each request in the caches of `layers` layers (kv[i], alike in heads, dim, pages and
+ * page_size): path[b][0..] (row stride ldp, T entries) names nodes in rising order, node path[b][i] >= i, and ends at the first entry
+ * that does not (-1, say); the entry at position base[b] + path[b][i] moves to base[b] + i, k, v and scales as they are.
+ * Where either lies in a hole or past the table nothing is moved.
+ */
+int kq_kv_keep(const kq_kv* const* kv, int layers, const int32_t* table, int64_t ldt, int seqs, int width, const int32_t* base,
+               const int32_t* path, int64_t ldp, int T, void* stream);
+
+/* Bytes of device workspace kq_verify needs (0 for invalid sizes). */
+size_t kq_verify_workspace(int B, int T, int V);
+
+/*
+ * Which drafted tokens of B trees of T nodes the target's probabilities accept, and the token that follows.  Node 0 is the
+ * root (parents[b][0] = -1; another value: the request sits out, accepted and token -1), a token that is settled; the others are drafts
+ * tokens[b][t] (row stride ldt; outside 0..V-1: none), each after its parent (ldp 0: one tree for all).  Row b * T + t of x (V
+ * logits, stride ldx) follows node t: p = softmax(x / temperature[b]) (NULL: 1; not above 0: the largest logit alone, the
+ * first of equal ones).  A logit of -inf or NaN has no probability.
+ *
+ * From the root on, a node's children are tried in rising order, with u = uniform[b][child] in [0, 1) (row stride ldu), Z = 1:
+ *   draft NULL:  accepted where u Z < p(token); else the token leaves: p(token) = 0, Z -= p(token);
+ *   draft given: its row b * T + t (V probabilities, stride ldd) is what the children of node t were drawn from, each by
+ *                itself: accepted where u Z q(token) < max(p(token) - a q(token), 0), a = 0 at first; else a += Z and
+ *                Z = sum max(p - a q, 0).
+ * An accepted child is the next node; where none is, token[b] is the smallest id at which the running sum of what is left
+ * exceeds uniform[b][0] times its total (of p, where nothing is left; -1 where p has no probability anywhere).  So tokens come with
+ * the target's own probabilities.  path[b][0..T-1] receives the nodes from the root on, then -1; accepted[b] their number without the
+ * root.  Weights and sums are held in 64 bits.  ws: 256-byte aligned, kq_verify_workspace bytes; calls sharing it
+ * must be ordered.  B * T up to 65535.
+ */
+int kq_verify(const float* x, int64_t ldx, int B, int T, int V, const int32_t* tokens, int64_t ldt, const int32_t* parents,
+              int64_t ldp, const float* uniform, int64_t ldu, const float* temperature, const float* draft, int64_t ldd,
+              int32_t* accepted, int32_t* path, int32_t* token, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

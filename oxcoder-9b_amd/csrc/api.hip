@@ -502,11 +502,10 @@ static int check_q_heads(const kq_kv* kv, int q_heads, const char* fn) {
     return KQ_OK;
 }
 
-int kq_kv_append(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, int N, const int32_t* seq,
-                 const int32_t* pos, const float* q, int64_t ldq, int q_heads, float* q_out, int64_t ldqo, const float* k,
-                 int64_t ldk, const float* v, int64_t ldv, const float* rope, int rope_rows, int rot, int interleaved,
-                 void* stream) {
-    static const char* fn = "kq_kv_append";
+static int append(const char* fn, const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, int N,
+                  const int32_t* seq, const int32_t* pos, const int32_t* slot, const float* q, int64_t ldq, int q_heads,
+                  float* q_out, int64_t ldqo, const float* k, int64_t ldk, const float* v, int64_t ldv, const float* rope,
+                  int rope_rows, int rot, int interleaved, const float* q_norm, const float* k_norm, float eps, void* stream) {
     AppendArgs a = {};
     KQ_TRY(check_kv(kv, fn));
     KQ_TRY(check_table(kv, table, ldt, seqs, width, fn, &a.table));
@@ -519,7 +518,11 @@ int kq_kv_append(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, i
             return fail(KQ_ERR_ARG, "%s: rot=%d must be a multiple of 8 up to dim=%d", fn, rot, kv->dim);
         if (rope_rows < 1) return fail(KQ_ERR_ARG, "%s: rope_rows=%d must be positive", fn, rope_rows);
     }
+    if (q_norm) KQ_TRY(check_ptr(q_norm, 4, "q_norm", fn));
+    if (k_norm) KQ_TRY(check_ptr(k_norm, 4, "k_norm", fn));
+    if ((q_norm || k_norm) && !(eps >= 0 && eps - eps == 0)) return fail(KQ_ERR_ARG, "%s: eps must be finite, at least 0", fn);
     if (N == 0) return KQ_OK;
+    if (slot) KQ_TRY(check_ptr(slot, 4, "slot", fn));
     KQ_TRY(check_ptr(seq, 4, "seq", fn));
     KQ_TRY(check_ptr(pos, 4, "pos", fn));
     const int64_t kw = (int64_t)kv->heads * kv->dim, qw = (int64_t)q_heads * kv->dim;
@@ -537,10 +540,87 @@ int kq_kv_append(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, i
     a.rope_rows = rope_rows;
     a.rot = rope ? rot : 0;
     a.interleaved = interleaved;
-    a.seq = seq, a.pos = pos, a.q = q, a.k = k, a.v = v, a.rope = rope, a.q_out = q_out;
+    a.seq = seq, a.pos = pos, a.slot = slot, a.q = q, a.k = k, a.v = v, a.rope = rope, a.q_out = q_out;
     a.ldq = ldq, a.ldqo = ldqo, a.ldk = ldk, a.ldv = ldv;
+    a.q_norm = q ? q_norm : nullptr, a.k_norm = k_norm, a.eps = eps;
     launch_kv_append(a, as_stream(stream));
     return check_launch(fn);
+}
+
+int kq_kv_append(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, int N, const int32_t* seq,
+                 const int32_t* pos, const float* q, int64_t ldq, int q_heads, float* q_out, int64_t ldqo, const float* k,
+                 int64_t ldk, const float* v, int64_t ldv, const float* rope, int rope_rows, int rot, int interleaved,
+                 void* stream) {
+    return append("kq_kv_append", kv, table, ldt, seqs, width, N, seq, pos, nullptr, q, ldq, q_heads, q_out, ldqo, k, ldk, v, ldv,
+                  rope, rope_rows, rot, interleaved, nullptr, nullptr, 0.0f, stream);
+}
+
+int kq_kv_append_norm(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, int N, const int32_t* seq,
+                      const int32_t* pos, const int32_t* slot, const float* q, int64_t ldq, int q_heads, float* q_out,
+                      int64_t ldqo, const float* k, int64_t ldk, const float* v, int64_t ldv, const float* rope, int rope_rows,
+                      int rot, int interleaved, const float* q_norm, const float* k_norm, float eps, void* stream) {
+    return append("kq_kv_append_norm", kv, table, ldt, seqs, width, N, seq, pos, slot, q, ldq, q_heads, q_out, ldqo, k, ldk, v,
+                  ldv, rope, rope_rows, rot, interleaved, q_norm, k_norm, eps, stream);
+}
+
+static int check_tree(int seqs, int T, const char* fn) {
+    if (seqs < 1 || seqs > 65535) return fail(KQ_ERR_ARG, "%s: seqs=%d must be 1..65535", fn, seqs);
+    if (T < 1 || T > KQ_MAX_TREE) return fail(KQ_ERR_ARG, "%s: T=%d must be 1..%d", fn, T, KQ_MAX_TREE);
+    return KQ_OK;
+}
+
+// Row strides of parents: 0 is one row for all.
+static int check_parents(const int32_t* parents, int64_t ldp, int T, const char* fn) {
+    KQ_TRY(check_ptr(parents, 4, "parents", fn));
+    if (ldp < 0 || (ldp > 0 && ldp < T)) return fail(KQ_ERR_ARG, "%s: ldp=%lld must be 0 or at least T=%d", fn, (long long)ldp, T);
+    return KQ_OK;
+}
+
+int kq_tree_plan(const int32_t* parents, int64_t ldp, const int32_t* base, int seqs, int T, uint64_t* seen, int32_t* seq,
+                 int32_t* pos, int32_t* slot, void* stream) {
+    static const char* fn = "kq_tree_plan";
+    KQ_TRY(check_tree(seqs, T, fn));
+    KQ_TRY(check_parents(parents, ldp, T, fn));
+    KQ_TRY(check_ptr(base, 4, "base", fn));
+    KQ_TRY(check_ptr(seen, 8, "seen", fn));
+    KQ_TRY(check_ptr(seq, 4, "seq", fn));
+    KQ_TRY(check_ptr(pos, 4, "pos", fn));
+    KQ_TRY(check_ptr(slot, 4, "slot", fn));
+    launch_tree_plan(TreeArgs{parents, base, ldp, T, seen, seq, pos, slot}, seqs, as_stream(stream));
+    return check_launch(fn);
+}
+
+int kq_kv_keep(const kq_kv* const* kv, int layers, const int32_t* table, int64_t ldt, int seqs, int width, const int32_t* base,
+               const int32_t* path, int64_t ldp, int T, void* stream) {
+    static const char* fn = "kq_kv_keep";
+    if (!kv || layers < 1) return fail(KQ_ERR_ARG, "%s: no layer", fn);
+    KeepArgs a = {};
+    for (int i = 0; i < layers; i++) {
+        KQ_TRY(check_kv(kv[i], fn));
+        if (kv[i]->heads != kv[0]->heads || kv[i]->dim != kv[0]->dim || kv[i]->pages != kv[0]->pages ||
+            kv[i]->page_size != kv[0]->page_size)
+            return fail(KQ_ERR_ARG, "%s: the layers' caches must have the same heads, dim, pages and page_size", fn);
+    }
+    KQ_TRY(check_table(kv[0], table, ldt, seqs, width, fn, &a.table));
+    KQ_TRY(check_tree(seqs, T, fn));
+    KQ_TRY(check_ptr(base, 4, "base", fn));
+    KQ_TRY(check_rows(path, ldp, seqs, T, "path", fn));
+    a.base = base, a.path = path, a.ldp = ldp, a.T = T;
+    a.pages = kv[0]->pages, a.page_size = kv[0]->page_size;
+    for (int i0 = 0; i0 < layers; i0 += KEEP_LAYERS) {
+        const int n = layers - i0 < KEEP_LAYERS ? layers - i0 : KEEP_LAYERS;
+        for (int i = 0; i < n; i++) {
+            const kq_kv* c = kv[i0 + i];
+            const bool i8 = c->type == KQ_KV_I8;
+            const int64_t e = i8 ? 1 : 2;
+            a.layer[i] = KeepLayer{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), i8 ? c->k_scale : nullptr,
+                                   i8 ? c->v_scale : nullptr, c->page_stride * e, c->head_stride * e, c->pos_stride * e,
+                                   c->scale_page_stride, c->scale_head_stride, c->scale_pos_stride, (int)(c->dim * e), c->heads};
+        }
+        launch_kv_keep(a, n, seqs, as_stream(stream));
+        KQ_TRY(check_launch(fn));
+    }
+    return KQ_OK;
 }
 
 size_t kq_attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len) {
@@ -550,16 +630,16 @@ size_t kq_attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_le
     return attn_paged_workspace(seqs, q_heads, dim, T, max_len);
 }
 
-int kq_attn_paged(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, const int32_t* lens,
-                  int max_len, int T, const float* q, int64_t ldq, int q_heads, float scale, float* out, int64_t ldo,
-                  void* ws, size_t ws_bytes, void* stream) {
-    static const char* fn = "kq_attn_paged";
+// lens: of trees (seen given) their bases.
+static int attention(const char* fn, const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width,
+                     const int32_t* lens, const uint64_t* seen, int max_len, int T, const float* q, int64_t ldq, int q_heads,
+                     float scale, float* out, int64_t ldo, void* ws, size_t ws_bytes, void* stream) {
     AttnArgs a = {};
     KQ_TRY(check_kv(kv, fn));
     KQ_TRY(check_table(kv, table, ldt, seqs, width, fn, &a.table));
     KQ_TRY(check_q_heads(kv, q_heads, fn));
-    KQ_TRY(check_ptr(lens, 4, "lens", fn));
-    if (T < 1 || T > KQ_MAX_BATCH) return fail(KQ_ERR_ARG, "%s: T=%d must be 1..%d", fn, T, KQ_MAX_BATCH);
+    KQ_TRY(check_ptr(lens, 4, seen ? "base" : "lens", fn));
+    if (!seen && (T < 1 || T > KQ_MAX_BATCH)) return fail(KQ_ERR_ARG, "%s: T=%d must be 1..%d", fn, T, KQ_MAX_BATCH);
     if (max_len < 1 || max_len > (1 << 30)) return fail(KQ_ERR_ARG, "%s: max_len=%d must be 1..2^30", fn, max_len);
     const int64_t rows = (int64_t)seqs * T, qw = (int64_t)q_heads * kv->dim;
     KQ_TRY(check_rows(q, ldq, rows, qw, "q", fn));
@@ -571,6 +651,7 @@ int kq_attn_paged(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, 
         return fail(KQ_ERR_ARG, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, need);
     a.kv = *kv;
     a.lens = lens;
+    a.seen = seen;
     a.max_len = max_len < a.table.cap ? max_len : a.table.cap;
     a.T = T;
     a.q_heads = q_heads;
@@ -578,6 +659,63 @@ int kq_attn_paged(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, 
     a.scale = scale;
     a.ws = static_cast<uint8_t*>(ws);
     launch_attn_paged(a, as_stream(stream));
+    return check_launch(fn);
+}
+
+int kq_attn_paged(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, const int32_t* lens,
+                  int max_len, int T, const float* q, int64_t ldq, int q_heads, float scale, float* out, int64_t ldo,
+                  void* ws, size_t ws_bytes, void* stream) {
+    return attention("kq_attn_paged", kv, table, ldt, seqs, width, lens, nullptr, max_len, T, q, ldq, q_heads, scale, out, ldo, ws,
+                     ws_bytes, stream);
+}
+
+size_t kq_attn_tree_workspace(int seqs, int q_heads, int dim, int T, int max_len) {
+    if (seqs < 1 || seqs > 65535 || q_heads < 1 || q_heads > 4096 || dim < 16 || dim > 256 || dim % 16 || T < 1 ||
+        T > KQ_MAX_TREE || max_len < 1 || max_len > (1 << 30))
+        return 0;
+    return attn_paged_workspace(seqs, q_heads, dim, T, max_len);
+}
+
+int kq_attn_tree(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, const int32_t* base,
+                 const uint64_t* seen, int max_len, int T, const float* q, int64_t ldq, int q_heads, float scale, float* out,
+                 int64_t ldo, void* ws, size_t ws_bytes, void* stream) {
+    static const char* fn = "kq_attn_tree";
+    KQ_TRY(check_tree(seqs, T, fn));
+    KQ_TRY(check_ptr(base, 4, "base", fn));
+    KQ_TRY(check_ptr(seen, 8, "seen", fn));
+    return attention(fn, kv, table, ldt, seqs, width, base, seen, max_len, T, q, ldq, q_heads, scale, out, ldo, ws, ws_bytes, stream);
+}
+
+size_t kq_verify_workspace(int B, int T, int V) {
+    if (B < 1 || T < 1 || T > KQ_MAX_TREE || V < 1 || V > (1 << 30) || (int64_t)B * T > 65535) return 0;
+    return verify_workspace(B, T, V);
+}
+
+int kq_verify(const float* x, int64_t ldx, int B, int T, int V, const int32_t* tokens, int64_t ldt, const int32_t* parents,
+              int64_t ldp, const float* uniform, int64_t ldu, const float* temperature, const float* draft, int64_t ldd,
+              int32_t* accepted, int32_t* path, int32_t* token, void* ws, size_t ws_bytes, void* stream) {
+    static const char* fn = "kq_verify";
+    KQ_TRY(check_tree(B, T, fn));
+    if ((int64_t)B * T > 65535) return fail(KQ_ERR_ARG, "%s: %d trees of %d nodes must be up to 65535 rows", fn, B, T);
+    if (V < 1 || V > (1 << 30)) return fail(KQ_ERR_ARG, "%s: V=%d must be 1..2^30", fn, V);
+    KQ_TRY(check_rows(x, ldx, (int64_t)B * T, V, "x", fn));
+    KQ_TRY(check_rows(tokens, ldt, B, T, "tokens", fn));
+    KQ_TRY(check_parents(parents, ldp, T, fn));
+    KQ_TRY(check_rows(uniform, ldu, B, T, "uniform", fn));
+    if (temperature) KQ_TRY(check_ptr(temperature, 4, "temperature", fn));
+    if (draft) KQ_TRY(check_rows(draft, ldd, (int64_t)B * T, V, "draft", fn));
+    KQ_TRY(check_ptr(accepted, 4, "accepted", fn));
+    KQ_TRY(check_ptr(path, 4, "path", fn));
+    KQ_TRY(check_ptr(token, 4, "token", fn));
+    KQ_TRY(check_ptr(ws, 256, "ws", fn));
+    const size_t need = verify_workspace(B, T, V);
+    if (ws_bytes < need) return fail(KQ_ERR_ARG, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, need);
+    VerifyArgs a = {};
+    a.x = x, a.ldx = ldx, a.B = B, a.T = T, a.V = V;
+    a.tokens = tokens, a.ldt = ldt, a.parents = parents, a.ldp = ldp, a.uniform = uniform, a.ldu = ldu;
+    a.temperature = temperature, a.draft = draft, a.ldd = ldd;
+    a.accepted = accepted, a.path = path, a.token = token, a.ws = static_cast<uint8_t*>(ws);
+    launch_verify(a, as_stream(stream));
     return check_launch(fn);
 }
 

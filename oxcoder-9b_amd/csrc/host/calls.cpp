@@ -19,7 +19,7 @@ struct Plan {
     int64_t ldt;
     int seqs, width, q_heads, heads, dim, max_len, rope_rows, rot, interleaved;
     const float* rope;
-    float scale;
+    float scale, eps;
     void* ws;
     size_t ws_bytes;
 };
@@ -86,15 +86,15 @@ PyObject* guarded(F f) {
 
 bool sizes_fit(int64_t a, int64_t b = 0) { return a <= INT_MAX && b <= INT_MAX; }
 
-// plan(table, rope, q_heads, heads, dim, max_len, interleaved, scale, ws): table (pointer, row stride, rows, columns),
+// plan(table, rope, q_heads, heads, dim, max_len, interleaved, scale, eps, ws): table (pointer, row stride, rows, columns),
 // rope (pointer or None, rows, columns), ws (pointer, bytes)
 PyObject* plan(PyObject*, PyObject* args) {
     Plan p = {};
     PyObject *table, *rope, *ws;
     long long ldt = 0;
     Py_ssize_t bytes = 0;
-    if (!PyArg_ParseTuple(args, "(OLii)(Oii)iiiiif(On)", &table, &ldt, &p.seqs, &p.width, &rope, &p.rope_rows, &p.rot, &p.q_heads,
-                          &p.heads, &p.dim, &p.max_len, &p.interleaved, &p.scale, &ws, &bytes))
+    if (!PyArg_ParseTuple(args, "(OLii)(Oii)iiiiiff(On)", &table, &ldt, &p.seqs, &p.width, &rope, &p.rope_rows, &p.rot, &p.q_heads,
+                          &p.heads, &p.dim, &p.max_len, &p.interleaved, &p.scale, &p.eps, &ws, &bytes))
         return nullptr;
     p.ldt = ldt;
     p.ws_bytes = (size_t)bytes;
@@ -107,13 +107,16 @@ PyObject* plan(PyObject*, PyObject* args) {
     return PyCapsule_New(held, "kq plan", drop_plan);
 }
 
-// append(plan, cache, stream, q, k, v, seq, pos, q_out)
+// append(plan, cache, stream, q, k, v, seq, pos, q_out), and append_norm with slot, q_norm and k_norm (pointers or None) behind
+template <bool NORM>
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        if (n != 9) Py_RETURN_NONE;
+        if (n != (NORM ? 12 : 9)) Py_RETURN_NONE;
         const Plan* p = plan_of(a[0]);
         const auto* kv = static_cast<const kq_kv*>(pointer(a[1]));
         void* stream = pointer(a[2]);
+        const float *q_norm = nullptr, *k_norm = nullptr;
+        if (NORM) q_norm = static_cast<const float*>(pointer(a[10])), k_norm = static_cast<const float*>(pointer(a[11]));
         if (PyErr_Occurred()) return nullptr;
         Look see;
         const int64_t N = see.rows(a[4]);
@@ -128,11 +131,16 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const float* v = see.mat<float>(a[5], F32, N, (int64_t)p->heads * p->dim, &ldv);
         const int32_t* seq = see.list<int32_t>(a[6], I32, N, true);
         const int32_t* pos = see.list<int32_t>(a[7], I32, N, true);
+        const int32_t* slot = NORM ? see.list<int32_t>(a[9], I32, N, false) : nullptr;
         if (!see.ok || !sizes_fit(N)) Py_RETURN_NONE;
         int rc;
         Py_BEGIN_ALLOW_THREADS
-        rc = kq_kv_append(kv, p->table, p->ldt, p->seqs, p->width, (int)N, seq, pos, q, ldq, p->q_heads, out, ldo,
-            k, ldk, v, ldv, p->rope, p->rope_rows, p->rot, p->interleaved, stream);
+        if (NORM)
+            rc = kq_kv_append_norm(kv, p->table, p->ldt, p->seqs, p->width, (int)N, seq, pos, slot, q, ldq, p->q_heads, out, ldo,
+                k, ldk, v, ldv, p->rope, p->rope_rows, p->rot, p->interleaved, q_norm, k_norm, p->eps, stream);
+        else
+            rc = kq_kv_append(kv, p->table, p->ldt, p->seqs, p->width, (int)N, seq, pos, q, ldq, p->q_heads, out, ldo,
+                k, ldk, v, ldv, p->rope, p->rope_rows, p->rot, p->interleaved, stream);
         Py_END_ALLOW_THREADS
         return PyLong_FromLong(rc);
     });
@@ -213,10 +221,129 @@ PyObject* pick(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// Parents of B trees of T nodes: a row each, or one for all (stride 0).
+const int32_t* parents_of(Look& see, PyObject* o, int64_t B, int64_t T, int64_t* ld) {
+    const bool shared = B > 1 && see.rows(o) == 1;
+    const int32_t* p = see.mat<int32_t>(o, I32, shared ? 1 : B, T, ld);
+    if (shared) *ld = 0;
+    else if (B == 1) *ld = T;
+    return p;
+}
+
+// tree_plan(seen, seq, pos, slot, stream, parents, base, requests, nodes)
+PyObject* tree_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 9) Py_RETURN_NONE;
+        auto* seen = static_cast<uint64_t*>(pointer(a[0]));
+        auto *seq = static_cast<int32_t*>(pointer(a[1])), *pos = static_cast<int32_t*>(pointer(a[2])),
+             *slot = static_cast<int32_t*>(pointer(a[3]));
+        void* stream = pointer(a[4]);
+        const long B = PyLong_AsLong(a[7]), T = PyLong_AsLong(a[8]);
+        if (PyErr_Occurred()) return nullptr;
+        Look see;
+        int64_t ldp = 0;
+        const int32_t* parents = parents_of(see, a[5], B, T, &ldp);
+        const int32_t* base = see.list<int32_t>(a[6], I32, B, true);
+        if (!see.ok) Py_RETURN_NONE;
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = kq_tree_plan(parents, ldp, base, (int)B, (int)T, seen, seq, pos, slot, stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(rc);
+    });
+}
+
+// attend_tree(plan, cache, stream, q, base, seen (pointer), out, nodes)
+PyObject* attend_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 8) Py_RETURN_NONE;
+        const Plan* p = plan_of(a[0]);
+        const auto* kv = static_cast<const kq_kv*>(pointer(a[1]));
+        void* stream = pointer(a[2]);
+        const auto* seen = static_cast<const uint64_t*>(pointer(a[5]));
+        const long T = PyLong_AsLong(a[7]);
+        if (PyErr_Occurred()) return nullptr;
+        if (T < 1 || T > KQ_MAX_TREE) Py_RETURN_NONE;
+        Look see;
+        int64_t ldq = 0, ldo = 0;
+        const int64_t rows = (int64_t)p->seqs * T, cols = (int64_t)p->q_heads * p->dim;
+        const float* q = see.mat<float>(a[3], F32, rows, cols, &ldq);
+        float* out = see.mat<float>(a[6], F32, rows, cols, &ldo);
+        const int32_t* base = see.list<int32_t>(a[4], I32, p->seqs, true);
+        if (!see.ok) Py_RETURN_NONE;
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = kq_attn_tree(kv, p->table, p->ldt, p->seqs, p->width, base, seen, p->max_len, (int)T, q, ldq, p->q_heads,
+            p->scale, out, ldo, p->ws, p->ws_bytes, stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(rc);
+    });
+}
+
+// keep(plan, caches (pointer to their pointers), layers, stream, path, base)
+PyObject* keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 6) Py_RETURN_NONE;
+        const Plan* p = plan_of(a[0]);
+        const auto* kv = static_cast<const kq_kv* const*>(pointer(a[1]));
+        const long layers = PyLong_AsLong(a[2]);
+        void* stream = pointer(a[3]);
+        if (PyErr_Occurred()) return nullptr;
+        Look see;
+        int64_t ldp = 0;
+        const int64_t T = see.cols(a[4]);
+        const int32_t* path = see.mat<int32_t>(a[4], I32, p->seqs, T, &ldp);
+        const int32_t* base = see.list<int32_t>(a[5], I32, p->seqs, true);
+        if (!see.ok || !sizes_fit(T)) Py_RETURN_NONE;
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = kq_kv_keep(kv, (int)layers, p->table, p->ldt, p->seqs, p->width, base, path, ldp, (int)T, stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(rc);
+    });
+}
+
+// verify(accepted, path, token, ws, ws_bytes, stream, logits, tokens, parents, uniform, temperature, draft)
+PyObject* verify(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 12) Py_RETURN_NONE;
+        auto *accepted = static_cast<int32_t*>(pointer(a[0])), *path = static_cast<int32_t*>(pointer(a[1])),
+             *token = static_cast<int32_t*>(pointer(a[2]));
+        void *ws = pointer(a[3]), *stream = pointer(a[5]);
+        const size_t bytes = PyLong_AsSize_t(a[4]);
+        if (PyErr_Occurred()) return nullptr;
+        Look see;
+        const int64_t B = see.rows(a[7]), T = see.cols(a[7]), V = see.cols(a[6]);
+        if (!see.ok || !sizes_fit(B, V) || !sizes_fit(T)) Py_RETURN_NONE;
+        int64_t ldx = 0, ldt = 0, ldp = 0, ldu = 0, ldd = 0;
+        const float* x = see.mat<float>(a[6], F32, B * T, V, &ldx);
+        const int32_t* tokens = see.mat<int32_t>(a[7], I32, B, T, &ldt);
+        const int32_t* parents = parents_of(see, a[8], B, T, &ldp);
+        const float* uniform = see.mat<float>(a[9], F32, B, T, &ldu);
+        const float* temperature = see.list<float>(a[10], F32, B, false);
+        const float* draft = a[11] == Py_None ? nullptr : see.mat<float>(a[11], F32, B * T, V, &ldd);
+        if (!see.ok) Py_RETURN_NONE;
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = kq_verify(x, ldx, (int)B, (int)T, (int)V, tokens, ldt, parents, ldp, uniform, ldu, temperature, draft, ldd,
+            accepted, path, token, ws, bytes, stream);
+        Py_END_ALLOW_THREADS
+        return PyLong_FromLong(rc);
+    });
+}
+
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(F)); }
+
 PyMethodDef methods[] = {{"plan", plan, METH_VARARGS, nullptr},
-                         {"append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(append)), METH_FASTCALL, nullptr},
-                         {"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attend)), METH_FASTCALL, nullptr},
-                         {"pick", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(pick)), METH_FASTCALL, nullptr},
+                         {"append", fast<append<false>>(), METH_FASTCALL, nullptr},
+                         {"append_norm", fast<append<true>>(), METH_FASTCALL, nullptr},
+                         {"attend", fast<attend>(), METH_FASTCALL, nullptr},
+                         {"pick", fast<pick>(), METH_FASTCALL, nullptr},
+                         {"tree_plan", fast<tree_plan>(), METH_FASTCALL, nullptr},
+                         {"attend_tree", fast<attend_tree>(), METH_FASTCALL, nullptr},
+                         {"keep", fast<keep>(), METH_FASTCALL, nullptr},
+                         {"verify", fast<verify>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", "Token-loop calls of libkq.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

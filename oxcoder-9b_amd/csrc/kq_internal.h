@@ -121,8 +121,10 @@ struct AppendArgs {
     kq_kv kv;
     PageTable table;
     int N, q_heads, rope_rows, rot, interleaved;
-    const int32_t *seq, *pos;
+    const int32_t *seq, *pos, *slot;            // slot: where a token is stored, NULL: at its position
     const float *q, *k, *v, *rope;
+    const float *q_norm, *k_norm;               // NULL: no norm
+    float eps;
     float* q_out;
     int64_t ldq, ldqo, ldk, ldv;
 };
@@ -133,7 +135,8 @@ struct AttnMl {
 struct AttnArgs {
     kq_kv kv;
     PageTable table;
-    const int32_t* lens;
+    const int32_t* lens;       // of a tree: where its first slot lies
+    const uint64_t* seen;      // [request][token]: the nodes that each node of a tree sees; NULL: the tokens are a chain
     int max_len, T, q_heads;
     const float* q;
     int64_t ldq, ldo;
@@ -148,10 +151,53 @@ struct AttnArgs {
     float* po;
     AttnMl* pml;
 };
-template <class KV>
+template <class KV, bool TREE>
 void launch_attn_part(const AttnArgs& a, hipStream_t s);
 size_t attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len);
 void launch_attn_paged(const AttnArgs& a, hipStream_t s);
+// A tree of drafted tokens (kv_tree.hip).
+constexpr int TREE_MOST = KQ_MAX_TREE;
+struct TreeArgs {
+    const int32_t *parents, *base;
+    int64_t ldp;
+    int T;
+    uint64_t* seen;
+    int32_t *seq, *pos, *slot;
+};
+void launch_tree_plan(const TreeArgs& a, int seqs, hipStream_t s);
+// A layer's cache as the kernel that moves entries takes it, in bytes.
+struct KeepLayer {
+    uint8_t *k, *v;
+    float *k_scale, *v_scale;
+    int64_t page, head, pos, scale_page, scale_head, scale_pos;
+    int row, heads;            // bytes of one head's entry
+};
+constexpr int KEEP_LAYERS = 32;
+struct KeepArgs {
+    KeepLayer layer[KEEP_LAYERS];
+    PageTable table;
+    const int32_t *base, *path;
+    int64_t ldp;
+    int T, pages, page_size;
+};
+void launch_kv_keep(const KeepArgs& a, int layers, int seqs, hipStream_t s);
+struct VerifyPart {
+    double sum;                // of 2^((x - m) scale)
+    float m;                   // the largest logit of a slice
+    int at;                    // its first place in the row
+};
+struct VerifyArgs {
+    const float *x, *draft, *uniform, *temperature;
+    const int32_t *tokens, *parents;
+    int64_t ldx, ldd, ldu, ldt, ldp;
+    int B, T, V;
+    int32_t *accepted, *path, *token;
+    uint8_t* ws;
+    // set by launch_verify
+    int slice, slices;         // ids of a slice, slices of a row
+};
+size_t verify_workspace(int B, int T, int V);
+void launch_verify(const VerifyArgs& a, hipStream_t s);
 struct LogitsArgs {
     const float* x;
     int64_t ldx, ldh, ldb, ldm, ldy;

@@ -40,7 +40,8 @@ __device__ __forceinline__ void store8(typename KV::T* p, int gap, f32x4 a, f32x
     }
 }
 
-template <class KV, bool V4>
+// NORMS: queries and keys may be normed, and stored apart from their position (kq_kv_append_norm).
+template <class KV, bool V4, bool NORMS>
 __global__ void __launch_bounds__(256) k_kv_append(AppendArgs a, int lanes) {
     const int D = a.kv.dim, H = a.q_heads + 2 * a.kv.heads;
     const int per = 256 / lanes;                              // heads per workgroup
@@ -48,8 +49,8 @@ __global__ void __launch_bounds__(256) k_kv_append(AppendArgs a, int lanes) {
     const int i = threadIdx.x % lanes;                        // group of 8 values in the head
     if (head >= (int64_t)a.N * H) return;                     // whole lane groups end together
     const int n = (int)(head / H), h = (int)(head % H);
-    const int pos = a.pos[n], seq = a.seq[n];
-    if (seq < 0 || seq >= a.table.seqs || pos < 0 || pos >= a.table.cap || (a.rot && pos >= a.rope_rows)) return;
+    const int pos = a.pos[n], seq = a.seq[n], slot = NORMS && a.slot ? a.slot[n] : pos;
+    if (seq < 0 || seq >= a.table.seqs || slot < 0 || slot >= a.table.cap || (a.rot && (pos < 0 || pos >= a.rope_rows))) return;
     const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + a.kv.heads;
     const int kh = is_q ? 0 : h - a.q_heads - (is_v ? a.kv.heads : 0);
     const float* x = is_q ? a.q + (int64_t)n * a.ldq + (int64_t)h * D
@@ -62,6 +63,22 @@ __global__ void __launch_bounds__(256) k_kv_append(AppendArgs a, int lanes) {
     if (live) {
         lo = ld4f<V4>(x + at);
         hi = ld4f<V4>(x + at + gap);
+    }
+    if constexpr (NORMS) {
+        const float* w = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;
+        if (w) {                                              // the same for a head's lanes
+            float ss = ((lo.x * lo.x + lo.y * lo.y) + (lo.z * lo.z + lo.w * lo.w)) +
+                       ((hi.x * hi.x + hi.y * hi.y) + (hi.z * hi.z + hi.w * hi.w));
+            f32x4 wl = {0, 0, 0, 0}, wh = {0, 0, 0, 0};
+            if (live) {
+                wl = ld4f<V4>(w + at);
+                wh = ld4f<V4>(w + at + gap);
+            }
+            for (int i = lanes >> 1; i; i >>= 1) ss += __shfl_xor(ss, i, 64);
+            const float r = 1.0f / sqrtf(ss / (float)D + a.eps);
+            lo = lo * r * wl;
+            hi = hi * r * wh;
+        }
     }
     if (live && turns) {
         const float* r = a.rope + (int64_t)pos * a.rot + 4 * i;
@@ -88,9 +105,9 @@ __global__ void __launch_bounds__(256) k_kv_append(AppendArgs a, int lanes) {
         }
         return;
     }
-    const int page = a.table.pages[(int64_t)seq * a.table.ld + pos / a.kv.page_size];
+    const int page = a.table.pages[(int64_t)seq * a.table.ld + slot / a.kv.page_size];
     if (page < 0 || page >= a.kv.pages) return;
-    const int off = pos & (a.kv.page_size - 1);
+    const int off = slot & (a.kv.page_size - 1);
     float scale = 0.0f;
     if constexpr (KV::id == KQ_KV_I8) {
         float m = fmaxf(fmaxf(fabsf(lo.x), fabsf(lo.y)), fmaxf(fabsf(lo.z), fabsf(lo.w)));
@@ -115,11 +132,16 @@ void launch_kv_append(const AppendArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)((heads + per - 1) / per));
     auto al = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0; };
     const bool v4 = al(a.k, a.ldk) && al(a.v, a.ldv) && (!a.q_heads || (al(a.q, a.ldq) && al(a.q_out, a.ldqo))) &&
-                    (!a.rot || al(a.rope, 0));
+                    (!a.rot || al(a.rope, 0)) && al(a.q_norm, 0) && al(a.k_norm, 0);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, lanes); };
-    if (a.kv.type == KQ_KV_F16) v4 ? go(k_kv_append<KvF16, true>) : go(k_kv_append<KvF16, false>);
-    else if (a.kv.type == KQ_KV_BF16) v4 ? go(k_kv_append<KvBf16, true>) : go(k_kv_append<KvBf16, false>);
-    else v4 ? go(k_kv_append<KvI8, true>) : go(k_kv_append<KvI8, false>);
+    auto of = [&](auto kv) {
+        typedef decltype(kv) KV;
+        if (a.q_norm || a.k_norm || a.slot) v4 ? go(k_kv_append<KV, true, true>) : go(k_kv_append<KV, false, true>);
+        else v4 ? go(k_kv_append<KV, true, false>) : go(k_kv_append<KV, false, false>);
+    };
+    if (a.kv.type == KQ_KV_F16) of(KvF16());
+    else if (a.kv.type == KQ_KV_BF16) of(KvBf16());
+    else of(KvI8());
 }
 
 }  // namespace kq

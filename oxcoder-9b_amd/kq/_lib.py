@@ -61,6 +61,16 @@ KQ_SYMBOLS = {
     "kq_logits_workspace": (C.c_size_t, [_i]),
     "kq_logits_penalize": (_i, [_vp, _i64, _i, _i, _vp, _i64, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _vp,
                                 _i64, _vp, _i64, _vp, C.c_size_t, _vp, _vp]),
+    "kq_tree_plan": (_i, [_vp, _i64, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "kq_kv_append_norm": (_i, [_vp, _vp, _i64, _i, _i, _i, _vp, _vp, _vp, _vp, _i64, _i, _vp, _i64, _vp, _i64, _vp, _i64,
+                               _vp, _i, _i, _i, _vp, _vp, C.c_float, _vp]),
+    "kq_attn_tree_workspace": (C.c_size_t, [_i, _i, _i, _i, _i]),
+    "kq_attn_tree": (_i, [_vp, _vp, _i64, _i, _i, _vp, _vp, _i, _i, _vp, _i64, _i, C.c_float, _vp, _i64, _vp, C.c_size_t,
+                          _vp]),
+    "kq_kv_keep": (_i, [_vp, _i, _vp, _i64, _i, _i, _vp, _vp, _i64, _i, _vp]),
+    "kq_verify_workspace": (C.c_size_t, [_i, _i, _i]),
+    "kq_verify": (_i, [_vp, _i64, _i, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp,
+                       C.c_size_t, _vp]),
 }
 KQHOST_SYMBOLS = {
     "kq_host_quantize_q4k": (_i, [_vp, _i64, _i, _vp]),
@@ -73,6 +83,7 @@ KQ_OK = 0
 KQ_ERR_ARG = -1
 KQ_ERR_HIP = -2
 KQ_MAX_BATCH = 16
+KQ_MAX_TREE = 64
 KQ_GEMM_STATIC_SCRATCH_BYTES = 32 << 20
 KQ_KV_F16, KQ_KV_I8, KQ_KV_BF16 = 1, 24, 30
 

@@ -10,6 +10,15 @@ keys and stores keys and values (kq_kv_append), ``attend`` runs their attention 
     att.append(layer, q, k, v, seq, pos, q)          # q is rotated in place
     att.attend(layer, q, lens, out)
 
+A step that verifies drafts feeds a tree of tokens per request, whose node j lies in slot base + j of the cache:
+
+    tree = Tree(requests, nodes)                      # one for all layers and steps
+    att = PagedAttention(cache, table, 32, nodes=nodes, rope=rope_table(4096, 128))
+    tree.plan(parents, base)                          # once a step
+    att.append(layer, q, k, v, tree.seq, tree.pos, q, slot=tree.slot)
+    att.attend_tree(layer, q, tree, out)
+    att.keep(path, base)                              # the accepted nodes (sampling.Verifier), in all layers at once
+
 ``table`` is int32 [requests][pages of one]: the page of each run of ``page_size`` positions; the program
 that owns the pool fills it, and may change it between calls (the kernels read it when they run).  An entry
 outside the pool is a hole: nothing is stored there, and attention passes over it.
@@ -86,6 +95,39 @@ class KVCache:
         self.ref = C.addressof(self._kv)      # the const kq_kv* of the C ABI; lives as long as this object
 
 
+class Tree:
+    """What the calls of every layer take of a step's trees: ``plan`` fills, from the parents of each request's nodes, seq, pos
+    and slot (int32 [requests * nodes], PagedAttention.append's) and seen (int64 [requests][nodes]: bit j of node t's
+    word says that it sees node j, its ancestors and itself; 0: no node)."""
+
+    def __init__(self, requests, nodes, device="cuda"):
+        if not 1 <= requests <= 65535 or not 1 <= nodes <= _lib.KQ_MAX_TREE:
+            raise ValueError("1..65535 requests of 1..%d nodes" % _lib.KQ_MAX_TREE)
+        self.requests, self.nodes = requests, nodes
+        self.seen = torch.zeros((requests, nodes), dtype=torch.int64, device=device)
+        self.seq, self.pos, self.slot = (torch.full((requests * nodes,), -1, dtype=torch.int32, device=device) for _ in range(3))
+        self.device, self.base = self.seen.device, None
+        # what every call passes on, as addresses: the tensors stay as long as the tree
+        self._held = tuple(t.data_ptr() for t in (self.seen, self.seq, self.pos, self.slot))
+        self._calls = _lib.calls() if self.device.type == "cuda" else None
+
+    def plan(self, parents, base):
+        """parents: int32 [requests][nodes], or [1][nodes] for all requests: the node that node t follows, below t, or -1 where
+        it follows the context; another value: no node, nor those that follow it.  base: int32 [requests], the
+        positions ahead of the tree; below 0: the request sits out.  Node t lies in slot base + t and
+        stands at position base + its ancestors' number.  base is read by attend_tree too: it stays as it is until
+        the step's last call."""
+        if not isinstance(base, torch.Tensor) or base.device != self.device:
+            raise ValueError("base must be a device tensor, on the tree's device")
+        rc = self._calls and self._calls.tree_plan(*self._held, ops._stream(self.device), parents, base, self.requests, self.nodes)
+        if rc is None:                       # a tensor is not as it should be
+            ops.tree_plan(parents, base, self.seen, self.seq, self.pos, self.slot, self.requests, self.nodes)
+        elif rc:
+            _lib.check(rc)
+        self.base = base
+        return self
+
+
 class PagedAttention:
     """The attention of a decoding program over its layers' caches, with the one workspace it needs.
 
@@ -94,10 +136,13 @@ class PagedAttention:
     (default: what its row of the table covers); rope: rope_table's, or None (nothing is rotated), whose width is
     the number of values that turn (append skips tokens at positions past its rows); interleaved: pairs (2i, 2i + 1)
     instead of (i, i + rot/2); scale: default dim ** -0.5.
+    q_norm, k_norm: float32 [layers][dim], weights of a norm of each head of q (of k) that append applies ahead of the
+    rotation, x / sqrt(mean(x^2) + eps) * w; nodes: the most nodes of a tree that attend_tree will see (0: none, up to 64).
     These are for the object's life: another table or rotation takes another object, what is in them may change.
     Calls on one PagedAttention share its workspace and so must be ordered: one stream, or synchronised."""
 
-    def __init__(self, caches, table, q_heads, tokens=1, max_len=None, rope=None, interleaved=False, scale=None):
+    def __init__(self, caches, table, q_heads, tokens=1, max_len=None, rope=None, interleaved=False, scale=None,
+                 q_norm=None, k_norm=None, eps=1e-6, nodes=0):
         if not caches:
             raise ValueError("one cache per layer")
         c = caches[0]
@@ -109,33 +154,56 @@ class PagedAttention:
             raise ValueError("tokens must be 1..%d" % _lib.KQ_MAX_BATCH)
         if q_heads < 1 or q_heads % c.heads:
             raise ValueError("q_heads must be a multiple of the cache's %d heads" % c.heads)
+        if not 0 <= nodes <= _lib.KQ_MAX_TREE:
+            raise ValueError("nodes must be 0..%d" % _lib.KQ_MAX_TREE)
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None and (w.shape != (len(caches), c.dim) or w.dtype != torch.float32 or not w.is_contiguous()
+                                  or w.device != c.device):
+                raise ValueError("%s must be float32 [%d layers][%d], contiguous, on the caches' device"
+                                 % (name, len(caches), c.dim))
+        if not (eps >= 0 and eps < float("inf")):
+            raise ValueError("eps must be finite, at least 0")
         self.caches, self.table, self.q_heads, self.tokens = tuple(caches), table, q_heads, tokens
         self.rope, self._interleaved = rope, 1 if interleaved else 0
         self.scale = c.dim ** -0.5 if scale is None else float(scale)
         self.max_len = table.shape[1] * c.page_size if max_len is None else int(max_len)
         n = ops.attn_paged_workspace_bytes(table.shape[0], q_heads, c.dim, tokens, self.max_len)
+        self.nodes, self.q_norm, self.k_norm, self.eps = nodes, q_norm, k_norm, float(eps)
+        if n and nodes:
+            n = max(n, ops.attn_tree_workspace_bytes(table.shape[0], q_heads, c.dim, nodes, self.max_len))
         if not n:
             raise ValueError("%d requests of %d positions, %d heads of %d: not supported"
                              % (table.shape[0], self.max_len, q_heads, c.dim))
         buf = torch.empty(n + 256, dtype=torch.uint8, device=c.device)
         self.ws = buf[-buf.data_ptr() % 256:][:n]
         # what every call passes on, as addresses: the tensors stay as long as the plan
-        self._plan, self._keep = None, (table, rope, buf)
+        self._plan, self._keep = None, (table, rope, q_norm, k_norm, buf)
+        self._refs = (C.c_void_p * len(self.caches))(*[x.ref for x in self.caches])
+        self._norms = [tuple(None if w is None else w.data_ptr() + 4 * c.dim * i for w in (q_norm, k_norm))
+                       for i in range(len(self.caches))] if q_norm is not None or k_norm is not None else None
         if c.device.type == "cuda":
             self._calls = _lib.calls()
             self._plan = self._calls.plan(ops._table(table), ops._rope(rope), q_heads, c.heads, c.dim, self.max_len,
-                                          self._interleaved, self.scale, (self.ws.data_ptr(), n))
+                                          self._interleaved, self.scale, self.eps, (self.ws.data_ptr(), n))
 
-    def append(self, layer, q, k, v, seq, pos, q_out=None):
-        """Rotate q [N][q_heads * dim] into q_out (q itself: in place; None: a new tensor) and k
+    def append(self, layer, q, k, v, seq, pos, q_out=None, slot=None):
+        """Norm (where the constructor has weights) and rotate q [N][q_heads * dim] into q_out (q itself: in place; None: a new tensor) and k
         [N][heads * dim], store k and v for token n of request seq[n] at position pos[n] (both int32 [N]).
-        q None: keys and values only.  Returns q_out."""
+        q None: keys and values only.  slot (int32 [N]): where the tokens are stored, in the place of pos, which then
+        only rotates.  Returns q_out."""
         if q is not None and q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         c = self.caches[layer]
-        rc = self._plan and self._calls.append(self._plan, c.ref, ops._stream(c.device), q, k, v, seq, pos, q_out)
+        if self._norms is None and slot is None:
+            rc = self._plan and self._calls.append(self._plan, c.ref, ops._stream(c.device), q, k, v, seq, pos, q_out)
+        else:
+            norms = self._norms[layer] if self._norms else (None, None)
+            rc = self._plan and self._calls.append_norm(self._plan, c.ref, ops._stream(c.device), q, k, v, seq, pos, q_out, slot,
+                                                        *norms)
         if rc is None:                       # a tensor is not as it should be
-            ops.kv_append(c, self.table, q, k, v, seq, pos, q_out, self.q_heads, self.rope, self._interleaved)
+            qn, kn = (w if w is None else w[layer] for w in (self.q_norm, self.k_norm))
+            ops.kv_append(c, self.table, q, k, v, seq, pos, q_out, self.q_heads, self.rope, self._interleaved, slot, qn, kn,
+                          self.eps)
         elif rc:
             _lib.check(rc)
         return q_out
@@ -155,3 +223,34 @@ class PagedAttention:
         elif rc:
             _lib.check(rc)
         return out
+
+    def attend_tree(self, layer, q, tree, out=None):
+        """Attention of every request's tree as ``tree`` (a Tree of this object's requests, planned) says: node t sees the
+        positions ahead of the tree, its ancestors and itself.  q and out [requests * nodes][q_heads * dim]; a node that is
+        none, or of a request that sits out, gets 0.  Returns out."""
+        T = tree.nodes
+        if tree.requests != self.table.shape[0] or T > self.nodes:
+            raise ValueError("a tree of %d requests and %d nodes, made for %d requests and up to %d nodes"
+                             % (tree.requests, T, self.table.shape[0], self.nodes))
+        c = self.caches[layer]
+        if tree.device != c.device or tree.base is None:
+            raise ValueError("the tree must be planned, on the caches' device")
+        if out is None:
+            out = torch.empty((q.shape[0], self.q_heads * c.dim), dtype=torch.float32, device=q.device)
+        rc = self._plan and self._calls.attend_tree(self._plan, c.ref, ops._stream(c.device), q, tree.base, tree._held[0], out, T)
+        if rc is None:                       # a tensor is not as it should be
+            ops.attn_tree(c, self.table, q, tree.base, tree.seen, out, self.q_heads, T, self.scale, self.max_len, self.ws)
+        elif rc:
+            _lib.check(rc)
+        return out
+
+    def keep(self, path, base):
+        """Move the entries of each request's accepted nodes together in every layer's cache: from position base[b] +
+        path[b][i] to base[b] + i, for i up to the first entry that names no node (below i, or not above the one
+        before; -1 ends it).  path: int32 [requests][up to 64], base: int32 [requests]."""
+        c = self.caches[0]
+        rc = self._plan and self._calls.keep(self._plan, C.addressof(self._refs), len(self.caches), ops._stream(c.device), path, base)
+        if rc is None:                       # a tensor is not as it should be
+            ops.kv_keep(self.caches, self.table, path, base)
+        elif rc:
+            _lib.check(rc)

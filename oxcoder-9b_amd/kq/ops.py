@@ -477,10 +477,12 @@ def _rope(rope):
     return (_dev(rope, "rope", torch.float32), *rope.shape)
 
 
-def kv_append(cache, table, q, k, v, seq, pos, q_out, q_heads, rope=None, interleaved=False):
+def kv_append(cache, table, q, k, v, seq, pos, q_out, q_heads, rope=None, interleaved=False, slot=None, q_norm=None,
+              k_norm=None, eps=0.0):
     """Rotate q [N][q_heads * dim] into q_out and k [N][heads * dim], and store k and v of token n at position pos[n]
     of request seq[n] in ``cache`` (a kv.KVCache) under ``table`` int32 [requests][width] (kq_kv_append).
-    q and q_out None: keys and values only; rope: kv.rope_table's, or None."""
+    q and q_out None: keys and values only; rope: kv.rope_table's, or None.  slot (int32 [N]): stored there, not at pos;
+    q_norm, k_norm (float [dim]): norms of each head ahead of the rotation (kq_kv_append_norm)."""
     f32, i32, D = torch.float32, torch.int32, cache.dim
     N, cols = k.shape[0], cache.heads * D
     if (q is None) != (q_out is None):
@@ -492,10 +494,82 @@ def kv_append(cache, table, q, k, v, seq, pos, q_out, q_heads, rope=None, interl
         po, ldo = _mat(q_out, "q_out", f32, N, q_heads * D)
     pk, ldk = _mat(k, "k", f32, N, cols)
     pv, ldv = _mat(v, "v", f32, N, cols)
-    _lib.check(_lib.kq().kq_kv_append(cache.ref, *_table(table), N, _need(seq, "seq", i32, N), _need(pos, "pos", i32, N), pq, ldq,
-                                      q_heads, po, ldo, pk, ldk, pv, ldv, *_rope(rope), 1 if interleaved else 0,
-                                      _stream(cache.device)))
+    head = (cache.ref, *_table(table), N, _need(seq, "seq", i32, N), _need(pos, "pos", i32, N))
+    rest = (pq, ldq, q_heads, po, ldo, pk, ldk, pv, ldv, *_rope(rope), 1 if interleaved else 0)
+    if slot is None and q_norm is None and k_norm is None:
+        _lib.check(_lib.kq().kq_kv_append(*head, *rest, _stream(cache.device)))
+    else:
+        _lib.check(_lib.kq().kq_kv_append_norm(*head, _opt(slot, "slot", i32, N), *rest, _opt(q_norm, "q_norm", f32, D),
+                                               _opt(k_norm, "k_norm", f32, D), eps, _stream(cache.device)))
     return q_out
+
+
+def _parents(t, requests, nodes):
+    """(pointer, row stride) of parents int32 [requests or 1][nodes]."""
+    if requests > 1 and isinstance(t, torch.Tensor) and t.dim() == 2 and t.shape[0] == 1:
+        return _mat(t, "parents", torch.int32, 1, nodes)[0], 0
+    p, ld = _mat(t, "parents", torch.int32, requests, nodes)
+    return p, ld if requests > 1 else nodes
+
+
+def tree_plan(parents, base, seen, seq, pos, slot, requests, nodes):
+    """What kv.Tree.plan says, into seen int64 and seq, pos and slot int32, each of requests * nodes values (kq_tree_plan)."""
+    n, i32 = requests * nodes, torch.int32
+    _lib.check(_lib.kq().kq_tree_plan(*_parents(parents, requests, nodes), _need(base, "base", i32, requests), requests, nodes,
+                                      _need(seen, "seen", torch.int64, n), _need(seq, "seq", i32, n), _need(pos, "pos", i32, n),
+                                      _need(slot, "slot", i32, n), _stream(seen.device)))
+
+
+def attn_tree_workspace_bytes(seqs, q_heads, dim, nodes, max_len):
+    """Device bytes of workspace attn_tree needs (kq_attn_tree_workspace; 0 for sizes it does not take)."""
+    return int(_lib.kq().kq_attn_tree_workspace(seqs, q_heads, dim, nodes, max_len))
+
+
+def attn_tree(cache, table, q, base, seen, out, q_heads, nodes, scale, max_len, ws):
+    """Attention of each request's tree of ``nodes`` nodes over ``cache`` under ``table``: q, out [requests * nodes]
+    [q_heads * dim], base int32 [requests], seen int64 [requests][nodes] (tree_plan's); ws of attn_tree_workspace_bytes,
+    256-byte aligned (kq_attn_tree)."""
+    table = _table(table)
+    rows, cols = table[2] * nodes, q_heads * cache.dim
+    pq, ldq = _mat(q, "q", torch.float32, rows, cols)
+    po, ldo = _mat(out, "out", torch.float32, rows, cols)
+    _lib.check(_lib.kq().kq_attn_tree(cache.ref, *table, _need(base, "base", torch.int32, table[2]),
+                                      _need(seen, "seen", torch.int64, rows), max_len, nodes, pq, ldq, q_heads, scale, po, ldo,
+                                      _dev(ws, "ws", torch.uint8), ws.numel(), _stream(cache.device)))
+    return out
+
+
+def kv_keep(caches, table, path, base):
+    """Move each request's entries at base[b] + path[b][i] to base[b] + i in every cache (kq_kv_keep): path int32
+    [requests][nodes], base int32 [requests]."""
+    table = _table(table)
+    nodes = path.shape[-1] if isinstance(path, torch.Tensor) and path.dim() == 2 else 0
+    pp, ldp = _mat(path, "path", torch.int32, table[2], nodes)
+    refs = (C.c_void_p * len(caches))(*[c.ref for c in caches])
+    _lib.check(_lib.kq().kq_kv_keep(C.addressof(refs), len(caches), *table, _need(base, "base", torch.int32, table[2]), pp, ldp,
+                                    nodes, _stream(caches[0].device)))
+
+
+def verify_workspace_bytes(requests, nodes, vocab):
+    """Device bytes of workspace verify needs (kq_verify_workspace; 0 for sizes it does not take)."""
+    return int(_lib.kq().kq_verify_workspace(requests, nodes, vocab))
+
+
+def verify(logits, tokens, parents, uniform, temperature, draft, accepted, path, token, ws):
+    """sampling.Verifier.verify's arguments, into accepted int32 [B], path int32 [B * T] and token int32 [B]; ws of
+    verify_workspace_bytes, 256-byte aligned (kq_verify)."""
+    f32, i32 = torch.float32, torch.int32
+    if not isinstance(tokens, torch.Tensor) or tokens.dim() != 2 or not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+        raise ValueError("tokens must be [requests][nodes], logits [requests * nodes][vocabulary]")
+    (B, T), V = tokens.shape, logits.shape[1]
+    px, ldx = _mat(logits, "logits", f32, B * T, V)
+    pt, ldt = _mat(tokens, "tokens", i32, B, T)
+    pu, ldu = _mat(uniform, "uniform", f32, B, T)
+    pd, ldd = (None, 0) if draft is None else _mat(draft, "draft", f32, B * T, V)
+    _lib.check(_lib.kq().kq_verify(px, ldx, B, T, V, pt, ldt, *_parents(parents, B, T), pu, ldu,
+                                   _opt(temperature, "temperature", f32, B), pd, ldd, _need(accepted, "accepted", i32, B),
+                                   _need(path, "path", i32, B * T), _need(token, "token", i32, B), _dev(ws, "ws", torch.uint8),
+                                   ws.numel(), _stream(logits.device)))
 
 
 def attn_paged_workspace_bytes(seqs, q_heads, dim, tokens, max_len):

@@ -26,7 +26,8 @@ ARCH = "gfx950"
 HIP_SOURCES = ["api.hip", "q8k_quantize.hip", "producers.hip", "argmax.hip", "gemv_q8k.hip", "gemv_mfma.hip",
                "gemv_f32.hip", "gemm_q8k.hip", "gemm_small.hip", "kv_append.hip", "attn_paged.hip",
                "attn_paged_f16.hip", "attn_paged_bf16.hip", "attn_paged_i8.hip", "logits.hip", "kv_tree.hip",
-               "attn_tree_f16.hip", "attn_tree_bf16.hip", "attn_tree_i8.hip", "verify.hip"]
+               "attn_tree.hip", "attn_tree_f16.hip", "attn_tree_bf16.hip",
+               "attn_tree_i8.hip", "verify.hip"]
 HIP_FLAGS = [
     "--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -646,19 +646,21 @@ static int attention(const char* fn, const kq_kv* kv, const int32_t* table, int6
     KQ_TRY(check_rows(out, ldo, rows, qw, "out", fn));
     if (!(scale - scale == 0)) return fail(KQ_ERR_ARG, "%s: scale must be finite", fn);
     KQ_TRY(check_ptr(ws, 256, "ws", fn));
-    const size_t need = attn_paged_workspace(seqs, q_heads, kv->dim, T, max_len);
+    const size_t need = seen ? attn_tree_bytes(seqs, kv->heads, q_heads / kv->heads, kv->dim, T, max_len)
+                             : attn_paged_workspace(seqs, q_heads, kv->dim, T, max_len);
     if (ws_bytes < need)
         return fail(KQ_ERR_ARG, "%s: workspace of %zu bytes, %zu needed", fn, ws_bytes, need);
     a.kv = *kv;
     a.lens = lens;
     a.seen = seen;
+    a.bound = max_len;
     a.max_len = max_len < a.table.cap ? max_len : a.table.cap;
     a.T = T;
     a.q_heads = q_heads;
     a.q = q, a.ldq = ldq, a.out = out, a.ldo = ldo;
     a.scale = scale;
     a.ws = static_cast<uint8_t*>(ws);
-    launch_attn_paged(a, as_stream(stream));
+    seen ? launch_attn_tree(a, as_stream(stream)) : launch_attn_paged(a, as_stream(stream));
     return check_launch(fn);
 }
 
@@ -673,7 +675,7 @@ size_t kq_attn_tree_workspace(int seqs, int q_heads, int dim, int T, int max_len
     if (seqs < 1 || seqs > 65535 || q_heads < 1 || q_heads > 4096 || dim < 16 || dim > 256 || dim % 16 || T < 1 ||
         T > KQ_MAX_TREE || max_len < 1 || max_len > (1 << 30))
         return 0;
-    return attn_paged_workspace(seqs, q_heads, dim, T, max_len);
+    return attn_tree_workspace(seqs, q_heads, dim, T, max_len);
 }
 
 int kq_attn_tree(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, const int32_t* base,

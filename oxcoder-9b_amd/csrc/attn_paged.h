@@ -242,18 +242,6 @@ struct Attn {
         }
         return bits;
     }
-    // The same for a row of a tree: a hole, or neither below the tree's first slot nor a node of `nodes`.
-    static __device__ __forceinline__ uint32_t hidden_tree(const Span& w, int u, int tree, uint64_t nodes, int g) {
-        uint32_t bits = 0;
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const int at = 32 * u + 16 * t + 4 * g, n = w.first + at - tree;  // of the four, the first's place in the tree
-            const uint32_t seen = n >= 0 ? (uint32_t)(n < 64 ? nodes >> n : 0) : n > -4 ? (uint32_t)(nodes << -n) | ((1u << -n) - 1u) : 15u;
-            const uint32_t out = ~(uint32_t)(w.there >> at) | ~seen;
-            bits |= (out & 15u) << (4 * t);
-        }
-        return bits;
-    }
     __device__ __forceinline__ void clear_v(uint32_t bits) {
 #pragma unroll
         for (int t = 0; t < 2; t++)
@@ -461,17 +449,9 @@ __device__ __forceinline__ void put_o(float* row, const f32x4 (&o)[ND], float k,
     }
 }
 
-// The positions of request b that are there: of a tree, its first slot (lens) and T more.
-template <bool TREE>
-__device__ __forceinline__ int at_length(const AttnArgs& a, int length) {
-    if constexpr (TREE) return length < 0 ? 0 : min(min(length, a.max_len) + a.T, a.max_len);
-    return min(length, a.max_len);
-}
-
 // NR: tiles of 16 rows that a workgroup takes at once; PAIRED: it takes chunks by twos (apart from the other, whose way is
-// shorter: one request of 611 positions 7.8 -> 7.0 us); TREE: the tokens are the nodes of a tree (kq_attn_tree), and a row sees
-// the context and the nodes of its word.
-template <class KV, int ND, int NR, bool PAIRED, bool TREE>
+// shorter: one request of 611 positions 7.8 -> 7.0 us).
+template <class KV, int ND, int NR, bool PAIRED>
 __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ? 3 : 4) k_attn_part(AttnArgs a) {
     typedef Attn<KV, ND, NR> A;
     __shared__ u32x4 sq[NR][A::QS][3][64];                      // q's parts [tile][share][part][lane]
@@ -503,22 +483,10 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
     const int length = a.lens[b];
     int page = entry(c * AT_CHUNK + 64 * wave);
     asm volatile("" : "+v"(page));
-    const int first = __builtin_amdgcn_readfirstlane(length), len = at_length<TREE>(a, first);
+    const int len = min(__builtin_amdgcn_readfirstlane(length), a.max_len);
     if (c * AT_CHUNK >= len && (c || a.joined)) return;         // the join knows the chunks that are there
     const int G = a.group, R = a.T * G;
-    int all = TREE ? min(first, len) : len - a.T + 1;           // positions that every token sees
-    uint64_t nodes[NR] = {}, some = 0;                          // TREE: those that the rows see, those that any row sees
-    if constexpr (TREE) {
-        const uint64_t* seen = a.seen + (int64_t)b * a.T;
-        const uint64_t mine = lane < a.T ? seen[lane] : 0;
-        if (__any(lane < a.T && !mine)) all = 0;                // a node that is none sees nothing
-        uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
-#pragma unroll
-        for (int i = 1; i < 64; i <<= 1) lo |= of_lane(lane ^ i, lo), hi |= of_lane(lane ^ i, hi);
-        some = (uint64_t)hi << 32 | lo;
-#pragma unroll
-        for (int n = 0; n < NR; n++) nodes[n] = seen[min((r0 + r + 16 * n) / G, a.T - 1)];
-    }
+    const int all = len - a.T + 1;                              // positions that every token sees
     A s;
     s.kb = static_cast<const uint8_t*>(a.kv.k) + (int64_t)kh * a.kv.head_stride * A::EB;
     s.vb = static_cast<const uint8_t*>(a.kv.v) + (int64_t)kh * a.kv.head_stride * A::EB;
@@ -715,21 +683,14 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
             if (partly) {
 #pragma unroll
                 for (int n = 0; n < NR; n++) {
-                    const uint32_t hid = TREE ? A::hidden_tree(w, u, nodes[n] ? first : -(1 << 29), nodes[n], g)
-                                              : A::hidden(w, u, row[n] < R ? all + t[n] : 0, g);
+                    const uint32_t hid = A::hidden(w, u, row[n] < R ? all + t[n] : 0, g);
 #pragma unroll
                     for (int j = 0; j < 8; j++)
                         if (hid >> j & 1u) e[n][j >> 2][j & 3] = -INFINITY;
                 }
                 // An infinity or NaN that only some tokens see would reach the others as 0 * inf: then the rows are done
                 // again, token by token, with the values that it does not see cleared.
-                uint32_t gone;
-                if constexpr (TREE) {
-                    const uint64_t see = apart ? a.seen[(int64_t)b * a.T + tok] : some;
-                    gone = A::hidden_tree(w, u, see ? first : -(1 << 29), see, g);
-                } else {
-                    gone = A::hidden(w, u, apart ? all + tok : len, g);
-                }
+                const uint32_t gone = A::hidden(w, u, apart ? all + tok : len, g);
                 if (a.T > 1 && !apart) found |= s.v_not_finite(A::hidden(w, u, all, g) & ~gone);
                 s.clear_v(gone);
             }
@@ -857,7 +818,7 @@ __global__ void __launch_bounds__(64 * AT_WAVES, ND > 8 || NR > 1 ? 2 : ND > 4 ?
     }
 }
 
-template <class KV, int ND, int NR, bool TREE>
+template <class KV, int ND, int NR>
 void launch_attn_part_nr(const AttnArgs& args, hipStream_t s) {
     AttnArgs a = args;
     const int R = a.T * a.group;
@@ -865,24 +826,24 @@ void launch_attn_part_nr(const AttnArgs& args, hipStream_t s) {
     const int live = a.paired && R < 16 ? R : 16, held = a.paired ? NR * (ND > 8 ? 2 : 1) * 512 : 0;
     const size_t lds = (size_t)live * (AT_WAVES * Attn<KV, ND, NR>::LD * 4 + held);
     const dim3 grid(a.kv.heads * a.row_groups, a.table.seqs, a.groups);
-    if (a.paired) hipLaunchKernelGGL((k_attn_part<KV, ND, NR, true, TREE>), grid, dim3(64 * AT_WAVES), lds, s, a);
-    else hipLaunchKernelGGL((k_attn_part<KV, ND, NR, false, TREE>), grid, dim3(64 * AT_WAVES), lds, s, a);
+    if (a.paired) hipLaunchKernelGGL((k_attn_part<KV, ND, NR, true>), grid, dim3(64 * AT_WAVES), lds, s, a);
+    else hipLaunchKernelGGL((k_attn_part<KV, ND, NR, false>), grid, dim3(64 * AT_WAVES), lds, s, a);
 }
 
-template <class KV, int ND, bool TREE>
+template <class KV, int ND>
 void launch_attn_part_nd(const AttnArgs& a, hipStream_t s) {
     if constexpr (ND <= 8)
-        if (a.T * a.group > 16) return launch_attn_part_nr<KV, ND, 2, TREE>(a, s);
-    launch_attn_part_nr<KV, ND, 1, TREE>(a, s);
+        if (a.T * a.group > 16) return launch_attn_part_nr<KV, ND, 2>(a, s);
+    launch_attn_part_nr<KV, ND, 1>(a, s);
 }
 
-template <class KV, bool TREE>
+template <class KV>
 void launch_attn_part(const AttnArgs& a, hipStream_t s) {
     static constexpr void (*go[16])(const AttnArgs&, hipStream_t) = {
-        launch_attn_part_nd<KV, 1, TREE>, launch_attn_part_nd<KV, 2, TREE>, launch_attn_part_nd<KV, 3, TREE>, launch_attn_part_nd<KV, 4, TREE>,
-        launch_attn_part_nd<KV, 5, TREE>, launch_attn_part_nd<KV, 6, TREE>, launch_attn_part_nd<KV, 7, TREE>, launch_attn_part_nd<KV, 8, TREE>,
-        launch_attn_part_nd<KV, 9, TREE>, launch_attn_part_nd<KV, 10, TREE>, launch_attn_part_nd<KV, 11, TREE>, launch_attn_part_nd<KV, 12, TREE>,
-        launch_attn_part_nd<KV, 13, TREE>, launch_attn_part_nd<KV, 14, TREE>, launch_attn_part_nd<KV, 15, TREE>, launch_attn_part_nd<KV, 16, TREE>};
+        launch_attn_part_nd<KV, 1>, launch_attn_part_nd<KV, 2>, launch_attn_part_nd<KV, 3>, launch_attn_part_nd<KV, 4>,
+        launch_attn_part_nd<KV, 5>, launch_attn_part_nd<KV, 6>, launch_attn_part_nd<KV, 7>, launch_attn_part_nd<KV, 8>,
+        launch_attn_part_nd<KV, 9>, launch_attn_part_nd<KV, 10>, launch_attn_part_nd<KV, 11>, launch_attn_part_nd<KV, 12>,
+        launch_attn_part_nd<KV, 13>, launch_attn_part_nd<KV, 14>, launch_attn_part_nd<KV, 15>, launch_attn_part_nd<KV, 16>};
     go[a.kv.dim / 16 - 1](a, s);
 }
 

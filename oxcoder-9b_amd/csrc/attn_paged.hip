@@ -9,13 +9,13 @@ namespace kq {
 // One workgroup per row and 32 N of its values: 32 groups of 8 lanes take every 32nd pair of chunks, in the steps of
 // the workgroup that had both where there was one; then the groups are added as a tree: a row's result depends on its
 // number of chunks alone.
-template <int N, bool PAIRED, bool TREE>
+template <int N, bool PAIRED>
 __global__ void __launch_bounds__(256) k_attn_join(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) f32x4 so[4][N][8];
     __shared__ float sl[4], sm[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, D = a.kv.dim;
     const int b = blockIdx.x / a.T, h = blockIdx.y, G = a.group, d = 32 * N * blockIdx.z + 4 * (tid & 7);
-    const int len = at_length<TREE>(a, a.lens[b]), n = len <= 0 ? 0 : (len + AT_CHUNK - 1) / AT_CHUNK, pairs = (n + 1) / 2;
+    const int len = min(a.lens[b], a.max_len), n = len <= 0 ? 0 : (len + AT_CHUNK - 1) / AT_CHUNK, pairs = (n + 1) / 2;
     const int64_t row = (((int64_t)b * a.kv.heads + h / G) * a.T * G + blockIdx.x % a.T * G + h % G) * a.parts;
     float top = -INFINITY;
     for (int c = tid; c < (PAIRED ? pairs : n); c += 256) top = fmaxf(top, a.pml[row + c].m);
@@ -87,8 +87,7 @@ size_t attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len) 
     return max_len <= AT_CHUNK ? 256 : up256(parts * dim * 4) + up256(parts * sizeof(AttnMl));
 }
 
-template <bool TREE>
-static void launch(const AttnArgs& args, hipStream_t s) {
+void launch_attn_paged(const AttnArgs& args, hipStream_t s) {
     AttnArgs a = args;
     a.scale *= 1.44269504088896341f;                           // scores in powers of 2
     a.group = a.q_heads / a.kv.heads;
@@ -108,9 +107,9 @@ static void launch(const AttnArgs& args, hipStream_t s) {
     const size_t parts = (size_t)a.table.seqs * a.T * a.q_heads * a.parts;
     a.po = reinterpret_cast<float*>(a.ws);
     a.pml = reinterpret_cast<AttnMl*>(a.ws + up256(parts * a.kv.dim * 4));
-    if (a.kv.type == KQ_KV_F16) launch_attn_part<KvF16, TREE>(a, s);
-    else if (a.kv.type == KQ_KV_BF16) launch_attn_part<KvBf16, TREE>(a, s);
-    else launch_attn_part<KvI8, TREE>(a, s);
+    if (a.kv.type == KQ_KV_F16) launch_attn_part<KvF16>(a, s);
+    else if (a.kv.type == KQ_KV_BF16) launch_attn_part<KvBf16>(a, s);
+    else launch_attn_part<KvI8>(a, s);
     if (!a.joined) return;
     // rows enough for the chip: four times fewer workgroups, that scan a row's maxima once for 128 values (512 rows of 20 chunks and
     // 256 values 7.4 -> 5 us; the 32 rows of 391 chunks 8 us with 32 values each, 13 us with 128)
@@ -118,10 +117,8 @@ static void launch(const AttnArgs& args, hipStream_t s) {
     const bool wide = rows >= device_cus();
     const dim3 grid(a.table.seqs * a.T, a.q_heads, wide ? (a.kv.dim + 127) / 128 : (a.kv.dim + 31) / 32);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
-    if (a.paired) wide ? go(k_attn_join<4, true, TREE>) : go(k_attn_join<1, true, TREE>);
-    else wide ? go(k_attn_join<4, false, TREE>) : go(k_attn_join<1, false, TREE>);
+    if (a.paired) wide ? go(k_attn_join<4, true>) : go(k_attn_join<1, true>);
+    else wide ? go(k_attn_join<4, false>) : go(k_attn_join<1, false>);
 }
-
-void launch_attn_paged(const AttnArgs& a, hipStream_t s) { a.seen ? launch<true>(a, s) : launch<false>(a, s); }
 
 }  // namespace kq

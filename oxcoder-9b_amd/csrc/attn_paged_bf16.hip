@@ -2,5 +2,5 @@
 #include "attn_paged.h"
 
 namespace kq {
-template void launch_attn_part<KvBf16, false>(const AttnArgs& a, hipStream_t s);
+template void launch_attn_part<KvBf16>(const AttnArgs& a, hipStream_t s);
 }

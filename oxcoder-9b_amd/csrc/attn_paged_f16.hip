@@ -2,5 +2,5 @@
 #include "attn_paged.h"
 
 namespace kq {
-template void launch_attn_part<KvF16, false>(const AttnArgs& a, hipStream_t s);
+template void launch_attn_part<KvF16>(const AttnArgs& a, hipStream_t s);
 }

@@ -1,6 +1,6 @@
 // Attention of trees of drafted tokens over a paged cache of bf16 values.
-#include "attn_paged.h"
+#include "attn_tree.h"
 
 namespace kq {
-template void launch_attn_part<KvBf16, true>(const AttnArgs& a, hipStream_t s);
+template void launch_attn_tree_part<KvBf16>(const AttnArgs& a, hipStream_t s);
 }

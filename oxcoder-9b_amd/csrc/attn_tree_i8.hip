@@ -1,6 +1,6 @@
 // Attention of trees of drafted tokens over a paged cache of 8-bit codes.
-#include "attn_paged.h"
+#include "attn_tree.h"
 
 namespace kq {
-template void launch_attn_part<KvI8, true>(const AttnArgs& a, hipStream_t s);
+template void launch_attn_tree_part<KvI8>(const AttnArgs& a, hipStream_t s);
 }

@@ -136,7 +136,7 @@ struct AttnArgs {
     kq_kv kv;
     PageTable table;
     const int32_t* lens;       // of a tree: where its first slot lies
-    const uint64_t* seen;      // [request][token]: the nodes that each node of a tree sees; NULL: the tokens are a chain
+    const uint64_t* seen;      // trees: [request][node], the nodes that each node sees
     int max_len, T, q_heads;
     const float* q;
     int64_t ldq, ldo;
@@ -150,11 +150,19 @@ struct AttnArgs {
     int row_groups;                     // workgroups that share a chunk, each for its rows
     float* po;
     AttnMl* pml;
+    // set by launch_attn_tree, with group, page_shift, joined and parts
+    int bound;                          // max_len as the caller gave it, which the split goes by
+    int split, tiles;                   // positions of a part; 16 rows each that a wave takes
 };
-template <class KV, bool TREE>
+template <class KV>
 void launch_attn_part(const AttnArgs& a, hipStream_t s);
 size_t attn_paged_workspace(int seqs, int q_heads, int dim, int T, int max_len);
 void launch_attn_paged(const AttnArgs& a, hipStream_t s);
+template <class KV>
+void launch_attn_tree_part(const AttnArgs& a, hipStream_t s);
+size_t attn_tree_bytes(int seqs, int heads, int group, int dim, int T, int max_len);
+size_t attn_tree_workspace(int seqs, int q_heads, int dim, int T, int max_len);
+void launch_attn_tree(const AttnArgs& a, hipStream_t s);
 // A tree of drafted tokens (kv_tree.hip).
 constexpr int TREE_MOST = KQ_MAX_TREE;
 struct TreeArgs {

@@ -21,37 +21,34 @@ namespace kq {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// The positions of a request that are there: those ahead of its tree, and T more.
-__device__ __forceinline__ int tree_length(const AttnArgs& a, int base) {
-    return base < 0 ? 0 : min(min(base, a.max_len) + a.T, a.max_len);
-}
-
-// Both elements' three parts, the first element in the low half.
-__device__ __forceinline__ void split3(float x, float y, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
-    auto cut = [](float a) { return fbits(ubits(a) & 0xffff0000u); };
-    const float rx = x - cut(x), ry = y - cut(y);
-    p0 = hi_halves(ubits(x), ubits(y));
-    p1 = hi_halves(ubits(rx), ubits(ry));
-    p2 = hi_halves(ubits(rx - cut(rx)), ubits(ry - cut(ry)));
-}
-
-// Eight f16 values as the sums of two bf16 values; an infinity or NaN stays in the first.
-__device__ __forceinline__ void f16_pair(u32x4 raw, u32x4& hi, u32x4& lo) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const float x = f16_lo(raw[j]), y = f16_hi(raw[j]);
-        const float cx = fbits(ubits(x) & 0xffff0000u), cy = fbits(ubits(y) & 0xffff0000u);
-        hi[j] = hi_halves(ubits(x), ubits(y));
-        const uint32_t r = hi_halves(ubits(x - cx), ubits(y - cy));
-        lo[j] = r;
+// What two values lose when they are cut to bf16: a dot product of the packed halves with (-1, 0) or (0, -1) and the value, whose
+// sum is exact as the rest has fewer bits than the value.  (In registers that the compiler does not see through: it takes the other
+// half of one of these as a literal.)
+struct Cut {
+    uint32_t x, y;
+    __device__ __forceinline__ Cut() : x(0x0000bf80u), y(0xbf800000u) { asm volatile("" : "+s"(x), "+s"(y)); }
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    __device__ __forceinline__ float rest(uint32_t p, uint32_t which, float v) const {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, which), v, false);
     }
-    // inf - inf and NaN - NaN are NaN: the second part of such a value is 0
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if ((hi[j] & 0x7f80u) == 0x7f80u) lo[j] &= 0xffff0000u;
-        if ((hi[j] >> 16 & 0x7f80u) == 0x7f80u) lo[j] &= 0xffffu;
+    // both values' three parts, the first value in the low half
+    __device__ __forceinline__ void split3(float v, float w, uint32_t& p0, uint32_t& p1, uint32_t& p2) const {
+        p0 = hi_halves(ubits(v), ubits(w));
+        v = rest(p0, x, v), w = rest(p0, y, w);
+        p1 = hi_halves(ubits(v), ubits(w));
+        v = rest(p1, x, v), w = rest(p1, y, w);
+        p2 = hi_halves(ubits(v), ubits(w));
     }
-}
+    // eight f16 values as the sums of two bf16 values; of an infinity or NaN the second is NaN
+    __device__ __forceinline__ void f16_pair(u32x4 raw, u32x4& hi, u32x4& lo) const {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float v = f16_lo(raw[j]), w = f16_hi(raw[j]);
+            hi[j] = hi_halves(ubits(v), ubits(w));
+            lo[j] = hi_halves(ubits(rest(hi[j], x, v)), ubits(rest(hi[j], y, w)));
+        }
+    }
+};
 
 __device__ __forceinline__ f32x4 mma_bf16(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -71,18 +68,18 @@ struct TreeAttn {
     static constexpr bool I8 = KV::id == KQ_KV_I8, F16 = KV::id == KQ_KV_F16;
     static constexpr int D = 16 * ND, EB = I8 ? 1 : 2, QS = ND / 2, P = 32;
     static constexpr int PLANES = F16 ? 2 : 1;
-    static constexpr int ROW = 2 * D + 16;                 // bytes of a position in LDS: rows fall on other banks each
-    static constexpr int PLANE = P * ROW, TILE = 2 * PLANES * PLANE;
+    // bytes of a position in LDS: 8 keys' pieces of 16, and 4 values' pieces of 32, each fall on all banks
+    static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 32;
+    static constexpr int KPLANE = P * KROW, VPLANE = P * VROW, VALUES = PLANES * KPLANE, TILE = VALUES + PLANES * VPLANE;
     static constexpr int NBUF = 2 * TILE <= 72 * 1024 ? 2 : 1;
     static constexpr int UNITS = D * EB / 16;              // 16-byte pieces of a position
     static constexpr int MINE = 8;                         // positions that a wave fetches
     static constexpr int PER = (MINE * UNITS + 63) / 64;   // pieces of a lane
-    static constexpr bool AHEAD = ND < 16 && NT == 1;      // fragments are read ahead of their use, where registers are left
     static constexpr size_t LDS = (size_t)TILE * NBUF;
 };
 
 template <class KV, int ND, int NT>
-__global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) k_attn_tree(AttnArgs a) {
+__global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 && NT == 1 ? 3 : 2) k_attn_tree(AttnArgs a) {
     typedef TreeAttn<KV, ND, NT> A;
     extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];
     __shared__ uint32_t there[A::NBUF][4];
@@ -96,6 +93,7 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) 
     if (from >= len && z) return;                              // the join knows the splits that are there
     const int row0 = 16 * NT * (4 * rb + wave);              // the wave's first
     const bool idle = row0 >= R;
+    const Cut cut;
 
     // what the rows see of the tree, and what any row does
     const uint64_t* seen = a.seen + (int64_t)b * a.T;
@@ -105,97 +103,110 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) 
     for (int i = 1; i < 64; i <<= 1) lo |= of_lane(lane ^ i, lo), hi |= of_lane(lane ^ i, hi);
     const uint64_t some = (uint64_t)__builtin_amdgcn_readfirstlane(hi) << 32 | __builtin_amdgcn_readfirstlane(lo);
     // (Read again where it is needed, and the thread's place below taken anew for each tile: neither is held.)
-    auto nodes_of = [&](int n) __attribute__((always_inline)) {
-        int row = row0 + 16 * n + (lane & 15);
-        asm volatile("" : "+v"(row));
-        return seen[min(row / G, a.T - 1)];
-    };
     auto here = [&]() __attribute__((always_inline)) {
-        int i = lane;
+        uint32_t i = lane;
         asm volatile("" : "+v"(i));
         return i;
+    };
+    auto nodes_of = [&](int n) __attribute__((always_inline)) {
+        return seen[min((row0 + 16 * n + (int)(here() & 15)) / G, a.T - 1)];
     };
 
     // Keys past the head's size stay 0 from here on.
     if (D < A::D)
         for (int i = tid; i < A::NBUF * A::PLANES * A::P; i += 256) {
-            uint8_t* row = tiles + i / (A::PLANES * A::P) * A::TILE + i % (A::PLANES * A::P) * A::ROW;
+            uint8_t* row = tiles + i / (A::PLANES * A::P) * A::TILE + i % (A::PLANES * A::P) * A::KROW;
             for (int d = D; d < A::D; d += 8) *reinterpret_cast<u32x4*>(row + 2 * d) = u32x4{0, 0, 0, 0};
         }
 
-    // Fetching: lane i of a wave looks after the place of position MINE wave + i of the tile, and holds PER pieces.
+    // Fetching: each wave MINE positions, a lane PER pieces of 16 bytes.  (Lanes past the last piece, and pieces past the head's size,
+    // take one that another lane has too.)
     const int32_t* table = a.table.pages + (int64_t)b * a.table.ld;
     const uint8_t* kb = static_cast<const uint8_t*>(a.kv.k) + (int64_t)kh * a.kv.head_stride * A::EB;
-    const uint8_t* vb = static_cast<const uint8_t*>(a.kv.v) + (int64_t)kh * a.kv.head_stride * A::EB;
-    auto entry = [&](int first) __attribute__((always_inline)) {
-        return table[min(first + A::MINE * wave + here() % A::MINE, a.table.cap - 1) >> a.page_shift];
+    const int64_t to_v = static_cast<const uint8_t*>(a.kv.v) - static_cast<const uint8_t*>(a.kv.k);
+    const uint32_t page_bytes = (uint32_t)a.kv.page_stride * A::EB, pos_bytes = (uint32_t)a.kv.pos_stride * A::EB;   // below 2^31 both
+    const uint32_t last = D * A::EB - 16;
+    auto pos_of = [&](int i, uint32_t lane) __attribute__((always_inline)) { return (int)((64 * i + lane) / A::UNITS % A::MINE); };
+    auto col_of = [&](int i, uint32_t lane) __attribute__((always_inline)) { return min(16 * ((64 * i + lane) % A::UNITS), last); };
+    int page[A::PER];
+    auto look = [&](int first) __attribute__((always_inline)) {
+        const uint32_t lane = here();
+#pragma unroll
+        for (int i = 0; i < A::PER; i++) page[i] = table[min(first + A::MINE * wave + pos_of(i, lane), a.table.cap - 1) >> a.page_shift];
     };
     u32x4 kreg[A::PER], vreg[A::PER];
-    uint32_t ok_bits = 0;
+    uint64_t ok_lanes[A::PER];
+    float ks[A::PER], vs[A::PER];
     bool wild = false;                                         // values that are not finite count as 0 (below)
-    float ks = 0.0f, vs = 0.0f;
-    auto fetch = [&](int first, int page) __attribute__((always_inline)) {
-        const int lane = here(), p = first + A::MINE * wave + lane % A::MINE, node = p - base;
-        const bool ok = p < to && (unsigned)page < (unsigned)a.kv.pages && (node < 0 || (node < 64 && (some >> node & 1u)));
-        const int off = p & (a.kv.page_size - 1);
-        const int64_t at = ok ? (page * a.kv.page_stride + off * a.kv.pos_stride) * A::EB : 0;
-        ok_bits = (uint32_t)__ballot(ok) & ((1u << A::MINE) - 1u);
-        if constexpr (A::I8) {
-            const int64_t e = page * a.kv.scale_page_stride + kh * a.kv.scale_head_stride + off * a.kv.scale_pos_stride;
-            ks = ok ? a.kv.k_scale[e] : 0.0f;
-            vs = ok ? a.kv.v_scale[e] : 0.0f;
-        }
-        const uint32_t at_lo = (uint32_t)at, at_hi = (uint32_t)(at >> 32);
+    auto fetch = [&](int first) __attribute__((always_inline)) {
+        const uint32_t lane = here();
 #pragma unroll
         for (int i = 0; i < A::PER; i++) {
-            const int u = 64 * i + lane, pos = u / A::UNITS % A::MINE, col = u % A::UNITS;
-            const int64_t place = (int64_t)((uint64_t)of_lane(pos, at_hi) << 32 | of_lane(pos, at_lo)) + 16 * col;
-            const bool live = ok_bits >> pos & 1u && 16 * col < D * A::EB;
-            u32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-            if (live) {
-                k = *reinterpret_cast<const u32x4*>(kb + place);
-                v = *reinterpret_cast<const u32x4*>(vb + place);
+            const int p = first + A::MINE * wave + pos_of(i, lane), node = p - base;
+            bool ok = (unsigned)page[i] < (unsigned)a.kv.pages;
+            if (first + A::P > min(base, to)) ok = ok && p < to && (node < 0 || (node < 64 && (some >> (node & 63) & 1u)));
+            const uint32_t pg = ok ? page[i] : 0, off = ok ? p & (a.kv.page_size - 1) : 0;
+            ok_lanes[i] = __ballot(ok);
+            const uint8_t* at = kb + (uint64_t)pg * page_bytes + (uint64_t)off * pos_bytes + col_of(i, lane);
+            kreg[i] = *reinterpret_cast<const u32x4*>(at);
+            vreg[i] = *reinterpret_cast<const u32x4*>(at + to_v);
+            if constexpr (A::I8) {
+                // a position's scales by the lane that has its first piece
+                if ((64 * i + lane) % A::UNITS == 0) {
+                    const int64_t e = pg * a.kv.scale_page_stride + kh * a.kv.scale_head_stride + off * a.kv.scale_pos_stride;
+                    ks[i] = ok ? a.kv.k_scale[e] : 0.0f;
+                    vs[i] = ok ? a.kv.v_scale[e] : 0.0f;
+                }
             }
-            kreg[i] = k, vreg[i] = v;
         }
     };
     auto put = [&](int buf) __attribute__((always_inline)) {
-        const int lane = here(), mine = A::MINE * wave + lane % A::MINE;
-        uint8_t* kt = tiles + buf * A::TILE + A::MINE * wave * A::ROW;
-        uint8_t* vt = kt + A::PLANES * A::PLANE;
+        const uint32_t lane = here();
+        uint8_t* kt = tiles + buf * A::TILE + A::MINE * wave * A::KROW;
+        uint8_t* vt = tiles + buf * A::TILE + A::VALUES + A::MINE * wave * A::VROW;
+        uint32_t ok_bits = (1u << A::MINE) - 1u;
+        uint64_t all = ~0ull;
+#pragma unroll
+        for (int i = 0; i < A::PER; i++) all &= ok_lanes[i];
+        if (all != ~0ull) {                                    // positions that are not there
+#pragma unroll
+            for (int i = 0; i < A::PER; i++)
+                if (!(ok_lanes[i] >> lane & 1u)) kreg[i] = vreg[i] = u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int p = 0; p < A::MINE; p++) {
+                constexpr int U = A::UNITS;
+                ok_bits &= ~((uint32_t)(~ok_lanes[p * U / 64] >> (p * U % 64) & 1u) << p);
+            }
+        }
+        if (!A::I8 && wild) {
+#pragma unroll
+            for (int i = 0; i < A::PER; i++) vreg[i] = finite<A::F16 ? 0x7c00u : 0x7f80u>(vreg[i]);
+        }
 #pragma unroll
         for (int i = 0; i < A::PER; i++) {
-            const int u = 64 * i + lane, pos = u / A::UNITS, col = u % A::UNITS;
-            u32x4 k = kreg[i], v = vreg[i];
-            const bool live = (A::MINE * A::UNITS % 64 == 0 || pos < A::MINE) && 16 * col < D * A::EB;
-            uint8_t *kp = kt + pos * A::ROW + 16 / A::EB * 2 * col, *vp = vt + pos * A::ROW + 16 / A::EB * 2 * col;
+            const uint32_t pos = pos_of(i, lane), col = col_of(i, lane);
+            uint8_t *kp = kt + pos * A::KROW + 2 / A::EB * col, *vp = vt + pos * A::VROW + 2 / A::EB * col;
+            const u32x4 k = kreg[i], v = vreg[i];
             if constexpr (A::I8) {
-                const u32x4 k0 = code_bf16(k.x, k.y), k1 = code_bf16(k.z, k.w), v0 = code_bf16(v.x, v.y), v1 = code_bf16(v.z, v.w);
-                if (live) {
-                    *reinterpret_cast<u32x4*>(kp) = k0, *reinterpret_cast<u32x4*>(kp + 16) = k1;
-                    *reinterpret_cast<u32x4*>(vp) = v0, *reinterpret_cast<u32x4*>(vp + 16) = v1;
-                }
+                *reinterpret_cast<u32x4*>(kp) = code_bf16(k.x, k.y), *reinterpret_cast<u32x4*>(kp + 16) = code_bf16(k.z, k.w);
+                *reinterpret_cast<u32x4*>(vp) = code_bf16(v.x, v.y), *reinterpret_cast<u32x4*>(vp + 16) = code_bf16(v.z, v.w);
+                if ((64 * i + lane) % A::UNITS == 0) scales[buf][0][A::MINE * wave + pos] = ks[i], scales[buf][1][A::MINE * wave + pos] = vs[i];
+            } else if constexpr (A::F16) {
+                u32x4 hi, lo;
+                cut.f16_pair(k, hi, lo);
+                if (wild) lo = finite<0x7f80u>(lo);            // the second part of an infinity or NaN is 0
+                *reinterpret_cast<u32x4*>(kp) = hi, *reinterpret_cast<u32x4*>(kp + A::KPLANE) = lo;
+                cut.f16_pair(v, hi, lo);
+                *reinterpret_cast<u32x4*>(vp) = hi, *reinterpret_cast<u32x4*>(vp + A::VPLANE) = lo;
             } else {
-                if (wild) v = finite<A::F16 ? 0x7c00u : 0x7f80u>(v);
-                if constexpr (A::PLANES == 2) {
-                    u32x4 kh, kl, vh, vl;
-                    f16_pair(k, kh, kl);
-                    f16_pair(v, vh, vl);
-                    if (live) {
-                        *reinterpret_cast<u32x4*>(kp) = kh, *reinterpret_cast<u32x4*>(kp + A::PLANE) = kl;
-                        *reinterpret_cast<u32x4*>(vp) = vh, *reinterpret_cast<u32x4*>(vp + A::PLANE) = vl;
-                    }
-                } else if (live) {
-                    *reinterpret_cast<u32x4*>(kp) = k;
-                    *reinterpret_cast<u32x4*>(vp) = v;
-                }
+                *reinterpret_cast<u32x4*>(kp) = k;
+                *reinterpret_cast<u32x4*>(vp) = v;
             }
         }
         if (lane == 0) there[buf][wave] = ok_bits;
-        if (A::I8 && lane < A::MINE) scales[buf][0][mine] = ks, scales[buf][1][mine] = vs;
     };
-    int page = entry(from);
-    fetch(from, page);
+    look(from);
+    fetch(from);
 
     // q's parts, in powers of 2
     u32x4 qp[NT][A::QS][3];
@@ -220,17 +231,20 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) 
             }
         }
     }
-    float m[NT], l[NT];
+    // e's exponents count from -under (0 at first), which moves where one passes MOST; any: the lanes whose rows have seen a position
+    constexpr float MOST = 8.0f;
+    float under[NT], l[NT];
+    uint64_t any[NT];
     f32x4 o[NT][ND];
-    // Once, and once more where an infinity or NaN among the values left a sum that is not finite: it reached rows that do not see it
-    // as 0 * inf.  Then such values count as 0, and are given to the rows that see them at the end.
+    // Once, and once more where an infinity or NaN in the cache left a sum that is not finite: a value reached rows that do not see
+    // it as 0 * inf.  Then such values count as 0, and are given to the rows that see them at the end.
     for (;;) {
-    page = entry(from + A::P);
+    look(from + A::P);
     put(0);
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        m[n] = -INFINITY, l[n] = 0.0f;
+        under[n] = 0.0f, l[n] = 0.0f, any[n] = 0;
 #pragma unroll
         for (int d = 0; d < ND; d++) o[n][d] = f32x4{0, 0, 0, 0};
     }
@@ -238,45 +252,38 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) 
     for (int first = from; first < to; first += A::P) {
         const bool on = first + A::P < to;
         if (on) {
-            fetch(first + A::P, page);
-            page = entry(first + 2 * A::P);
+            fetch(first + A::P);
+            look(first + 2 * A::P);
         }
         if (!idle) {
             const uint8_t* kt = tiles + buf * A::TILE;
-            const uint8_t* vt = kt + A::PLANES * A::PLANE;
-            f32x4 acc[NT][2] = {};
-            // a step of d for both 16 positions, the next one's on its way while it is multiplied (no more, which would cost
-            // registers); the two in turn, so that no product waits for the one just before it
-            u32x4 k[A::AHEAD ? 2 : 1][2][A::PLANES];
-            auto key = [&](int i, u32x4 (&to)[2][A::PLANES]) __attribute__((always_inline)) {
+            const uint8_t* vt = kt + A::VALUES;
+            f32x4 acc[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                const float x = A::I8 ? 0.0f : under[n];
+                acc[n][0] = acc[n][1] = f32x4{x, x, x, x};
+            }
+            // A step of d (of f16, of the second parts, then of the first) for both 16 positions, the next one's on its way while it is
+            // multiplied; the two in turn, so that no product waits for the one just before it.
+            constexpr int KN = A::QS * A::PLANES;
+            u32x4 k[2][2];
+            auto key = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
                 for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int j = 0; j < A::PLANES; j++)
-                        to[t][j] = *reinterpret_cast<const u32x4*>(kt + (16 * t + r) * A::ROW + 64 * i + 16 * g + j * A::PLANE);
+                    k[i & 1][t] = *reinterpret_cast<const u32x4*>(kt + (16 * t + r) * A::KROW + 64 * (i / A::PLANES) + 16 * g +
+                                                                  (A::PLANES - 1 - i % A::PLANES) * A::KPLANE);
             };
-            if (A::AHEAD) key(0, k[0]);
+            key(0);
 #pragma unroll
-            for (int i = 0; i < A::QS; i++) {
-                constexpr int B = A::AHEAD ? 1 : 0;
-                if (!A::AHEAD) key(i, k[0]);
-                else if (i + 1 < A::QS) key(i + 1, k[(i + 1) & B]);
-                u32x4 kh[2], kl[2];
+            for (int i = 0; i < KN; i++) {
+                if (i + 1 < KN) key(i + 1);
+                const bool first_part = i % A::PLANES == A::PLANES - 1;
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    kh[t] = k[i & B][t][0];
-                    if constexpr (A::F16) kl[t] = k[i & B][t][A::PLANES - 1];
-                }
-                if constexpr (A::F16) {
+                for (int j = first_part ? 2 : 1; j >= 0; j--)
 #pragma unroll
-                    for (int j = 1; j >= 0; j--)
-#pragma unroll
-                        for (int n = 0; n < 2 * NT; n++) acc[n >> 1][n & 1] = mma_bf16(kl[n & 1], qp[n >> 1][i][j], acc[n >> 1][n & 1]);
-                }
-#pragma unroll
-                for (int j = 2; j >= 0; j--)
-#pragma unroll
-                    for (int n = 0; n < 2 * NT; n++) acc[n >> 1][n & 1] = mma_bf16(kh[n & 1], qp[n >> 1][i][j], acc[n >> 1][n & 1]);
+                    for (int n = 0; n < 2 * NT; n++)
+                        acc[n >> 1][n & 1] = mma_bf16(k[i & 1][n & 1], qp[n >> 1][i / A::PLANES][j], acc[n >> 1][n & 1]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (A::I8) {
@@ -284,7 +291,9 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) 
                 for (int t = 0; t < 2; t++) {
                     const f32x4 x = *reinterpret_cast<const f32x4*>(&scales[buf][0][16 * t + 4 * g]);
 #pragma unroll
-                    for (int n = 0; n < NT; n++) acc[n][t] *= x;
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[n][t][i] = __builtin_fmaf(acc[n][t][i], x[i], under[n]);
                 }
             }
             uint32_t ok = 0;                                   // the step's positions that are there
@@ -310,81 +319,77 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) 
                 float top = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = fmaxf(top, acc[n][i >> 2][i & 3]);
-                top = fmaxf(m[n], xor32_max(xor16_max(top)));
-                const float keep = m[n] == top ? 1.0f : __builtin_amdgcn_exp2f(m[n] - top);
-                if (!__all(keep == 1.0f)) {
+                if (__ballot(top > MOST) | (__ballot(top > -INFINITY) & ~any[n])) {
+                    top = xor32_max(xor16_max(top));
+                    // (by the tile's largest itself: what rounding `under` moves, far from 0, must not leave e above 1)
+                    const bool had = any[n] >> lane & 1u, up = top > (had ? MOST : -INFINITY);
+                    const float by = up ? top : 0.0f, keep = had ? __builtin_amdgcn_exp2f(-by) : 1.0f;
+                    under[n] -= by;
+                    any[n] |= __ballot(up);
                     l[n] *= keep;
 #pragma unroll
                     for (int d = 0; d < ND; d++) o[n][d] *= keep;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) acc[n][i >> 2][i & 3] -= by;
                 }
-                m[n] = top;
-                const float under = top == -INFINITY ? 0.0f : top;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float x = __builtin_amdgcn_exp2f(acc[n][i >> 2][i & 3] - under);
+                    const float x = __builtin_amdgcn_exp2f(acc[n][i >> 2][i & 3]);
                     acc[n][i >> 2][i & 3] = x;
                     l[n] += x;
                 }
             }
             {
                 u32x4 ep[NT][3];
-                f32x4 x[2];
-                if constexpr (A::I8)
+                if constexpr (A::I8) {
+                    f32x4 x[2];
 #pragma unroll
                     for (int t = 0; t < 2; t++) x[t] = *reinterpret_cast<const f32x4*>(&scales[buf][1][16 * t + 4 * g]);
+                    auto scaled = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int i = 0; i < 8 * NT; i++) {
+                            const float e = acc[i >> 3][i >> 2 & 1][i & 3], y = e * x[i >> 2 & 1][i & 3];
+                            acc[i >> 3][i >> 2 & 1][i & 3] = decltype(careful)::value && e == 0.0f ? e : y;
+                        }
+                    };
+                    if (partly) scaled(std::true_type());      // a position that a row does not see takes no part, whatever its scale
+                    else scaled(std::false_type());
+                }
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        float e0 = acc[n][j >> 1][2 * (j & 1)], e1 = acc[n][j >> 1][2 * (j & 1) + 1];
-                        if constexpr (A::I8) {                 // a NaN stays one, a 0 takes no part
-                            e0 = e0 == 0.0f ? e0 : e0 * x[j >> 1][2 * (j & 1)];
-                            e1 = e1 == 0.0f ? e1 : e1 * x[j >> 1][2 * (j & 1) + 1];
-                        }
+                        const float e0 = acc[n][j >> 1][2 * (j & 1)], e1 = acc[n][j >> 1][2 * (j & 1) + 1];
                         uint32_t q0, q1, q2;
-                        split3(e0, e1, q0, q1, q2);
+                        cut.split3(e0, e1, q0, q1, q2);
                         ep[n][0][j] = q0, ep[n][1][j] = q1, ep[n][2][j] = q2;
                     }
                 // four positions' values at a time, transposed: lane r's d, positions 4 g + 0..3 of each 16
-                const uint8_t* at = vt + (4 * g + (r >> 2)) * A::ROW + 8 * (r & 3);
-                auto value = [&](int d, u32x4 (&to)[2][A::PLANES]) __attribute__((always_inline)) {
+                const uint8_t* at = vt + (4 * g + (r >> 2)) * A::VROW + 8 * (r & 3);
+                constexpr int VN = ND / 2 * A::PLANES;
+                u32x4 v[2][2];
+                auto value = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int w = 0; w < 2; w++)
-#pragma unroll
-                        for (int j = 0; j < A::PLANES; j++) {
-                            const uint8_t* from = at + j * A::PLANE + 32 * (d + w);
-                            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)from));
-                            const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(from + 16 * A::ROW)));
-                            to[w][j] = u32x4{x.x, x.y, y.x, y.y};
-                        }
-                };
-                {
-                    u32x4 v[A::AHEAD ? 2 : 1][2][A::PLANES];
-                    constexpr int B = A::AHEAD ? 1 : 0;
-                    if (A::AHEAD) value(0, v[0]);
-#pragma unroll
-                    for (int d = 0; d < ND; d += 2) {
-                        if (!A::AHEAD) value(d, v[0]);
-                        else if (d + 2 < ND) value(d + 2, v[((d >> 1) + 1) & B]);
-                        u32x4 vh[2], vl[2];
-#pragma unroll
-                        for (int w = 0; w < 2; w++) {
-                            const u32x4 raw = v[d >> 1 & B][w][0];
-                            vh[w] = raw;
-                            if constexpr (A::F16) vl[w] = v[d >> 1 & B][w][A::PLANES - 1];
-                        }
-                        if constexpr (A::F16) {
-#pragma unroll
-                            for (int j = 1; j >= 0; j--)
-#pragma unroll
-                                for (int n = 0; n < 2 * NT; n++) o[n >> 1][d + (n & 1)] = mma_bf16(vl[n & 1], ep[n >> 1][j], o[n >> 1][d + (n & 1)]);
-                        }
-#pragma unroll
-                        for (int j = 2; j >= 0; j--)
-#pragma unroll
-                            for (int n = 0; n < 2 * NT; n++) o[n >> 1][d + (n & 1)] = mma_bf16(vh[n & 1], ep[n >> 1][j], o[n >> 1][d + (n & 1)]);
-                        __builtin_amdgcn_sched_barrier(0);
+                    for (int w = 0; w < 2; w++) {
+                        const uint8_t* from = at + 64 * (i / A::PLANES) + 32 * w + (A::PLANES - 1 - i % A::PLANES) * A::VPLANE;
+                        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)from));
+                        const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(from + 16 * A::VROW)));
+                        v[i & 1][w] = u32x4{x.x, x.y, y.x, y.y};
                     }
+                };
+                value(0);
+#pragma unroll
+                for (int i = 0; i < VN; i++) {
+                    if (i + 1 < VN) value(i + 1);
+                    const bool first_part = i % A::PLANES == A::PLANES - 1;
+#pragma unroll
+                    for (int j = first_part ? 2 : 1; j >= 0; j--)
+#pragma unroll
+                        for (int n = 0; n < 2 * NT; n++) {
+                            f32x4& to = o[n >> 1][2 * (i / A::PLANES) + (n & 1)];
+                            to = mma_bf16(v[i & 1][n & 1], ep[n >> 1][j], to);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
         }
@@ -404,8 +409,10 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) 
             if (16 * d < D) zero += o[n][d] * 0.0f;
     if (!__syncthreads_or(!idle && !(zero.x + zero.y + (zero.z + zero.w) == 0.0f))) break;
     wild = true;
-    fetch(from, entry(from));
+    look(from);
+    fetch(from);
     }
+    const int me = here(), row_of_me = me & 15, d_of_me = 4 * (me >> 4);
     if (!A::I8 && wild && !idle) {
         uint64_t nodes[NT];
 #pragma unroll
@@ -414,7 +421,7 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) 
             for (int p = from; p < to; p++) {
                 const int page = __builtin_amdgcn_readfirstlane(table[p >> a.page_shift]);
                 if ((unsigned)page >= (unsigned)a.kv.pages) continue;
-                const uint8_t* at = vb + (page * a.kv.page_stride + (p & (a.kv.page_size - 1)) * a.kv.pos_stride) * A::EB + 8 * g;
+                const uint8_t* at = kb + to_v + (uint64_t)page * page_bytes + (uint64_t)(p & (a.kv.page_size - 1)) * pos_bytes + 2 * d_of_me;
                 const int node = p - base;
 #pragma unroll
                 for (int d = 0; d < ND; d++)
@@ -435,7 +442,7 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) 
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         l[n] = xor32_sum(xor16_sum(l[n]));
-        if (!nodes_of(n)) m[n] = -INFINITY, l[n] = 0.0f;          // no node: it has seen nothing
+        if (!nodes_of(n)) l[n] = 0.0f;                           // no node: it has seen nothing
     }
     const int64_t part0 = (((int64_t)b * a.kv.heads + kh) * R) * a.parts + z;
     auto out_of = [&](int row) {
@@ -445,14 +452,14 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 ? 3 : 2) 
     if (idle) return;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const int row = row0 + 16 * n + r;
+        const int row = row0 + 16 * n + row_of_me;
         if (row >= R) continue;
-        if (a.joined && g == 0) a.pml[part0 + (int64_t)row * a.parts] = AttnMl{m[n], l[n]};
+        if (a.joined && d_of_me == 0) a.pml[part0 + (int64_t)row * a.parts] = AttnMl{l[n] != 0.0f ? -under[n] : -INFINITY, l[n]};
         float* to = out_of(row);
 #pragma unroll
         for (int d = 0; d < ND; d++)
             if (16 * d < D)
-                *reinterpret_cast<f32x4_a4*>(to + 16 * d + 4 * g) = l[n] == 0.0f ? f32x4{0, 0, 0, 0} : a.joined ? o[n][d] : o[n][d] / l[n];
+                *reinterpret_cast<f32x4_a4*>(to + 16 * d + d_of_me) = l[n] == 0.0f ? f32x4{0, 0, 0, 0} : a.joined ? o[n][d] : o[n][d] / l[n];
     }
 }
 

@@ -1,40 +1,60 @@
 // Attention of trees of drafted tokens over a paged key-value cache (include/kq.h: kq_attn_tree): how the positions are
 // split, and the join of the parts that attn_tree.h's kernels leave.
-#include "attn_tree.h"
+#include <math.h>
+
+#include "kv_device.h"
 
 namespace kq {
 
-// ROWS rows a workgroup, 256 / ROWS threads each: lanes of 4 values, in groups that take every so many parts.
+// ROWS rows a workgroup, 256 / ROWS threads each: lanes of 4 values, in groups that take every so many parts.  The parts'
+// largest scores and sums are looked at by all of a row's threads, and their weights left in LDS.
+constexpr int TJ_MOST = 2048;                // parts of a row at most
 template <int ROWS>
 __global__ void __launch_bounds__(256) k_attn_tree_join(AttnArgs a, int lanes) {
-    __shared__ f32x4 so[256];
-    __shared__ float sl[256];
-    const int tid = threadIdx.x, per = 256 / ROWS, groups = per / lanes, at = tid % per, group = at / lanes, d = 4 * (at % lanes);
-    const int D = a.kv.dim, G = a.group, H = a.q_heads;
-    const int64_t i = (int64_t)blockIdx.x * ROWS + tid / per, rows = (int64_t)a.table.seqs * a.T * H;
-    const int64_t bt = min(i, rows - 1) / H;
-    const int h = (int)(min(i, rows - 1) % H), b = (int)(bt / a.T), t = (int)(bt % a.T);
+    extern __shared__ float weight[];                          // [row][part], then the groups' sums
+    __shared__ float stat[ROWS];
+    const int per = 256 / ROWS, mine = threadIdx.x / per, at = threadIdx.x % per, groups = per / lanes, group = at / lanes;
+    const int d = 4 * (at % lanes), D = a.kv.dim, G = a.group, H = a.q_heads;
+    const int64_t rows = (int64_t)a.table.seqs * a.T * H, i = min((int64_t)blockIdx.x * ROWS + mine, rows - 1), bt = i / H;
+    const int h = (int)(i % H), b = (int)(bt / a.T), t = (int)(bt % a.T);
     const int len = tree_length(a, a.lens[b]), n = (len + a.split - 1) / a.split;
     const int64_t row = (((int64_t)b * a.kv.heads + h / G) * a.T * G + t * G + h % G) * a.parts;
-    float top = -INFINITY;
-    for (int c = 0; c < n; c++) top = fmaxf(top, a.pml[row + c].m);
-    f32x4 sum = {0, 0, 0, 0};
-    float total = 0.0f;
-    if (group < groups && d < D)
-        for (int c = group; c < n; c += groups) {
+    float* const w = weight + mine * a.parts;
+    // the first wave of a row's threads (or the part of one that they are)
+    if (at < 64) {
+        const int step = min(per, 64);
+        float top = -INFINITY, total = 0.0f;
+        for (int c = at; c < n; c += step) top = fmaxf(top, a.pml[row + c].m);
+        for (int x = step >> 1; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+        for (int c = at; c < n; c += step) {
             const AttnMl ml = a.pml[row + c];
-            const f32x4 x = *reinterpret_cast<const f32x4*>(a.po + (row + c) * D + d);
             const float k = ml.l != 0.0f ? __builtin_amdgcn_exp2f(ml.m - top) : 0.0f;   // 0: the row saw nothing (a NaN counts)
-            if (ml.l != 0.0f) sum += x * k;
+            w[c] = k;
             total += ml.l * k;
         }
+        for (int x = step >> 1; x; x >>= 1) total += __shfl_xor(total, x, 64);
+        if (at == 0) stat[mine] = total;
+    }
+    __syncthreads();
+    f32x4 sum = {0, 0, 0, 0};
+    if (d < D) {
+        const float* po = a.po + row * D + d;
+#pragma unroll 4
+        for (int c = group; c < n; c += groups) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(po + (int64_t)c * D);
+            const float k = w[c];
+            sum += k != 0.0f ? x * k : f32x4{0, 0, 0, 0};
+        }
+    }
     if (groups > 1) {
-        so[tid] = sum, sl[tid] = total;
+        f32x4* so = reinterpret_cast<f32x4*>(weight + (ROWS * a.parts + 3) / 4 * 4);
+        so[threadIdx.x] = sum;
         __syncthreads();
         if (group == 0)
-            for (int w = 1; w < groups; w++) sum += so[tid + w * lanes], total += sl[tid + w * lanes];
+            for (int x = 1; x < groups; x++) sum += so[threadIdx.x + x * lanes];
     }
-    if (group == 0 && d < D && i < rows)
+    const float total = stat[mine];
+    if (group == 0 && d < D && (int64_t)blockIdx.x * ROWS + mine < rows)
         *reinterpret_cast<f32x4_a4*>(a.out + bt * a.ldo + (int64_t)h * D + d) = total == 0.0f ? f32x4{0, 0, 0, 0} : sum / total;
 }
 
@@ -47,10 +67,9 @@ static TreeSplit split_of(int seqs, int heads, int group, int dim, int T, int ma
     const int R = T * group;
     s.tiles = R <= 64 || dim > 128 ? 1 : 2;
     const int64_t columns = (int64_t)seqs * heads * ((R + 64 * s.tiles - 1) / (64 * s.tiles));
-    const int64_t want = (2048 + columns - 1) / columns;
+    const int64_t want = ((s.tiles == 2 ? 512 : 2048) + columns - 1) / columns;
     int64_t split = (max_len + want - 1) / want;
-    if (split < 64) split = 64;
-    if (split < (max_len + 65534) / 65535) split = (max_len + 65534) / 65535;
+    if (split < (max_len + TJ_MOST - 1) / TJ_MOST) split = (max_len + TJ_MOST - 1) / TJ_MOST;
     split = (split + 31) / 32 * 32;
     s.split = (int)split;
     s.parts = (int)((max_len + split - 1) / split);
@@ -93,9 +112,15 @@ void launch_attn_tree(const AttnArgs& args, hipStream_t s) {
     if (!a.joined) return;
     const int64_t rows = (int64_t)a.table.seqs * a.T * a.q_heads;
     const int lanes = a.kv.dim <= 64 ? 16 : a.kv.dim <= 128 ? 32 : 64;
-    if (a.parts <= 16 && lanes <= 32) hipLaunchKernelGGL(k_attn_tree_join<8>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, s, a, lanes);
-    else if (a.parts <= 16) hipLaunchKernelGGL(k_attn_tree_join<4>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a, lanes);
-    else hipLaunchKernelGGL(k_attn_tree_join<1>, dim3((unsigned)rows), dim3(256), 0, s, a, lanes);
+    // few parts: a row's threads are its lanes alone, and several rows share a workgroup
+    auto go = [&](auto kernel, int each) {
+        const size_t lds = ((size_t)each * a.parts + 3) / 4 * 16 + (256 / each > lanes ? 4096 : 0);
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + each - 1) / each)), dim3(256), lds, s, a, lanes);
+    };
+    if (a.parts > 16) go(k_attn_tree_join<1>, 1);
+    else if (lanes == 64) go(k_attn_tree_join<4>, 4);
+    else if (lanes == 32) go(k_attn_tree_join<8>, 8);
+    else go(k_attn_tree_join<16>, 16);
 }
 
 }  // namespace kq

@@ -17,4 +17,9 @@ __device__ __forceinline__ uint32_t bf16_rne(float x) {
     return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
 }
 
+// The positions of a request with a tree that are there: those ahead of its tree, and T more.
+__device__ __forceinline__ int tree_length(const AttnArgs& a, int base) {
+    return base < 0 ? 0 : min(min(base, a.max_len) + a.T, a.max_len);
+}
+
 }  // namespace kq

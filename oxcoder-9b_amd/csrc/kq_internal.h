@@ -202,7 +202,8 @@ struct VerifyArgs {
     int32_t *accepted, *path, *token;
     uint8_t* ws;
     // set by launch_verify
-    int slice, slices;         // ids of a slice, slices of a row
+    int slice, slices, shift;  // ids of a slice (2^shift), slices of a row
+    size_t parts_at, sums_at;  // places in the workspace
 };
 size_t verify_workspace(int B, int T, int V);
 void launch_verify(const VerifyArgs& a, hipStream_t s);

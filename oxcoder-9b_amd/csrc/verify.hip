@@ -5,18 +5,22 @@
 // a_0 = 0, Z_0 = 1, a_k+1 = a_k + Z_k, Z_k+1 = sum max(p - a_k+1 q, 0).  So what is left is one number a and the row.  For a
 // child that was not drawn (q holds it alone) what is left is p without the refused tokens.
 //
-// The first kernel takes every row's softmax statistics slice by slice; the second, one workgroup a request, walks the tree on
-// the rows' statistics and its tokens' logits, all fetched at once, and draws the next token: over the slices' sums, then
-// inside one slice.
+// A round is two kernels: the first takes softmax statistics, slice by slice, of the row that a request's walk stands at and of as
+// many levels of nodes below it as fit a budget of rows; the second, one workgroup a request, walks on over those and, where
+// the walk ends, draws the next token: over the slices' sums, then inside one slice.  Rows that no walk comes to need not be
+// read: a batch of large trees takes four rounds, the last of which reads whatever is left below the few walks that still go on.
+// Where a draft's probabilities leave something else than p, two more kernels sum what is left slice by slice and draw.
 #include "kq_device.h"
 #include "kq_internal.h"
 
 namespace kq {
 
-constexpr int VF_T = 256;                    // threads of the first kernel
-constexpr int VF_MOST = 8192;                // ids of its largest slice
-constexpr int VF_LEAST = 2048;
-constexpr int VF_W = 1024;                   // threads of the second
+constexpr int VF_T = 256;                    // threads of the kernels that read rows
+constexpr int VF_MOST = 8192;                // ids of their largest slice (half, and a quarter, are the others)
+constexpr int VF_LEAST = 2048;               // and of the smallest
+constexpr int VF_W = 1024;                   // threads of the walk
+constexpr int VF_EACH = VF_MOST / VF_W;      // ids of one of them in a slice
+constexpr int VF_ROUNDS = 4;
 
 // Weights are held in 64 bits as well: a vocabulary's running sum has a border for every id, and fp32 weights, off by 2^-24
 // each, would put one draw in some hundred on the border's other side.
@@ -27,82 +31,170 @@ struct VfScale {
 __device__ __forceinline__ VfScale vf_scale(const VerifyArgs& a, int b) {
     const float t = a.temperature ? a.temperature[b] : 1.0f;
     const bool greedy = !(t > 0.0f);
-    return VfScale{greedy ? 0.0 : 1.4426950408889634 / (double)t, greedy};
+    return VfScale{greedy ? 0.0 : 1.4426950408889634 / fmin((double)t, 3e38), greedy};
 }
-// 2^z, z <= 0: ln(2)^k / k! f^k summed to k = 11 over the fraction f in -1/2..1/2, off by at most (ln(2)/2)^12 / 12! = 6.3e-15
-// of it; below 2^-1000, and for a NaN, 0.
-__device__ __forceinline__ double vf_exp2(double z) {
-    if (!(z > -1000.0)) return 0.0;
-    const double n = rint(z), f = z - n;
-    double p = 4.44553827187081e-10;
-    p = fma(p, f, 7.054911620801121e-09);
-    p = fma(p, f, 1.0178086009239696e-07);
-    p = fma(p, f, 1.3215486790144305e-06);
-    p = fma(p, f, 1.5252733804059838e-05);
-    p = fma(p, f, 0.00015403530393381606);
-    p = fma(p, f, 0.0013333558146428441);
-    p = fma(p, f, 0.009618129107628477);
-    p = fma(p, f, 0.055504108664821576);
-    p = fma(p, f, 0.2402265069591007);
-    p = fma(p, f, 0.6931471805599453);
-    return ldexp(fma(p, f, 1.0), (int)n);
-}
-// x's weight beside the largest logit m: 1 for m itself, 0 for -inf and NaN.
-__device__ __forceinline__ double vf_weight(const VfScale& s, float x, float m) {
-    return x == m ? 1.0 : vf_exp2(((double)x - (double)m) * s.c);
-}
+// x's weight beside the row's largest logit m, 2^(c (x - m)): 0 for -inf and NaN; beside +inf, 1 for that alone.  To within 4e-14 of
+// it: 2^f over the fraction f of the exponent, in -1/2..1/2, is the polynomial of degree 9 that equals it at Chebyshev's points
+// (2e-14 off at most; c x - c m would be off by the rounding of c m, which a low temperature makes large).
+struct VfTop {
+    float m;
+    double c, least;                                           // least: a difference whose weight is 0
+    __device__ __forceinline__ VfTop(const VfScale& s, float top) : m(top), c(s.c), least(-2000.0 / s.c) {}
+    __device__ __forceinline__ double weight(float x) const {
+        if (m == INFINITY) return x == m ? 1.0 : 0.0;
+        const double z = fmax((double)x - (double)m, least) * c;
+        const double t = z + 0x1.8p52;                         // its low half is z to the nearest integer
+        const double f = z - (t - 0x1.8p52);
+        double p = 1.0205905413765595e-07;
+        p = fma(p, f, 1.325964524488711e-06);
+        p = fma(p, f, 1.5252672924850737e-05);
+        p = fma(p, f, 0.0001540343375125101);
+        p = fma(p, f, 0.0013333558200794592);
+        p = fma(p, f, 0.009618129193934313);
+        p = fma(p, f, 0.05550410866465167);
+        p = fma(p, f, 0.2402265069564034);
+        p = fma(p, f, 0.6931471805599462);
+        p = fma(p, f, 1.0000000000000135);
+        return ldexp(p, (int)__builtin_bit_cast(uint64_t, t));
+    }
+};
+__device__ __forceinline__ double vf_weight(const VfScale& s, float x, float m) { return VfTop(s, m).weight(x); }
 
 __device__ __forceinline__ double vf_wave_sum(double v) {
     for (int w = 32; w; w >>= 1) v += __shfl_xor(v, w, 64);
     return v;
 }
 
-template <bool V4>
-__global__ void __launch_bounds__(VF_T) k_verify_stats(VerifyArgs a) {
+// Where a request's walk stands.
+enum { VF_WALKING, VF_DONE, VF_LEFT };       // VF_LEFT: a draft was refused, and what that leaves is still to be summed
+struct VfState {
+    int cur, n, status, child; // the node, accepted drafts, the child that was refused
+    int first;                 // the row's largest logit: its place
+    float m;                   // and it
+    double per;                // 1 / the sum of the row's weights
+};
+__device__ __forceinline__ VfState* vf_state(const VerifyArgs& a, int b) { return reinterpret_cast<VfState*>(a.ws) + b; }
+__device__ __forceinline__ VerifyPart* vf_parts(const VerifyArgs& a, int64_t row) {
+    return reinterpret_cast<VerifyPart*>(a.ws + a.parts_at) + row * a.slices;
+}
+__device__ __forceinline__ double* vf_sums(const VerifyArgs& a, int b) {
+    return reinterpret_cast<double*>(a.ws + a.sums_at) + (int64_t)b * a.slices;
+}
+
+// The nodes whose rows a round looks at, by a whole wave with up = the lane's node's parent (-2: none): cur, and as many whole levels
+// below it as leave at most `most` nodes.
+__device__ __forceinline__ uint64_t vf_round(int up, int cur, int most) {
+    const int lane = threadIdx.x & 63;
+    // steps up to cur, by doubling; far: not below cur
+    int link = up, steps = 1;
+    bool there = lane == cur;
+    if (there) link = lane, steps = 0;
+#pragma unroll 1
+    for (int i = 0; i < 6; i++) {
+        const int from = max(link, 0);
+        const int on = __shfl(link, from, 64), more = __shfl(steps, from, 64);
+        if (link >= 0 && !there) {
+            steps += more;
+            link = on;
+        }
+    }
+    const bool below = link == cur;
+    uint64_t nodes = 1ull << cur;
+#pragma unroll 1
+    for (int level = 1; level < TREE_MOST; level++) {
+        const uint64_t more = __ballot(below && steps <= level);
+        if (more == nodes || __popcll(more) > most) break;
+        nodes = more;
+    }
+    return nodes;
+}
+// The lane's node's parent, -2 where it is none.
+__device__ __forceinline__ int vf_up(const VerifyArgs& a, int b, int t) {
+    const int up = t < a.T ? a.parents[(int64_t)b * a.ldp + t] : -2;
+    return t ? (up >= 0 && up < t ? up : -2) : up;
+}
+
+// A slice's nv values into LDS; returns the thread's largest.  (Here and below, loops that take an exponential each are kept rolled and
+// code is shared where it can be: a kernel of some microseconds waits for its own instructions, some tenths of one for each KB.)
+template <bool V4, int SLICE>
+__device__ __forceinline__ float vf_stage(const float* x, int nv, float* to) {
+    constexpr int QUADS = SLICE / VF_T / 4;
+    float m = -INFINITY;
+    if (nv == SLICE) {
+        f32x4 v[QUADS];
+#pragma unroll
+        for (int n = 0; n < QUADS; n++) {
+            const float* at = x + 4 * (n * VF_T + threadIdx.x);
+            if constexpr (V4) v[n] = *reinterpret_cast<const f32x4*>(at);
+            else v[n] = *reinterpret_cast<const f32x4_a4*>(at);
+        }
+#pragma unroll
+        for (int n = 0; n < QUADS; n++) {
+            m = fmaxf(m, fmaxf(fmaxf(v[n].x, v[n].y), fmaxf(v[n].z, v[n].w)));
+            *reinterpret_cast<f32x4*>(to + 4 * (n * VF_T + threadIdx.x)) = v[n];
+        }
+    } else {
+#pragma unroll 1
+        for (int i = threadIdx.x; i < nv; i += VF_T) {
+            const float v = x[i];
+            to[i] = v;
+            m = fmaxf(m, v);
+        }
+    }
+    return m;
+}
+
+template <bool V4, int SLICE>
+__global__ void __launch_bounds__(VF_T) k_verify_stats(VerifyArgs a, int round, int most) {
+    extern __shared__ __attribute__((aligned(16))) float vf_lds[];
     __shared__ float sm[VF_T / 64];
     __shared__ double ss[VF_T / 64];
     __shared__ int sa[VF_T / 64];
-    const int64_t row = blockIdx.y;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, v0 = blockIdx.x * a.slice, nv = min(a.slice, a.V - v0);
-    const float* x = a.x + row * a.ldx + v0;
-    const VfScale s = vf_scale(a, (int)(row / a.T));
-    f32x4 v[VF_MOST / VF_T / 4];
-#pragma unroll
-    for (int n = 0; n < VF_MOST / VF_T / 4; n++) {
-        const int i = 4 * (n * VF_T + tid);
-        v[n] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (i + 3 < nv) {
-            if constexpr (V4) v[n] = *reinterpret_cast<const f32x4*>(x + i);
-            else v[n] = *reinterpret_cast<const f32x4_a4*>(x + i);
-        } else {
-            for (int k = 0; k < 3; k++)
-                if (i + k < nv) v[n][k] = x[i + k];
+    const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int up = vf_up(a, b, lane);
+    int cur = 0;
+    if (round) {
+        const VfState* state = vf_state(a, b);
+        if (state->status != VF_WALKING) return;
+        cur = state->cur;
+    } else if (__shfl(up, 0, 64) != -1) {
+        return;
+    }
+    uint64_t nodes = vf_round(up, cur, most);
+    const int v0 = blockIdx.x * SLICE, nv = min(SLICE, a.V - v0);
+    const VfScale s = vf_scale(a, b);
+#pragma unroll 1
+    for (int k = 0; nodes; nodes &= nodes - 1, k++) {
+        if (k % (int)gridDim.z != (int)blockIdx.z) continue;
+        const int64_t row = (int64_t)b * a.T + __builtin_ctzll(nodes);
+        const float* x = a.x + row * a.ldx + v0;
+        float m = vf_stage<V4, SLICE>(x, nv, vf_lds);
+        for (int w = 32; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
+        __syncthreads();
+        if (lane == 0) sm[wave] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+        double sum = 0.0;
+        int at = INT_MAX;
+        if (m > -INFINITY) {
+            const VfTop top(s, m);
+            if (s.greedy) {                                    // its place alone counts
+                for (int i = tid; i < nv && at == INT_MAX; i += VF_T)
+                    if (vf_lds[i] == m) at = i;
+            } else {
+#pragma unroll 2
+                for (int i = tid; i < nv; i += VF_T) sum += top.weight(vf_lds[i]);
+            }
+        }
+        sum = vf_wave_sum(sum);
+        for (int w = 32; w; w >>= 1) at = min(at, __shfl_xor(at, w, 64));
+        if (lane == 0) ss[wave] = sum, sa[wave] = at;
+        __syncthreads();
+        if (tid == 0) {
+            at = min(min(sa[0], sa[1]), min(sa[2], sa[3]));
+            vf_parts(a, row)[blockIdx.x] = VerifyPart{(ss[0] + ss[1]) + (ss[2] + ss[3]), m, s.greedy && m > -INFINITY ? v0 + at : 0};
         }
     }
-    float m = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < VF_MOST / VF_T / 4; n++) m = fmaxf(m, fmaxf(fmaxf(v[n].x, v[n].y), fmaxf(v[n].z, v[n].w)));
-    for (int w = 32; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
-    if (lane == 0) sm[wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    double sum = 0.0;
-    int at = INT_MAX;
-#pragma unroll
-    for (int n = VF_MOST / VF_T / 4 - 1; n >= 0; n--)
-#pragma unroll
-        for (int k = 3; k >= 0; k--) {
-            if (v[n][k] == m) at = 4 * (n * VF_T + tid) + k;
-            if (m > -INFINITY) sum += vf_weight(s, v[n][k], m);
-        }
-    sum = vf_wave_sum(sum);
-    for (int w = 32; w; w >>= 1) at = min(at, __shfl_xor(at, w, 64));
-    if (lane == 0) ss[wave] = sum, sa[wave] = at;
-    __syncthreads();
-    if (tid) return;
-    VerifyPart* part = reinterpret_cast<VerifyPart*>(a.ws) + row * a.slices + blockIdx.x;
-    at = min(min(sa[0], sa[1]), min(sa[2], sa[3]));
-    *part = VerifyPart{(ss[0] + ss[1]) + (ss[2] + ss[3]), m, m > -INFINITY ? v0 + at : 0};
 }
 
 // A row's distribution as the walk left it: weights of p, less the refused tokens or a times q's.
@@ -117,200 +209,430 @@ struct VfLeft {
 struct VfShared {
     int tok[TREE_MOST], up[TREE_MOST], top_at[TREE_MOST], refused[TREE_MOST];
     float m[TREE_MOST], u[TREE_MOST], x[TREE_MOST], q[TREE_MOST];
-    double sum[TREE_MOST];
-    double seg[VF_W], wave[VF_W / 64];
-    int found;
+    double sum[TREE_MOST], gone[TREE_MOST];  // gone: the refused tokens' weights
+    double wave[VF_W / 64];
+    int found, last;
+    uint64_t nodes;
 };
 
-__device__ __forceinline__ double vf_left(const VfShared& S, const VfScale& s, const VfLeft& f, int i) {
-    const double e = s.greedy ? (i == f.first ? 1.0 : 0.0) : vf_weight(s, f.x[i], f.m);
-    if (f.q) return fmax(e * f.per - f.a * (double)f.q[i], 0.0);
+__device__ __forceinline__ double vf_left(const VfShared& S, const VfScale& s, const VfLeft& f, int i, float x, float q) {
+    const double e = s.greedy ? (i == f.first ? 1.0 : 0.0) : vf_weight(s, x, f.m);
+    if (f.q) return fmax(e * f.per - f.a * (double)q, 0.0);
     for (int k = 0; k < f.gone; k++)
         if (S.refused[k] == i) return 0.0;
     return e;
 }
 
-// Sums of the row's segments of `len` ids into S.seg, and their total.
-__device__ double vf_segments(VfShared& S, const VfScale& s, const VfLeft& f, int V, int len) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = (V + len - 1) / len;
-    __syncthreads();
-    for (int g = wave; g < n; g += VF_W / 64) {
-        const int end = min((g + 1) * len, V);
-        double sum = 0.0;
-        for (int i = g * len + lane; i < end; i += 64) sum += vf_left(S, s, f, i);
-        sum = vf_wave_sum(sum);
-        if (lane == 0) S.seg[g] = sum;
-    }
-    __syncthreads();
-    double total = 0.0;
-    for (int g = lane; g < n; g += 64) total += S.seg[g];
-    return vf_wave_sum(total);
+__device__ __forceinline__ double vf_left(const VfShared& S, const VfScale& s, const VfLeft& f, int i) {
+    return vf_left(S, s, f, i, f.x[i], f.q ? f.q[i] : 0.0f);
 }
 
-// The smallest id of [from, to) at which before + the running sum exceeds the target; the last one with a weight where
-// none does (the sums' own rounding), -1 where none has one.
-__device__ int vf_pick(VfShared& S, const VfScale& s, const VfLeft& f, int from, int to, double before, double target) {
+// Sum of weight(i) over [0, n), by the whole workgroup.
+template <class F>
+__device__ double vf_sum(VfShared& S, F weight, int n) {
+    double sum = 0.0;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += VF_W) sum += weight(i);
+    sum = vf_wave_sum(sum);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) S.wave[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int k = 0; k < VF_W / 64; k++) sum += S.wave[k];
+    return sum;
+}
+
+// The token that follows: the smallest id at which the running sum of what is left exceeds its share of the total, by the
+// whole workgroup.  First over the slices, whose sums come from their statistics, or from `sums`; then inside one.  Where
+// there are no sums of the slices (`rows`), and where the slice found has none left (what rounding left of refused tokens
+// was its sum), over the row itself: its total, and then the id.
+__device__ int vf_draw(VfShared& S, const VerifyArgs& a, const VfScale& s, const VfLeft& f, double left, const VerifyPart* parts,
+                       const double* sums, bool rows) {
+    extern __shared__ __attribute__((aligned(16))) double vf_w[];      // VF_MOST weights, then as many floats of q where there is one
+    float* const vf_q = reinterpret_cast<float*>(vf_w + VF_MOST);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int last = -1;
-    for (int i0 = from; i0 < to; i0 += VF_W) {
-        const int i = i0 + tid;
-        const double w = i < to ? vf_left(S, s, f, i) : 0.0;
-        double run = w;
-        for (int k = 1; k < 64; k <<= 1) {
-            const double y = __shfl_up(run, k, 64);
-            if (lane >= k) run += y;
-        }
+    const VfTop top(s, f.m);
+    double target = (double)S.u[0] * left, before = 0.0;
+    int from = 0, to = a.slices;
+    enum { SLICES, IDS, TOTAL, FIND };
+    int found = -1;
+#pragma unroll 1
+    for (int what = rows ? TOTAL : SLICES; what <= FIND; what++) {
+        if (what >= TOTAL) from = 0, to = a.V, before = 0.0;
+        if (what == TOTAL) target = INFINITY;
+        int last = -1;
         __syncthreads();
-        if (tid == 0) S.found = INT_MAX;
-        if (lane == 63) S.wave[wave] = run;
-        __syncthreads();
-        double ahead = before;
-        for (int k = 0; k < wave; k++) ahead += S.wave[k];
-        if (w > 0.0 && ahead + run > target) atomicMin(&S.found, i);
-        const uint64_t some = __ballot(w > 0.0);
-        if (some) last = i0 + 64 * wave + 63 - __builtin_clzll(some);
-        for (int k = 0; k < VF_W / 64; k++) before += S.wave[k];
-        __syncthreads();
-        if (S.found != INT_MAX) return S.found;
-    }
-    __syncthreads();
-    if (tid == 0) S.found = -1;
-    __syncthreads();
-    if (lane == 0) atomicMax(&S.found, last);
-    __syncthreads();
-    return S.found;
-}
-
-__global__ void __launch_bounds__(VF_W) k_verify_walk(VerifyArgs a) {
-    __shared__ VfShared S;
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, T = a.T;
-    const VfScale s = vf_scale(a, b);
-    const int64_t row0 = (int64_t)b * T;
-    const VerifyPart* parts = reinterpret_cast<const VerifyPart*>(a.ws) + row0 * a.slices;
-    if (tid < T) {
-        const int up = a.parents[(int64_t)b * a.ldp + tid], tok = a.tokens[(int64_t)b * a.ldt + tid];
-        const bool ok = up >= 0 && up < tid, in = ok && tok >= 0 && tok < a.V;
-        S.tok[tid] = in ? tok : -1;
-        S.up[tid] = tid == 0 ? up : ok ? up : -2;
-        S.u[tid] = a.uniform[(int64_t)b * a.ldu + tid];
-        S.x[tid] = in ? a.x[(row0 + up) * a.ldx + tok] : -INFINITY;
-        S.q[tid] = in && a.draft ? a.draft[(row0 + up) * a.ldd + tok] : 0.0f;
-    }
-    // every row's statistics: the slices' brought to the row's largest logit
-    for (int t = wave; t < T; t += VF_W / 64) {
-        const VerifyPart* p = parts + (int64_t)t * a.slices;
-        float m = -INFINITY;
-        for (int i = lane; i < a.slices; i += 64) m = fmaxf(m, p[i].m);
-        for (int w = 32; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
-        double sum = 0.0;
-        int at = INT_MAX;
-        for (int i = lane; i < a.slices; i += 64) {
-            const VerifyPart y = p[i];
-            if (y.m == m) at = min(at, y.at);
-            sum += y.sum * vf_weight(s, y.m, m);
-        }
-        sum = vf_wave_sum(sum);
-        for (int w = 32; w; w >>= 1) at = min(at, __shfl_xor(at, w, 64));
-        if (lane == 0) S.m[t] = m, S.sum[t] = m == -INFINITY ? 0.0 : s.greedy ? 1.0 : sum, S.top_at[t] = at;
-    }
-    __syncthreads();
-    int* path = a.path + row0;
-    const int seg_len = ((a.V + VF_W - 1) / VF_W + 255) / 256 * 256;
-    int cur = 0, n = 0;
-    VfLeft f = {};
-    double left = 0.0;
-    if (S.up[0] == -1) {
-        if (tid == 0) path[0] = 0;
-        for (;;) {
-            f = VfLeft{a.x + (row0 + cur) * a.ldx, nullptr, S.m[cur], S.top_at[cur], 0.0, 0.0, 0};
-            left = S.sum[cur];
-            int next = -1;
-            if (left > 0.0) {
-                f.per = 1.0 / left;
-                if (a.draft) left = 1.0;
-                uint64_t children = __ballot(lane < T && lane > 0 && S.up[lane < T ? lane : 0] == cur);
-                for (; children; children &= children - 1) {
-                    const int c = __builtin_ctzll(children), tok = S.tok[c];
-                    if (tok < 0) continue;                     // no token: refused, and nothing leaves
-                    const double e = s.greedy ? (tok == f.first ? 1.0 : 0.0) : vf_weight(s, S.x[c], f.m);
-                    if (a.draft) {
-                        const double q = (double)S.q[c];
-                        if ((double)S.u[c] * left * q < fmax(e * f.per - f.a * q, 0.0)) next = c;
-                        if (next >= 0) break;
-                        f.a += left;
-                        f.q = a.draft + (row0 + cur) * a.ldd;
-                        left = vf_segments(S, s, f, a.V, seg_len);
-                    } else {
-                        bool again = false;                    // refused already: it holds nothing any more
-                        for (int k = 0; k < f.gone; k++) again |= S.refused[k] == tok;
-                        const double w = again ? 0.0 : e;
-                        if ((double)S.u[c] * left < w) next = c;
-                        if (next >= 0) break;
-                        left -= w;
-                        __syncthreads();
-                        if (tid == 0) S.refused[f.gone] = tok;
-                        __syncthreads();
-                        f.gone++;
-                    }
+        if (tid == 0) S.found = INT_MAX, S.last = -1;
+#pragma unroll 1
+        for (int i0 = from; i0 < to; i0 += VF_MOST) {
+            const int n = min(to - i0, VF_MOST);
+            if (what != SLICES) {
+                float x[VF_EACH];
+#pragma unroll
+                for (int k = 0; k < VF_EACH; k++) x[k] = f.x[i0 + min(k * VF_W + tid, n - 1)];
+#pragma unroll
+                for (int k = 0; k < VF_EACH; k++) vf_w[k * VF_W + tid] = (double)x[k];
+                if (f.q) {
+#pragma unroll
+                    for (int k = 0; k < VF_EACH; k++) x[k] = f.q[i0 + min(k * VF_W + tid, n - 1)];
+#pragma unroll
+                    for (int k = 0; k < VF_EACH; k++) vf_q[k * VF_W + tid] = x[k];
                 }
             }
-            if (next < 0) break;
+#pragma unroll 1
+            for (int i = tid; i < n; i += VF_W) {
+                const int at = i0 + i, mine = what == SLICES ? a.shift : 0;
+                float x = 0.0f;
+                double times = 1.0;
+                if (what != SLICES) x = (float)vf_w[i];
+                else if (sums) times = sums[at];
+                else x = parts[at].m, times = parts[at].sum;
+                double w = s.greedy ? (at == f.first >> mine ? 1.0 : 0.0) : top.weight(x) * times;
+                if (what == SLICES) {
+                    if (sums) w = times;
+                } else if (f.q) {
+                    w = fmax(w * f.per - f.a * (double)vf_q[i], 0.0);
+                }
+                for (int k = 0; k < f.gone; k++)
+                    if (S.refused[k] >> mine == at) w -= S.gone[k];
+                vf_w[i] = w;
+            }
+            __syncthreads();
+            // VF_EACH neighbours a thread
+            const int mine = tid * VF_EACH, end = min(mine + VF_EACH, n);
+            double sum = 0.0;
+#pragma unroll 1
+            for (int i = mine; i < end; i++) {
+                sum += vf_w[i];
+                if (vf_w[i] > 0.0) last = i0 + i;
+            }
+            double run = sum;
+#pragma unroll 1
+            for (int k = 1; k < 64; k <<= 1) {
+                const double y = __shfl_up(run, k, 64);
+                if (lane >= k) run += y;
+            }
+            if (lane == 63) S.wave[wave] = run;
+            __syncthreads();
+            double ahead = before;
+#pragma unroll
+            for (int k = 0; k < VF_W / 64; k++) {
+                const double x = S.wave[k];
+                ahead += k < wave ? x : 0.0;
+                before += x;
+            }
+            ahead += run - sum;
+            if (last >= i0 + mine && ahead + sum > target) atomicMin(&S.found, tid);
+            __syncthreads();
+            const int who = S.found;
+            if (who != INT_MAX) {
+                __syncthreads();
+                if (tid == who) {
+                    int at = last;
+#pragma unroll 1
+                    for (int i = mine; i0 + i < last; i++) {
+                        if (vf_w[i] > 0.0 && ahead + vf_w[i] > target) {
+                            at = i0 + i;
+                            break;
+                        }
+                        ahead += vf_w[i];
+                    }
+                    S.last = at, S.wave[0] = ahead;
+                }
+                break;
+            }
+        }
+        const bool passed = S.found != INT_MAX;
+        if (!passed && last >= 0) atomicMax(&S.last, last);    // the last with a weight: the sums' own rounding
+        __syncthreads();
+        found = S.last;
+        if (what == SLICES) {
+            if (found < 0) {
+                what = IDS;
+                continue;
+            }
+            from = found << a.shift, to = min(from + a.slice, a.V);
+            before = passed ? S.wave[0] : 0.0;
+            if (!passed) target = INFINITY;
+        } else if (what == IDS) {
+            if (found >= 0) break;
+        } else if (what == TOTAL) {
+            if (found < 0) break;
+            target = (double)S.u[0] * before;
+        }
+    }
+    return found;
+}
+
+// The request's drafts, their logits and probabilities, into LDS.
+__device__ void vf_drafts(VfShared& S, const VerifyArgs& a, int b) {
+    const int tid = threadIdx.x;
+    if (tid >= a.T) return;
+    const int up = vf_up(a, b, tid), tok = a.tokens[(int64_t)b * a.ldt + tid];
+    const bool in = tid && up >= 0 && tok >= 0 && tok < a.V;
+    const int64_t row = (int64_t)b * a.T + max(up, 0);
+    S.tok[tid] = in ? tok : -1;
+    S.up[tid] = up;
+    S.u[tid] = a.uniform[(int64_t)b * a.ldu + tid];
+    S.x[tid] = in ? a.x[row * a.ldx + tok] : -INFINITY;
+    S.q[tid] = in && a.draft ? a.draft[row * a.ldd + tok] : 0.0f;
+}
+
+// A row's statistics from its slices' by one wave: brought to the row's largest logit.
+__device__ void vf_row(VfShared& S, const VerifyArgs& a, const VfScale& s, int b, int t) {
+    const int lane = threadIdx.x & 63;
+    const VerifyPart* p = vf_parts(a, (int64_t)b * a.T + t);
+    float m = -INFINITY;
+    for (int i = lane; i < a.slices; i += 64) m = fmaxf(m, p[i].m);
+    for (int w = 32; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
+    double sum = 0.0;
+    int at = INT_MAX;
+    const VfTop top(s, m);
+#pragma unroll 1
+    for (int i = lane; i < a.slices; i += 64) {
+        const VerifyPart y = p[i];
+        if (y.m == m) at = min(at, y.at);
+        sum += y.sum * top.weight(y.m);
+    }
+    sum = vf_wave_sum(sum);
+    for (int w = 32; w; w >>= 1) at = min(at, __shfl_xor(at, w, 64));
+    if (lane == 0) S.m[t] = m, S.sum[t] = m == -INFINITY ? 0.0 : s.greedy ? 1.0 : sum, S.top_at[t] = at;
+}
+// The same from the row itself, by the whole workgroup (the same sums: slice by slice, in the first kernel's order).
+__device__ void vf_row_anew(VfShared& S, const VerifyArgs& a, const VfScale& s, int b, int t) {
+    const float* x = a.x + ((int64_t)b * a.T + t) * a.ldx;
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < a.V; i += VF_W) m = fmaxf(m, x[i]);
+    for (int w = 32; w; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) S.wave[threadIdx.x >> 6] = (double)m;
+    if (threadIdx.x == 0) S.found = INT_MAX;
+    __syncthreads();
+    for (int k = 0; k < VF_W / 64; k++) m = fmaxf(m, (float)S.wave[k]);
+    int at = INT_MAX;
+    for (int i = threadIdx.x; i < a.V; i += VF_W)
+        if (x[i] == m) at = min(at, i);
+    if (at != INT_MAX) atomicMin(&S.found, at);
+    const double sum = m == -INFINITY ? 0.0 : vf_sum(S, [&](int i) { return vf_weight(s, x[i], m); }, a.V);
+    __syncthreads();
+    if (threadIdx.x == 0) S.m[t] = m, S.sum[t] = m == -INFINITY ? 0.0 : s.greedy ? 1.0 : sum, S.top_at[t] = S.found;
+    __syncthreads();
+}
+
+__device__ __forceinline__ VfLeft vf_at(const VfShared& S, const VerifyArgs& a, int b, int cur) {
+    return VfLeft{a.x + ((int64_t)b * a.T + cur) * a.ldx, nullptr, S.m[cur], S.top_at[cur], 0.0, 1.0 / S.sum[cur], 0};
+}
+__device__ __forceinline__ double vf_child(const VfShared& S, const VfScale& s, const VfLeft& f, int c) {
+    return s.greedy ? (S.tok[c] == f.first ? 1.0 : 0.0) : vf_weight(s, S.x[c], f.m);
+}
+// cur's children with a token, those behind `past`.
+__device__ __forceinline__ uint64_t vf_children(const VfShared& S, int T, int cur, int past) {
+    const int t = threadIdx.x & 63;
+    return __ballot(t < T && t > past && S.up[min(t, T - 1)] == cur && S.tok[min(t, T - 1)] >= 0);
+}
+
+// Walks on while the node's row has been looked at; what it says goes to the outputs, or to the state for the next round.
+__global__ void __launch_bounds__(VF_W) k_verify_walk(VerifyArgs a, int round, int most) {
+    __shared__ VfShared S;
+    const int b = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, T = a.T;
+    VfState* const state = vf_state(a, b);
+    int cur = 0, n = 0;
+    if (round) {
+        if (state->status != VF_WALKING) return;
+        cur = state->cur, n = state->n;
+    }
+    const VfScale s = vf_scale(a, b);
+    vf_drafts(S, a, b);
+    const uint64_t nodes = vf_round(vf_up(a, b, tid & 63), cur, most);
+    if (!round && a.parents[(int64_t)b * a.ldp] != -1) {       // the request sits out
+        if (tid < T) a.path[(int64_t)b * T + tid] = -1;
+        if (tid == 0) a.accepted[b] = a.token[b] = -1, state->status = VF_DONE;
+        return;
+    }
+    for (int t = wave; t < T; t += VF_W / 64)
+        if (nodes >> t & 1u) vf_row(S, a, s, b, t);
+    __syncthreads();
+    int* path = a.path + (int64_t)b * T;
+    if (!round && tid == 0) path[0] = 0;
+    for (;;) {
+        VfLeft f = vf_at(S, a, b, cur);
+        double left = S.sum[cur];
+        int next = -1, refused = -1;
+        if (left > 0.0) {
+            uint64_t children = vf_children(S, T, cur, 0);
+            for (; children; children &= children - 1) {
+                const int c = __builtin_ctzll(children), tok = S.tok[c];
+                const double e = vf_child(S, s, f, c), u = (double)S.u[c];
+                if (a.draft) {
+                    if (u * (double)S.q[c] < e * f.per) next = c;
+                    else refused = c;
+                    break;
+                }
+                bool again = false;                            // refused already: it holds nothing any more
+                for (int k = 0; k < f.gone; k++) again |= S.refused[k] == tok;
+                const double w = again ? 0.0 : e;
+                if (u * left < w) {
+                    next = c;
+                    break;
+                }
+                left -= w;
+                if (!again) {
+                    __syncthreads();
+                    if (tid == 0) S.refused[f.gone] = tok, S.gone[f.gone] = w;
+                    __syncthreads();
+                    f.gone++;
+                }
+            }
+        }
+        if (next >= 0) {
             cur = next;
             n++;
             if (tid == 0) path[n] = next;
-            __syncthreads();
+            if (nodes >> cur & 1u) {
+                __syncthreads();
+                continue;
+            }
+            if (tid == 0) state->cur = cur, state->n = n, state->status = VF_WALKING;
+            return;
         }
-    } else {
-        n = -1;
+        if (refused >= 0) {
+            if (tid == 0) *state = VfState{cur, n, VF_LEFT, refused, f.first, f.m, f.per};
+            return;
+        }
+        int token = -1;
+        if (S.sum[cur] > 0.0) {
+            if (!(left > 0.0)) left = S.sum[cur], f.gone = 0;  // nothing is left: drawn from p itself
+            token = vf_draw(S, a, s, f, left, vf_parts(a, (int64_t)b * T + cur), nullptr, false);
+        }
+        for (int i = n + 1 + tid; i < T; i += VF_W) path[i] = -1;
+        if (tid == 0) a.accepted[b] = n, a.token[b] = token, state->status = VF_DONE;
+        return;
+    }
+}
+
+// Sums over slices of max(p - q, 0) for the requests whose draft was refused.
+template <bool V4, int SLICE>
+__global__ void __launch_bounds__(VF_T) k_verify_left(VerifyArgs a) {
+    extern __shared__ __attribute__((aligned(16))) float vf_lds[];
+    __shared__ double ss[VF_T / 64];
+    const int b = blockIdx.y, tid = threadIdx.x;
+    const VfState state = *vf_state(a, b);
+    if (state.status != VF_LEFT) return;
+    const int64_t row = (int64_t)b * a.T + state.cur;
+    const int v0 = blockIdx.x * SLICE, nv = min(SLICE, a.V - v0);
+    const VfScale s = vf_scale(a, b);
+    vf_stage<V4, SLICE>(a.x + row * a.ldx + v0, nv, vf_lds);
+    vf_stage<V4, SLICE>(a.draft + row * a.ldd + v0, nv, vf_lds + SLICE);
+    double sum = 0.0;
+    __syncthreads();
+    const VfTop top(s, state.m);
+#pragma unroll 2
+    for (int i = tid; i < nv; i += VF_T) {
+        const double e = s.greedy ? (v0 + i == state.first ? 1.0 : 0.0) : top.weight(vf_lds[i]);
+        sum += fmax(e * state.per - (double)vf_lds[SLICE + i], 0.0);
+    }
+    sum = vf_wave_sum(sum);
+    if ((tid & 63) == 0) ss[tid >> 6] = sum;
+    __syncthreads();
+    if (tid == 0) vf_sums(a, b)[blockIdx.x] = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+}
+
+// From a refused draft on: its siblings, and the token.  (A sibling that is taken leads on to nodes whose rows may not have been
+// looked at, and to other sums: this workgroup then does both by itself.)
+__global__ void __launch_bounds__(VF_W) k_verify_rest(VerifyArgs a) {
+    __shared__ VfShared S;
+    const int b = blockIdx.x, tid = threadIdx.x, T = a.T;
+    const VfState state = *vf_state(a, b);
+    if (state.status != VF_LEFT) return;
+    const VfScale s = vf_scale(a, b);
+    vf_drafts(S, a, b);
+    if (tid == 0) S.m[state.cur] = state.m, S.top_at[state.cur] = state.first, S.sum[state.cur] = 1.0 / state.per;
+    __syncthreads();
+    int* path = a.path + (int64_t)b * T;
+    int cur = state.cur, n = state.n, past = state.child;
+    VfLeft f = vf_at(S, a, b, cur);
+    f.per = state.per;
+    f.q = a.draft + ((int64_t)b * T + cur) * a.ldd;
+    f.a = 1.0;
+    const double* sums = vf_sums(a, b);
+    double left = vf_sum(S, [&](int i) { return sums[i]; }, a.slices);
+    bool summed = true;                                        // sums are those of what is left
+    for (;;) {
+        int next = -1;
+        if (S.sum[cur] > 0.0)
+            for (uint64_t children = vf_children(S, T, cur, past); children; children &= children - 1) {
+                const int c = __builtin_ctzll(children);
+                const double q = (double)S.q[c];
+                if ((double)S.u[c] * left * q < fmax(vf_child(S, s, f, c) * f.per - f.a * q, 0.0)) {
+                    next = c;
+                    break;
+                }
+                f.a += left;
+                f.q = a.draft + ((int64_t)b * T + cur) * a.ldd;
+                left = vf_sum(S, [&](int i) { return vf_left(S, s, f, i); }, a.V);
+                summed = false;
+            }
+        if (next < 0) break;
+        cur = next, past = 0;
+        n++;
+        if (tid == 0) path[n] = next;
+        vf_row_anew(S, a, s, b, cur);
+        f = vf_at(S, a, b, cur);
+        left = 1.0;
+        summed = false;
+    }
+    int token = -1;
+    if (S.sum[cur] > 0.0) {
+        if (!(left > 0.0)) {                                   // nothing is left: drawn from p itself
+            f.q = nullptr, f.a = 0.0;
+            summed = false;
+        }
+        token = vf_draw(S, a, s, f, left, nullptr, sums, !summed);
     }
     for (int i = n + 1 + tid; i < T; i += VF_W) path[i] = -1;
-    int token = -1;
-    if (n >= 0 && S.sum[cur] > 0.0) {
-        if (!(left > 0.0)) f.q = nullptr, f.a = 0.0, f.gone = 0;   // nothing is left: drawn from p itself
-        left = vf_segments(S, s, f, a.V, seg_len);
-        const double target = (double)S.u[0] * left;
-        // the first segment at which the running sum exceeds the target
-        const int segs = (a.V + seg_len - 1) / seg_len;
-        double run = 0.0, ahead = 0.0;
-        int at = -1, last = -1;
-        for (int g = 0; g < segs; g++) {
-            const double w = S.seg[g];
-            if (w > 0.0) {
-                last = g;
-                if (at < 0 && run + w > target) at = g, ahead = run;
-            }
-            run += w;
-        }
-        if (at < 0) {
-            at = last;
-            ahead = -1.0;                                      // (rounding: whatever comes last)
-        }
-        if (at >= 0) token = vf_pick(S, s, f, at * seg_len, min((at + 1) * seg_len, a.V), ahead < 0.0 ? 0.0 : ahead, ahead < 0.0 ? INFINITY : target);
-    }
-    if (tid == 0) {
-        a.accepted[b] = n;
-        a.token[b] = token;
-    }
+    if (tid == 0) a.accepted[b] = n, a.token[b] = token;
 }
 
-static int vf_slice(int B, int T, int V) {
-    (void)B, (void)T;
-    return V <= VF_LEAST ? VF_LEAST : VF_MOST;
-}
+static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// The states, the slices' statistics of every row and a row of sums for each request, for the smallest slices.
 size_t verify_workspace(int B, int T, int V) {
-    const int slice = vf_slice(B, T, V);
-    return ((size_t)B * T * ((V + slice - 1) / slice) * sizeof(VerifyPart) + 255) & ~(size_t)255;
+    const size_t slices = ((size_t)V + VF_LEAST - 1) / VF_LEAST;
+    return up256(B * sizeof(VfState)) + up256((size_t)B * T * slices * sizeof(VerifyPart)) + up256(B * slices * sizeof(double));
 }
 
 void launch_verify(const VerifyArgs& args, hipStream_t s) {
     VerifyArgs a = args;
-    a.slice = vf_slice(a.B, a.T, a.V);
+    // Rows of a round: all of them up to 160 MB, which one round reads in the time of the others' launches and waits (32 chains of 8
+    // over 151936 ids: 155 MB); else 64 MB for all requests, and in the last round whatever is left.
+    const int64_t row_bytes = (int64_t)a.B * a.V * 4, fit = (64 << 20) / row_bytes;
+    const bool once = row_bytes * a.T <= (160 << 20);
+    const int most = once || fit >= a.T ? a.T : fit < 1 ? 1 : (int)fit, rounds = most < a.T ? VF_ROUNDS : 1;
+    // the largest slice that leaves two workgroups a CU in the first round
+    a.slice = VF_MOST;
+    while (a.slice > VF_LEAST && (int64_t)a.B * most * ((a.V + a.slice - 1) / a.slice) < 2 * device_cus()) a.slice /= 2;
+    a.shift = __builtin_ctz((unsigned)a.slice);
     a.slices = (a.V + a.slice - 1) / a.slice;
-    auto go = [&](auto kernel, dim3 grid, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, a); };
-    const bool v4 = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx % 4 == 0;
-    go(v4 ? k_verify_stats<true> : k_verify_stats<false>, dim3(a.slices, a.B * a.T), VF_T);
-    go(k_verify_walk, dim3(a.B), VF_W);
+    a.parts_at = up256(a.B * sizeof(VfState));
+    a.sums_at = a.parts_at + up256((size_t)a.B * a.T * a.slices * sizeof(VerifyPart));
+    auto al = [](const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0; };
+    const bool v4 = al(a.x, a.ldx) && (!a.draft || al(a.draft, a.ldd));
+    const size_t lds = a.slice * sizeof(float), all = VF_MOST * sizeof(double);
+    for (int round = 0; round < rounds; round++) {
+        const int rows = round + 1 < rounds ? most : a.T;
+        const dim3 grid(a.slices, a.B, rows < 4 ? rows : 4);
+        auto stats = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(VF_T), lds, s, a, round, rows); };
+        if (a.slice == 8192) v4 ? stats(k_verify_stats<true, 8192>) : stats(k_verify_stats<false, 8192>);
+        else if (a.slice == 4096) v4 ? stats(k_verify_stats<true, 4096>) : stats(k_verify_stats<false, 4096>);
+        else v4 ? stats(k_verify_stats<true, 2048>) : stats(k_verify_stats<false, 2048>);
+        hipLaunchKernelGGL(k_verify_walk, dim3(a.B), dim3(VF_W), all, s, a, round, rows);
+    }
+    if (!a.draft) return;
+    auto sums = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.slices, a.B), dim3(VF_T), 2 * lds, s, a); };
+    if (a.slice == 8192) v4 ? sums(k_verify_left<true, 8192>) : sums(k_verify_left<false, 8192>);
+    else if (a.slice == 4096) v4 ? sums(k_verify_left<true, 4096>) : sums(k_verify_left<false, 4096>);
+    else v4 ? sums(k_verify_left<true, 2048>) : sums(k_verify_left<false, 2048>);
+    hipLaunchKernelGGL(k_verify_rest, dim3(a.B), dim3(VF_W), all + VF_MOST * sizeof(float), s, a);
 }
 
 }  // namespace kq

@@ -88,6 +88,20 @@ def test_large(dev):
     check(dev, x, tokens, parents, u)
 
 
+@pytest.mark.parametrize("B,T,V,draft", [(40, 24, 60001, False), (17, 64, 50000, False), (170, 5, 100000, False),
+                                         (20, 16, 140000, True)])
+def test_more_rows_than_are_read_at_once(dev, B, T, V, draft):
+    """Walks that go on where the rows read so far end, in chains, trees and stars; accepted to the last node by random numbers of 0."""
+    for seed in range(2):
+        parents = chain(B, T).numpy() if draft else random_parents(B, T, seed).numpy()
+        parents[B // 2:] = np.maximum(np.arange(T) - 1, 0) - (np.arange(T) == 0)
+        parents[0, 1:] = 0
+        x, tokens, parents, u, q = inputs(B, T, V, seed=seed, draft=draft, parents=parents)
+        u[1::3, 1:] = 0
+        got = check(dev, x, tokens, parents, u, draft=q)
+        assert max(got[0]) == T - 1
+
+
 @pytest.mark.parametrize("draft", [False, True])
 def test_temperatures(dev, draft):
     """Cold, hot, greedy (0, below, NaN); infinitely hot: every finite logit alike."""

@@ -16,8 +16,8 @@
 namespace kq {
 
 constexpr int VF_T = 256;                    // threads of the kernels that read rows
-constexpr int VF_MOST = 8192;                // ids of their largest slice (half, and a quarter, are the others)
-constexpr int VF_LEAST = 2048;               // and of the smallest
+constexpr int VF_MOST = 4096;                // ids of their slices
+constexpr int VF_LEAST = 2048;               // or half of that
 constexpr int VF_W = 1024;                   // threads of the walk
 constexpr int VF_EACH = VF_MOST / VF_W;      // ids of one of them in a slice
 constexpr int VF_ROUNDS = 4;
@@ -140,6 +140,7 @@ __device__ __forceinline__ float vf_stage(const float* x, int nv, float* to) {
             to[i] = v;
             m = fmaxf(m, v);
         }
+        if ((int)threadIdx.x < (-nv & 3)) to[nv + threadIdx.x] = -INFINITY;    // whole quads
     }
     return m;
 }
@@ -182,8 +183,14 @@ __global__ void __launch_bounds__(VF_T) k_verify_stats(VerifyArgs a, int round, 
                 for (int i = tid; i < nv && at == INT_MAX; i += VF_T)
                     if (vf_lds[i] == m) at = i;
             } else {
-#pragma unroll 2
-                for (int i = tid; i < nv; i += VF_T) sum += top.weight(vf_lds[i]);
+                double more = 0.0;                             // (two chains: a 64-bit instruction's result comes late)
+#pragma unroll 1
+                for (int i = 4 * tid; i < nv; i += 4 * VF_T) {
+                    const f32x4 v = *reinterpret_cast<const f32x4*>(vf_lds + i);
+                    sum += top.weight(v.x) + top.weight(v.y);
+                    more += top.weight(v.z) + top.weight(v.w);
+                }
+                sum += more;
             }
         }
         sum = vf_wave_sum(sum);
@@ -526,10 +533,16 @@ __global__ void __launch_bounds__(VF_T) k_verify_left(VerifyArgs a) {
     double sum = 0.0;
     __syncthreads();
     const VfTop top(s, state.m);
-#pragma unroll 2
-    for (int i = tid; i < nv; i += VF_T) {
-        const double e = s.greedy ? (v0 + i == state.first ? 1.0 : 0.0) : top.weight(vf_lds[i]);
-        sum += fmax(e * state.per - (double)vf_lds[SLICE + i], 0.0);
+#pragma unroll 1
+    for (int i = 4 * tid; i < nv; i += 4 * VF_T) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(vf_lds + i), q = *reinterpret_cast<const f32x4*>(vf_lds + SLICE + i);
+        double left[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const double e = s.greedy ? (v0 + i + k == state.first ? 1.0 : 0.0) : top.weight(x[k]);
+            left[k] = i + k < nv ? fmax(e * state.per - (double)q[k], 0.0) : 0.0;
+        }
+        sum += (left[0] + left[1]) + (left[2] + left[3]);
     }
     sum = vf_wave_sum(sum);
     if ((tid & 63) == 0) ss[tid >> 6] = sum;
@@ -622,15 +635,13 @@ void launch_verify(const VerifyArgs& args, hipStream_t s) {
         const int rows = round + 1 < rounds ? most : a.T;
         const dim3 grid(a.slices, a.B, rows < 4 ? rows : 4);
         auto stats = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(VF_T), lds, s, a, round, rows); };
-        if (a.slice == 8192) v4 ? stats(k_verify_stats<true, 8192>) : stats(k_verify_stats<false, 8192>);
-        else if (a.slice == 4096) v4 ? stats(k_verify_stats<true, 4096>) : stats(k_verify_stats<false, 4096>);
+        if (a.slice == 4096) v4 ? stats(k_verify_stats<true, 4096>) : stats(k_verify_stats<false, 4096>);
         else v4 ? stats(k_verify_stats<true, 2048>) : stats(k_verify_stats<false, 2048>);
         hipLaunchKernelGGL(k_verify_walk, dim3(a.B), dim3(VF_W), all, s, a, round, rows);
     }
     if (!a.draft) return;
     auto sums = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.slices, a.B), dim3(VF_T), 2 * lds, s, a); };
-    if (a.slice == 8192) v4 ? sums(k_verify_left<true, 8192>) : sums(k_verify_left<false, 8192>);
-    else if (a.slice == 4096) v4 ? sums(k_verify_left<true, 4096>) : sums(k_verify_left<false, 4096>);
+    if (a.slice == 4096) v4 ? sums(k_verify_left<true, 4096>) : sums(k_verify_left<false, 4096>);
     else v4 ? sums(k_verify_left<true, 2048>) : sums(k_verify_left<false, 2048>);
     hipLaunchKernelGGL(k_verify_rest, dim3(a.B), dim3(VF_W), all + VF_MOST * sizeof(float), s, a);
 }

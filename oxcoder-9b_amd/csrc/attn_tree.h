@@ -239,204 +239,202 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 && NT == 
     // Once, and once more where an infinity or NaN in the cache left a sum that is not finite: a value reached rows that do not see
     // it as 0 * inf.  Then such values count as 0, and are given to the rows that see them at the end.
     for (;;) {
-    look(from + A::P);
-    put(0);
-    __syncthreads();
+        look(from + A::P);
+        put(0);
+        __syncthreads();
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        under[n] = 0.0f, l[n] = 0.0f, any[n] = 0;
+        for (int n = 0; n < NT; n++) {
+            under[n] = 0.0f, l[n] = 0.0f, any[n] = 0;
 #pragma unroll
-        for (int d = 0; d < ND; d++) o[n][d] = f32x4{0, 0, 0, 0};
-    }
-    int buf = 0;
-    for (int first = from; first < to; first += A::P) {
-        const bool on = first + A::P < to;
-        if (on) {
-            fetch(first + A::P);
-            look(first + 2 * A::P);
+            for (int d = 0; d < ND; d++) o[n][d] = f32x4{0, 0, 0, 0};
         }
-        if (!idle) {
-            const uint8_t* kt = tiles + buf * A::TILE;
-            const uint8_t* vt = kt + A::VALUES;
-            f32x4 acc[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const float x = A::I8 ? 0.0f : under[n];
-                acc[n][0] = acc[n][1] = f32x4{x, x, x, x};
+        int buf = 0;
+        for (int first = from; first < to; first += A::P) {
+            const bool on = first + A::P < to;
+            if (on) {
+                fetch(first + A::P);
+                look(first + 2 * A::P);
             }
-            // A step of d (of f16, of the second parts, then of the first) for both 16 positions, the next one's on its way while it is
-            // multiplied; the two in turn, so that no product waits for the one just before it.
-            constexpr int KN = A::QS * A::PLANES;
-            u32x4 k[2][2];
-            auto key = [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-                for (int t = 0; t < 2; t++)
-                    k[i & 1][t] = *reinterpret_cast<const u32x4*>(kt + (16 * t + r) * A::KROW + 64 * (i / A::PLANES) + 16 * g +
-                                                                  (A::PLANES - 1 - i % A::PLANES) * A::KPLANE);
-            };
-            key(0);
-#pragma unroll
-            for (int i = 0; i < KN; i++) {
-                if (i + 1 < KN) key(i + 1);
-                const bool first_part = i % A::PLANES == A::PLANES - 1;
-#pragma unroll
-                for (int j = first_part ? 2 : 1; j >= 0; j--)
-#pragma unroll
-                    for (int n = 0; n < 2 * NT; n++)
-                        acc[n >> 1][n & 1] = mma_bf16(k[i & 1][n & 1], qp[n >> 1][i / A::PLANES][j], acc[n >> 1][n & 1]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if constexpr (A::I8) {
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const f32x4 x = *reinterpret_cast<const f32x4*>(&scales[buf][0][16 * t + 4 * g]);
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) acc[n][t][i] = __builtin_fmaf(acc[n][t][i], x[i], under[n]);
-                }
-            }
-            uint32_t ok = 0;                                   // the step's positions that are there
-#pragma unroll
-            for (int i = 0; i < 4; i++) ok |= there[buf][i] << A::MINE * i;
-            ok = __builtin_amdgcn_readfirstlane(ok);
-            const bool partly = ok != ~0u || first + 32 > base;
-            uint32_t shown[NT];                                // bit i: the row sees position first + i
-            if (partly) {
+            if (!idle) {
+                const uint8_t* kt = tiles + buf * A::TILE;
+                const uint8_t* vt = kt + A::VALUES;
+                f32x4 acc[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    const int at = first - base;                 // the first's place in the tree
-                    const uint64_t nodes = nodes_of(n);
-                    const uint64_t see = at >= 64 ? 0 : at >= 0 ? nodes >> at : at > -32 ? nodes << -at | ((1u << -at) - 1u) : ~0ull;
-                    shown[n] = ok & (uint32_t)see;
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (!(shown[n] >> (16 * (i >> 2) + 4 * g + (i & 3)) & 1u)) acc[n][i >> 2][i & 3] = -INFINITY;
+                    const float x = A::I8 ? 0.0f : under[n];
+                    acc[n][0] = acc[n][1] = f32x4{x, x, x, x};
                 }
-            }
+                // A step of d (of f16, of the second parts, then of the first) for both 16 positions, the next one's on its way while it is
+                // multiplied; the two in turn, so that no product waits for the one just before it.
+                constexpr int KN = A::QS * A::PLANES;
+                u32x4 k[2][2];
+                auto key = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 8; i++) top = fmaxf(top, acc[n][i >> 2][i & 3]);
-                if (__ballot(top > MOST) | (__ballot(top > -INFINITY) & ~any[n])) {
-                    top = xor32_max(xor16_max(top));
-                    // (by the tile's largest itself: what rounding `under` moves, far from 0, must not leave e above 1)
-                    const bool had = any[n] >> lane & 1u, up = top > (had ? MOST : -INFINITY);
-                    const float by = up ? top : 0.0f, keep = had ? __builtin_amdgcn_exp2f(-by) : 1.0f;
-                    under[n] -= by;
-                    any[n] |= __ballot(up);
-                    l[n] *= keep;
-#pragma unroll
-                    for (int d = 0; d < ND; d++) o[n][d] *= keep;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) acc[n][i >> 2][i & 3] -= by;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float x = __builtin_amdgcn_exp2f(acc[n][i >> 2][i & 3]);
-                    acc[n][i >> 2][i & 3] = x;
-                    l[n] += x;
-                }
-            }
-            {
-                u32x4 ep[NT][3];
-                if constexpr (A::I8) {
-                    f32x4 x[2];
-#pragma unroll
-                    for (int t = 0; t < 2; t++) x[t] = *reinterpret_cast<const f32x4*>(&scales[buf][1][16 * t + 4 * g]);
-                    auto scaled = [&](auto careful) __attribute__((always_inline)) {
-#pragma unroll
-                        for (int i = 0; i < 8 * NT; i++) {
-                            const float e = acc[i >> 3][i >> 2 & 1][i & 3], y = e * x[i >> 2 & 1][i & 3];
-                            acc[i >> 3][i >> 2 & 1][i & 3] = decltype(careful)::value && e == 0.0f ? e : y;
-                        }
-                    };
-                    if (partly) scaled(std::true_type());      // a position that a row does not see takes no part, whatever its scale
-                    else scaled(std::false_type());
-                }
-#pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float e0 = acc[n][j >> 1][2 * (j & 1)], e1 = acc[n][j >> 1][2 * (j & 1) + 1];
-                        uint32_t q0, q1, q2;
-                        cut.split3(e0, e1, q0, q1, q2);
-                        ep[n][0][j] = q0, ep[n][1][j] = q1, ep[n][2][j] = q2;
-                    }
-                // four positions' values at a time, transposed: lane r's d, positions 4 g + 0..3 of each 16
-                const uint8_t* at = vt + (4 * g + (r >> 2)) * A::VROW + 8 * (r & 3);
-                constexpr int VN = ND / 2 * A::PLANES;
-                u32x4 v[2][2];
-                auto value = [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-                    for (int w = 0; w < 2; w++) {
-                        const uint8_t* from = at + 64 * (i / A::PLANES) + 32 * w + (A::PLANES - 1 - i % A::PLANES) * A::VPLANE;
-                        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)from));
-                        const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(from + 16 * A::VROW)));
-                        v[i & 1][w] = u32x4{x.x, x.y, y.x, y.y};
-                    }
+                    for (int t = 0; t < 2; t++)
+                        k[i & 1][t] = *reinterpret_cast<const u32x4*>(kt + (16 * t + r) * A::KROW + 64 * (i / A::PLANES) + 16 * g +
+                                                                      (A::PLANES - 1 - i % A::PLANES) * A::KPLANE);
                 };
-                value(0);
+                key(0);
 #pragma unroll
-                for (int i = 0; i < VN; i++) {
-                    if (i + 1 < VN) value(i + 1);
+                for (int i = 0; i < KN; i++) {
+                    if (i + 1 < KN) key(i + 1);
                     const bool first_part = i % A::PLANES == A::PLANES - 1;
 #pragma unroll
                     for (int j = first_part ? 2 : 1; j >= 0; j--)
 #pragma unroll
-                        for (int n = 0; n < 2 * NT; n++) {
-                            f32x4& to = o[n >> 1][2 * (i / A::PLANES) + (n & 1)];
-                            to = mma_bf16(v[i & 1][n & 1], ep[n >> 1][j], to);
-                        }
+                        for (int n = 0; n < 2 * NT; n++)
+                            acc[n >> 1][n & 1] = mma_bf16(k[i & 1][n & 1], qp[n >> 1][i / A::PLANES][j], acc[n >> 1][n & 1]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                if constexpr (A::I8) {
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        const f32x4 x = *reinterpret_cast<const f32x4*>(&scales[buf][0][16 * t + 4 * g]);
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) acc[n][t][i] = __builtin_fmaf(acc[n][t][i], x[i], under[n]);
+                    }
+                }
+                uint32_t ok = 0;                                   // the step's positions that are there
+#pragma unroll
+                for (int i = 0; i < 4; i++) ok |= there[buf][i] << A::MINE * i;
+                ok = __builtin_amdgcn_readfirstlane(ok);
+                const bool partly = ok != ~0u || first + 32 > base;
+                uint32_t shown[NT];                                // bit i: the row sees position first + i
+                if (partly) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const int at = first - base;                 // the first's place in the tree
+                        const uint64_t nodes = nodes_of(n);
+                        const uint64_t see = at >= 64 ? 0 : at >= 0 ? nodes >> at : at > -32 ? nodes << -at | ((1u << -at) - 1u) : ~0ull;
+                        shown[n] = ok & (uint32_t)see;
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if (!(shown[n] >> (16 * (i >> 2) + 4 * g + (i & 3)) & 1u)) acc[n][i >> 2][i & 3] = -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) top = fmaxf(top, acc[n][i >> 2][i & 3]);
+                    if (__ballot(top > MOST) | (__ballot(top > -INFINITY) & ~any[n])) {
+                        top = xor32_max(xor16_max(top));
+                        // (by the tile's largest itself: what rounding `under` moves, far from 0, must not leave e above 1)
+                        const bool had = any[n] >> lane & 1u, up = top > (had ? MOST : -INFINITY);
+                        const float by = up ? top : 0.0f, keep = had ? __builtin_amdgcn_exp2f(-by) : 1.0f;
+                        under[n] -= by;
+                        any[n] |= __ballot(up);
+                        l[n] *= keep;
+#pragma unroll
+                        for (int d = 0; d < ND; d++) o[n][d] *= keep;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) acc[n][i >> 2][i & 3] -= by;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float x = __builtin_amdgcn_exp2f(acc[n][i >> 2][i & 3]);
+                        acc[n][i >> 2][i & 3] = x;
+                        l[n] += x;
+                    }
+                }
+                {
+                    u32x4 ep[NT][3];
+                    if constexpr (A::I8) {
+                        f32x4 x[2];
+#pragma unroll
+                        for (int t = 0; t < 2; t++) x[t] = *reinterpret_cast<const f32x4*>(&scales[buf][1][16 * t + 4 * g]);
+                        auto scaled = [&](auto careful) __attribute__((always_inline)) {
+#pragma unroll
+                            for (int i = 0; i < 8 * NT; i++) {
+                                const float e = acc[i >> 3][i >> 2 & 1][i & 3], y = e * x[i >> 2 & 1][i & 3];
+                                acc[i >> 3][i >> 2 & 1][i & 3] = decltype(careful)::value && e == 0.0f ? e : y;
+                            }
+                        };
+                        if (partly) scaled(std::true_type());      // a position that a row does not see takes no part, whatever its scale
+                        else scaled(std::false_type());
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const float e0 = acc[n][j >> 1][2 * (j & 1)], e1 = acc[n][j >> 1][2 * (j & 1) + 1];
+                            uint32_t q0, q1, q2;
+                            cut.split3(e0, e1, q0, q1, q2);
+                            ep[n][0][j] = q0, ep[n][1][j] = q1, ep[n][2][j] = q2;
+                        }
+                    // four positions' values at a time, transposed: lane r's d, positions 4 g + 0..3 of each 16
+                    const uint8_t* at = vt + (4 * g + (r >> 2)) * A::VROW + 8 * (r & 3);
+                    constexpr int VN = ND / 2 * A::PLANES;
+                    u32x4 v[2][2];
+                    auto value = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int w = 0; w < 2; w++) {
+                            const uint8_t* from = at + 64 * (i / A::PLANES) + 32 * w + (A::PLANES - 1 - i % A::PLANES) * A::VPLANE;
+                            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)from));
+                            const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(from + 16 * A::VROW)));
+                            v[i & 1][w] = u32x4{x.x, x.y, y.x, y.y};
+                        }
+                    };
+                    value(0);
+#pragma unroll
+                    for (int i = 0; i < VN; i++) {
+                        if (i + 1 < VN) value(i + 1);
+                        const bool first_part = i % A::PLANES == A::PLANES - 1;
+#pragma unroll
+                        for (int j = first_part ? 2 : 1; j >= 0; j--)
+#pragma unroll
+                            for (int n = 0; n < 2 * NT; n++) {
+                                f32x4& to = o[n >> 1][2 * (i / A::PLANES) + (n & 1)];
+                                to = mma_bf16(v[i & 1][n & 1], ep[n >> 1][j], to);
+                            }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
             }
+            if (A::NBUF == 1) __syncthreads();                     // the tile has been read
+            if (on) put(A::NBUF == 2 ? buf ^ 1 : 0);
+            __syncthreads();
+            if (A::NBUF == 2) buf ^= 1;
         }
-        if (A::NBUF == 1) __syncthreads();                     // the tile has been read
-        if (on) put(A::NBUF == 2 ? buf ^ 1 : 0);
-        __syncthreads();
-        if (A::NBUF == 2) buf ^= 1;
-    }
 
-    if (A::I8 || wild) break;
-    // 0 * x is 0 for every finite x
-    f32x4 zero = {0, 0, 0, 0};
+        if (A::I8 || wild) break;
+        // 0 * x is 0 for every finite x
+        f32x4 zero = {0, 0, 0, 0};
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+        for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-            if (16 * d < D) zero += o[n][d] * 0.0f;
-    if (!__syncthreads_or(!idle && !(zero.x + zero.y + (zero.z + zero.w) == 0.0f))) break;
-    wild = true;
-    look(from);
-    fetch(from);
+            for (int d = 0; d < ND; d++)
+                if (16 * d < D) zero += o[n][d] * 0.0f;
+        if (!__syncthreads_or(!idle && !(zero.x + zero.y + (zero.z + zero.w) == 0.0f))) break;
+        wild = true;
+        look(from);
+        fetch(from);
     }
     const int me = here(), row_of_me = me & 15, d_of_me = 4 * (me >> 4);
     if (!A::I8 && wild && !idle) {
         uint64_t nodes[NT];
 #pragma unroll
         for (int n = 0; n < NT; n++) nodes[n] = nodes_of(n);
-        {
-            for (int p = from; p < to; p++) {
-                const int page = __builtin_amdgcn_readfirstlane(table[p >> a.page_shift]);
-                if ((unsigned)page >= (unsigned)a.kv.pages) continue;
-                const uint8_t* at = kb + to_v + (uint64_t)page * page_bytes + (uint64_t)(p & (a.kv.page_size - 1)) * pos_bytes + 2 * d_of_me;
-                const int node = p - base;
+        for (int p = from; p < to; p++) {
+            const int page = __builtin_amdgcn_readfirstlane(table[p >> a.page_shift]);
+            if ((unsigned)page >= (unsigned)a.kv.pages) continue;
+            const uint8_t* at = kb + to_v + (uint64_t)page * page_bytes + (uint64_t)(p & (a.kv.page_size - 1)) * pos_bytes + 2 * d_of_me;
+            const int node = p - base;
 #pragma unroll
-                for (int d = 0; d < ND; d++)
-                    if (16 * d < D) {
-                        const u32x2 raw = *reinterpret_cast<const u32x2*>(at + 32 * d);
+            for (int d = 0; d < ND; d++)
+                if (16 * d < D) {
+                    const u32x2 raw = *reinterpret_cast<const u32x2*>(at + 32 * d);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t half = i & 1 ? raw[i >> 1] >> 16 : raw[i >> 1] & 0xffffu;
-                            const float v = A::F16 ? f16_lo(half) : fbits(half << 16);
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t half = i & 1 ? raw[i >> 1] >> 16 : raw[i >> 1] & 0xffffu;
+                        const float v = A::F16 ? f16_lo(half) : fbits(half << 16);
 #pragma unroll
-                            for (int n = 0; n < NT; n++)
-                                if (!(fabsf(v) < INFINITY) && (node < 0 || nodes[n] >> node & 1u)) o[n][d][i] += v;
-                        }
+                        for (int n = 0; n < NT; n++)
+                            if (!(fabsf(v) < INFINITY) && (node < 0 || nodes[n] >> node & 1u)) o[n][d][i] += v;
                     }
-            }
+                }
         }
     }
 #pragma unroll

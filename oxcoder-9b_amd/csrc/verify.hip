@@ -25,21 +25,22 @@ constexpr int VF_ROUNDS = 4;
 // Weights are held in 64 bits as well: a vocabulary's running sum has a border for every id, and fp32 weights, off by 2^-24
 // each, would put one draw in some hundred on the border's other side.
 struct VfScale {
-    double c;                  // log2(e) / temperature
+    double c, least;           // log2(e) / temperature; a difference of logits whose weight is 0
     bool greedy;               // temperature 0: the first of the largest logits alone
 };
 __device__ __forceinline__ VfScale vf_scale(const VerifyArgs& a, int b) {
     const float t = a.temperature ? a.temperature[b] : 1.0f;
     const bool greedy = !(t > 0.0f);
-    return VfScale{greedy ? 0.0 : 1.4426950408889634 / fmin((double)t, 3e38), greedy};
+    const double x = greedy ? 1.0 : fmin((double)t, 3e38);
+    return VfScale{1.4426950408889634 / x, -1400.0 * x, greedy};
 }
 // x's weight beside the row's largest logit m, 2^(c (x - m)): 0 for -inf and NaN; beside +inf, 1 for that alone.  To within 4e-14 of
 // it: 2^f over the fraction f of the exponent, in -1/2..1/2, is the polynomial of degree 9 that equals it at Chebyshev's points
 // (2e-14 off at most; c x - c m would be off by the rounding of c m, which a low temperature makes large).
 struct VfTop {
     float m;
-    double c, least;                                           // least: a difference whose weight is 0
-    __device__ __forceinline__ VfTop(const VfScale& s, float top) : m(top), c(s.c), least(-2000.0 / s.c) {}
+    double c, least;
+    __device__ __forceinline__ VfTop(const VfScale& s, float top) : m(top), c(s.c), least(s.least) {}
     __device__ __forceinline__ double weight(float x) const {
         if (m == INFINITY) return x == m ? 1.0 : 0.0;
         const double z = fmax((double)x - (double)m, least) * c;
@@ -61,6 +62,7 @@ struct VfTop {
 __device__ __forceinline__ double vf_weight(const VfScale& s, float x, float m) { return VfTop(s, m).weight(x); }
 
 __device__ __forceinline__ double vf_wave_sum(double v) {
+#pragma unroll 1
     for (int w = 32; w; w >>= 1) v += __shfl_xor(v, w, 64);
     return v;
 }
@@ -216,7 +218,7 @@ struct VfLeft {
 struct VfShared {
     int tok[TREE_MOST], up[TREE_MOST], top_at[TREE_MOST], refused[TREE_MOST];
     float m[TREE_MOST], u[TREE_MOST], x[TREE_MOST], q[TREE_MOST];
-    double sum[TREE_MOST], gone[TREE_MOST];  // gone: the refused tokens' weights
+    double sum[TREE_MOST], e[TREE_MOST], gone[TREE_MOST];     // the drafts' weights, the refused tokens'
     double wave[VF_W / 64];
     int found, last;
     uint64_t nodes;
@@ -329,7 +331,9 @@ __device__ int vf_draw(VfShared& S, const VerifyArgs& a, const VfScale& s, const
                 before += x;
             }
             ahead += run - sum;
-            if (last >= i0 + mine && ahead + sum > target) atomicMin(&S.found, tid);
+            // (one lane a wave: a hundred lanes' minimum of one word takes microseconds)
+            const uint64_t past = __ballot(last >= i0 + mine && ahead + sum > target);
+            if (past && lane == 0) atomicMin(&S.found, 64 * wave + __builtin_ctzll(past));
             __syncthreads();
             const int who = S.found;
             if (who != INT_MAX) {
@@ -371,18 +375,23 @@ __device__ int vf_draw(VfShared& S, const VerifyArgs& a, const VfScale& s, const
     return found;
 }
 
-// The request's drafts, their logits and probabilities, into LDS.
-__device__ void vf_drafts(VfShared& S, const VerifyArgs& a, int b) {
-    const int tid = threadIdx.x;
-    if (tid >= a.T) return;
-    const int up = vf_up(a, b, tid), tok = a.tokens[(int64_t)b * a.ldt + tid];
-    const bool in = tid && up >= 0 && tok >= 0 && tok < a.V;
+// The request's drafts, their logits and probabilities: a thread's, and all of them in LDS.
+struct VfDraft {
+    int up, tok;
+    float u, x, q;
+};
+__device__ __forceinline__ VfDraft vf_draft(const VerifyArgs& a, int b) {
+    const int t = min((int)threadIdx.x, a.T - 1);
+    const int up = vf_up(a, b, t), tok = a.tokens[(int64_t)b * a.ldt + t];
+    const bool in = t && up >= 0 && tok >= 0 && tok < a.V;
     const int64_t row = (int64_t)b * a.T + max(up, 0);
-    S.tok[tid] = in ? tok : -1;
-    S.up[tid] = up;
-    S.u[tid] = a.uniform[(int64_t)b * a.ldu + tid];
-    S.x[tid] = in ? a.x[row * a.ldx + tok] : -INFINITY;
-    S.q[tid] = in && a.draft ? a.draft[row * a.ldd + tok] : 0.0f;
+    const int at = in ? tok : 0;
+    const float u = a.uniform[(int64_t)b * a.ldu + t], x = a.x[row * a.ldx + at], q = a.draft ? a.draft[row * a.ldd + at] : 0.0f;
+    return VfDraft{up, in ? tok : -1, u, in ? x : -INFINITY, in ? q : 0.0f};
+}
+__device__ __forceinline__ void vf_put(VfShared& S, const VerifyArgs& a, const VfDraft& d) {
+    const int t = threadIdx.x;
+    if (t < a.T) S.tok[t] = d.tok, S.up[t] = d.up, S.u[t] = d.u, S.x[t] = d.x, S.q[t] = d.q;
 }
 
 // A row's statistics from its slices' by one wave: brought to the row's largest logit.
@@ -449,8 +458,9 @@ __global__ void __launch_bounds__(VF_W) k_verify_walk(VerifyArgs a, int round, i
         cur = state->cur, n = state->n;
     }
     const VfScale s = vf_scale(a, b);
-    vf_drafts(S, a, b);
+    const VfDraft mine = vf_draft(a, b);
     const uint64_t nodes = vf_round(vf_up(a, b, tid & 63), cur, most);
+    vf_put(S, a, mine);
     if (!round && a.parents[(int64_t)b * a.ldp] != -1) {       // the request sits out
         if (tid < T) a.path[(int64_t)b * T + tid] = -1;
         if (tid == 0) a.accepted[b] = a.token[b] = -1, state->status = VF_DONE;
@@ -458,6 +468,12 @@ __global__ void __launch_bounds__(VF_W) k_verify_walk(VerifyArgs a, int round, i
     }
     for (int t = wave; t < T; t += VF_W / 64)
         if (nodes >> t & 1u) vf_row(S, a, s, b, t);
+    __syncthreads();
+    // every child's weight in its parent's row
+    if (tid < T && S.up[tid] >= 0 && nodes >> S.up[tid] & 1u) {
+        const int up = S.up[tid];
+        S.e[tid] = s.greedy ? (S.tok[tid] == S.top_at[up] ? 1.0 : 0.0) : vf_weight(s, S.x[tid], S.m[up]);
+    }
     __syncthreads();
     int* path = a.path + (int64_t)b * T;
     if (!round && tid == 0) path[0] = 0;
@@ -469,7 +485,7 @@ __global__ void __launch_bounds__(VF_W) k_verify_walk(VerifyArgs a, int round, i
             uint64_t children = vf_children(S, T, cur, 0);
             for (; children; children &= children - 1) {
                 const int c = __builtin_ctzll(children), tok = S.tok[c];
-                const double e = vf_child(S, s, f, c), u = (double)S.u[c];
+                const double e = S.e[c], u = (double)S.u[c];
                 if (a.draft) {
                     if (u * (double)S.q[c] < e * f.per) next = c;
                     else refused = c;
@@ -558,7 +574,7 @@ __global__ void __launch_bounds__(VF_W) k_verify_rest(VerifyArgs a) {
     const VfState state = *vf_state(a, b);
     if (state.status != VF_LEFT) return;
     const VfScale s = vf_scale(a, b);
-    vf_drafts(S, a, b);
+    vf_put(S, a, vf_draft(a, b));
     if (tid == 0) S.m[state.cur] = state.m, S.top_at[state.cur] = state.first, S.sum[state.cur] = 1.0 / state.per;
     __syncthreads();
     int* path = a.path + (int64_t)b * T;

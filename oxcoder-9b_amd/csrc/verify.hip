@@ -34,29 +34,55 @@ __device__ __forceinline__ VfScale vf_scale(const VerifyArgs& a, int b) {
     const double x = greedy ? 1.0 : fmin((double)t, 3e38);
     return VfScale{1.4426950408889634 / x, -1400.0 * x, greedy};
 }
+// 2^f of f in -1/2..1/2 to within 2e-14 of it: the polynomial of degree 9 that equals it at Chebyshev's points, the highest power first.
+constexpr int VF_TERMS = 10;
+__device__ constexpr double VF_POLY[VF_TERMS] = {1.0205905413765595e-07, 1.325964524488711e-06, 1.5252672924850737e-05, 0.0001540343375125101, 0.0013333558200794592,
+                                                 0.009618129193934313, 0.05550410866465167, 0.2402265069564034, 0.6931471805599462, 1.0000000000000135};
+// For a loop of them: in scalar registers (as literals the compiler copies one for each step).
+struct VfPoly {
+    double c[VF_TERMS];
+    __device__ __forceinline__ VfPoly() {
+#pragma unroll
+        for (int k = 0; k < VF_TERMS; k++) {
+            c[k] = VF_POLY[k];
+            asm volatile("" : "+s"(c[k]));
+        }
+    }
+};
 // x's weight beside the row's largest logit m, 2^(c (x - m)): 0 for -inf and NaN; beside +inf, 1 for that alone.  To within 4e-14 of
-// it: 2^f over the fraction f of the exponent, in -1/2..1/2, is the polynomial of degree 9 that equals it at Chebyshev's points
-// (2e-14 off at most; c x - c m would be off by the rounding of c m, which a low temperature makes large).
+// it.  (c x - c m would be off by the rounding of c m, which a low temperature makes large.)
 struct VfTop {
     float m;
     double c, least;
     __device__ __forceinline__ VfTop(const VfScale& s, float top) : m(top), c(s.c), least(s.least) {}
+    // N of them side by side, as a 64-bit instruction's result comes late
+    template <int N>
+    __device__ __forceinline__ void weights(const double (&poly)[VF_TERMS], const float (&x)[N], double (&w)[N]) const {
+        if (m == INFINITY) {
+#pragma unroll
+            for (int i = 0; i < N; i++) w[i] = x[i] == m ? 1.0 : 0.0;
+            return;
+        }
+        double f[N], t[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const double z = fmax((double)x[i] - (double)m, least) * c;
+            t[i] = z + 0x1.8p52;                               // its low half is z to the nearest integer
+            f[i] = z - (t[i] - 0x1.8p52);
+            w[i] = poly[0];
+        }
+#pragma unroll
+        for (int k = 1; k < VF_TERMS; k++)
+#pragma unroll
+            for (int i = 0; i < N; i++) w[i] = fma(w[i], f[i], poly[k]);
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = ldexp(w[i], (int)__builtin_bit_cast(uint64_t, t[i]));
+    }
     __device__ __forceinline__ double weight(float x) const {
-        if (m == INFINITY) return x == m ? 1.0 : 0.0;
-        const double z = fmax((double)x - (double)m, least) * c;
-        const double t = z + 0x1.8p52;                         // its low half is z to the nearest integer
-        const double f = z - (t - 0x1.8p52);
-        double p = 1.0205905413765595e-07;
-        p = fma(p, f, 1.325964524488711e-06);
-        p = fma(p, f, 1.5252672924850737e-05);
-        p = fma(p, f, 0.0001540343375125101);
-        p = fma(p, f, 0.0013333558200794592);
-        p = fma(p, f, 0.009618129193934313);
-        p = fma(p, f, 0.05550410866465167);
-        p = fma(p, f, 0.2402265069564034);
-        p = fma(p, f, 0.6931471805599462);
-        p = fma(p, f, 1.0000000000000135);
-        return ldexp(p, (int)__builtin_bit_cast(uint64_t, t));
+        const float one[1] = {x};
+        double w[1];
+        weights(VF_POLY, one, w);
+        return w[0];
     }
 };
 __device__ __forceinline__ double vf_weight(const VfScale& s, float x, float m) { return VfTop(s, m).weight(x); }
@@ -185,14 +211,15 @@ __global__ void __launch_bounds__(VF_T) k_verify_stats(VerifyArgs a, int round, 
                 for (int i = tid; i < nv && at == INT_MAX; i += VF_T)
                     if (vf_lds[i] == m) at = i;
             } else {
-                double more = 0.0;                             // (two chains: a 64-bit instruction's result comes late)
+                const VfPoly poly;
 #pragma unroll 1
                 for (int i = 4 * tid; i < nv; i += 4 * VF_T) {
                     const f32x4 v = *reinterpret_cast<const f32x4*>(vf_lds + i);
-                    sum += top.weight(v.x) + top.weight(v.y);
-                    more += top.weight(v.z) + top.weight(v.w);
+                    const float x[4] = {v.x, v.y, v.z, v.w};
+                    double w[4];
+                    top.weights(poly.c, x, w);
+                    sum += (w[0] + w[1]) + (w[2] + w[3]);
                 }
-                sum += more;
             }
         }
         sum = vf_wave_sum(sum);
@@ -549,13 +576,16 @@ __global__ void __launch_bounds__(VF_T) k_verify_left(VerifyArgs a) {
     double sum = 0.0;
     __syncthreads();
     const VfTop top(s, state.m);
+    const VfPoly poly;
 #pragma unroll 1
     for (int i = 4 * tid; i < nv; i += 4 * VF_T) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(vf_lds + i), q = *reinterpret_cast<const f32x4*>(vf_lds + SLICE + i);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(vf_lds + i), q = *reinterpret_cast<const f32x4*>(vf_lds + SLICE + i);
+        const float x[4] = {v.x, v.y, v.z, v.w};
         double left[4];
+        top.weights(poly.c, x, left);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const double e = s.greedy ? (v0 + i + k == state.first ? 1.0 : 0.0) : top.weight(x[k]);
+            const double e = s.greedy ? (v0 + i + k == state.first ? 1.0 : 0.0) : left[k];
             left[k] = i + k < nv ? fmax(e * state.per - (double)q[k], 0.0) : 0.0;
         }
         sum += (left[0] + left[1]) + (left[2] + left[3]);

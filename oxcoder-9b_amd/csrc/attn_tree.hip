@@ -7,7 +7,8 @@
 namespace kq {
 
 // ROWS rows a workgroup, 256 / ROWS threads each: lanes of 4 values, in groups that take every so many parts.  The parts'
-// largest scores and sums are looked at by all of a row's threads, and their weights left in LDS.
+// largest scores and sums are looked at by all of a row's threads, and their weights left in LDS.  Bound by the parts' bytes and the
+// chain of loads: 4 us for 256 rows of 20 parts, 12 for 2048 of 32 (34 MB).
 constexpr int TJ_MOST = 2048;                // parts of a row at most
 template <int ROWS>
 __global__ void __launch_bounds__(256) k_attn_tree_join(AttnArgs a, int lanes) {
@@ -61,7 +62,10 @@ __global__ void __launch_bounds__(256) k_attn_tree_join(AttnArgs a, int lanes) {
 struct TreeSplit {
     int tiles, split, parts;   // 16 rows each that a wave takes; positions of a part; parts
 };
-// How a call's rows and positions are shared out.
+// How a call's rows and positions are shared out.  Workgroups enough to fill the card once where each is long (two tiles of rows a wave,
+// two workgroups a CU: 512; 64 nodes over 50001 positions take 148 us, and 159 with 1024, which leave twice the parts to join), and
+// some four times where a wave takes one and requests are ragged (2048: batches of 16 in f16 and 32 in 8 bits 175 and 161 us; 1024:
+// 192 and 164, 4096: 207 and 170).
 static TreeSplit split_of(int seqs, int heads, int group, int dim, int T, int max_len) {
     TreeSplit s;
     const int R = T * group;

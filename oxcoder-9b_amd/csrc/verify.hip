@@ -10,6 +10,11 @@
 // the walk ends, draws the next token: over the slices' sums, then inside one slice.  Rows that no walk comes to need not be
 // read: a batch of large trees takes four rounds, the last of which reads whatever is left below the few walks that still go on.
 // Where a draft's probabilities leave something else than p, two more kernels sum what is left slice by slice and draw.
+//
+// The statistics are bound by 64-bit arithmetic beside the loads (155 MB, 39 million weights: 47 us, 3.3 TB/s; 70 with a polynomial of
+// degree 11, one weight after another), the walks by latency: 4 us where nothing is drawn, 12 with a draw (its two scans), for a
+// whole batch at once.  One request of 5 nodes over 151936 ids: 19 us; 32 chains of 8 with draft probabilities: 87; 16 trees of
+// 64 nodes over 248320 ids: 90, where a copy's rate would take 200 for all 1 GB of their rows.
 #include "kq_device.h"
 #include "kq_internal.h"
 
@@ -663,7 +668,7 @@ size_t verify_workspace(int B, int T, int V) {
 void launch_verify(const VerifyArgs& args, hipStream_t s) {
     VerifyArgs a = args;
     // Rows of a round: all of them up to 160 MB, which one round reads in the time of the others' launches and waits (32 chains of 8
-    // over 151936 ids: 155 MB); else 64 MB for all requests, and in the last round whatever is left.
+    // over 151936 ids, 155 MB: 99 us, and 105 in rounds); else 64 MB for all requests, and in the last round whatever is left.
     const int64_t row_bytes = (int64_t)a.B * a.V * 4, fit = (64 << 20) / row_bytes;
     const bool once = row_bytes * a.T <= (160 << 20);
     const int most = once || fit >= a.T ? a.T : fit < 1 ? 1 : (int)fit, rounds = most < a.T ? VF_ROUNDS : 1;

@@ -600,6 +600,9 @@ int kq_kv_keep(const kq_kv* const* kv, int layers, const int32_t* table, int64_t
         if (kv[i]->heads != kv[0]->heads || kv[i]->dim != kv[0]->dim || kv[i]->pages != kv[0]->pages ||
             kv[i]->page_size != kv[0]->page_size)
             return fail(KQ_ERR_ARG, "%s: the layers' caches must have the same heads, dim, pages and page_size", fn);
+        for (int j = 0; j < i; j++)
+            if ((kv[j]->k == kv[i]->k) != (kv[j]->v == kv[i]->v))
+                return fail(KQ_ERR_ARG, "%s: layers %d and %d share one of k and v", fn, j, i);
     }
     KQ_TRY(check_table(kv[0], table, ldt, seqs, width, fn, &a.table));
     KQ_TRY(check_tree(seqs, T, fn));
@@ -607,18 +610,21 @@ int kq_kv_keep(const kq_kv* const* kv, int layers, const int32_t* table, int64_t
     KQ_TRY(check_rows(path, ldp, seqs, T, "path", fn));
     a.base = base, a.path = path, a.ldp = ldp, a.T = T;
     a.pages = kv[0]->pages, a.page_size = kv[0]->page_size;
-    for (int i0 = 0; i0 < layers; i0 += KEEP_LAYERS) {
-        const int n = layers - i0 < KEEP_LAYERS ? layers - i0 : KEEP_LAYERS;
-        for (int i = 0; i < n; i++) {
-            const kq_kv* c = kv[i0 + i];
-            const bool i8 = c->type == KQ_KV_I8;
-            const int64_t e = i8 ? 1 : 2;
-            a.layer[i] = KeepLayer{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), i8 ? c->k_scale : nullptr,
-                                   i8 ? c->v_scale : nullptr, c->page_stride * e, c->head_stride * e, c->pos_stride * e,
-                                   c->scale_page_stride, c->scale_head_stride, c->scale_pos_stride, (int)(c->dim * e), c->heads};
-        }
+    int n = 0;
+    for (int i = 0; i < layers; i++) {
+        const kq_kv* c = kv[i];
+        bool again = false;                                    // layers that share a cache: its entries move once
+        for (int j = 0; j < i && !again; j++) again = kv[j]->k == c->k;
+        const bool i8 = c->type == KQ_KV_I8;
+        const int64_t e = i8 ? 1 : 2;
+        if (!again)
+            a.layer[n++] = KeepLayer{static_cast<uint8_t*>(c->k), static_cast<uint8_t*>(c->v), i8 ? c->k_scale : nullptr,
+                                     i8 ? c->v_scale : nullptr, c->page_stride * e, c->head_stride * e, c->pos_stride * e,
+                                     c->scale_page_stride, c->scale_head_stride, c->scale_pos_stride, (int)(c->dim * e), c->heads};
+        if ((n < KEEP_LAYERS && i + 1 < layers) || !n) continue;
         launch_kv_keep(a, n, seqs, as_stream(stream));
         KQ_TRY(check_launch(fn));
+        n = 0;
     }
     return KQ_OK;
 }

@@ -150,3 +150,12 @@ def test_refusals_on_the_device(dev):
             att.keep(*a)
     torch.cuda.synchronize()
     assert torch.equal(cache.k, before)
+
+
+@pytest.mark.parametrize("layers", [2, 33, 64])
+def test_layers_that_share_a_cache(dev, layers):
+    """Their entries move once, among a launch's layers and across launches."""
+    base, T = [3, 20], 12
+    table, pages = page_table([n + T for n in base], 16, extra=1)
+    own = [make_cache("bf16", pages, 2, 16, 64, dev, seed=i) for i in range(max(layers - 2, 1))]
+    check(dev, own + [own[0]] * (layers - len(own)), table, base, paths(2, T, 5), 16)

@@ -94,6 +94,7 @@ def test_keep_argument_errors():
     refused(keep(c, None), "kv is NULL")
     for change in (dict(heads=4), dict(dim=48), dict(pages=5), dict(page_size=32)):
         refused(keep(c, cache_struct(**change)), "the same heads")
+    refused(keep(c, cache_struct(), cache_struct(v=P + 4096)), "layers 0 and 2 share one of k and v")
     for change, msg in ((dict(table=None), "table is NULL"), (dict(base=None), "base is NULL"), (dict(path=None), "path is NULL"),
                         (dict(ldp=7), "7 of path"), (dict(T=0), "T=0"), (dict(T=65, ldp=65), "T=65"), (dict(seqs=0), "seqs=0")):
         refused(keep(c, c, **change), msg)

@@ -41,8 +41,10 @@ __device__ __forceinline__ VfScale vf_scale(const VerifyArgs& a, int b) {
 }
 // 2^f of f in -1/2..1/2 to within 2e-14 of it: the polynomial of degree 9 that equals it at Chebyshev's points, the highest power first.
 constexpr int VF_TERMS = 10;
-__device__ constexpr double VF_POLY[VF_TERMS] = {1.0205905413765595e-07, 1.325964524488711e-06, 1.5252672924850737e-05, 0.0001540343375125101, 0.0013333558200794592,
-                                                 0.009618129193934313, 0.05550410866465167, 0.2402265069564034, 0.6931471805599462, 1.0000000000000135};
+__device__ constexpr double VF_POLY[VF_TERMS] = {
+    1.0205905413765595e-07, 1.325964524488711e-06, 1.5252672924850737e-05, 0.0001540343375125101,
+    0.0013333558200794592, 0.009618129193934313, 0.05550410866465167, 0.2402265069564034,
+    0.6931471805599462, 1.0000000000000135};
 // For a loop of them: in scalar registers (as literals the compiler copies one for each step).
 struct VfPoly {
     double c[VF_TERMS];

@@ -102,3 +102,71 @@ def test_quantized_activations(dev):
     out, _ = decoder(dev, 4, "f16", 16, "q8k").generate_tree(ids, 16)
     assert out == decoder(dev, 4, "f16", 16, "q8k").generate_tree(ids, 16)[0]
     assert all(len(row) == 16 and all(0 <= t < 1024 for t in row) for row in out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache", ["f16", "i8"])
+def test_a_captured_step(dev, cache):
+    """Plan, append, attention, verification and the kept entries of two layers as one graph: each replay, with other trees, bases and
+    random numbers in its tensors and eager work between, leaves the bits of the eager calls."""
+    from kq import kv, sampling
+    from tree_helpers import random_parents
+    B, T, H, KV, D, V, W = 3, 24, 4, 2, 64, 5000, 12
+    table = torch.randperm(B * W, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(B, W).to(dev)
+    g = torch.Generator().manual_seed(2)
+    norm = (1 + 0.1 * torch.randn((2, D), generator=g)).to(dev)
+
+    class Side:
+        def __init__(self):
+            self.caches = [kv.KVCache(B * W, 16, KV, D, cache, dev) for _ in range(2)]
+            self.att = kv.PagedAttention(self.caches, table, H, rope=kv.rope_table(W * 16, D, device=dev), q_norm=norm, k_norm=norm,
+                                         nodes=T)
+            self.tree, self.ver = kv.Tree(B, T, dev), sampling.Verifier(B, T, V, dev)
+            self.out = [torch.zeros((B * T, H * D), device=dev) for _ in range(2)]
+            self.turned = torch.zeros((B * T, H * D), device=dev)
+
+        def step(self, x):
+            self.tree.plan(x["parents"], x["base"])
+            for i in range(2):
+                self.att.append(i, x["q"], x["k"], x["v"], self.tree.seq, self.tree.pos, self.turned, slot=self.tree.slot)
+                self.att.attend_tree(i, self.turned, self.tree, self.out[i])
+            accepted, path, token = self.ver.verify(x["logits"], x["tokens"], x["parents"], x["uniform"])
+            self.att.keep(path, x["base"])
+            return accepted, path, token
+
+        def held(self):
+            return [t for c in self.caches for t in (c.k, c.v)] + self.out
+
+    def given(i):
+        g = torch.Generator().manual_seed(10 + i)
+        logits = torch.randn((B * T, V), generator=g)
+        tokens = torch.randint(0, V, (B, T), generator=g, dtype=torch.int32)
+        logits.view(B, T, V).scatter_add_(2, tokens.long()[:, None].expand(B, T, T).contiguous(), torch.full((B, T, T), 9.0))
+        base = torch.tensor([[5, 70, 0], [9, -1, 17], [31, 80, 2], [0, 100, 160]][i], dtype=torch.int32)
+        return dict(logits=logits, tokens=tokens, parents=random_parents(B, T, i), base=base, uniform=torch.rand((B, T), generator=g),
+                    q=torch.randn((B * T, H * D), generator=g), k=torch.randn((B * T, KV * D), generator=g),
+                    v=torch.randn((B * T, KV * D), generator=g))
+
+    eager, replayed = Side(), Side()
+    x = {n: t.to(dev) for n, t in given(0).items()}
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        replayed.step(x)                                       # (every kernel is loaded)
+    s.synchronize()
+    eager.step(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = replayed.step(x)
+    some = 0
+    for i in (1, 2, 3, 1):
+        for n, t in given(i).items():
+            x[n].copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        mine = [t.clone() for t in got]
+        want = eager.step(x)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(mine, want))
+        assert all(torch.equal(a, b) for a, b in zip(replayed.held(), eager.held()))
+        some += int(mine[0].clamp(min=0).sum())
+    assert some > 0

@@ -239,8 +239,11 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 && NT == 
             }
         }
     }
-    // e's exponents count from -under (0 at first), which moves where one passes MOST; any: the lanes whose rows have seen a position
-    constexpr float MOST = 8.0f;
+    // e's exponents count from -under (0 at first), which moves where one passes MOST; any: the lanes whose rows have seen a position.
+    // Scores' sums start at `under`, but not where all that a row has seen lies more than FAR below 0: there the sum would be rounded
+    // at its size, and a later, larger score lose its own bits to it.  Such a row's scores are summed from 0, and `under` comes after.
+    constexpr float MOST = 8.0f, FAR = 16.0f;
+    auto apart = [](float under) __attribute__((always_inline)) { return under > FAR ? under : 0.0f; };
     float under[NT], l[NT];
     uint64_t any[NT];
     f32x4 o[NT][ND];
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 && NT == 
                 f32x4 acc[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    const float x = A::I8 ? 0.0f : under[n];
+                    const float x = A::I8 ? 0.0f : under[n] - apart(under[n]);
                     acc[n][0] = acc[n][1] = f32x4{x, x, x, x};
                 }
                 // A step of d (of f16, of the second parts, then of the first) for both 16 positions, the next one's on its way while it is
@@ -299,9 +302,11 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 && NT == 
                     for (int t = 0; t < 2; t++) {
                         const f32x4 x = *reinterpret_cast<const f32x4*>(&scales[buf][0][16 * t + 4 * g]);
 #pragma unroll
-                        for (int n = 0; n < NT; n++)
+                        for (int n = 0; n < NT; n++) {
+                            const float from = under[n] - apart(under[n]);
 #pragma unroll
-                            for (int i = 0; i < 4; i++) acc[n][t][i] = __builtin_fmaf(acc[n][t][i], x[i], under[n]);
+                            for (int i = 0; i < 4; i++) acc[n][t][i] = __builtin_fmaf(acc[n][t][i], x[i], from);
+                        }
                     }
                 }
                 uint32_t ok = 0;                                   // the step's positions that are there
@@ -327,12 +332,13 @@ __global__ void __launch_bounds__(256, ND * NT <= 4 ? 4 : ND * NT <= 8 && NT == 
                     float top = -INFINITY;
 #pragma unroll
                     for (int i = 0; i < 8; i++) top = fmaxf(top, acc[n][i >> 2][i & 3]);
-                    if (__ballot(top > MOST) | (__ballot(top > -INFINITY) & ~any[n])) {
+                    if (__ballot(top > MOST || under[n] > FAR) | (__ballot(top > -INFINITY) & ~any[n])) {
                         top = xor32_max(xor16_max(top));
                         // (by the tile's largest itself: what rounding `under` moves, far from 0, must not leave e above 1)
-                        const bool had = any[n] >> lane & 1u, up = top > (had ? MOST : -INFINITY);
-                        const float by = up ? top : 0.0f, keep = had ? __builtin_amdgcn_exp2f(-by) : 1.0f;
-                        under[n] -= by;
+                        const float rest = apart(under[n]);
+                        const bool had = any[n] >> lane & 1u, up = top + rest > (had ? MOST : -INFINITY);
+                        const float by = up ? top : -rest, keep = had && up ? __builtin_amdgcn_exp2f(-(top + rest)) : 1.0f;
+                        under[n] = up ? under[n] - rest - by : under[n];
                         any[n] |= __ballot(up);
                         l[n] *= keep;
 #pragma unroll

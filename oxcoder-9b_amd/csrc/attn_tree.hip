@@ -44,7 +44,9 @@ __global__ void __launch_bounds__(256) k_attn_tree_join(AttnArgs a, int lanes) {
         for (int c = group; c < n; c += groups) {
             const f32x4 x = *reinterpret_cast<const f32x4*>(po + (int64_t)c * D);
             const float k = w[c];
-            sum += k != 0.0f ? x * k : f32x4{0, 0, 0, 0};
+            // an infinity or NaN that the row saw counts however small the part's weight
+#pragma unroll
+            for (int i = 0; i < 4; i++) sum[i] += k != 0.0f ? x[i] * k : fabsf(x[i]) < INFINITY ? 0.0f : x[i];
         }
     }
     if (groups > 1) {

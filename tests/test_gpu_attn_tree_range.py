@@ -24,6 +24,35 @@ def test_weights_far_below_the_largest(dev, dtype, gap, D, T):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("gap", [0, 20, 80, 120, 1000])
+@pytest.mark.parametrize("D,T", [(64, 1), (128, 40), (256, 4)])
+def test_infinite_values_of_small_weight(dev, dtype, gap, D, T):
+    """An infinity or NaN that a row sees counts however small its weight, in whichever part of the context it lies; the other
+    columns keep their sums."""
+    lens = [700, 40]
+    print("tree infinite values", dtype, gap, D, T, flush=True)
+    cache, table, q = sinks(dev, dtype, D, gap, lens, T)
+    # one in a tile with a position that takes all the weight, one in a tile without
+    hits = [(330, 10), (100, 20)]
+    for p, d in hits:
+        cache.v[table[0, p // 16], 0, p % 16:p % 16 + 2, d:d + 4] = 0
+    ref, bound = attention(cache, table, q, lens, T, 2, 1.0)
+    # exp(-120) is below fp32's least normal number 2^-126: such a weight may be lost, and with it 2^-126 |v| a position
+    bound += 2.0 ** -126 * 700 * float(cache.v.abs().max())
+    for p, d in hits:
+        page, off = table[0, p // 16], p % 16
+        cache.v[page, 0, off, d:d + 4] = torch.tensor([math.inf, -math.inf, math.nan, math.inf], device=dev).to(cache.v.dtype)
+        cache.v[page, 0, off + 1, d + 3] = -math.inf
+    got = attend(dev, cache, table, q, [n - T for n in lens], chain(2, T), 2, scale=1.0).view(2, T, 2, D)
+    for p, d in hits:
+        hit = got[0, :, :, d:d + 4].cpu()
+        assert (hit[..., 0] == math.inf).all() and (hit[..., 1] == -math.inf).all() and hit[..., 2:].isnan().all()
+        for x in (got, ref.view(2, T, 2, D), bound.view(2, T, 2, D)):
+            x[0, :, :, d:d + 4] = 0
+    check_attention(got.view(2 * T, -1), ref, bound)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("D,T", [(64, 1), (128, 20), (240, 4)])
 def test_infinite_keys_that_are_seen(dev, dtype, D, T):
     """A key of -inf in one channel: no weight where the query is positive there, however small, and a NaN row where it is

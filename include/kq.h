@@ -372,7 +372,7 @@ int kq_kv_append_norm(const kq_kv* kv, const int32_t* table, int64_t ldt, int se
                       int64_t ldqo, const float* k, int64_t ldk, const float* v, int64_t ldv, const float* rope, int rope_rows,
                       int rot, int interleaved, const float* q_norm, const float* k_norm, float eps, void* stream);
 
-/* Bytes of device workspace kq_attn_tree needs (0 for invalid sizes). */
+/* Bytes of device workspace kq_attn_tree needs for up to so many requests, nodes and positions (0 for invalid sizes). */
 size_t kq_attn_tree_workspace(int seqs, int q_heads, int dim, int T, int max_len);
 
 /*

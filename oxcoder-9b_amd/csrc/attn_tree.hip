@@ -68,12 +68,17 @@ struct TreeSplit {
 // two workgroups a CU: 512; 64 nodes over 50001 positions take 148 us, and 159 with 1024, which leave twice the parts to join), and
 // some four times where a wave takes one and requests are ragged (2048: batches of 16 in f16 and 32 in 8 bits 175 and 161 us; 1024:
 // 192 and 164, 4096: 207 and 170).
+static int tiles_of(int R, int dim) { return R <= 64 || dim > 128 ? 1 : 2; }
+static int64_t columns_of(int seqs, int heads, int R, int tiles) {
+    return (int64_t)seqs * heads * ((R + 64 * tiles - 1) / (64 * tiles));
+}
+static int workgroups_of(int tiles) { return tiles == 2 ? 512 : 2048; }
 static TreeSplit split_of(int seqs, int heads, int group, int dim, int T, int max_len) {
     TreeSplit s;
     const int R = T * group;
-    s.tiles = R <= 64 || dim > 128 ? 1 : 2;
-    const int64_t columns = (int64_t)seqs * heads * ((R + 64 * s.tiles - 1) / (64 * s.tiles));
-    const int64_t want = ((s.tiles == 2 ? 512 : 2048) + columns - 1) / columns;
+    s.tiles = tiles_of(R, dim);
+    const int64_t columns = columns_of(seqs, heads, R, s.tiles);
+    const int64_t want = (workgroups_of(s.tiles) + columns - 1) / columns;
     int64_t split = (max_len + want - 1) / want;
     if (split < (max_len + TJ_MOST - 1) / TJ_MOST) split = (max_len + TJ_MOST - 1) / TJ_MOST;
     split = (split + 31) / 32 * 32;
@@ -84,19 +89,29 @@ static TreeSplit split_of(int seqs, int heads, int group, int dim, int T, int ma
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-size_t attn_tree_bytes(int seqs, int heads, int group, int dim, int T, int max_len) {
-    const TreeSplit s = split_of(seqs, heads, group, dim, T, max_len);
-    const size_t parts = (size_t)seqs * T * heads * group * s.parts;
-    return s.parts == 1 ? 256 : up256(parts * dim * 4) + up256(parts * sizeof(AttnMl));
+static size_t bytes_of(size_t rows, int dim, int64_t parts) {
+    return parts == 1 ? 256 : up256(rows * parts * dim * 4) + up256(rows * parts * sizeof(AttnMl));
 }
 
-// What trees of up to T nodes need, whatever the key-value heads.
+size_t attn_tree_bytes(int seqs, int heads, int group, int dim, int T, int max_len) {
+    return bytes_of((size_t)seqs * T * heads * group, dim, split_of(seqs, heads, group, dim, T, max_len).parts);
+}
+
+// The most that any call needs of up to so many requests, nodes and positions, whatever the key-value heads.  Parts come up to
+// the least of what the workgroups ask for and the tiles of max_len, and some shorter max_len meets that; several requests that share the
+// workgroups may need less than fewer do, and past as many as the workgroups each has one part.
 size_t attn_tree_workspace(int seqs, int q_heads, int dim, int T, int max_len) {
     size_t most = 256;
+    const int64_t tiles_long = (max_len + 31) / 32;
     for (int heads = 1; heads <= q_heads; heads++)
         for (int t = 1; t <= T && q_heads % heads == 0; t++) {
-            const size_t n = attn_tree_bytes(seqs, heads, q_heads / heads, dim, t, max_len);
-            most = n > most ? n : most;
+            const int R = t * (q_heads / heads), tiles = tiles_of(R, dim), all = workgroups_of(tiles);
+            for (int b = 1; b <= seqs; b++) {
+                const int64_t columns = columns_of(b, heads, R, tiles), want = (all + columns - 1) / columns;
+                const size_t n = bytes_of((size_t)b * t * q_heads, dim, want < tiles_long ? want : tiles_long);
+                most = n > most ? n : most;
+                if (want == 1) break;
+            }
         }
     return most;
 }

@@ -521,7 +521,8 @@ def tree_plan(parents, base, seen, seq, pos, slot, requests, nodes):
 
 
 def attn_tree_workspace_bytes(seqs, q_heads, dim, nodes, max_len):
-    """Device bytes of workspace attn_tree needs (kq_attn_tree_workspace; 0 for sizes it does not take)."""
+    """Device bytes of workspace attn_tree needs for up to so many requests, nodes and positions (kq_attn_tree_workspace; 0 for
+    sizes it does not take)."""
     return int(_lib.kq().kq_attn_tree_workspace(seqs, q_heads, dim, nodes, max_len))
 
 

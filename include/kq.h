@@ -379,7 +379,9 @@ size_t kq_attn_tree_workspace(int seqs, int q_heads, int dim, int T, int max_len
  * kq_attn_paged for trees of T (1..KQ_MAX_TREE) nodes: row b * T + t of q and out is node t of request b, which sees the
  * positions below base[b] and slot base[b] + j for each bit j of seen[b * T + t] (kq_tree_plan's); its own word 0, or a base
  * below 0: it sees nothing, and its row is 0.  Positions from max_len on, or past the table's, are not there.
- * What lies in positions that a row does not see, infinities and NaN too, has no effect on it.
+ * What lies in positions that a row does not see, infinities and NaN too, has no effect on it.  How a row's positions are shared out goes by
+ * seqs, T, the heads and max_len (not by the requests' lengths), so its fp32 sums are added in another order where those differ; with
+ * those alike its bits do not depend on the other requests.
  */
 int kq_attn_tree(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, int width, const int32_t* base,
                  const uint64_t* seen, int max_len, int T, const float* q, int64_t ldq, int q_heads, float scale, float* out,

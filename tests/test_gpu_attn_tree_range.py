@@ -7,7 +7,7 @@ import torch
 from decode_helpers import U, attention, check_attention, values
 from test_gpu_attn_range import sinks
 from test_gpu_attn_tree import attend, setup
-from tree_helpers import chain
+from tree_helpers import chain, tree_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,22 @@ def test_scores_that_rise_from_far_below(dev, dtype, far, D, T, H):
                 cache.k[(*at, 0)] = -127 if dtype == "i8" else -far * part
     got = attend(dev, cache, table, q, base, chain(4, T), H, scale=1.0 / 8)
     check_attention(got, *own(cache, table, q, base, T, H, 1.0 / 8))
+
+
+@pytest.mark.parametrize("dtype,D,H", [("f16", 128, 8), ("bf16", 64, 4), ("i8", 80, 2), ("bf16", 256, 16)])
+def test_a_row_beside_other_sizes_of_call(dev, dtype, D, H):
+    """How many requests, nodes and positions a call is made for changes the order of a row's sums alone: each time it is
+    the formula's, and with the same sizes the same bits."""
+    T, n, most = 8, 1000, 64
+    cache, table, q = setup(dev, dtype, D, H, 2, 16, [n], most)
+    want, bound = tree_attention(cache, table, q[:T], [n], chain(1, T), H, D ** -0.5)
+    for seqs, nodes, max_len in ((1, T, 1016), (1, T, 60000), (2, T, 1016), (9, T, 5000), (70, T, 1064), (1, most, 1064), (1, most, 60000),
+                                 (5, 40, 2000)):
+        wide = torch.full((seqs, 60000 // 16 + 1), -1, dtype=torch.int32)
+        wide[:, :table.shape[1]] = table
+        rows = q[:nodes].repeat(seqs, 1)
+        base = [n] + [n - 7 * b for b in range(1, seqs)]
+        got = attend(dev, cache, wide, rows, base, chain(seqs, nodes), H, max_len=max_len)
+        print("sizes", dtype, D, H, seqs, nodes, max_len, flush=True)
+        check_attention(got[:T], want, bound)
+        assert torch.equal(got[:T], attend(dev, cache, wide, rows, [n] + [5] * (seqs - 1), chain(seqs, nodes), H, max_len=max_len)[:T])

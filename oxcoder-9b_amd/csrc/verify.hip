@@ -15,6 +15,8 @@
 // degree 11, one weight after another), the walks by latency: 4 us where nothing is drawn, 12 with a draw (its two scans), for a
 // whole batch at once.  One request of 5 nodes over 151936 ids: 19 us; 32 chains of 8 with draft probabilities: 87; 16 trees of
 // 64 nodes over 248320 ids: 90, where a copy's rate would take 200 for all 1 GB of their rows.
+#include <algorithm>
+
 #include "kq_device.h"
 #include "kq_internal.h"
 
@@ -669,10 +671,15 @@ size_t verify_workspace(int B, int T, int V) {
 
 void launch_verify(const VerifyArgs& args, hipStream_t s) {
     VerifyArgs a = args;
-    // Rows of a round: all of them up to 160 MB, which one round reads in the time of the others' launches and waits (32 chains of 8
-    // over 151936 ids, 155 MB: 99 us, and 105 in rounds); else 64 MB for all requests, and in the last round whatever is left.
-    const int64_t row_bytes = (int64_t)a.B * a.V * 4, fit = (64 << 20) / row_bytes;
-    const bool once = row_bytes * a.T <= (160 << 20);
+    // Rows of a round: 8 nodes of each request, fewer where those are more than 64 MB, and in the last round whatever is left.  All at
+    // once where there are no more than 8 nodes (of up to 240 MB), or 24 of 64 MB in all: one round then costs less than the launches and
+    // waits of several.  Measured, all at once and by this rule's rounds: 32 chains of 8 over 151936 ids (148 MB) 63 and 75 us, 48
+    // with drawn drafts (223 MB) 112 and 116, but 64 chains (297 MB) 100 to 111 and 99; 8 trees of 10 (46 MB) 33 and 51, 4 of 24 (56 MB) 43 and 50; but 8 chains of 16 (74 MB) 44 and 41; one tree of 64
+    // (37 MB) 65 and 29, four (148 MB) 86 and 44; 16 of 64 over 16000 ids (62 MB) 125 and 75, over 32000 (125 MB) 146 and 69.  Of 16 nodes a
+    // request in place of 8 the last two take 79 and 77; of 4, four trees of 64 take 52 and 64 chains of 16 over 32000 ids 68, as with 8 (70).
+    // More than 64 MB a round: 16 trees of 64 over 248320 ids 90 us, 101 with 128 MB.
+    const int64_t row_bytes = (int64_t)a.B * a.V * 4, all_bytes = row_bytes * a.T, fit = std::min<int64_t>(8, (64 << 20) / row_bytes);
+    const bool once = all_bytes <= (64 << 20) ? a.T <= 24 : a.T <= 8 && all_bytes <= (240 << 20);
     const int most = once || fit >= a.T ? a.T : fit < 1 ? 1 : (int)fit, rounds = most < a.T ? VF_ROUNDS : 1;
     // the largest slice that leaves two workgroups a CU in the first round
     a.slice = VF_MOST;

@@ -257,7 +257,6 @@ struct VfShared {
     double sum[TREE_MOST], e[TREE_MOST], gone[TREE_MOST];     // the drafts' weights, the refused tokens'
     double wave[VF_W / 64];
     int found, last;
-    uint64_t nodes;
 };
 
 __device__ __forceinline__ double vf_left(const VfShared& S, const VfScale& s, const VfLeft& f, int i, float x, float q) {
@@ -450,7 +449,7 @@ __device__ void vf_row(VfShared& S, const VerifyArgs& a, const VfScale& s, int b
     for (int w = 32; w; w >>= 1) at = min(at, __shfl_xor(at, w, 64));
     if (lane == 0) S.m[t] = m, S.sum[t] = m == -INFINITY ? 0.0 : s.greedy ? 1.0 : sum, S.top_at[t] = at;
 }
-// The same from the row itself, by the whole workgroup (the same sums: slice by slice, in the first kernel's order).
+// The same from the row itself, by the whole workgroup: a sum in another order, equal to the slices' up to 64-bit rounding.
 __device__ void vf_row_anew(VfShared& S, const VerifyArgs& a, const VfScale& s, int b, int t) {
     const float* x = a.x + ((int64_t)b * a.T + t) * a.ldx;
     float m = -INFINITY;

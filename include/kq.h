@@ -389,8 +389,8 @@ int kq_attn_tree(const kq_kv* kv, const int32_t* table, int64_t ldt, int seqs, i
 
 /*
  * Keep the accepted nodes of each request in the caches of `layers` layers (kv[i], alike in heads, dim, pages and
- * page_size): path[b][0..] (row stride ldp, T entries) names nodes in rising order, node path[b][i] >= i, and ends at the first entry
- * that does not (-1, say); the entry at position base[b] + path[b][i] moves to base[b] + i, k, v and scales as they are.
+ * page_size): path[b][0..] (row stride ldp, T entries) names nodes of a tree of T in rising order, node path[b][i] >= i, and ends at the
+ * first entry that does not (-1, say; T or more); the entry at position base[b] + path[b][i] moves to base[b] + i, k, v and scales as they are.
  * Where either lies in a hole or past the table nothing is moved.  A cache that several layers share (the same k and v) is
  * moved once; caches that overlap otherwise are the caller's error.
  */

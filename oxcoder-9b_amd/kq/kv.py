@@ -246,8 +246,9 @@ class PagedAttention:
 
     def keep(self, path, base):
         """Move the entries of each request's accepted nodes together in every layer's cache: from position base[b] +
-        path[b][i] to base[b] + i, for i up to the first entry that names no node (below i, or not above the one
-        before; -1 ends it).  path: int32 [requests][up to 64], base: int32 [requests]."""
+        path[b][i] to base[b] + i, for i up to the first entry that names no node (below i, not above the one
+        before, or at least the row's width; -1 ends it).  path: int32 [requests][nodes], as wide as the trees and not cut to
+        the longest path, since its width says how many nodes there are; base: int32 [requests]."""
         c = self.caches[0]
         rc = self._plan and self._calls.keep(self._plan, C.addressof(self._refs), len(self.caches), ops._stream(c.device), path, base)
         if rc is None:                       # a tensor is not as it should be

@@ -297,7 +297,7 @@ __device__ int vf_draw(VfShared& S, const VerifyArgs& a, const VfScale& s, const
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const VfTop top(s, f.m);
     double target = (double)S.u[0] * left, before = 0.0;
-    int from = 0, to = a.slices;
+    int from = 0, to = a.slices, gone = f.gone;
     enum { SLICES, IDS, TOTAL, FIND };
     int found = -1;
 #pragma unroll 1
@@ -337,7 +337,7 @@ __device__ int vf_draw(VfShared& S, const VerifyArgs& a, const VfScale& s, const
                 } else if (f.q) {
                     w = fmax(w * f.per - f.a * (double)vf_q[i], 0.0);
                 }
-                for (int k = 0; k < f.gone; k++)
+                for (int k = 0; k < gone; k++)
                     if (S.refused[k] >> mine == at) w -= S.gone[k];
                 vf_w[i] = w;
             }
@@ -403,8 +403,9 @@ __device__ int vf_draw(VfShared& S, const VerifyArgs& a, const VfScale& s, const
         } else if (what == IDS) {
             if (found >= 0) break;
         } else if (what == TOTAL) {
-            if (found < 0) break;
-            target = (double)S.u[0] * before;
+            if (found < 0 && !gone) break;
+            if (found < 0) gone = 0, what = IDS;               // nothing but refused tokens: `left` was rounding, the total anew from p itself
+            else target = (double)S.u[0] * before;
         }
     }
     return found;

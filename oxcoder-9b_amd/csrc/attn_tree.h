@@ -14,13 +14,14 @@
 // bf16 values are exact, and sums fp32.  8-bit codes are bf16 values; an f16 value is the sum of two, its top 8 bits and the 3
 // that they leave, of which the second meets the first two parts of q and e (the third would add below 2^-24 of the product).
 //
-// Bound by the matrix units where there are many rows: 64 nodes over 50001 positions, 32 on 8 heads of 128, bf16, take three times
-// 52 GFLOP in 133 us, 1.18 PFLOP/s, 94 % of a large bf16 product's rate (a kernel whose waves each read the cache for
-// themselves, as for a few tokens a request: 240).  With fewer, by what is done once a tile: fetching, converting and storing
-// it for 64 rows (16 requests of 24 nodes, 16 on 4 heads of 256, f16: 162 us, whose products alone would take 68; 32 of 16 nodes, 8-bit:
-// 150, and 85).  Two tiles of rows a wave (NT = 2) halve that where there are more than 64 rows (the long
-// context 148 us against 173), but heads above 128 leave no registers for them.  Tiles are in LDS twice where two fit in 72 KB,
-// so that one is filled while the other is read (a barrier a tile instead of two).
+// Nearest its products where there are many rows: 64 nodes over 50001 positions, 32 on 8 heads of 128, bf16, take three times
+// 52 GFLOP in 147 us, 1.07 PFLOP/s, 86 % of a large bf16 product's rate; the matrix units are busy 58 % of the clocks, and waves wait
+// for their turn to issue 40 % of theirs (a kernel whose waves each read the cache for themselves, as for a few tokens a request:
+// 240).  With fewer, by what is done once a tile: fetching, converting and storing it for 64 rows (16 requests of 24 nodes, 16 on
+// 4 heads of 256, f16: 179 us, whose products alone would take 68; 32 of 16 nodes, 8-bit: 161, and 85).  Two tiles of rows a wave
+// (NT = 2) halve that where there are more than 64 rows (the long context 148 us against 173), but heads above 128 leave no registers
+// for them.  Tiles are in LDS twice where two fit in 72 KB, so that one is filled while the other is read (a barrier a tile instead of
+// two).  Times of the kernel alone, from a trace.
 #pragma once
 #include "attn_paged.h"
 

@@ -8,7 +8,7 @@ namespace kq {
 
 // ROWS rows a workgroup, 256 / ROWS threads each: lanes of 4 values, in groups that take every so many parts.  The parts'
 // largest scores and sums are looked at by all of a row's threads, and their weights left in LDS.  Bound by the parts' bytes and the
-// chain of loads: 4 us for 256 rows of 20 parts, 12 for 2048 of 32 (34 MB).
+// chain of loads: 4.3 us for 256 rows of 20 parts, 9.4 for 2048 of 32 (34 MB).
 constexpr int TJ_MOST = 2048;                // parts of a row at most
 template <int ROWS>
 __global__ void __launch_bounds__(256) k_attn_tree_join(AttnArgs a, int lanes) {
@@ -67,7 +67,9 @@ struct TreeSplit {
 // How a call's rows and positions are shared out.  Workgroups enough to fill the card once where each is long (two tiles of rows a wave,
 // two workgroups a CU: 512; 64 nodes over 50001 positions take 148 us, and 159 with 1024, which leave twice the parts to join), and
 // some four times where a wave takes one and requests are ragged (2048: batches of 16 in f16 and 32 in 8 bits 175 and 161 us; 1024:
-// 192 and 164, 4096: 207 and 170).
+// 192 and 164, 4096: 207 and 170).  All by max_len, which the host knows, and not by the lengths: with a max_len of 131072 the same four
+// calls (one of 8 nodes, one of 64, 16 and 32 requests) have longer parts for fewer workgroups and take 29, 225, 535 and 371 us in place
+// of 13, 145, 173 and 159.
 static int tiles_of(int R, int dim) { return R <= 64 || dim > 128 ? 1 : 2; }
 static int64_t columns_of(int seqs, int heads, int R, int tiles) {
     return (int64_t)seqs * heads * ((R + 64 * tiles - 1) / (64 * tiles));

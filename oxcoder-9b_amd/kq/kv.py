@@ -138,6 +138,8 @@ class PagedAttention:
     instead of (i, i + rot/2); scale: default dim ** -0.5.
     q_norm, k_norm: float32 [layers][dim], weights of a norm of each head of q (of k) that append applies ahead of the
     rotation, x / sqrt(mean(x^2) + eps) * w; nodes: the most nodes of a tree that attend_tree will see (0: none, up to 64).
+    attend_tree shares a request's positions out by max_len, not by their number: it is fastest where that is near the longest
+    request's (16 requests of 5000 positions: 173 us with 5027, 535 with 131072).
     These are for the object's life: another table or rotation takes another object, what is in them may change.
     Calls on one PagedAttention share its workspace and so must be ordered: one stream, or synchronised."""
 
